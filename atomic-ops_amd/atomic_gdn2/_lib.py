@@ -49,6 +49,28 @@ class Gdn2DecodeDesc(ctypes.Structure):
                 ("fuse_prologue", _c_int), ("cap", _c_int), ("scale", _c_dbl), ("stability_tau", _c_dbl)]
 
 
+class Gdn2LmPremixStep(ctypes.Structure):
+    """``struct gdn2_lm_premix_step`` (include/gdn2.h)."""
+    _fields_ = [("R", _c_int), ("S", _c_int), ("H", _c_int), ("D", _c_int), ("ldy", _c_int), ("parent_type", _c_int),
+                ("g_max", ctypes.c_float), ("y", _vp), ("history", _vp), ("parents", _vp), ("conv_w", _vp * 3),
+                ("conv_b", _vp * 3), ("gate_b", _vp * 2), ("decay_b", _vp), ("decay_a", _vp), ("out", _vp * 6),
+                ("og", _vp), ("new_history", _vp)]
+
+
+class Gdn2W4(ctypes.Structure):
+    """``struct gdn2_w4`` (include/gdn2.h)."""
+    _fields_ = [("M", _c_int), ("K", _c_int), ("N", _c_int), ("group", _c_int), ("dtype", _c_int),
+                ("ldx", ctypes.c_int64), ("ldr", ctypes.c_int64)] + [
+                    (n, _vp) for n in ("x", "q", "meta", "bias", "residual", "y")]
+
+
+class Gdn2Beam(ctypes.Structure):
+    """``struct gdn2_beam`` (include/gdn2.h)."""
+    _fields_ = [("B", _c_int), ("K", _c_int), ("V", _c_int), ("n", _c_int), ("eos", _c_int), ("dtype", _c_int),
+                ("ld", ctypes.c_int64)] + [
+                    (n, _vp) for n in ("logits", "scores", "finished", "tokens", "rows", "out_scores", "out_finished")]
+
+
 class Gdn2Error(RuntimeError):
     pass
 
@@ -81,6 +103,12 @@ def lib():
         L.gdn2_decode.argtypes = [P(Gdn2DecodeDesc)] + [_vp] * 13
         L.gdn2_prefill_prep.argtypes = [_c_int] * 6 + [_vp, _c_int] + [_vp] * 5
         L.gdn2_decode_flags.argtypes = [P(Gdn2DecodeDesc), _c_int] + [_vp] * 13
+        L.gdn2_decode_from.argtypes = [P(Gdn2DecodeDesc), _c_int] + [_vp] * 9 + [_c_int, _vp, _c_int] + [_vp] * 4
+        L.gdn2_lm_premix_step_fwd.argtypes = [_vp, _vp]
+        L.gdn2_w4_linear.argtypes = [P(Gdn2W4), _vp]
+        L.gdn2_beam_workspace_bytes.argtypes = [_c_int] * 4
+        L.gdn2_beam_workspace_bytes.restype = _c_size
+        L.gdn2_beam_step.argtypes = [P(Gdn2Beam), _vp, _vp]
         L.gdn2_bwd.argtypes = [P(Gdn2Desc)] + [_vp] * 18
         L.gdn2_wy_stage.argtypes = [P(Gdn2Desc)] + [_vp] * 15
         L.gdn2_scores.argtypes = [P(Gdn2Desc)] + [_vp] * 7
@@ -107,7 +135,8 @@ def lib():
                    "gdn2_fwd_prefill",
                    "gdn2_decode", "gdn2_prefill_prep", "gdn2_decode_flags", "gdn2_bwd", "gdn2_wy_stage", "gdn2_scores", "gdn2_debug_gemm", "gdn2_debug_stream",
                    "gdn2_debug_mfma", "gdn2_lm_premix_fwd", "gdn2_lm_premix_bwd", "gdn2_lm_rms_fwd", "gdn2_lm_rms_bwd",
-                   "gdn2_lm_swiglu", "gdn2_lm_columns", "gdn2_prof_begin", "gdn2_prof_end"):
+                   "gdn2_lm_swiglu", "gdn2_lm_columns", "gdn2_decode_from", "gdn2_lm_premix_step_fwd", "gdn2_w4_linear", "gdn2_beam_step",
+                   "gdn2_prof_begin", "gdn2_prof_end"):
             getattr(L, fn).restype = _c_int
         if L.gdn2_abi_version() != ABI_VERSION:
             raise Gdn2Error("libgdn2_hip.so ABI version mismatch")
@@ -117,7 +146,7 @@ def lib():
 
 _BIND = None
 _BIND_ABI = ("gdn2_residual_layout", "gdn2_fwd_workspace_bytes", "gdn2_bwd_workspace_bytes", "gdn2_fwd", "gdn2_fwd_bf16",
-             "gdn2_bwd", "gdn2_decode_flags", "gdn2_default_state_ckpt", "gdn2_last_error")
+             "gdn2_bwd", "gdn2_decode_from", "gdn2_default_state_ckpt", "gdn2_last_error")
 
 
 def bind():

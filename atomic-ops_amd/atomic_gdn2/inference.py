@@ -101,7 +101,7 @@ def _aligned(t):
 
 
 def _run_decode(xs, in_dtype, B, H, D, n_tok, seq_ld, scale, state_in, state_code, o, out_code,
-                reset=None, fuse=False, a_log=None, dt_bias=None, tau=None, offset=0):
+                reset=None, fuse=False, a_log=None, dt_bias=None, tau=None, offset=0, parents=None):
     dev = xs[0].device
     xs = [_aligned(x) for x in xs]
     state_in = _aligned(state_in)
@@ -112,16 +112,18 @@ def _run_decode(xs, in_dtype, B, H, D, n_tok, seq_ld, scale, state_in, state_cod
                              int(tau is not None), float(scale), float(tau) if tau is not None else 0.0)
     L_ = _lib.lib()
     with torch.cuda.device(dev):
-        _lib.check(L_.gdn2_decode(ctypes.byref(dd), *(_lib.ptr(x, offset) for x in xs), _lib.ptr(a_log),
-                                  _lib.ptr(dt_bias), _lib.ptr(reset), _lib.ptr(state_in), _lib.ptr(o, offset),
-                                  _lib.ptr(state_out), _lib.stream_handle(dev)), "gdn2_decode")
+        _lib.check(L_.gdn2_decode_from(ctypes.byref(dd), 0, *(_lib.ptr(x, offset) for x in xs), _lib.ptr(a_log),
+                                       _lib.ptr(dt_bias), _lib.ptr(reset),
+                                       0 if parents is None else _ID_TYPES[parents.dtype], _lib.ptr(parents),
+                                       0 if parents is None else state_in.shape[0], _lib.ptr(state_in),
+                                       _lib.ptr(o, offset), _lib.ptr(state_out), _lib.stream_handle(dev)), "gdn2_decode")
     return state_out
 
 
 def decode_step(q=None, k=None, v=None, w=None, b=None, g=None, state=None,
                 scale: float = 1.0, reset=None, state_dtype=torch.float32,
                 stability_tau=None, fuse_prologue: bool = False, a_log=None,
-                dt_bias=None, inputs: "LayerInputs | None" = None, cfg=None):
+                dt_bias=None, inputs: "LayerInputs | None" = None, cfg=None, parents=None):
     """Single-token recurrence for serving (reference ``decode_step``).
 
     q, k, v, w, b, g: (B, H, D), g this token's log-decay (positive values act as 0, as in
@@ -130,6 +132,10 @@ def decode_step(q=None, k=None, v=None, w=None, b=None, g=None, state=None,
     b, w raw logits (sigmoid) and g the raw gate, g = -exp(a_log[h]) * softplus(g + dt_bias[d]),
     with a_log (H,) and dt_bias (D,).  stability_tau: cap on each head's Frobenius norm of the
     new state.  NaN / +-Inf entries of the new state and of o become 0.
+
+    parents (B,) int32 or int64, with a state (S, H, D, D) of any number of rows: row b continues state
+    row parents[b] (the beams of a search, whose states are reordered in the read that the step makes
+    anyway); a row outside 0 .. S-1 starts from a zero state.
 
     Returns (o (B, H, D) in q's dtype, new_state (B, H, D, D) in state_dtype).  Compute is fp32;
     the incoming state is first cast to state_dtype (as the reference does)."""
@@ -142,7 +148,7 @@ def decode_step(q=None, k=None, v=None, w=None, b=None, g=None, state=None,
         # plain calls (csrc/bind.cpp) go native; None = not one, and what follows handles it
         out = _lib.bind().decode(q, k, v, w, b, g, state, float(scale), reset, _STATE_DTYPES[state_dtype] == 1,
                                  None if stability_tau is None else float(stability_tau), fuse_prologue,
-                                 a_log if fuse_prologue else None, dt_bias if fuse_prologue else None)
+                                 a_log if fuse_prologue else None, dt_bias if fuse_prologue else None, parents)
         if out is not None:
             return out
     bsz, H, D = q.shape
@@ -153,7 +159,7 @@ def decode_step(q=None, k=None, v=None, w=None, b=None, g=None, state=None,
     if stability_tau is not None and not isinstance(stability_tau, (int, float)):
         raise ValueError(
             "stability_tau must be a concrete Python float (B4)")
-    if tuple(state.shape) != (bsz, H, D, D):
+    if tuple(state.shape[-3:]) != (H, D, D) or state.dim() != 4 or (parents is None and state.shape[0] != bsz):
         raise ValueError(f"state must be (B,H,D,D), got {tuple(state.shape)}")
     sc = _state_code(state_dtype)
     rst = None
@@ -180,13 +186,23 @@ def decode_step(q=None, k=None, v=None, w=None, b=None, g=None, state=None,
     xs, in_dtype = _inputs_for_kernel(ts)
     st = state.to(_torch_dtype(sc)).contiguous()
     out_code = 1 if q.dtype == torch.bfloat16 else 0
+    if parents is not None:
+        if tuple(parents.shape) != (bsz,):
+            raise ValueError(f"parents must be (B,), got {tuple(parents.shape)}")
+        if parents.is_floating_point() or parents.is_complex() or parents.dtype == torch.bool:
+            raise TypeError(f"parents must be whole numbers, got {parents.dtype}")
+        if parents.device != dev:
+            raise ValueError(f"parents is on {parents.device}, q on {dev}")
+        if state.shape[0] == 0:
+            raise ValueError("parents need a state to start from")
+        parents = (parents if parents.dtype in _ID_TYPES else parents.to(torch.int64)).contiguous()
     o = torch.empty((bsz, H, D), dtype=_torch_dtype(out_code), device=dev)
     flags = None if rst is None else rst.to(device=dev, dtype=torch.uint8).contiguous()
     if fuse_prologue:
         a_log = a_log.to(device=dev, dtype=torch.float32).contiguous()
         dt_bias = dt_bias.to(device=dev, dtype=torch.float32).contiguous()
     new = _run_decode(xs, in_dtype, bsz, H, D, 1, 1, scale, st, sc, o, out_code, reset=flags,
-                      fuse=fuse_prologue, a_log=a_log, dt_bias=dt_bias, tau=stability_tau)
+                      fuse=fuse_prologue, a_log=a_log, dt_bias=dt_bias, tau=stability_tau, parents=parents)
     if o.dtype != q.dtype:
         o = o.to(q.dtype)
     return o, new

@@ -41,7 +41,7 @@ struct Abi {
   decltype(&gdn2_fwd) fwd;
   decltype(&gdn2_fwd_bf16) fwd_bf16;
   decltype(&gdn2_bwd) bwd;
-  decltype(&gdn2_decode_flags) decode;
+  decltype(&gdn2_decode_from) decode;
   decltype(&gdn2_default_state_ckpt) default_ckpt;
   decltype(&gdn2_last_error) last_error;
 } abi{};
@@ -318,22 +318,30 @@ PyObject* py_sequence(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// Row indices as the kernels take them: n of int32 or int64 (kind), contiguous on the device.
+bool row_indices(const Tensor& t, const c10::Device& dev, int64_t n, int* kind) {
+  if (!plain(t, dev) || !t.is_contiguous() || t.dim() != 1 || t.numel() != n) return false;
+  *kind = t.scalar_type() == at::kInt ? GDN2_FLAG_INT32 : GDN2_FLAG_INT64;
+  return t.scalar_type() == at::kInt || t.scalar_type() == at::kLong;
+}
+
 // decode(q, k, v, w, b, g, state, scale, reset or None, state is bf16, tau or None, fuse, a_log or
-// None, dt_bias or None) -> (o, new state), or None: not a plain call
+// None, dt_bias or None[, parents or None]) -> (o, new state), or None: not a plain call
 PyObject* py_decode(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 14) return PyErr_Format(PyExc_TypeError, "decode takes 14 arguments");
+  if (n != 14 && n != 15) return PyErr_Format(PyExc_TypeError, "decode takes 14 or 15 arguments");
   for (int i = 0; i < 7; ++i)
     if (!THPVariable_Check(args[i])) return none();
-  for (int i : {8, 12, 13})
-    if (args[i] != Py_None && !THPVariable_Check(args[i])) return none();
+  for (int i : {8, 12, 13, 14})
+    if (i < n && args[i] != Py_None && !THPVariable_Check(args[i])) return none();
   if (!PyFloat_Check(args[7]) || (args[10] != Py_None && !PyFloat_Check(args[10]))) return none();
-  Tensor x[7], reset, a_log, dt_bias;
+  Tensor x[7], reset, a_log, dt_bias, parents;
   for (int i = 0; i < 7; ++i) x[i] = THPVariable_Unpack(args[i]);
   if (args[8] != Py_None) reset = THPVariable_Unpack(args[8]);
   const bool sbf = PyObject_IsTrue(args[9]) == 1, fuse = PyObject_IsTrue(args[11]) == 1;
   if (args[12] != Py_None) a_log = THPVariable_Unpack(args[12]);
   if (args[13] != Py_None) dt_bias = THPVariable_Unpack(args[13]);
+  if (n == 15 && args[14] != Py_None) parents = THPVariable_Unpack(args[14]);
   if (!plain_mode() || !x[0].is_cuda() || x[0].dim() != 3 || x[0].numel() == 0) return none();
   const c10::Device dev = x[0].device();
   const int64_t B = x[0].size(0), H = x[0].size(1), D = x[0].size(2);
@@ -344,7 +352,9 @@ PyObject* py_decode(PyObject*, PyObject* const* args, Py_ssize_t n) {
   };
   for (int i = 0; i < 6; ++i)
     if (!ready(x[i], dt) || x[i].sizes() != x[0].sizes()) return none();
-  if (!ready(x[6], sdt) || x[6].dim() != 4 || x[6].size(0) != B || x[6].size(1) != H || x[6].size(2) != D || x[6].size(3) != D)
+  int from = 0;
+  if (parents.defined() && !row_indices(parents, dev, B, &from)) return none();
+  if (!ready(x[6], sdt) || x[6].dim() != 4 || (from ? x[6].size(0) < 1 || x[6].size(0) > INT32_MAX : x[6].size(0) != B) || x[6].size(1) != H || x[6].size(2) != D || x[6].size(3) != D)
     return none();
   int kind = 0;
   if (reset.defined()) {
@@ -376,7 +386,8 @@ PyObject* py_decode(PyObject*, PyObject* const* args, Py_ssize_t n) {
     st = empty_on(x[0], {B, H, D, D}, sdt);
     auto p = [&](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
     status = abi.decode(&d, kind, p(x[0]), p(x[1]), p(x[2]), p(x[3]), p(x[4]), p(x[5]),
-                        fuse ? f32_at(a_log) : nullptr, fuse ? f32_at(dt_bias) : nullptr, p(reset), p(x[6]), p(o), p(st),
+                        fuse ? f32_at(a_log) : nullptr, fuse ? f32_at(dt_bias) : nullptr, p(reset), from, p(parents),
+                        (int)x[6].size(0), p(x[6]), p(o), p(st),
                         stream_of(dev));
   });
   return status ? none() : pair(o, st);

@@ -392,6 +392,14 @@ int gdn2_decode(const gdn2_decode_desc* d, const void* q, const void* k, const v
 int gdn2_decode_flags(const gdn2_decode_desc* d, int flag_type, const void* q, const void* k, const void* v,
                       const void* w, const void* b, const void* g, const float* a_log, const float* dt_bias,
                       const void* reset, const void* state_in, void* o, void* state_out, void* stream) {
+  return gdn2_decode_from(d, flag_type, q, k, v, w, b, g, a_log, dt_bias, reset, 0, nullptr, 0, state_in, o, state_out,
+                          stream);
+}
+
+int gdn2_decode_from(const gdn2_decode_desc* d, int flag_type, const void* q, const void* k, const void* v,
+                     const void* w, const void* b, const void* g, const float* a_log, const float* dt_bias,
+                     const void* reset, int parent_type, const void* parents, int n_states, const void* state_in,
+                     void* o, void* state_out, void* stream) {
   if (flag_type < GDN2_FLAG_BYTE || flag_type > GDN2_FLAG_INT64) return fail(GDN2_ERR_INVALID, "unknown flag type");
   if (!d) return fail(GDN2_ERR_INVALID, "null descriptor");
   if (d->B < 1 || d->H < 1 || d->n_tok < 1) return fail(GDN2_ERR_INVALID, "non-positive shape");
@@ -402,6 +410,17 @@ int gdn2_decode_flags(const gdn2_decode_desc* d, int flag_type, const void* q, c
     if (f != 0 && f != 1) return fail(GDN2_ERR_INVALID, "dtype / flag fields must be 0 or 1");
   if (!q || !k || !v || !w || !b || !g || !o || !state_out) return fail(GDN2_ERR_INVALID, "null tensor pointer");
   if (d->fuse_prologue && (!a_log || !dt_bias)) return fail(GDN2_ERR_INVALID, "fuse_prologue needs a_log and dt_bias");
+  if (parents) {
+    if (parent_type != GDN2_FLAG_INT32 && parent_type != GDN2_FLAG_INT64)
+      return fail(GDN2_ERR_INVALID, "parents are int32 or int64");
+    if (d->n_tok != 1) return fail(GDN2_ERR_UNSUPPORTED, "parents with one token only");
+    if (!state_in || n_states < 1) return fail(GDN2_ERR_INVALID, "parents need a state to start from");
+    // (what a row starts from may be another row's state)
+    const size_t row = (size_t)d->H * d->D * d->D * (d->state_dtype ? 2 : 4);
+    const char *si = static_cast<const char*>(state_in), *so = static_cast<const char*>(state_out);
+    if (si < so + row * d->B && so < si + row * n_states)
+      return fail(GDN2_ERR_INVALID, "with parents, state_out must not overlap state_in");
+  }
   gdn2::DecodeArgs a{};
   a.q = q; a.k = k; a.v = v; a.w = w; a.b = b; a.g = g;
   a.a_log = a_log; a.dt_bias = dt_bias; a.reset = reset; a.flag_type = flag_type; a.state_in = state_in;
@@ -410,6 +429,7 @@ int gdn2_decode_flags(const gdn2_decode_desc* d, int flag_type, const void* q, c
   a.in_bf16 = d->in_dtype; a.out_bf16 = d->out_dtype; a.state_bf16 = d->state_dtype;
   a.fuse = d->fuse_prologue; a.cap = d->cap;
   a.scale = (float)d->scale; a.tau = (float)d->stability_tau;
+  a.parents = parents; a.parent64 = parent_type == GDN2_FLAG_INT64; a.n_states = n_states;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const hipError_t e = timed(8, s, [&] { return gdn2::launch_decode(d->D, a, d->B * d->H, s); });
   if (e != hipSuccess) return hip_fail(e, "decode launch");
@@ -757,6 +777,112 @@ int gdn2_lm_columns(int split, float* const parts[], const int32_t widths[], int
   a.rows = rows;
   a.ld = ld;
   return lm_done(gdn2::launch_lm_columns(a, split != 0, reinterpret_cast<hipStream_t>(stream)), "lm columns launch");
+}
+
+int gdn2_lm_premix_step_fwd(const gdn2_lm_premix_step* p, void* stream) {
+  if (!p) return fail(GDN2_ERR_INVALID, "null argument block");
+  if (p->R < 1 || p->S < 1 || p->H < 1) return fail(GDN2_ERR_INVALID, "non-positive shape");
+  if (p->D != 64 && p->D != 128) return fail(GDN2_ERR_UNSUPPORTED, "D in {64, 128} only");
+  if (p->H > 4096 || (int64_t)p->R * p->H > (int64_t(1) << 28)) return fail(GDN2_ERR_UNSUPPORTED, "shape too large");
+  if (p->ldy < 6 * p->H * p->D + p->H) return fail(GDN2_ERR_INVALID, "ldy too small");
+  if (p->parents && p->parent_type != GDN2_FLAG_INT32 && p->parent_type != GDN2_FLAG_INT64)
+    return fail(GDN2_ERR_INVALID, "parents are int32 or int64");
+  if (!p->parents && p->S != p->R) return fail(GDN2_ERR_INVALID, "without parents every row continues its own history: S = R");
+  gdn2::LmPremixStepArgs a{};
+  bool ok = p->y && p->history && p->decay_b && p->decay_a && p->og && p->new_history;
+  for (int i = 0; i < 3; ++i) {
+    a.cw[i] = p->conv_w[i];
+    a.cb[i] = p->conv_b[i];
+    ok = ok && p->conv_w[i] && p->conv_b[i] && aligned16({p->conv_w[i]});
+  }
+  for (int i = 0; i < 2; ++i) {
+    a.gb[i] = p->gate_b[i];
+    ok = ok && p->gate_b[i];
+  }
+  for (int i = 0; i < 6; ++i) {
+    a.out[i] = p->out[i];
+    ok = ok && p->out[i];
+  }
+  if (!ok) return fail(GDN2_ERR_INVALID, "null pointer, or taps not 16-byte aligned");
+  const size_t row = (size_t)9 * p->H * p->D;
+  if (p->history < p->new_history + row * p->R && p->new_history < p->history + row * p->S)
+    return fail(GDN2_ERR_INVALID, "new_history must not overlap history");
+  a.y = p->y; a.history = p->history; a.parents = p->parents;
+  a.decay_b = p->decay_b; a.decay_a = p->decay_a; a.og = p->og; a.new_history = p->new_history;
+  a.R = p->R; a.S = p->S; a.H = p->H; a.ldy = p->ldy;
+  a.parent64 = p->parent_type == GDN2_FLAG_INT64;
+  a.g_max = p->g_max;
+  return lm_done(gdn2::launch_lm_premix_step(p->D, a, reinterpret_cast<hipStream_t>(stream)), "lm premix step launch");
+}
+
+static_assert(GDN2_F32 == gdn2::W4_F32 && GDN2_BF16 == gdn2::W4_BF16 && GDN2_F16 == gdn2::W4_F16, "header constants");
+
+int gdn2_w4_linear(const gdn2_w4* p, void* stream) {
+  if (!p) return fail(GDN2_ERR_INVALID, "null argument block");
+  if (p->M < 1 || p->K < 1 || p->N < 1) return fail(GDN2_ERR_INVALID, "non-positive shape");
+  if (p->group != 32 && p->group != 64 && p->group != 128) return fail(GDN2_ERR_UNSUPPORTED, "groups of 32, 64 or 128 rows");
+  if (p->dtype < GDN2_F32 || p->dtype > GDN2_F16) return fail(GDN2_ERR_INVALID, "unknown dtype");
+  if (p->M > (1 << 20) || p->K > (1 << 24) || p->N > (1 << 24)) return fail(GDN2_ERR_UNSUPPORTED, "shape too large");
+  if (p->ldx < p->K || (p->residual && p->ldr < p->N)) return fail(GDN2_ERR_INVALID, "row stride below the row");
+  if (!p->x || !p->q || !p->meta || !p->y || !aligned16({p->q, p->meta}))
+    return fail(GDN2_ERR_INVALID, "null pointer, or weights not 16-byte aligned");
+  const uintptr_t e = p->dtype == GDN2_F32 ? 4 : 2;
+  if ((reinterpret_cast<uintptr_t>(p->x) | reinterpret_cast<uintptr_t>(p->y) | reinterpret_cast<uintptr_t>(p->bias) |
+       reinterpret_cast<uintptr_t>(p->residual)) & (e - 1))
+    return fail(GDN2_ERR_INVALID, "pointer not aligned to its elements");
+  gdn2::W4Args a{};
+  a.x = p->x; a.q = static_cast<const uint32_t*>(p->q); a.meta = static_cast<const uint32_t*>(p->meta);
+  a.bias = p->bias; a.res = p->residual; a.y = p->y;
+  a.M = p->M; a.K = p->K; a.N = p->N;
+  a.nkb = (p->K + gdn2::W4_KB - 1) / gdn2::W4_KB;
+  a.nnb = (p->N + 15) / 16;
+  a.ldx = (size_t)p->ldx; a.ldr = (size_t)p->ldr;
+  a.vec = aligned16({p->x}) && p->K % 8 == 0 && p->ldx % (16 / e) == 0;
+  return lm_done(gdn2::launch_w4(p->dtype, p->group, a, reinterpret_cast<hipStream_t>(stream)), "w4 launch");
+}
+
+namespace {
+int beam_shape(int B, int K, int V, int n) {
+  if (B < 1 || K < 1 || V < 1 || n < 1) return fail(GDN2_ERR_INVALID, "non-positive shape");
+  if (n > gdn2::BEAM_MAX_N || K > gdn2::BEAM_MAX_K) return fail(GDN2_ERR_UNSUPPORTED, "at most 128 beams a group, kept or given");
+  if ((int64_t)K * V >= (int64_t(1) << 31) || (int64_t)B * K > 65535) return fail(GDN2_ERR_UNSUPPORTED, "shape too large");
+  if ((int64_t)n > (int64_t)K * V) return fail(GDN2_ERR_INVALID, "n above K V");
+  if ((int64_t)K * n * gdn2::beam_splits(B * K, V) >= (int64_t(1) << 31))
+    return fail(GDN2_ERR_UNSUPPORTED, "shape too large");
+  return GDN2_OK;
+}
+size_t beam_cand_bytes(int B, int K, int V, int n) {
+  return align_up((size_t)B * K * gdn2::beam_splits(B * K, V) * n * 8);
+}
+}  // namespace
+
+size_t gdn2_beam_workspace_bytes(int B, int K, int V, int n) {
+  if (beam_shape(B, K, V, n)) return 0;
+  return beam_cand_bytes(B, K, V, n) + (size_t)B * K * gdn2::beam_splits(B * K, V) * 8;
+}
+
+int gdn2_beam_step(const gdn2_beam* p, void* workspace, void* stream) {
+  if (!p) return fail(GDN2_ERR_INVALID, "null argument block");
+  const int st = beam_shape(p->B, p->K, p->V, p->n);
+  if (st) return st;
+  if (p->dtype < GDN2_F32 || p->dtype > GDN2_F16) return fail(GDN2_ERR_INVALID, "unknown dtype");
+  if (p->eos < -1 || p->eos >= p->V) return fail(GDN2_ERR_INVALID, "eos outside the vocabulary");
+  if (p->finished && p->eos < 0) return fail(GDN2_ERR_INVALID, "finished beams need an eos token");
+  if (p->ld < p->V) return fail(GDN2_ERR_INVALID, "row stride below the row");
+  if (!p->logits || !p->scores || !p->tokens || !p->rows || !p->out_scores || !workspace || !aligned16({workspace}))
+    return fail(GDN2_ERR_INVALID, "null pointer, or workspace not 16-byte aligned");
+  const int e = p->dtype == GDN2_F32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(p->logits) % e) return fail(GDN2_ERR_INVALID, "pointer not aligned to its elements");
+  gdn2::BeamArgs a{};
+  a.logits = p->logits; a.scores = p->scores; a.finished = p->finished;
+  a.cand = static_cast<unsigned long long*>(workspace);
+  a.part = at<float>(workspace, beam_cand_bytes(p->B, p->K, p->V, p->n));
+  a.tokens = p->tokens; a.rows = p->rows; a.out_scores = p->out_scores; a.out_finished = p->out_finished;
+  a.B = p->B; a.K = p->K; a.V = p->V; a.n = p->n; a.eos = p->eos;
+  a.splits = gdn2::beam_splits(p->B * p->K, p->V);
+  a.ld = (size_t)p->ld;
+  a.vec = aligned16({p->logits}) && p->ld * e % 16 == 0;
+  return lm_done(gdn2::launch_beam(p->dtype, a, reinterpret_cast<hipStream_t>(stream)), "beam launch");
 }
 
 int gdn2_debug_scan_copies(int n_bh, int D, int nc, int in_place, int cus) {

@@ -87,11 +87,13 @@ __global__ __launch_bounds__(CW / 4 * 16) void decode_step_kernel(DecodeArgs a) 
   const int bi = bh / a.H, hi = bh - bi * a.H;
   const int l = lane_id(), wv = tid / WAVE;
   const size_t sb = (size_t)bh * D * D;
+  const int from = a.parents ? row_index(a.parents, a.parent64, bi, a.n_states) : bi;
+  const size_t sp = ((size_t)from * a.H + hi) * D * D;
 
   float4 h[KPK];
 #pragma unroll
   for (int i = 0; i < KPK; ++i)
-    h[i] = a.state_in ? ld_quad<SBF>(a.state_in, sb + (size_t)(d0 + i) * D + j0) : make_float4(0.f, 0.f, 0.f, 0.f);
+    h[i] = a.state_in && from >= 0 ? ld_quad<SBF>(a.state_in, sp + (size_t)(d0 + i) * D + j0) : make_float4(0.f, 0.f, 0.f, 0.f);
 
   const size_t io = (size_t)bh * a.seq_ld * D;
   // this thread's columns of w and v, issued with the key vectors' loads (one round trip)

@@ -243,6 +243,9 @@ struct DecodeArgs {
   int H, n_tok, seq_ld;
   int in_bf16, out_bf16, state_bf16, fuse, cap;
   float scale, tau;
+  // one token only: row b starts from state row parents[b] of n_states (from zero outside them)
+  const void* parents;
+  int parent64, n_states;
 };
 
 hipError_t launch_decode(int D, const DecodeArgs& a, int n_bh, hipStream_t s);
@@ -366,6 +369,66 @@ hipError_t launch_lm_rms_fwd(const LmRmsArgs& a, hipStream_t s);
 hipError_t launch_lm_rms_bwd(const LmRmsArgs& a, hipStream_t s);
 hipError_t launch_lm_swiglu(const float* gu, const float* dact, float* out, int rows, int M, hipStream_t s);
 hipError_t launch_lm_columns(const LmColumnsArgs& a, bool split, hipStream_t s);
+
+// One token of the block between its input projections and the recurrence (gdn2_lm.hip): y rows of
+// ldy floats as in LmPremixArgs; history: S rows of the three projections before it, oldest first,
+// 3 C floats each (q | k | v); parents: null or a history row for each of the R rows (zero history
+// outside [0, S)).  out: q, k, v, w, b, g (R, H, D); og (R, C); new_history like history, R rows.
+struct LmPremixStepArgs {
+  const float *y, *history;
+  const void* parents;
+  const float *cw[3], *cb[3], *gb[2], *decay_b, *decay_a;
+  float *out[6], *og, *new_history;
+  int R, S, H, ldy, parent64;
+  float g_max;
+};
+hipError_t launch_lm_premix_step(int D, const LmPremixStepArgs& a, hipStream_t s);
+
+// Element i of a row index tensor (int32 or int64), -1 outside [0, n).
+__device__ __forceinline__ int row_index(const void* p, int is64, int i, int n) {
+  if (is64) {
+    const int64_t x = static_cast<const int64_t*>(p)[i];
+    return x >= 0 && x < n ? (int)x : -1;
+  }
+  const int x = static_cast<const int32_t*>(p)[i];
+  return x >= 0 && x < n ? x : -1;
+}
+
+// Rows times a matrix of 4-bit weights (gdn2_w4.hip).  x (M, K) rows of ldx elements; q: for each 16
+// columns and 128 rows of the matrix, 64 lanes of four words; lane l's word j holds rows
+// 32 j + 8 (l / 16) + e of column l % 16, element e < 4 in nibble 2 e, e >= 4 in nibble 2 e - 7; meta:
+// for each 16 columns and group a word a column, scale | zero << 16 as bfloat16 bits.  Rows past K and
+// columns past N have scale 0.  res (M, N) rows of ldr elements, y (M, N).
+constexpr int W4_F32 = 0, W4_BF16 = 1, W4_F16 = 2;
+constexpr int W4_KB = 128;
+struct W4Args {
+  const void* x;
+  const uint32_t *q, *meta;
+  const void *bias, *res;
+  void* y;
+  int M, K, N, nkb, nnb;
+  size_t ldx, ldr;
+  int vec;                     // whole 16-byte accesses of x: alignment, ldx and K allow them
+};
+hipError_t launch_w4(int dtype, int group, const W4Args& a, hipStream_t s);
+
+// Beam search's selection (gdn2_beam.hip).  logits (B K, V) rows of ld elements; part: per row and split
+// (maximum, sum of exp); cand: per row and split n keys.
+constexpr int BEAM_MAX_N = 128, BEAM_MAX_K = 128;
+struct BeamArgs {
+  const void* logits;
+  const float* scores;
+  const uint8_t* finished;
+  float* part;
+  unsigned long long* cand;
+  int64_t *tokens, *rows;
+  float* out_scores;
+  uint8_t* out_finished;
+  int B, K, V, n, eos, splits, vec;
+  size_t ld;
+};
+int beam_splits(int rows, int V);
+hipError_t launch_beam(int dtype, const BeamArgs& a, hipStream_t s);
 
 // Linear work index of this workgroup such that consecutive indices (workgroups of one
 // (batch, head), which read the same chunk operands) land on the same XCD (blockIdx % 8 picks

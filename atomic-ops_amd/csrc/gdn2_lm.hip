@@ -355,6 +355,68 @@ __global__ __launch_bounds__(256) void lm_premix_bwd_kernel(LmPremixBwdArgs a) {
   }
 }
 
+// ------------------------------------------------------------------------------------
+// premix of one token from cached projections: the convolutions' window is the row's parent's last
+// three projections and y itself.  One wave a row, head and role (the roles of premix), lanes over the
+// channels, so that rows of any alignment are read whole.
+// ------------------------------------------------------------------------------------
+template <int D>
+__global__ __launch_bounds__(256) void lm_premix_step_kernel(LmPremixStepArgs a) {
+  constexpr int NC = D / WAVE;                       // channels of a lane
+  const int id = blockIdx.x * 4 + wave_id(), n = a.R * a.H, role = id / n;
+  if (role >= 7) return;
+  const int rh = id - role * n, row = rh / a.H, h = rh - row * a.H, l = lane_id(), C = a.H * D;
+  const float* __restrict__ y = a.y + (size_t)row * a.ldy;
+  const size_t ob = (size_t)rh * D + l;
+  if (role < 3) {
+    const int from = a.parents ? row_index(a.parents, a.parent64, row, a.S) : row;
+    const float* __restrict__ past = a.history + ((size_t)max(from, 0) * 9 + role) * C;
+    float* __restrict__ keep = a.new_history + ((size_t)row * 9 + role) * C;
+    float s[NC], ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int ch = h * D + l + WAVE * i;
+      const F4 wt = ldf(a.cw[role] + 4 * ch);
+      float x[4];
+#pragma unroll
+      for (int j = 0; j < 3; ++j) x[j] = from >= 0 ? past[(size_t)3 * C * j + ch] : 0.f;
+      x[3] = y[role * C + ch];
+      float u = fmaf(x[3], wt.v[3], a.cb[role][ch]);
+#pragma unroll
+      for (int j = 2; j >= 0; --j) u = fmaf(x[j], wt.v[j], u);
+      s[i] = u * sigmoid_1ulp(u);
+      ss = fmaf(s[i], s[i], ss);
+#pragma unroll
+      for (int j = 0; j < 3; ++j) keep[(size_t)3 * C * j + ch] = x[j + 1];
+    }
+    if (role < 2) {
+      const float r = rsqrtf(lanes_sum<WAVE>(ss) + 1e-6f);
+#pragma unroll
+      for (int i = 0; i < NC; ++i) s[i] *= r;
+    } else {
+#pragma unroll
+      for (int i = 0; i < NC; ++i) s[i] = clip_nan(s[i], -50.f, 50.f);
+    }
+#pragma unroll
+    for (int i = 0; i < NC; ++i) a.out[role][ob + WAVE * i] = s[i];
+    return;
+  }
+  if (role < 6) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int ch = h * D + l + WAVE * i;
+      const float x = y[role * C + ch];
+      if (role == 5) a.og[(size_t)row * C + ch] = x;
+      else a.out[7 - role][ob + WAVE * i] = sigmoid_1ulp(x + a.gb[role - 3][ch]);
+    }
+    return;
+  }
+  const float ldh = -expf(clip_nan(a.decay_a[h], -20.f, 20.f)) * softplus_t(y[6 * C + h] + a.decay_b[h]);
+  const float ld = ldh != ldh ? 0.f : (ldh == __builtin_inff() ? 0.f : (ldh == -__builtin_inff() ? -20.f : ldh));
+#pragma unroll
+  for (int i = 0; i < NC; ++i) a.out[5][ob + WAVE * i] = -fminf(fabsf(ld), a.g_max);
+}
+
 // out[r] = sum_p part[p][r], p ascending within four quarters that are then added in order
 __global__ __launch_bounds__(256) void lm_reduce_kernel(const float* part, float* out, int rows, int cols) {
   __shared__ float red[256];
@@ -548,6 +610,13 @@ hipError_t launch_lm_premix_fwd(int D, const LmPremixArgs& a, hipStream_t s) {
   const dim3 grid(a.B * a.H * ((a.L + LM_TOK - 1) / LM_TOK), 7);
   if (D == 128) hipLaunchKernelGGL((lm_premix_fwd_kernel<128>), grid, dim3(256), 0, s, a);
   else hipLaunchKernelGGL((lm_premix_fwd_kernel<64>), grid, dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_lm_premix_step(int D, const LmPremixStepArgs& a, hipStream_t s) {
+  const dim3 grid((a.R * a.H * 7 + 3) / 4);
+  if (D == 128) hipLaunchKernelGGL((lm_premix_step_kernel<128>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((lm_premix_step_kernel<64>), grid, dim3(256), 0, s, a);
   return hipGetLastError();
 }
 

@@ -199,6 +199,16 @@ int gdn2_decode_flags(const gdn2_decode_desc* d, int flag_type, const void* q, c
                       const float* a_log, const float* dt_bias, const void* reset,
                       const void* state_in, void* o, void* state_out, void* stream);
 
+/* gdn2_decode_flags for one token (n_tok = 1), batch row b starting from row parents[b] of a state
+ * (n_states, H, D, D): the reordering of a beam search's states in the read that the step makes
+ * anyway.  parents: B rows, int32 (parent_type GDN2_FLAG_INT32) or int64 (GDN2_FLAG_INT64); a row
+ * outside [0, n_states) starts from a zero state.  state_out must not overlap state_in. */
+int gdn2_decode_from(const gdn2_decode_desc* d, int flag_type, const void* q, const void* k,
+                     const void* v, const void* w, const void* b, const void* g,
+                     const float* a_log, const float* dt_bias, const void* reset, int parent_type,
+                     const void* parents, int n_states, const void* state_in, void* o,
+                     void* state_out, void* stream);
+
 /* Forward of one segment without a residual, like gdn2_fwd(d, ..., residual = NULL, ...), with
  * the workspace in a fixed 64 MiB (67108864-byte) device array inside the library instead of
  * a caller buffer.  No counterpart in the reference: it is for callers that cannot allocate
@@ -288,6 +298,63 @@ int gdn2_lm_swiglu(const float* gu, const float* d_act, float* out, int rows, in
  * rows <= 65535. */
 int gdn2_lm_columns(int split, float* const parts[], const int32_t widths[], int n, float* wide, int rows,
                     int ld, void* stream);
+
+/* One token of gdn2_lm_premix_fwd from the cached projections of the three tokens before it.  y (R, ldy)
+ * as there, any ldy >= 6*H*D + H and alignment; history (S, 3, 3*H*D): the projections of q, k and v
+ * side by side, the oldest token first (zeros before the first token); parents: NULL (row r continues
+ * history row r, S = R) or R row indices, int32 (GDN2_FLAG_INT32) or int64 (GDN2_FLAG_INT64), a row
+ * outside [0, S) having zero history.  out: q, k, v, w, b, g (R, H, D); og (R, H*D); new_history
+ * (R, 3, 3*H*D), not overlapping history. */
+typedef struct gdn2_lm_premix_step {
+  int32_t R, S, H, D;     /* D in {64, 128} */
+  int32_t ldy, parent_type;
+  float g_max;
+  const float *y, *history;
+  const void* parents;
+  const float *conv_w[3], *conv_b[3], *gate_b[2], *decay_b, *decay_a;
+  float *out[6], *og, *new_history;
+} gdn2_lm_premix_step;
+int gdn2_lm_premix_step_fwd(const gdn2_lm_premix_step* p, void* stream);
+
+/* ---- token generation ------------------------------------------------------------------------ */
+
+/* y = x W (+ bias) (+ residual), W[k][n] = scale (q - zero): x (M, K) rows of ldx elements, bias (N),
+ * residual (M, N) rows of ldr, y (M, N) contiguous, all of one dtype: 0 float32, 1 bfloat16, 2 float16.
+ * W in the layout of the kernels, K and N padded to Kp (a multiple of 128) and Np (of 16):
+ *   q     (Np / 16, Kp / 128, 64, 4) words; word j of lane l holds rows 32 j + 8 (l / 16) + e,
+ *         e = 0 .. 7, of column l % 16, element e < 4 in nibble 2 e, e >= 4 in nibble 2 e - 7;
+ *   meta  (Np / 16, Kp / group, 16) words, scale | zero << 16 as bfloat16 bits; 0 past K and N.
+ * group: 32, 64 or 128 rows of W share a scale and a zero.  q and meta 16-byte aligned.  Sums are
+ * float32 and products exact; y is rounded once.  A row of x with an infinity or NaN gives NaN. */
+enum { GDN2_F32 = 0, GDN2_BF16 = 1, GDN2_F16 = 2 };
+typedef struct gdn2_w4 {
+  int32_t M, K, N, group, dtype;
+  int64_t ldx, ldr;
+  const void *x, *q, *meta, *bias, *residual;
+  void* y;
+} gdn2_w4;
+int gdn2_w4_linear(const gdn2_w4* p, void* stream);
+
+/* The n best of the K V continuations of each of B groups of K beams, the best first, equal scores by
+ * the lower k V + v:  scores[b][k] + log_softmax(logits[b K + k])[v], float32.  logits (B*K, V) rows of
+ * ld elements; scores (B, K); NaN among either counts as -inf, and so does every continuation of a
+ * beam whose score or whose logits are all -inf.  finished NULL or B*K bytes: a beam with a nonzero one has a single
+ * continuation, the token eos at the beam's own score (0 <= eos < V).  eos -1: none.
+ * tokens, rows (B, n): v and b K + k; out_scores (B, n); out_finished NULL or (B, n) bytes: whether
+ * the beam was finished or v is eos.  1 <= n <= 128, n <= K V, K <= 128, K V < 2^31.
+ * workspace: gdn2_beam_workspace_bytes, 16-byte aligned. */
+typedef struct gdn2_beam {
+  int32_t B, K, V, n, eos, dtype;
+  int64_t ld;
+  const void* logits;
+  const float* scores;
+  const uint8_t* finished;
+  int64_t *tokens, *rows;
+  float* out_scores;
+  uint8_t* out_finished;
+} gdn2_beam;
+size_t gdn2_beam_workspace_bytes(int B, int K, int V, int n);
+int gdn2_beam_step(const gdn2_beam* p, void* workspace, void* stream);
 
 /* Diagnostics: C[M,N] = A[M,K] B[K,N] (row-major float32) through the kernels' MFMA tile
  * routine in the given dot mode.  M, N <= 64, K <= 128, all multiples of 16. */
