@@ -146,7 +146,8 @@ def lib():
 
 _BIND = None
 _BIND_ABI = ("gdn2_residual_layout", "gdn2_fwd_workspace_bytes", "gdn2_bwd_workspace_bytes", "gdn2_fwd", "gdn2_fwd_bf16",
-             "gdn2_bwd", "gdn2_decode_from", "gdn2_default_state_ckpt", "gdn2_last_error")
+             "gdn2_bwd", "gdn2_decode_from", "gdn2_default_state_ckpt", "gdn2_w4_linear", "gdn2_beam_workspace_bytes",
+             "gdn2_beam_step", "gdn2_lm_premix_step_fwd", "gdn2_last_error")
 
 
 def bind():

@@ -62,6 +62,12 @@ def beam_step(logits, scores, n: Optional[int] = None, finished=None, eos_id: Op
     lowest of the others follow, at -inf.  finished (B, K) bool, with eos_id: a finished beam has one
     continuation, eos_id at its own score; a beam that takes eos_id is finished.  Each group's
     result does not depend on the others, and equal inputs give equal bits."""
+    if isinstance(logits, torch.Tensor) and logits.is_cuda and (finished is None or eos_id is not None) \
+            and (eos_id is None or type(eos_id) is int and eos_id >= 0) and (n is None or type(n) is int):
+        # plain calls (csrc/bind.cpp) go native; None = not one, and what follows handles it
+        out = _lib.bind().beam(logits, scores, scores.shape[-1] if n is None else n, finished, -1 if eos_id is None else eos_id)
+        if out is not None:
+            return BeamStep(*out, None) if eos_id is None else BeamStep(*out)
     if scores.dim() != 2 or scores.numel() == 0:
         raise ValueError(f"scores must be (B, K), got {tuple(scores.shape)}")
     B, K = scores.shape
@@ -111,6 +117,10 @@ def premix_step(y, history, conv_w, conv_b, gate_b, decay_b, decay_a, n_heads: i
     the convolutions' taps and biases for q, k, v; gate_b two (C,): the erase and write gates' biases;
     decay_b, decay_a (H,).  parents (R,) int32 or int64: the history row that each row continues (one
     outside 0 .. S-1 has none: zeros); None: its own.  All float32 but parents."""
+    if isinstance(y, torch.Tensor) and y.is_cuda and type(n_heads) is int and type(g_max) is float:
+        out = _lib.bind().premix_step(y, history, (*conv_w, *conv_b, *gate_b, decay_b, decay_a), n_heads, g_max, parents)
+        if out is not None:
+            return PremixStep(*out)
     H = int(n_heads)
     if y.dim() != 2 or history.dim() != 3 or H < 1 or history.shape[1] != 3 or history.shape[2] % (3 * H) or history.shape[2] == 0:
         raise ValueError(f"y must be (R, columns) and history (S, 3, 3 H D), got {tuple(y.shape)} and {tuple(history.shape)}")

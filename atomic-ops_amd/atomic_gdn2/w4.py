@@ -154,6 +154,11 @@ def w4_linear(x, weight: W4Weight, bias=None, residual=None):
 
     bias (out,) and residual (..., out) are cast to x's dtype.  Rows may be strided (a slice of wider
     rows); sums are float32.  A row of x that holds an infinity or NaN gives NaN."""
+    if type(weight) is W4Weight and isinstance(x, torch.Tensor) and x.is_cuda:
+        # plain calls (csrc/bind.cpp) go native; None = not one, and what follows handles it
+        y = _lib.bind().w4(x, weight.q, weight.meta, weight.in_features, weight.out_features, weight.group_size, bias, residual)
+        if y is not None:
+            return y
     if not isinstance(weight, W4Weight):
         raise TypeError(f"weight must be a W4Weight (pack_w4, quantize_w4), got {type(weight).__name__}")
     if x.dtype not in _DTYPES:

@@ -7,7 +7,8 @@
 // dispatch modes, functorch wrappers or forward-mode tangents.  For anything else, and for whatever
 // the library refuses, they return None and the caller goes on in Python, which casts, validates
 // and raises.  MI355X, per pass: B1 H2 L256 gradient evaluation 209 -> 135 us, B1 H6 decode step
-// 23.0 -> 6.4 us, B8 H16 with raw inputs and reset flags 36.4 -> 7.7 us.
+// 23.0 -> 6.4 us, B8 H16 with raw inputs and reset flags 36.4 -> 7.7 us.  The steps of token generation
+// (w4, beam, premix_step) come the same way.
 //
 // Nothing is kept between calls but the configuration a caller passed to op().
 #include <ATen/ATen.h>
@@ -43,6 +44,10 @@ struct Abi {
   decltype(&gdn2_bwd) bwd;
   decltype(&gdn2_decode_from) decode;
   decltype(&gdn2_default_state_ckpt) default_ckpt;
+  decltype(&gdn2_w4_linear) w4;
+  decltype(&gdn2_beam_workspace_bytes) beam_ws;
+  decltype(&gdn2_beam_step) beam;
+  decltype(&gdn2_lm_premix_step_fwd) premix_step;
   decltype(&gdn2_last_error) last_error;
 } abi{};
 
@@ -394,6 +399,203 @@ PyObject* py_decode(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+bool tensors_of(PyObject* t) {
+  if (!PyTuple_Check(t)) return false;
+  for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(t); ++i)
+    if (!THPVariable_Check(PyTuple_GET_ITEM(t, i))) return false;
+  return true;
+}
+// A whole number of a call's arguments; false with no error set: not one.
+bool whole(PyObject* o, int64_t* x) {
+  if (!PyLong_CheckExact(o)) return false;
+  int over = 0;
+  *x = PyLong_AsLongLongAndOverflow(o, &over);
+  return !over;
+}
+// GDN2_F32, GDN2_BF16, GDN2_F16, or -1
+int float_kind(at::ScalarType t) { return t == at::kFloat ? 0 : t == at::kBFloat16 ? 1 : t == at::kHalf ? 2 : -1; }
+// The stride of t's rows of n elements, t (..., n): t is contiguous or a matrix with whole rows; else 0.
+int64_t row_stride(const Tensor& t, int64_t n) {
+  if (t.is_contiguous()) return n;
+  return t.dim() == 2 && t.stride(1) == 1 && (t.stride(0) >= n || t.size(0) == 1) ? std::max(t.stride(0), n) : 0;
+}
+PyObject* tuple_of(std::initializer_list<const Tensor*> ts) {
+  PyObject* out = PyTuple_New((Py_ssize_t)ts.size());
+  Py_ssize_t i = 0;
+  for (const Tensor* t : ts) {
+    PyObject* x = out ? THPVariable_Wrap(*t) : nullptr;
+    if (!x) {
+      Py_XDECREF(out);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(out, i++, x);
+  }
+  return out;
+}
+
+// w4(x, q, meta, in, out, group, bias or None, residual or None) -> y, or None: not a plain call
+PyObject* py_w4(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 8) return PyErr_Format(PyExc_TypeError, "w4 takes 8 arguments");
+  int64_t K, N, group;
+  if (!THPVariable_Check(args[0]) || !THPVariable_Check(args[1]) || !THPVariable_Check(args[2]) || !whole(args[3], &K) ||
+      !whole(args[4], &N) || !whole(args[5], &group))
+    return none();
+  Tensor x = THPVariable_Unpack(args[0]), q = THPVariable_Unpack(args[1]), meta = THPVariable_Unpack(args[2]), bias, res;
+  for (int i : {6, 7}) {
+    if (args[i] == Py_None) continue;
+    if (!THPVariable_Check(args[i])) return none();
+    (i == 6 ? bias : res) = THPVariable_Unpack(args[i]);
+  }
+  if (!plain_mode() || !x.is_cuda() || x.dim() < 1 || x.numel() == 0 || x.size(-1) != K) return none();
+  const c10::Device dev = x.device();
+  const at::ScalarType dt = x.scalar_type();
+  const int kind = float_kind(dt);
+  const int64_t M = x.numel() / K, ldx = row_stride(x, K);
+  if (kind < 0 || !ldx || !plain(x, dev) || M > INT32_MAX || K > INT32_MAX || N > INT32_MAX) return none();
+  for (const Tensor* t : {&q, &meta})
+    if (!plain(*t, dev) || t->scalar_type() != at::kInt || !t->is_contiguous()) return none();
+  if (bias.defined() && (!plain(bias, dev) || bias.scalar_type() != dt || bias.dim() != 1 || bias.size(0) != N || !bias.is_contiguous()))
+    return none();
+  int64_t ldr = 0;
+  if (res.defined()) {
+    if (!plain(res, dev) || res.scalar_type() != dt || res.dim() != x.dim() || res.size(-1) != N) return none();
+    for (int64_t i = 0; i + 1 < x.dim(); ++i)
+      if (res.size(i) != x.size(i)) return none();
+    if (!(ldr = row_stride(res, N))) return none();
+  }
+  gdn2_w4 a{};
+  a.M = (int32_t)M; a.K = (int32_t)K; a.N = (int32_t)N; a.group = (int32_t)group;
+  a.dtype = kind; a.ldx = ldx; a.ldr = ldr;
+  a.x = x.data_ptr(); a.q = q.data_ptr(); a.meta = meta.data_ptr();
+  a.bias = bias.defined() ? bias.data_ptr() : nullptr;
+  a.residual = res.defined() ? res.data_ptr() : nullptr;
+  Tensor y;
+  int status = 0;
+  unlocked([&] {
+    c10::DeviceGuard guard(dev);
+    at::DimVector size(x.sizes());
+    size.back() = N;
+    y = empty_on(x, size, dt);
+    a.y = y.data_ptr();
+    status = abi.w4(&a, stream_of(dev));
+  });
+  return status ? none() : THPVariable_Wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
+// beam(logits, scores, n, finished or None, eos or -1) -> (tokens, rows, scores[, finished]), or None:
+// not a plain call
+PyObject* py_beam(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  if (n_args != 5) return PyErr_Format(PyExc_TypeError, "beam takes 5 arguments");
+  int64_t n, eos;
+  if (!THPVariable_Check(args[0]) || !THPVariable_Check(args[1]) || !whole(args[2], &n) || !whole(args[4], &eos) ||
+      (args[3] != Py_None && !THPVariable_Check(args[3])))
+    return none();
+  const Tensor x = THPVariable_Unpack(args[0]), scores = THPVariable_Unpack(args[1]);
+  Tensor fin;
+  if (args[3] != Py_None) fin = THPVariable_Unpack(args[3]);
+  if (!plain_mode() || !x.is_cuda() || scores.dim() != 2 || scores.numel() == 0 || x.dim() < 2 || x.dim() > 3 || x.numel() == 0)
+    return none();
+  const c10::Device dev = x.device();
+  const int64_t B = scores.size(0), K = scores.size(1), V = x.size(-1), ld = row_stride(x, V);
+  const int kind = float_kind(x.scalar_type());
+  if (kind < 0 || !ld || !plain(x, dev) || !plain(scores, dev) || scores.scalar_type() != at::kFloat || !scores.is_contiguous())
+    return none();
+  if (x.dim() == 2 ? x.size(0) != B * K : x.size(0) != B || x.size(1) != K) return none();
+  if (fin.defined() && (!plain(fin, dev) || fin.scalar_type() != at::kBool || fin.dim() != 2 || fin.size(0) != B || fin.size(1) != K ||
+                        !fin.is_contiguous()))
+    return none();
+  if (B > 65535 || K > 65535 || V > INT32_MAX || n < 1 || n > INT32_MAX || eos < -1 || eos > INT32_MAX) return none();
+  gdn2_beam a{};
+  a.B = (int32_t)B; a.K = (int32_t)K; a.V = (int32_t)V; a.n = (int32_t)n; a.eos = (int32_t)eos;
+  a.dtype = kind; a.ld = ld;
+  a.logits = x.data_ptr(); a.scores = f32_at(scores);
+  a.finished = fin.defined() ? static_cast<const uint8_t*>(fin.data_ptr()) : nullptr;
+  Tensor tokens, rows, out, done;
+  int status = 0;
+  unlocked([&] {
+    c10::DeviceGuard guard(dev);
+    const size_t bytes = abi.beam_ws(a.B, a.K, a.V, a.n);
+    if (!bytes) {
+      status = 1;
+      return;
+    }
+    tokens = empty_on(x, {B, n}, at::kLong);
+    rows = empty_on(x, {B, n}, at::kLong);
+    out = empty_on(x, {B, n}, at::kFloat);
+    if (eos >= 0) done = empty_on(x, {B, n}, at::kBool);
+    const Tensor ws = empty_on(x, {(int64_t)bytes}, at::kByte);
+    a.tokens = static_cast<int64_t*>(tokens.data_ptr());
+    a.rows = static_cast<int64_t*>(rows.data_ptr());
+    a.out_scores = f32_at(out);
+    a.out_finished = done.defined() ? static_cast<uint8_t*>(done.data_ptr()) : nullptr;
+    status = abi.beam(&a, ws.data_ptr(), stream_of(dev));
+  });
+  if (status) return none();
+  return done.defined() ? tuple_of({&tokens, &rows, &out, &done}) : tuple_of({&tokens, &rows, &out});
+  END_HANDLE_TH_ERRORS
+}
+
+// premix_step(y, history, (taps of q, k, v, their biases, the gates' biases, decay_b, decay_a), heads, g_max,
+// parents or None) -> (q, k, v, w, b, g, gate, history), or None: not a plain call
+PyObject* py_premix_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6) return PyErr_Format(PyExc_TypeError, "premix_step takes 6 arguments");
+  int64_t H;
+  if (!THPVariable_Check(args[0]) || !THPVariable_Check(args[1]) || !tensors_of(args[2]) || PyTuple_GET_SIZE(args[2]) != 10 ||
+      !whole(args[3], &H) || !PyFloat_Check(args[4]) || (args[5] != Py_None && !THPVariable_Check(args[5])))
+    return none();
+  const Tensor y = THPVariable_Unpack(args[0]), past = THPVariable_Unpack(args[1]);
+  Tensor parents;
+  if (args[5] != Py_None) parents = THPVariable_Unpack(args[5]);
+  if (!plain_mode() || !y.is_cuda() || y.dim() != 2 || past.dim() != 3 || y.numel() == 0 || past.numel() == 0 || H < 1 ||
+      past.size(1) != 3 || past.size(2) % (3 * H))
+    return none();
+  const c10::Device dev = y.device();
+  const int64_t R = y.size(0), S = past.size(0), C = past.size(2) / 3, D = C / H, ldy = row_stride(y, y.size(1));
+  auto ready = [&](const Tensor& t) { return plain(t, dev) && t.scalar_type() == at::kFloat; };
+  if ((D != 64 && D != 128) || !ldy || ldy > INT32_MAX || y.size(1) < 6 * C + H || R * H > (int64_t(1) << 28) || S > INT32_MAX ||
+      !ready(y) || !ready(past) || !past.is_contiguous())
+    return none();
+  gdn2_lm_premix_step a{};
+  if (parents.defined() ? !row_indices(parents, dev, R, &a.parent_type) : S != R) return none();
+  const float* ps[10];
+  for (int i = 0; i < 10; ++i) {
+    const Tensor& t = THPVariable_Unpack(PyTuple_GET_ITEM(args[2], i));
+    const int64_t len = i < 8 ? C : H;
+    if (!ready(t) || !t.is_contiguous() || t.numel() != (i < 3 ? 4 * C : len) || t.size(0) != len || t.dim() != (i < 3 ? 2 : 1))
+      return none();
+    ps[i] = f32_at(t);
+  }
+  a.R = (int32_t)R; a.S = (int32_t)S; a.H = (int32_t)H; a.D = (int32_t)D; a.ldy = (int32_t)ldy;
+  a.g_max = (float)PyFloat_AS_DOUBLE(args[4]);
+  a.y = f32_at(y); a.history = f32_at(past);
+  a.parents = parents.defined() ? parents.data_ptr() : nullptr;
+  for (int i = 0; i < 3; ++i) {
+    a.conv_w[i] = ps[i];
+    a.conv_b[i] = ps[3 + i];
+  }
+  a.gate_b[0] = ps[6]; a.gate_b[1] = ps[7]; a.decay_b = ps[8]; a.decay_a = ps[9];
+  Tensor out[6], gate, now;
+  int status = 0;
+  unlocked([&] {
+    c10::DeviceGuard guard(dev);
+    for (int i = 0; i < 6; ++i) {
+      out[i] = empty_on(y, {R, H, D}, at::kFloat);
+      a.out[i] = f32_at(out[i]);
+    }
+    gate = empty_on(y, {R, C}, at::kFloat);
+    now = empty_on(y, {R, 3, 3 * C}, at::kFloat);
+    a.og = f32_at(gate);
+    a.new_history = f32_at(now);
+    status = abi.premix_step(&a, stream_of(dev));
+  });
+  return status ? none() : tuple_of({&out[0], &out[1], &out[2], &out[3], &out[4], &out[5], &gate, &now});
+  END_HANDLE_TH_ERRORS
+}
+
 // What a saved tensor looked like (lm_kernels.py): forty of them a block, looked over in Python at 1.5 us
 // each, would be a fifth of a small block's host time.
 struct Form {
@@ -403,12 +605,6 @@ struct Form {
 };
 const char* const kFormsName = "atomic_gdn2._bind.forms";
 void free_forms(PyObject* cap) { delete static_cast<std::vector<Form>*>(PyCapsule_GetPointer(cap, kFormsName)); }
-bool tensors_of(PyObject* t) {
-  if (!PyTuple_Check(t)) return false;
-  for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(t); ++i)
-    if (!THPVariable_Check(PyTuple_GET_ITEM(t, i))) return false;
-  return true;
-}
 
 // forms(tensors): their sizes, dtypes and devices
 PyObject* py_forms(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -488,6 +684,9 @@ PyMethodDef methods[] = {
     {"differ", (PyCFunction)(void (*)())py_differ, METH_FASTCALL, "differ(forms, tensors)"},
     {"dense", (PyCFunction)(void (*)())py_dense, METH_FASTCALL, "dense(tensors, x)"},
     {"decode", (PyCFunction)(void (*)())py_decode, METH_FASTCALL, "decode(...)"},
+    {"w4", (PyCFunction)(void (*)())py_w4, METH_FASTCALL, "w4(x, q, meta, in, out, group, bias, residual)"},
+    {"beam", (PyCFunction)(void (*)())py_beam, METH_FASTCALL, "beam(logits, scores, n, finished, eos)"},
+    {"premix_step", (PyCFunction)(void (*)())py_premix_step, METH_FASTCALL, "premix_step(y, history, weights, heads, g_max, parents)"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module{PyModuleDef_HEAD_INIT, "_bind", "native call path of the operator", -1, methods};
 
