@@ -105,7 +105,9 @@ def lib():
         L.gdn2_decode_flags.argtypes = [P(Gdn2DecodeDesc), _c_int] + [_vp] * 13
         L.gdn2_decode_from.argtypes = [P(Gdn2DecodeDesc), _c_int] + [_vp] * 9 + [_c_int, _vp, _c_int] + [_vp] * 4
         L.gdn2_lm_premix_step_fwd.argtypes = [_vp, _vp]
-        L.gdn2_w4_linear.argtypes = [P(Gdn2W4), _vp]
+        L.gdn2_w4_workspace_bytes.argtypes = [P(Gdn2W4)]
+        L.gdn2_w4_workspace_bytes.restype = _c_size
+        L.gdn2_w4_linear.argtypes = [P(Gdn2W4), _vp, _vp]
         L.gdn2_beam_workspace_bytes.argtypes = [_c_int] * 4
         L.gdn2_beam_workspace_bytes.restype = _c_size
         L.gdn2_beam_step.argtypes = [P(Gdn2Beam), _vp, _vp]
@@ -146,7 +148,7 @@ def lib():
 
 _BIND = None
 _BIND_ABI = ("gdn2_residual_layout", "gdn2_fwd_workspace_bytes", "gdn2_bwd_workspace_bytes", "gdn2_fwd", "gdn2_fwd_bf16",
-             "gdn2_bwd", "gdn2_decode_from", "gdn2_default_state_ckpt", "gdn2_w4_linear", "gdn2_beam_workspace_bytes",
+             "gdn2_bwd", "gdn2_decode_from", "gdn2_default_state_ckpt", "gdn2_w4_workspace_bytes", "gdn2_w4_linear", "gdn2_beam_workspace_bytes",
              "gdn2_beam_step", "gdn2_lm_premix_step_fwd", "gdn2_last_error")
 
 

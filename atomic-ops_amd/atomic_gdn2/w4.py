@@ -187,6 +187,7 @@ def w4_linear(x, weight: W4Weight, bias=None, residual=None):
                     0 if residual is None else N if M == 1 else residual.stride(0), x.data_ptr(), weight.q.data_ptr(),
                     weight.meta.data_ptr(), None if bias is None else bias.data_ptr(),
                     None if residual is None else residual.data_ptr(), y.data_ptr())
+    ws = torch.empty(_lib.lib().gdn2_w4_workspace_bytes(ctypes.byref(a)), dtype=torch.uint8, device=dev)
     with torch.cuda.device(dev):
-        _lib.check(_lib.lib().gdn2_w4_linear(ctypes.byref(a), _lib.stream_handle(dev)), "gdn2_w4_linear")
+        _lib.check(_lib.lib().gdn2_w4_linear(ctypes.byref(a), _lib.ptr(ws), _lib.stream_handle(dev)), "gdn2_w4_linear")
     return y

@@ -44,6 +44,7 @@ struct Abi {
   decltype(&gdn2_bwd) bwd;
   decltype(&gdn2_decode_from) decode;
   decltype(&gdn2_default_state_ckpt) default_ckpt;
+  decltype(&gdn2_w4_workspace_bytes) w4_ws;
   decltype(&gdn2_w4_linear) w4;
   decltype(&gdn2_beam_workspace_bytes) beam_ws;
   decltype(&gdn2_beam_step) beam;
@@ -478,7 +479,9 @@ PyObject* py_w4(PyObject*, PyObject* const* args, Py_ssize_t n) {
     size.back() = N;
     y = empty_on(x, size, dt);
     a.y = y.data_ptr();
-    status = abi.w4(&a, stream_of(dev));
+    const int64_t bytes = (int64_t)abi.w4_ws(&a);
+    const Tensor ws = bytes ? empty_on(x, {bytes}, at::kByte) : Tensor();
+    status = abi.w4(&a, bytes ? ws.data_ptr() : nullptr, stream_of(dev));
   });
   return status ? none() : THPVariable_Wrap(y);
   END_HANDLE_TH_ERRORS

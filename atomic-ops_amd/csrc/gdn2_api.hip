@@ -817,12 +817,14 @@ int gdn2_lm_premix_step_fwd(const gdn2_lm_premix_step* p, void* stream) {
 
 static_assert(GDN2_F32 == gdn2::W4_F32 && GDN2_BF16 == gdn2::W4_BF16 && GDN2_F16 == gdn2::W4_F16, "header constants");
 
-int gdn2_w4_linear(const gdn2_w4* p, void* stream) {
+namespace {
+// the product's arguments, checked, without its workspace
+int w4_args(const gdn2_w4* p, gdn2::W4Args* a) {
   if (!p) return fail(GDN2_ERR_INVALID, "null argument block");
   if (p->M < 1 || p->K < 1 || p->N < 1) return fail(GDN2_ERR_INVALID, "non-positive shape");
-  if (p->group != 32 && p->group != 64 && p->group != 128) return fail(GDN2_ERR_UNSUPPORTED, "groups of 32, 64 or 128 rows");
   if (p->dtype < GDN2_F32 || p->dtype > GDN2_F16) return fail(GDN2_ERR_INVALID, "unknown dtype");
   if (p->M > (1 << 20) || p->K > (1 << 24) || p->N > (1 << 24)) return fail(GDN2_ERR_UNSUPPORTED, "shape too large");
+  if (p->group != 32 && p->group != 64 && p->group != 128) return fail(GDN2_ERR_UNSUPPORTED, "groups of 32, 64 or 128 rows");
   if (p->ldx < p->K || (p->residual && p->ldr < p->N)) return fail(GDN2_ERR_INVALID, "row stride below the row");
   if (!p->x || !p->q || !p->meta || !p->y || !aligned16({p->q, p->meta}))
     return fail(GDN2_ERR_INVALID, "null pointer, or weights not 16-byte aligned");
@@ -830,14 +832,31 @@ int gdn2_w4_linear(const gdn2_w4* p, void* stream) {
   if ((reinterpret_cast<uintptr_t>(p->x) | reinterpret_cast<uintptr_t>(p->y) | reinterpret_cast<uintptr_t>(p->bias) |
        reinterpret_cast<uintptr_t>(p->residual)) & (e - 1))
     return fail(GDN2_ERR_INVALID, "pointer not aligned to its elements");
+  a->x = p->x; a->q = static_cast<const uint32_t*>(p->q); a->meta = static_cast<const uint32_t*>(p->meta);
+  a->bias = p->bias; a->res = p->residual; a->y = p->y;
+  a->M = p->M; a->K = p->K; a->N = p->N;
+  a->nkb = (p->K + gdn2::W4_KB - 1) / gdn2::W4_KB;
+  a->nnb = (p->N + 15) / 16;
+  a->ldx = (size_t)p->ldx; a->ldr = (size_t)p->ldr;
+  // (the last bound: a tile's rows within the 2^30 bytes of a buffer)
+  a->vec = aligned16({p->x}) && p->K % 8 == 0 && p->ldx % (16 / e) == 0 && p->ldx <= (int64_t(1) << 20);
+  a->wide = aligned16({p->y, p->bias, p->residual}) && p->N % 4 == 0 && p->ldr % 4 == 0;
+  return GDN2_OK;
+}
+}  // namespace
+
+size_t gdn2_w4_workspace_bytes(const gdn2_w4* p) {
   gdn2::W4Args a{};
-  a.x = p->x; a.q = static_cast<const uint32_t*>(p->q); a.meta = static_cast<const uint32_t*>(p->meta);
-  a.bias = p->bias; a.res = p->residual; a.y = p->y;
-  a.M = p->M; a.K = p->K; a.N = p->N;
-  a.nkb = (p->K + gdn2::W4_KB - 1) / gdn2::W4_KB;
-  a.nnb = (p->N + 15) / 16;
-  a.ldx = (size_t)p->ldx; a.ldr = (size_t)p->ldr;
-  a.vec = aligned16({p->x}) && p->K % 8 == 0 && p->ldx % (16 / e) == 0;
+  return w4_args(p, &a) ? 0 : gdn2::w4_workspace_bytes(p->dtype, a);
+}
+
+int gdn2_w4_linear(const gdn2_w4* p, void* workspace, void* stream) {
+  gdn2::W4Args a{};
+  const int st = w4_args(p, &a);
+  if (st) return st;
+  if (!aligned16({workspace}) || (!workspace && gdn2::w4_workspace_bytes(p->dtype, a)))
+    return fail(GDN2_ERR_INVALID, "null workspace, or not 16-byte aligned");
+  a.part = static_cast<float*>(workspace);
   return lm_done(gdn2::launch_w4(p->dtype, p->group, a, reinterpret_cast<hipStream_t>(stream)), "w4 launch");
 }
 

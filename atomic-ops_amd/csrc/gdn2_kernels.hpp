@@ -406,10 +406,13 @@ struct W4Args {
   const uint32_t *q, *meta;
   const void *bias, *res;
   void* y;
+  float* part;                 // w4_workspace_bytes
   int M, K, N, nkb, nnb;
   size_t ldx, ldr;
   int vec;                     // whole 16-byte accesses of x: alignment, ldx and K allow them
+  int wide;                    // four columns at a time of y, bias and res
 };
+size_t w4_workspace_bytes(int dtype, const W4Args& a);
 hipError_t launch_w4(int dtype, int group, const W4Args& a, hipStream_t s);
 
 // Beam search's selection (gdn2_beam.hip).  logits (B K, V) rows of ld elements; part: per row and split

@@ -64,45 +64,72 @@ __device__ __forceinline__ void w4_split(const float* x, W4Frag<W4_F32>& f) {
   f.p[2] = __builtin_bit_cast(s8, make_uint4(h[0], h[1], h[2], h[3]));
 }
 
-// x[m][k .. k+7], zero outside M and K
+// Eight activations as loaded: 16 or (float32) 32 bytes
 template <int XT>
-__device__ __forceinline__ W4Frag<XT> w4_load_x(const W4Args& a, int m, int k) {
+struct W4Raw {
+  static constexpr int NV = XT == W4_F32 ? 2 : 1;
+  uint4 v[NV];
+};
+template <int XT>
+__device__ __forceinline__ W4Frag<XT> w4_frag(const W4Raw<XT>& x) {
   W4Frag<XT> f;
   if constexpr (XT == W4_F32) {
+    const uint32_t u[8] = {x.v[0].x, x.v[0].y, x.v[0].z, x.v[0].w, x.v[1].x, x.v[1].y, x.v[1].z, x.v[1].w};
     float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = 0.f;
-    if (m < a.M) {
-      const float* p = static_cast<const float*>(a.x) + (size_t)m * a.ldx + k;
-      if (a.vec) {
-        if (k < a.K) {
-          const float4 u = *reinterpret_cast<const float4*>(p), w = *reinterpret_cast<const float4*>(p + 4);
-          v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
-          v[4] = w.x; v[5] = w.y; v[6] = w.z; v[7] = w.w;
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (k + e < a.K) v[e] = p[e];
-      }
-    }
+    for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(u[e]);
     w4_split(v, f);
   } else {
-    uint4 u = make_uint4(0u, 0u, 0u, 0u);
-    if (m < a.M) {
-      const uint16_t* p = static_cast<const uint16_t*>(a.x) + (size_t)m * a.ldx + k;
-      if (a.vec) {
-        if (k < a.K) u = *reinterpret_cast<const uint4*>(p);
-      } else {
-        uint32_t v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = k + e < a.K ? p[e] : 0u;
-        u = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
-      }
-    }
-    f.p[0] = __builtin_bit_cast(s8, u);
+    f.p[0] = __builtin_bit_cast(s8, x.v[0]);
   }
   return f;
+}
+// Their sum
+typedef _Float16 h2v __attribute__((ext_vector_type(2)));
+template <int XT>
+__device__ __forceinline__ float w4_sum8(const W4Raw<XT>& x) {
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < W4Raw<XT>::NV; ++i) {
+    const uint32_t u[4] = {x.v[i].x, x.v[i].y, x.v[i].z, x.v[i].w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (XT == W4_F32) s += __uint_as_float(u[e]);
+      else if constexpr (XT == W4_BF16)
+        s = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2v, u[e]), __builtin_bit_cast(b2v, 0x3f803f80u), s, false);
+      else s = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2v, u[e]), __builtin_bit_cast(h2v, 0x3c003c00u), s, false);
+    }
+  }
+  return s;
+}
+// x[m][k .. k+7] element by element, zero outside M and K: rows that 16-byte accesses cannot take
+template <int XT>
+__device__ __forceinline__ W4Raw<XT> w4_load_odd(const W4Args& a, int m, int k) {
+  W4Raw<XT> r;
+  if constexpr (XT == W4_F32) {
+    const float* p = static_cast<const float*>(a.x) + (size_t)min(m, a.M - 1) * a.ldx + k;
+    uint32_t v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = m < a.M && k + e < a.K ? __float_as_uint(p[e]) : 0u;
+    r.v[0] = make_uint4(v[0], v[1], v[2], v[3]);
+    r.v[1] = make_uint4(v[4], v[5], v[6], v[7]);
+  } else {
+    const uint16_t* p = static_cast<const uint16_t*>(a.x) + (size_t)min(m, a.M - 1) * a.ldx + k;
+    uint32_t v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = m < a.M && k + e < a.K ? p[e] : 0u;
+    r.v[0] = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+  }
+  return r;
+}
+// ... and by buffer loads from base + off: an offset past the buffer's end reads zero, without a branch
+constexpr uint32_t W4_OUT = 0x60000000u;             // above any offset of a buffer (at most 2^30)
+typedef unsigned u4v __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t w4_buffer(const void* p, size_t at, int64_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(p)) + at, 0, (int)bytes, 0x00027000);
+}
+__device__ __forceinline__ uint4 w4_buffer16(__amdgpu_buffer_rsrc_t b, uint32_t off, int uniform) {
+  return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(b, (int)off, uniform, 0));
 }
 
 template <int XT>
@@ -120,117 +147,529 @@ __device__ __forceinline__ void w4_st(void* p, size_t i, float v) {
 
 __device__ __forceinline__ void w4_hold(f4& a) { asm volatile("" : "+v"(a)); }
 
-// A workgroup takes 16 NB columns and 16 MT rows; its waves take the 128-deep blocks of the sum in
-// turn and add their parts through LDS in wave order.
-template <int XT, int GROUP, int MT, int NB>
-__global__ __launch_bounds__(512) void w4_rows_kernel(W4Args a) {
+template <int N>
+__device__ __forceinline__ s8 w4_down(const s8& x) {         // lane i of a row of 16 takes lane i + N's
+  if constexpr (N == 0) return x;
+  uint4 u = __builtin_bit_cast(uint4, x);
+  auto f = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x100 | N, 0xf, 0xf, true); };
+  return __builtin_bit_cast(s8, make_uint4(f(u.x), f(u.y), f(u.z), f(u.w)));
+}
+template <int XT, int N>
+__device__ __forceinline__ W4Frag<XT> w4_frag_down(const W4Frag<XT>& x) {
+  W4Frag<XT> y;
+#pragma unroll
+  for (int p = 0; p < W4Frag<XT>::NP; ++p) y.p[p] = w4_down<N>(x.p[p]);
+  return y;
+}
+
+// Four results of a row: plus bias and residual, rounded, stored; whole where a.wide allows it
+template <int XT>
+__device__ __forceinline__ float4 w4_ld4(const void* p, size_t i) {
+  if constexpr (XT == W4_F32) return *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+  const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
+  if constexpr (XT == W4_BF16)
+    return make_float4(bf16_val(u.x & 0xffffu), __uint_as_float(u.x & 0xffff0000u), bf16_val(u.y & 0xffffu), __uint_as_float(u.y & 0xffff0000u));
+  const h2v a = __builtin_bit_cast(h2v, u.x), b = __builtin_bit_cast(h2v, u.y);
+  return make_float4((float)a[0], (float)a[1], (float)b[0], (float)b[1]);
+}
+template <int XT>
+__device__ __forceinline__ void w4_out4(const W4Args& a, int m, int n, float4 v) {
+  const size_t at = (size_t)m * a.N + n;
+  if (a.wide) {
+    if (a.bias) v = add4(v, w4_ld4<XT>(a.bias, n));
+    if (a.res) v = add4(v, w4_ld4<XT>(a.res, (size_t)m * a.ldr + n));
+    if constexpr (XT == W4_F32) *reinterpret_cast<float4*>(static_cast<float*>(a.y) + at) = v;
+    else {
+      uint2 u;
+      if constexpr (XT == W4_BF16) u = make_uint2(bf16_pack(v.x, v.y), bf16_pack(v.z, v.w));
+      else u = make_uint2(__builtin_bit_cast(uint32_t, h2v{(_Float16)v.x, (_Float16)v.y}), __builtin_bit_cast(uint32_t, h2v{(_Float16)v.z, (_Float16)v.w}));
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.y) + at) = u;
+    }
+    return;
+  }
+  const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (n + e >= a.N) return;
+    float y = f[e];
+    if (a.bias) y += w4_ld<XT>(a.bias, n + e);
+    if (a.res) y += w4_ld<XT>(a.res, (size_t)m * a.ldr + n + e);
+    w4_st<XT>(a.y, at + e, y);
+  }
+}
+__device__ __forceinline__ void w4_part4(const W4Args& a, size_t at, int n, const float4& v) {
+  if (a.N % 4 == 0) {
+    *reinterpret_cast<float4*>(a.part + at) = v;
+    return;
+  }
+  const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (n + e < a.N) a.part[at + e] = f[e];
+}
+
+template <int CTRL>
+__device__ __forceinline__ float w4_dpp(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float w4_quad_sum(float x) {      // over the four lanes of a quad
+  x += w4_dpp<0xb1>(x);
+  return x + w4_dpp<0x4e>(x);
+}
+
+// Waves of a workgroup at most
+constexpr int w4_waves(int XT, int NB) { return XT != W4_F32 && NB == 1 ? 16 : 8; }
+
+// Few rows: bound by the bytes of the weights.  A workgroup takes 16 NB columns and 16 / SP rows; its waves take the 128-deep blocks of the sum in turn, the next one's
+// loads issued before the products of this one, and add their parts through LDS in wave order.
+//   x is the products' left operand, so a lane's results are rows 4 (l / 16) + e of one column and it
+// needs one scale.  With few rows an operand's 16 rows hold SP steps' pieces of each: row m's at rows
+// SP m, SP m + 1, ...: one load then serves SP steps, the later ones after a move by lanes (whose other
+// rows' products are not looked at), and only 4 / SP of a lane's four results are used.
+template <int XT, int GROUP, int SP, int NB>
+__global__ __launch_bounds__(w4_waves(XT, NB) * WAVE) void w4_rows_kernel(W4Args a) {
   constexpr bool F16 = XT == W4_F16;
-  constexpr int NP = W4Frag<XT>::NP, NG = W4_KB / GROUP, SG = GROUP / 32;
-  extern __shared__ f4 red[];                        // [wave][nb][mt][lane]
+  constexpr int NP = W4Frag<XT>::NP, NG = W4_KB / GROUP, SG = GROUP / 32, E = XT == W4_F32 ? 4 : 2;
+  constexpr int XL = 4 / SP, NE = 4 / SP, MR = 16 / SP;       // loads of x a block, results a lane, rows a tile
+  extern __shared__ float red[];                     // [wave][nb][e][lane]
   const int l = lane_id(), r = l & 15, c = l >> 4, w = wave_id(), W = blockDim.x / WAVE;
-  const int nb0 = blockIdx.x * NB, m0 = blockIdx.y * 16 * MT;
+  const int nb0 = blockIdx.x * NB, m0 = blockIdx.y * MR;
   const s8 ones = __builtin_bit_cast(s8, F16 ? make_uint4(0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u)
                                              : make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u));
-  f4 tot[NB][MT];
+  // a lane's offsets are fixed and a block's are uniform, so that a load takes no address arithmetic
+  const int rows = min(MR, a.M - m0), nbs = min(NB, a.nnb - nb0);
+  const __amdgpu_buffer_rsrc_t xb =
+      w4_buffer(a.x, (size_t)m0 * a.ldx * E, a.vec ? ((rows - 1) * (int64_t)a.ldx + a.K) * E : 0);
+  const __amdgpu_buffer_rsrc_t qb = w4_buffer(a.q, (size_t)nb0 * a.nkb * 1024, (int64_t)nbs * a.nkb * 1024);
+  const __amdgpu_buffer_rsrc_t sb = w4_buffer(a.meta, (size_t)nb0 * a.nkb * (NG * 64), (int64_t)nbs * a.nkb * (NG * 64));
+  const int xk = 32 * (r % SP) + 8 * c;              // the lane's first k of a load
+  const uint32_t xoff = r / SP < rows ? (uint32_t)(r / SP * a.ldx + xk) * E : W4_OUT;
+  uint32_t qoff[NB], soff[NB];
+#pragma unroll
+  for (int i = 0; i < NB; ++i) {                     // (columns past the last: zero codes and scales)
+    qoff[i] = (uint32_t)i * a.nkb * 1024 + 16 * l;
+    soff[i] = (uint32_t)i * a.nkb * (NG * 64) + 4 * r;
+  }
+  float tot[NB][NE];
 #pragma unroll
   for (int i = 0; i < NB; ++i)
 #pragma unroll
-    for (int j = 0; j < MT; ++j) tot[i][j] = f4{0.f, 0.f, 0.f, 0.f};
-  for (int kb = w; kb < a.nkb; kb += W) {
-    uint4 q[NB], mt[NB][NG];
+    for (int e = 0; e < NE; ++e) tot[i][e] = 0.f;
+  struct Block {
+    uint4 q[NB];
+    uint32_t sz[NB][NG];
+    W4Raw<XT> x[XL];
+  };
+  auto load = [&](Block& o, int kb) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
-      const size_t nb = min(nb0 + i, a.nnb - 1);
-      q[i] = reinterpret_cast<const uint4*>(a.q)[(nb * a.nkb + kb) * WAVE + l];
+      o.q[i] = w4_buffer16(qb, qoff[i], kb * 1024);
 #pragma unroll
       for (int g = 0; g < NG; ++g)
-        mt[i][g] = reinterpret_cast<const uint4*>(a.meta)[((nb * a.nkb + kb) * NG + g) * 4 + c];
+        o.sz[i][g] = __builtin_amdgcn_raw_buffer_load_b32(sb, (int)(soff[i] + 64 * g), kb * (NG * 64), 0);
     }
+    if (!a.vec) {
+#pragma unroll
+      for (int u = 0; u < XL; ++u)
+          o.x[u] = w4_load_odd<XT>(a, r / SP < rows ? m0 + r / SP : a.M, kb * W4_KB + 32 * SP * u + xk);
+    } else if ((kb + 1) * W4_KB <= a.K) {
+#pragma unroll
+      for (int u = 0; u < XL; ++u)
+#pragma unroll
+          for (int v = 0; v < W4Raw<XT>::NV; ++v)
+            o.x[u].v[v] = w4_buffer16(xb, xoff + 32 * SP * u * E + 16 * v, kb * (W4_KB * E));
+    } else {
+#pragma unroll
+      for (int u = 0; u < XL; ++u) {
+        const uint32_t out = kb * W4_KB + 32 * SP * u + xk < a.K ? 0u : W4_OUT;
+#pragma unroll
+        for (int v = 0; v < W4Raw<XT>::NV; ++v)
+          o.x[u].v[v] = w4_buffer16(xb, (xoff + 32 * SP * u * E + 16 * v) | out, kb * (W4_KB * E));
+      }
+    }
+  };
+  auto add = [&](const Block& o) __attribute__((always_inline)) {
+    W4Frag<XT> x[XL];
+#pragma unroll
+    for (int u = 0; u < XL; ++u) x[u] = w4_frag<XT>(o.x[u]);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      f4 acc[NB][MT], xs[MT];
+      f4 acc[NB], xs;
 #pragma unroll
       for (int s = 0; s < SG; ++s) {
         const int j = g * SG + s;
-        W4Frag<XT> x[MT];
+        const W4Frag<XT>& f = x[j / SP];
+        const W4Frag<XT> xj = j % SP == 0   ? f
+                              : j % SP == 1 ? w4_frag_down<XT, 1>(f)
+                              : j % SP == 2 ? w4_frag_down<XT, 2>(f)
+                                            : w4_frag_down<XT, 3>(f);
+        s8 op[NB];
 #pragma unroll
-        for (int t = 0; t < MT; ++t) x[t] = w4_load_x<XT>(a, m0 + 16 * t + r, kb * W4_KB + 32 * j + 8 * c);
+        for (int i = 0; i < NB; ++i)
+          op[i] = w4_operand<F16>(j == 0 ? o.q[i].x : j == 1 ? o.q[i].y : j == 2 ? o.q[i].z : o.q[i].w);
 #pragma unroll
-        for (int i = 0; i < NB; ++i) {
-          const s8 op = w4_operand<F16>(j == 0 ? q[i].x : j == 1 ? q[i].y : j == 2 ? q[i].z : q[i].w);
+        for (int p = 0; p < NP; ++p) {
 #pragma unroll
-          for (int t = 0; t < MT; ++t)
-#pragma unroll
-            for (int p = 0; p < NP; ++p) {
-              if (s == 0 && p == 0) w4_mfma_first<F16>(acc[i][t], op, x[t].p[p]);
-              else w4_mfma<F16>(acc[i][t], op, x[t].p[p]);
-            }
-        }
-#pragma unroll
-        for (int t = 0; t < MT; ++t)
-#pragma unroll
-          for (int p = 0; p < NP; ++p) {
-            if (s == 0 && p == 0) w4_mfma_first<F16>(xs[t], ones, x[t].p[p]);
-            else w4_mfma<F16>(xs[t], ones, x[t].p[p]);
+          for (int i = 0; i < NB; ++i) {
+            if (s == 0 && p == 0) w4_mfma_first<F16>(acc[i], xj.p[p], op[i]);
+            else w4_mfma<F16>(acc[i], xj.p[p], op[i]);
           }
+          if (s == 0 && p == 0) w4_mfma_first<F16>(xs, xj.p[p], ones);
+          else w4_mfma<F16>(xs, xj.p[p], ones);
+        }
       }
-      drain(xs[0]);
+      drain(xs);
 #pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        w4_hold(xs[t]);
-#pragma unroll
-        for (int i = 0; i < NB; ++i) w4_hold(acc[i][t]);
-      }
+      for (int i = 0; i < NB; ++i) w4_hold(acc[i]);
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
-        const uint32_t sz[4] = {mt[i][g].x, mt[i][g].y, mt[i][g].z, mt[i][g].w};
+        const float s = bf16_val(o.sz[i][g] & 0xffffu), z = __uint_as_float(o.sz[i][g] & 0xffff0000u);
 #pragma unroll
-        for (int t = 0; t < MT; ++t)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float s = bf16_val(sz[e] & 0xffffu), z = __uint_as_float(sz[e] & 0xffff0000u);
-            tot[i][t][e] = fmaf(s, fmaf(-z, xs[t][e], acc[i][t][e]), tot[i][t][e]);
-          }
+        for (int e = 0; e < NE; ++e) tot[i][e] = fmaf(s, fmaf(-z, xs[e * SP], acc[i][e * SP]), tot[i][e]);
       }
+    }
+  };
+  if (w < a.nkb) {                                   // (the launch gives every wave a block)
+    Block even, odd;
+    int kb = w;
+    load(even, kb);
+    for (;;) {
+      if (kb + W < a.nkb) load(odd, kb + W);
+      add(even);
+      if ((kb += W) >= a.nkb) break;
+      if (kb + W < a.nkb) load(even, kb + W);
+      add(odd);
+      if ((kb += W) >= a.nkb) break;
     }
   }
 #pragma unroll
   for (int i = 0; i < NB; ++i)
 #pragma unroll
-    for (int t = 0; t < MT; ++t) red[((w * NB + i) * MT + t) * WAVE + l] = tot[i][t];
+    for (int e = 0; e < NE; ++e) red[((w * NB + i) * NE + e) * WAVE + l] = tot[i][e];
   __syncthreads();
-  for (int x = threadIdx.x; x < NB * MT * WAVE; x += blockDim.x) {
-    f4 s = red[x];
-    for (int v = 1; v < W; ++v) {
-      const f4 u = red[v * NB * MT * WAVE + x];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[e] += u[e];
-    }
-    const int lane = x & 63, t = (x / WAVE) % MT, i = x / (WAVE * MT);
-    const int m = m0 + 16 * t + (lane & 15), n = (nb0 + i) * 16 + 4 * (lane >> 4);
-    if (m >= a.M) continue;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (n + e >= a.N) break;
-      float v = s[e];
-      if (a.bias) v += w4_ld<XT>(a.bias, n + e);
-      if (a.res) v += w4_ld<XT>(a.res, (size_t)m * a.ldr + n + e);
-      w4_st<XT>(a.y, (size_t)m * a.N + n + e, v);
-    }
+  constexpr int ALL = NB * NE * WAVE;
+  for (int x = threadIdx.x; x < ALL; x += blockDim.x) {
+    float v = red[x];
+    for (int u = 1; u < W; ++u) v += red[u * ALL + x];
+    const int lane = x % WAVE, e = x / WAVE % NE, i = x / (WAVE * NE);
+    const int m = m0 + NE * (lane >> 4) + e, n = (nb0 + i) * 16 + (lane & 15);
+    if (m >= a.M || n >= a.N) continue;
+    if (a.bias) v += w4_ld<XT>(a.bias, n);
+    if (a.res) v += w4_ld<XT>(a.res, (size_t)m * a.ldr + n);
+    w4_st<XT>(a.y, (size_t)m * a.N + n, v);
   }
 }
 
-template <int XT, int GROUP>
-static void w4_go(const W4Args& a, hipStream_t s) {
-  auto go = [&](auto mt, auto nb) {
-    constexpr int MT = decltype(mt)::value, NB = decltype(nb)::value;
-    const int W = a.nkb < 8 ? a.nkb : 8;
-    const dim3 grid((a.nnb + NB - 1) / NB, (a.M + 16 * MT - 1) / (16 * MT));
-    hipLaunchKernelGGL((w4_rows_kernel<XT, GROUP, MT, NB>), grid, dim3(W * WAVE), (size_t)W * NB * MT * WAVE * 16, s, a);
+// More rows: a workgroup of WM x WN x WK waves takes 16 MT WM rows and 16 NBW WN columns, and one of the
+// sum's gridDim.z parts, WK 128-deep blocks of it at a time (one for each wave along WK).  The waves stage the
+// blocks of x in LDS as operands (float32 split once), with each group's sum, so that x crosses the
+// caches once for all the columns: a CU takes about 34 bytes a nanosecond from the L2, and with x in
+// every wave's registers that was the bound.  The next blocks are loaded while these are multiplied.
+// With several parts the sums go to a.part (part, M, N), which w4_join_kernel adds in order.
+template <int XT_, int GROUP_, int MT_, int NBW_, int WM_, int WN_, int WK_>
+struct W4Tile {
+  static constexpr int XT = XT_, GROUP = GROUP_, MT = MT_, NBW = NBW_, WM = WM_, WN = WN_, WK = WK_;
+  static constexpr int W = WM * WN * WK, NP = W4Frag<XT>::NP, NG = W4_KB / GROUP;
+  static constexpr int UNITS = WK * WM * MT;         // 16 rows of a block each
+  static constexpr int UNIT = 4 * NP * WAVE * 16;    // bytes of a unit's operands
+  static constexpr int BUF = UNITS * (UNIT + NG * 64);
+  static constexpr int BM = 16 * MT * WM, BN = 16 * NBW * WN;
+  static constexpr int LDO = BN + 4;                 // floats of a row of results in LDS
+  static constexpr int LDS = 2 * BUF > BM * LDO * 4 ? 2 * BUF : BM * LDO * 4;
+};
+template <class C>
+__global__ __launch_bounds__(C::W * WAVE) void w4_tile_kernel(W4Args a) {
+  constexpr int XT = C::XT, GROUP = C::GROUP, MT = C::MT, NBW = C::NBW, WM = C::WM, WN = C::WN, WK = C::WK, W = C::W;
+  constexpr bool F16 = XT == W4_F16;
+  constexpr int NP = C::NP, NG = C::NG, SG = GROUP / 32, E = XT == W4_F32 ? 4 : 2, NU = (C::UNITS + W - 1) / W;
+  extern __shared__ char lds[];
+  auto frag = [&](int buf, int unit, int p, int j) { return reinterpret_cast<uint4*>(lds + buf * C::BUF + unit * C::UNIT + (p * 4 + j) * (WAVE * 16)); };
+  auto sums = [&](int buf, int unit, int g) { return reinterpret_cast<float*>(lds + buf * C::BUF + C::UNITS * C::UNIT + (unit * NG + g) * 64); };
+  const int l = lane_id(), r = l & 15, c = l >> 4, w = wave_id();
+  const int wk = w / (WM * WN), wm = w / WN % WM, wn = w % WN;
+  const int nb0 = __builtin_amdgcn_readfirstlane((blockIdx.x * WN + wn) * NBW), m0 = blockIdx.y * C::BM, parts = gridDim.z;
+  const int kb0 = (int)((int64_t)a.nkb * blockIdx.z / parts), kb1 = (int)((int64_t)a.nkb * (blockIdx.z + 1) / parts);
+  const int rows = min(C::BM, a.M - m0), k_end = min(a.K, kb1 * W4_KB);
+  const __amdgpu_buffer_rsrc_t xb =
+      w4_buffer(a.x, (size_t)m0 * a.ldx * E, ((rows - 1) * (int64_t)a.ldx + (a.K + 7) / 8 * 8) * E);
+  // (columns past the last: zero codes and scales)
+  const int nbs = max(0, min(NBW, a.nnb - nb0));
+  const size_t nbc = nbs ? nb0 : 0;
+  const __amdgpu_buffer_rsrc_t qb = w4_buffer(a.q, nbc * a.nkb * 1024, (int64_t)nbs * a.nkb * 1024);
+  const __amdgpu_buffer_rsrc_t sb = w4_buffer(a.meta, nbc * a.nkb * (NG * 64), (int64_t)nbs * a.nkb * (NG * 64));
+  f4 tot[NBW][MT];
+#pragma unroll
+  for (int i = 0; i < NBW; ++i)
+#pragma unroll
+    for (int t = 0; t < MT; ++t) tot[i][t] = f4{0.f, 0.f, 0.f, 0.f};
+  struct Block {
+    uint4 q[NBW];
+    uint32_t sz[NBW][NG];
   };
-  using std::integral_constant;
-  if (a.M <= 16) go(integral_constant<int, 1>{}, integral_constant<int, 1>{});
-  else go(integral_constant<int, 2>{}, integral_constant<int, 2>{});
+  W4Raw<XT> xr[NU][4];
+  // the wave's own block kb + wk of the weights, and its units of x of the blocks kb .. kb + WK - 1 (past the
+  // part's last block: zeros of x); lane l takes rows l / 8 (+ 8) and k 8 (l % 8) (+ 64) of a unit
+  uint32_t xoff[NU][2];
+#pragma unroll
+  for (int i = 0; i < NU; ++i) {
+    const int unit = w + W * i;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int m = 16 * (unit % (MT * WM)) + (l >> 3) + 8 * h;
+      xoff[i][h] = unit < C::UNITS && m < rows ? (uint32_t)(m * a.ldx + unit / (MT * WM) * W4_KB + 8 * (l & 7)) * E : W4_OUT;
+    }
+  }
+  auto load = [&](Block& o, int kb) __attribute__((always_inline)) {
+    const int kw = __builtin_amdgcn_readfirstlane(min(kb + wk, a.nkb - 1));
+#pragma unroll
+    for (int i = 0; i < NU; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {                  // rows 8 (j / 2) .., k 64 (j % 2) ..
+        const int k = (kb + (w + W * i) / (MT * WM)) * W4_KB + 64 * (j % 2) + 8 * (l & 7);
+        const uint32_t off = (k < k_end ? xoff[i][j / 2] : W4_OUT) + 64 * (j % 2) * E;
+#pragma unroll
+        for (int v = 0; v < W4Raw<XT>::NV; ++v) xr[i][j].v[v] = w4_buffer16(xb, off + 16 * v, kb * (W4_KB * E));
+      }
+#pragma unroll
+    for (int i = 0; i < NBW; ++i) {
+      o.q[i] = w4_buffer16(qb, i * a.nkb * 1024 + 16 * l, kw * 1024);
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+        o.sz[i][g] = __builtin_amdgcn_raw_buffer_load_b32(sb, i * a.nkb * (NG * 64) + 64 * g + 4 * r, kw * (NG * 64), 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);               // issued here, not where they are used
+  };
+  // An operand's lane (row, c) lies at slot 16 c + (row ^ (c + 4 (step & 1))): eight lanes that hold a
+  // row's 128 bytes then write to eight different banks, and a wave's reads are whole lines.
+  auto stage = [&](int buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+      const int unit = w + W * i;
+      if (C::UNITS % W && unit >= C::UNITS) continue;      // (uniform)
+      const int ch = l & 7;
+      float sum[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const W4Frag<XT> x = w4_frag<XT>(xr[i][j]);
+        const int row = (l >> 3) + 8 * (j / 2);
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+          frag(buf, unit, p, 0)[(2 * (j % 2) + (ch >> 2)) * WAVE + 16 * (ch & 3) + (row ^ ch)] = __builtin_bit_cast(uint4, x.p[p]);
+        sum[j] = w4_sum8<XT>(xr[i][j]);
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int row = (l >> 3) + 8 * j;
+        float s0 = sum[2 * j], s1 = sum[2 * j + 1];
+        if constexpr (NG == 1) s0 += s1;
+        s0 = w4_quad_sum(s0);
+        if constexpr (NG > 1) s1 = w4_quad_sum(s1);
+        if constexpr (NG <= 2) s0 += w4_dpp<0x141>(s0);
+        if constexpr (NG == 2) s1 += w4_dpp<0x141>(s1);
+        if constexpr (NG == 4) {
+          if ((ch & 3) == 0) {
+            sums(buf, unit, ch >> 2)[row] = s0;
+            sums(buf, unit, 2 + (ch >> 2))[row] = s1;
+          }
+        } else if (ch == 0) {
+          sums(buf, unit, 0)[row] = s0;
+          if constexpr (NG == 2) sums(buf, unit, 1)[row] = s1;
+        }
+      }
+    }
+  };
+  auto add = [&](const Block& o, int buf) __attribute__((always_inline)) {
+    const int u0 = wk * (MT * WM) + wm * MT, slot = l ^ c;
+    // operands of x in the order of their use, read AHEAD of it
+    constexpr int STEPS = 4 * NP * MT, AHEAD = NBW >= 4 ? 2 : 4;
+    auto read = [&](int i) __attribute__((always_inline)) {
+      const int t = i % MT, p = i / MT % NP, j = i / (MT * NP);
+      return __builtin_bit_cast(s8, frag(buf, u0 + t, p, j)[j & 1 ? slot ^ 4 : slot]);
+    };
+    s8 x[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) x[i] = read(i);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      f4 acc[NBW][MT];
+#pragma unroll
+      for (int s = 0; s < SG; ++s) {
+        const int j = g * SG + s;
+        s8 op[NBW];
+#pragma unroll
+        for (int i = 0; i < NBW; ++i)
+          op[i] = w4_operand<F16>(j == 0 ? o.q[i].x : j == 1 ? o.q[i].y : j == 2 ? o.q[i].z : o.q[i].w);
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            const int at = (j * NP + p) * MT + t;
+            const s8 xt = x[at % AHEAD];
+#pragma unroll
+            for (int i = 0; i < NBW; ++i) {
+              if (s == 0 && p == 0) w4_mfma_first<F16>(acc[i][t], xt, op[i]);
+              else w4_mfma<F16>(acc[i][t], xt, op[i]);
+            }
+            if (at + AHEAD < STEPS) x[at % AHEAD] = read(at + AHEAD);
+            __builtin_amdgcn_sched_barrier(0x3ff & ~0x300);      // (reads of LDS stay where they are)
+          }
+      }
+      auto sum = [&](int t) __attribute__((always_inline)) { return *reinterpret_cast<const f4*>(sums(buf, u0 + t, g) + 4 * c); };
+      f4 xs = sum(0);
+      drain(acc[0][0]);
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int i = 0; i < NBW; ++i) w4_hold(acc[i][t]);
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        const f4 next = sum(t + 1 < MT ? t + 1 : t);
+#pragma unroll
+        for (int i = 0; i < NBW; ++i) {
+          const float s = bf16_val(o.sz[i][g] & 0xffffu), z = __uint_as_float(o.sz[i][g] & 0xffff0000u);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) tot[i][t][e] = fmaf(s, fmaf(-z, xs[e], acc[i][t][e]), tot[i][t][e]);
+          w4_hold(tot[i][t]);                        // (before the next group's products: registers)
+        }
+        xs = next;
+      }
+    }
+  };
+  Block even, odd;
+  int kb = kb0, buf = 0;
+  load(even, kb);
+  stage(0);
+  __syncthreads();
+  for (;;) {
+    if (kb + WK < kb1) load(odd, kb + WK);
+    add(even, buf);
+    if ((kb += WK) >= kb1) break;
+    stage(buf ^= 1);
+    __syncthreads();
+    if (kb + WK < kb1) load(even, kb + WK);
+    add(odd, buf);
+    if ((kb += WK) >= kb1) break;
+    stage(buf ^= 1);
+    __syncthreads();
+  }
+  // results through LDS, the waves along the sum one after the other, so that whole lines are written
+  float* out = reinterpret_cast<float*>(lds);
+#pragma unroll
+  for (int v = 0; v < WK; ++v) {
+    __syncthreads();
+    if (wk != v) continue;
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int i = 0; i < NBW; ++i) {
+          float& o = out[(16 * (wm * MT + t) + 4 * c + e) * C::LDO + 16 * (wn * NBW + i) + r];
+          o = v ? o + tot[i][t][e] : tot[i][t][e];
+        }
+  }
+  __syncthreads();
+  const int n0 = blockIdx.x * C::BN;
+  for (int x = threadIdx.x; x < C::BM * C::BN / 4; x += W * WAVE) {
+    const int row = x / (C::BN / 4), col = 4 * (x % (C::BN / 4)), m = m0 + row, n = n0 + col;
+    if (row >= rows || n >= a.N) continue;
+    const float4 v = *reinterpret_cast<const float4*>(out + row * C::LDO + col);
+    if (parts > 1) w4_part4(a, ((size_t)blockIdx.z * a.M + m) * a.N + n, n, v);
+    else w4_out4<XT>(a, m, n, v);
+  }
+}
+
+// Rows that 16-byte accesses cannot take, as rows that they can: ld elements, zero past K
+template <typename T>
+__global__ __launch_bounds__(256) void w4_align_kernel(const T* x, T* out, int K, size_t ldx, int ld) {
+  const size_t m = blockIdx.x;
+  for (int k = blockIdx.y * 256 + threadIdx.x; k < ld; k += 256 * gridDim.y) out[m * ld + k] = k < K ? x[m * ldx + k] : T(0);
+}
+
+// The parts of a sum, in order; four columns a thread
+template <int XT>
+__global__ __launch_bounds__(256) void w4_join_kernel(W4Args a, int parts) {
+  const int cols = (a.N + 3) / 4, x = blockIdx.x * 256 + threadIdx.x, m = x / cols, n = 4 * (x - m * cols);
+  if (m >= a.M) return;
+  const size_t at = (size_t)m * a.N + n, step = (size_t)a.M * a.N;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (a.N % 4 == 0) {
+#pragma unroll 8
+    for (int p = 0; p < parts; ++p) v = add4(v, *reinterpret_cast<const float4*>(a.part + p * step + at));
+  } else {
+    float f[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int p = 0; p < parts; ++p)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n + e < a.N) f[e] += a.part[p * step + at + e];
+    v = make_float4(f[0], f[1], f[2], f[3]);
+  }
+  w4_out4<XT>(a, m, n, v);
+}
+
+// How a product runs: parts 0: rows; else tiles, the sum in parts.
+//   rows: one launch, x and (over 16 rows) the weights read again by each tile of rows.  Up to 8 rows
+//     always; more where the weights come from the caches again, 2^15 tiles of 16 rows and 128 x 16
+//     weights, and the sum is not long beside the columns (bfloat16, us, rows against tiles: 64 rows of
+//     2048 x 2048 5.6, 8.2; 64 of 4096 x 4096 11.6, 12.4; 128 of 4096 x 4096 20, 17; 16 of
+//     14336 x 4096 19, 14.8).
+//   parts: two workgroups a CU where that leaves 14 blocks of 128 or more to each, else one, with
+//     four blocks at least (64 rows of 14336 x 4096, 1 / 4 / 8 / 16 parts: 74, 25, 21, 27; 256 of
+//     4096 x 4096, 1 / 2: 21.8, 23.5).
+template <int XT, int GROUP>
+using W4Tiles = W4Tile<XT, GROUP, 2, 2, 1, 4, 2>;
+static int w4_parts(int M, int nkb, int nnb) {
+  using C = W4Tiles<W4_BF16, 128>;
+  if (M <= 8 || (nkb <= 64 && (int64_t)nkb * nnb * ((M + 15) / 16) <= 32768)) return 0;
+  const int64_t tiles = (int64_t)((16 * nnb + C::BN - 1) / C::BN) * ((M + C::BM - 1) / C::BM), cus = cu_count();
+  const int64_t two = 2 * cus / tiles, one = cus / tiles;
+  const int64_t p = two >= 1 && nkb / two >= 14 ? two : one < nkb / 4 ? one : nkb / 4;
+  return p < 1 ? 1 : (int)p;
+}
+
+static size_t w4_align_bytes(int dtype, const W4Args& a) {
+  return a.vec ? 0 : ((size_t)a.M * ((a.K + 7) / 8 * 8) * (dtype == W4_F32 ? 4 : 2) + 255) / 256 * 256;
+}
+size_t w4_workspace_bytes(int dtype, const W4Args& a) {
+  const int parts = w4_parts(a.M, a.nkb, a.nnb);
+  return parts ? w4_align_bytes(dtype, a) + (parts > 1 ? (size_t)parts * a.M * a.N * 4 : 0) : 0;
+}
+
+template <int XT, int GROUP, int SP, int NB>
+static void w4_rows(const W4Args& a, hipStream_t s) {
+  constexpr int most = w4_waves(XT, NB);
+  const int W = a.nkb < most ? a.nkb : most;
+  const dim3 grid((a.nnb + NB - 1) / NB, (a.M + 16 / SP - 1) / (16 / SP));
+  hipLaunchKernelGGL((w4_rows_kernel<XT, GROUP, SP, NB>), grid, dim3(W * WAVE), (size_t)W * NB * (4 / SP) * WAVE * 4, s, a);
+}
+
+template <int XT, int GROUP>
+static void w4_go(W4Args a, hipStream_t s) {
+  const int parts = w4_parts(a.M, a.nkb, a.nnb);
+  if (parts == 0) {
+    // two columns' blocks a wave where two workgroups a CU are left (one row of 4096 x 14336 float32:
+    // 14.6 -> 11.8 us, 16 of 4096 x 11008 14.7 -> 12.5; one of 4096 x 4096 4.5 -> 5.1)
+    const bool two = (int64_t)a.nnb * ((a.M + 15) / 16) >= 2 * cu_count();
+    if (a.M <= 4) two ? w4_rows<XT, GROUP, 4, 2>(a, s) : w4_rows<XT, GROUP, 4, 1>(a, s);
+    else if (a.M <= 8) two ? w4_rows<XT, GROUP, 2, 2>(a, s) : w4_rows<XT, GROUP, 2, 1>(a, s);
+    else two ? w4_rows<XT, GROUP, 1, 2>(a, s) : w4_rows<XT, GROUP, 1, 1>(a, s);
+    return;
+  }
+  if (!a.vec) {
+    using T = std::conditional_t<XT == W4_F32, uint32_t, uint16_t>;
+    const int ld = (a.K + 7) / 8 * 8;
+    T* x = reinterpret_cast<T*>(a.part);
+    a.part = reinterpret_cast<float*>(reinterpret_cast<char*>(a.part) + w4_align_bytes(XT, a));
+    hipLaunchKernelGGL((w4_align_kernel<T>), dim3(a.M, ld < 2048 ? 1 : ld / 1024 < 64 ? ld / 1024 : 64), dim3(256), 0, s,
+                       static_cast<const T*>(a.x), x, a.K, a.ldx, ld);
+    a.x = x;
+    a.ldx = ld;
+  }
+  using C = W4Tiles<XT, GROUP>;
+  const dim3 grid((a.N + C::BN - 1) / C::BN, (a.M + C::BM - 1) / C::BM, parts);
+  hipLaunchKernelGGL((w4_tile_kernel<C>), grid, dim3(C::W * WAVE), C::LDS, s, a);
+  if (parts > 1)
+    hipLaunchKernelGGL((w4_join_kernel<XT>), dim3(((int64_t)a.M * ((a.N + 3) / 4) + 255) / 256), dim3(256), 0, s, a, parts);
 }
 
 template <int XT>
@@ -241,6 +680,7 @@ static void w4_go_group(int group, const W4Args& a, hipStream_t s) {
 }
 
 hipError_t launch_w4(int dtype, int group, const W4Args& a, hipStream_t s) {
+
   if (dtype == W4_F32) w4_go_group<W4_F32>(group, a, s);
   else if (dtype == W4_BF16) w4_go_group<W4_BF16>(group, a, s);
   else w4_go_group<W4_F16>(group, a, s);

@@ -324,7 +324,8 @@ int gdn2_lm_premix_step_fwd(const gdn2_lm_premix_step* p, void* stream);
  *   q     (Np / 16, Kp / 128, 64, 4) words; word j of lane l holds rows 32 j + 8 (l / 16) + e,
  *         e = 0 .. 7, of column l % 16, element e < 4 in nibble 2 e, e >= 4 in nibble 2 e - 7;
  *   meta  (Np / 16, Kp / group, 16) words, scale | zero << 16 as bfloat16 bits; 0 past K and N.
- * group: 32, 64 or 128 rows of W share a scale and a zero.  q and meta 16-byte aligned.  Sums are
+ * group: 32, 64 or 128 rows of W share a scale and a zero.  q and meta 16-byte aligned; workspace
+ * gdn2_w4_workspace_bytes (0: none), 16-byte aligned.  Sums are
  * float32 and products exact; y is rounded once.  A row of x with an infinity or NaN gives NaN. */
 enum { GDN2_F32 = 0, GDN2_BF16 = 1, GDN2_F16 = 2 };
 typedef struct gdn2_w4 {
@@ -333,7 +334,8 @@ typedef struct gdn2_w4 {
   const void *x, *q, *meta, *bias, *residual;
   void* y;
 } gdn2_w4;
-int gdn2_w4_linear(const gdn2_w4* p, void* stream);
+size_t gdn2_w4_workspace_bytes(const gdn2_w4* p);
+int gdn2_w4_linear(const gdn2_w4* p, void* workspace, void* stream);
 
 /* The n best of the K V continuations of each of B groups of K beams, the best first, equal scores by
  * the lower k V + v:  scores[b][k] + log_softmax(logits[b K + k])[v], float32.  logits (B*K, V) rows of
