@@ -103,7 +103,7 @@ def beam_step(logits, scores, n: Optional[int] = None, finished=None, eos_id: Op
                       None if new is None else new.data_ptr())
     ws = torch.empty(L_.gdn2_beam_workspace_bytes(B, K, V, n), dtype=torch.uint8, device=dev)
     with torch.cuda.device(dev):
-        _lib.check(L_.gdn2_beam_step(ctypes.byref(a), ws.data_ptr(), _lib.stream_handle(dev)), "gdn2_beam_step")
+        _lib.check(L_.gdn2_beam_step(ctypes.byref(a), _lib.ptr(ws), _lib.stream_handle(dev)), "gdn2_beam_step")
     return BeamStep(*out, new)
 
 

@@ -521,20 +521,16 @@ PyObject* py_beam(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   unlocked([&] {
     c10::DeviceGuard guard(dev);
     const size_t bytes = abi.beam_ws(a.B, a.K, a.V, a.n);
-    if (!bytes) {
-      status = 1;
-      return;
-    }
     tokens = empty_on(x, {B, n}, at::kLong);
     rows = empty_on(x, {B, n}, at::kLong);
     out = empty_on(x, {B, n}, at::kFloat);
     if (eos >= 0) done = empty_on(x, {B, n}, at::kBool);
-    const Tensor ws = empty_on(x, {(int64_t)bytes}, at::kByte);
+    const Tensor ws = bytes ? empty_on(x, {(int64_t)bytes}, at::kByte) : Tensor();
     a.tokens = static_cast<int64_t*>(tokens.data_ptr());
     a.rows = static_cast<int64_t*>(rows.data_ptr());
     a.out_scores = f32_at(out);
     a.out_finished = done.defined() ? static_cast<uint8_t*>(done.data_ptr()) : nullptr;
-    status = abi.beam(&a, ws.data_ptr(), stream_of(dev));
+    status = abi.beam(&a, bytes ? ws.data_ptr() : nullptr, stream_of(dev));
   });
   if (status) return none();
   return done.defined() ? tuple_of({&tokens, &rows, &out, &done}) : tuple_of({&tokens, &rows, &out});

@@ -866,18 +866,18 @@ int beam_shape(int B, int K, int V, int n) {
   if (n > gdn2::BEAM_MAX_N || K > gdn2::BEAM_MAX_K) return fail(GDN2_ERR_UNSUPPORTED, "at most 128 beams a group, kept or given");
   if ((int64_t)K * V >= (int64_t(1) << 31) || (int64_t)B * K > 65535) return fail(GDN2_ERR_UNSUPPORTED, "shape too large");
   if ((int64_t)n > (int64_t)K * V) return fail(GDN2_ERR_INVALID, "n above K V");
-  if ((int64_t)K * n * gdn2::beam_splits(B * K, V) >= (int64_t(1) << 31))
+  if ((int64_t)K * n * gdn2::beam_splits(B * K, K, V) >= (int64_t(1) << 31))
     return fail(GDN2_ERR_UNSUPPORTED, "shape too large");
   return GDN2_OK;
 }
 size_t beam_cand_bytes(int B, int K, int V, int n) {
-  return align_up((size_t)B * K * gdn2::beam_splits(B * K, V) * n * 8);
+  return align_up((size_t)B * K * gdn2::beam_splits(B * K, K, V) * n * 8);
 }
 }  // namespace
 
 size_t gdn2_beam_workspace_bytes(int B, int K, int V, int n) {
   if (beam_shape(B, K, V, n)) return 0;
-  return beam_cand_bytes(B, K, V, n) + (size_t)B * K * gdn2::beam_splits(B * K, V) * 8;
+  return beam_cand_bytes(B, K, V, n) + (size_t)B * K * gdn2::beam_splits(B * K, K, V) * 8;
 }
 
 int gdn2_beam_step(const gdn2_beam* p, void* workspace, void* stream) {
@@ -888,7 +888,8 @@ int gdn2_beam_step(const gdn2_beam* p, void* workspace, void* stream) {
   if (p->eos < -1 || p->eos >= p->V) return fail(GDN2_ERR_INVALID, "eos outside the vocabulary");
   if (p->finished && p->eos < 0) return fail(GDN2_ERR_INVALID, "finished beams need an eos token");
   if (p->ld < p->V) return fail(GDN2_ERR_INVALID, "row stride below the row");
-  if (!p->logits || !p->scores || !p->tokens || !p->rows || !p->out_scores || !workspace || !aligned16({workspace}))
+  if (!p->logits || !p->scores || !p->tokens || !p->rows || !p->out_scores || !aligned16({workspace}) ||
+      (!workspace && gdn2_beam_workspace_bytes(p->B, p->K, p->V, p->n)))
     return fail(GDN2_ERR_INVALID, "null pointer, or workspace not 16-byte aligned");
   const int e = p->dtype == GDN2_F32 ? 4 : 2;
   if (reinterpret_cast<uintptr_t>(p->logits) % e) return fail(GDN2_ERR_INVALID, "pointer not aligned to its elements");
@@ -898,7 +899,7 @@ int gdn2_beam_step(const gdn2_beam* p, void* workspace, void* stream) {
   a.part = at<float>(workspace, beam_cand_bytes(p->B, p->K, p->V, p->n));
   a.tokens = p->tokens; a.rows = p->rows; a.out_scores = p->out_scores; a.out_finished = p->out_finished;
   a.B = p->B; a.K = p->K; a.V = p->V; a.n = p->n; a.eos = p->eos;
-  a.splits = gdn2::beam_splits(p->B * p->K, p->V);
+  a.splits = gdn2::beam_splits(p->B * p->K, p->K, p->V);
   a.ld = (size_t)p->ld;
   a.vec = aligned16({p->logits}) && p->ld * e % 16 == 0;
   return lm_done(gdn2::launch_beam(p->dtype, a, reinterpret_cast<hipStream_t>(stream)), "beam launch");

@@ -3,7 +3,7 @@
 //   c[k][v] = score[k] + ((x[k][v] - m_k) - ln sum_v exp(x[k][v] - m_k)),   m_k = max_v x[k][v];
 // a finished beam has one continuation, the end token at its own score; NaN counts as -inf.
 //
-// One pass over the logits (beam_part_kernel): a workgroup keeps a piece of a row in registers, forms
+// One pass over the logits, bound by their bytes (beam_part_kernel): a workgroup keeps a piece of a row in registers, forms
 // its maximum and sum, and its n best entries, which are the row's best whatever the row's sum is.
 // beam_join_kernel then has a few hundred entries a group: it joins the sums, forms the scores in
 // float32 as written above, and selects among them.
@@ -26,6 +26,54 @@ __device__ __forceinline__ float beam_key_value(u64 k) {
 }
 __device__ __forceinline__ uint32_t beam_key_index(u64 k) { return 0xffffffffu - (uint32_t)k; }
 
+// Over the wave's lanes, by lane moves within rows of 16, then the four rows' results
+template <int ROR>
+__device__ __forceinline__ float beam_ror(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x120 | ROR, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float beam_lane(float x, int l) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), l));
+}
+__device__ __forceinline__ float wave_maxf(float x) {
+  x = fmaxf(x, beam_ror<8>(x));
+  x = fmaxf(x, beam_ror<4>(x));
+  x = fmaxf(x, beam_ror<2>(x));
+  x = fmaxf(x, beam_ror<1>(x));
+  return fmaxf(fmaxf(beam_lane(x, 0), beam_lane(x, 16)), fmaxf(beam_lane(x, 32), beam_lane(x, 48)));
+}
+__device__ __forceinline__ float wave_sumf(float x) {
+  x += beam_ror<8>(x);
+  x += beam_ror<4>(x);
+  x += beam_ror<2>(x);
+  x += beam_ror<1>(x);
+  return (beam_lane(x, 0) + beam_lane(x, 16)) + (beam_lane(x, 32) + beam_lane(x, 48));
+}
+// exp(x - m) for x <= m, 1 where x is m (also at +inf)
+__device__ __forceinline__ float beam_exp(float x, float m) { return x == m ? 1.f : fast_exp(x - m); }
+// sum over v[0 .. PT) of exp(v - m), m > -inf their maximum or above
+template <int PT>
+__device__ __forceinline__ float beam_exps(const float* v, float m) {
+  float s = 0.f;
+  if (m == __builtin_inff()) {                       // (uniform)
+#pragma unroll
+    for (int i = 0; i < PT; ++i) s += v[i] == m ? 1.f : 0.f;
+  } else {
+#pragma unroll
+    for (int i = 0; i < PT; ++i) s += fast_exp(v[i] - m);
+  }
+  return s;
+}
+
+constexpr int BEAM_T = 256, BEAM_W = BEAM_T / WAVE;
+constexpr int BEAM_LIST = 1024;                 // entries that a selection ranks
+
+struct BeamShared {
+  u64 list[BEAM_LIST + 8];
+  u64 best[2][BEAM_W];
+  float t[2 * BEAM_W];
+  int count;
+};
+
 __device__ __forceinline__ u64 shfl_xor64(u64 x, int m) {
   return (u64)__shfl_xor((uint32_t)(x >> 32), m) << 32 | __shfl_xor((uint32_t)x, m);
 }
@@ -37,22 +85,7 @@ __device__ __forceinline__ u64 wave_max64(u64 x) {
   }
   return x;
 }
-__device__ __forceinline__ float wave_maxf(float x) {
-#pragma unroll
-  for (int m = WAVE / 2; m >= 1; m >>= 1) x = fmaxf(x, __shfl_xor(x, m));
-  return x;
-}
-__device__ __forceinline__ float wave_sumf(float x) {
-#pragma unroll
-  for (int m = WAVE / 2; m >= 1; m >>= 1) x += __shfl_xor(x, m);
-  return x;
-}
-// exp(x - m) for x <= m, 1 where x is m (also at +inf)
-__device__ __forceinline__ float beam_exp(float x, float m) { return x == m ? 1.f : fast_exp(x - m); }
-
-constexpr int BEAM_T = 256, BEAM_W = BEAM_T / WAVE;
-
-// The largest key of the workgroup, in every thread.  best: 2 BEAM_W words used in turn by parity.
+// The largest key of the workgroup, in every thread; best is used in turn by parity.
 __device__ __forceinline__ u64 block_max64(u64 x, u64 (*best)[BEAM_W], int parity) {
   x = wave_max64(x);
   if (lane_id() == 0) best[parity][wave_id()] = x;
@@ -61,6 +94,79 @@ __device__ __forceinline__ u64 block_max64(u64 x, u64 (*best)[BEAM_W], int parit
 #pragma unroll
   for (int i = 1; i < BEAM_W; ++i) y = best[parity][i] > y ? best[parity][i] : y;
   return y;
+}
+
+// The n best of the workgroup's entries, out[0 .. n) in order (0: no more entries).  key(i), i < PT:
+// a thread's entries, 0 for none; v[i]: their values; m: the largest v of the thread.
+//   Of a wave's lanes' maxima, the n-th largest bounds the n best from below, and so does the least of the
+// four waves' ceil(n / 4)-th largest (n entries at least reach either).  A few times n entries reach the
+// higher of the two; they are gathered and ranked by counting.  Where more than BEAM_LIST reach it (long ties, rows that are almost
+// all masked), n rounds of the largest key of all take their place.
+template <int PT, class Key>
+__device__ __forceinline__ void beam_select(BeamShared& sh, const float* v, float m, int n, u64* out, Key key) {
+  const int tid = threadIdx.x, l = lane_id();
+  const int share = (n + BEAM_W - 1) / BEAM_W, rounds = n <= 16 ? n : share;
+  float t = 0.f, ts = 0.f;
+  for (int i = 0; i < rounds; ++i) {
+    t = wave_maxf(m);
+    if (i + 1 == share) ts = t;
+    const u64 at = __ballot(m == t);
+    if (l == __ffsll(at) - 1) m = -__builtin_inff();
+  }
+  if (l == 0) {
+    sh.t[wave_id()] = ts;
+    sh.t[BEAM_W + wave_id()] = rounds == n ? t : -__builtin_inff();
+  }
+  if (tid == 0) sh.count = 0;
+  __syncthreads();
+  t = fmaxf(fminf(fminf(sh.t[0], sh.t[1]), fminf(sh.t[2], sh.t[3])),
+            fmaxf(fmaxf(sh.t[4], sh.t[5]), fmaxf(sh.t[6], sh.t[7])));
+#pragma unroll
+  for (int i = 0; i < PT; ++i) {
+    bool in = v[i] >= t;
+    if (__ballot(in) == 0) continue;                 // (uniform in the wave)
+    const u64 k = in ? key(i) : 0;
+    in = k != 0;
+    const u64 who = __ballot(in);
+    if (who == 0) continue;
+    int base = 0;
+    if (l == __ffsll(who) - 1) base = atomicAdd(&sh.count, __popcll(who));
+    base = __shfl(base, __ffsll(who) - 1);
+    const int at = base + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+    if (in && at < BEAM_LIST) sh.list[at] = k;
+  }
+  __syncthreads();
+  const int count = sh.count;
+  if (count <= BEAM_LIST) {
+    if (tid < 8) sh.list[count + tid] = 0;           // (ranked eight at a time)
+    __syncthreads();
+    for (int i = tid; i < count; i += BEAM_T) {
+      const u64 k = sh.list[i];
+      int rank = 0;
+      for (int j = 0; j < count; j += 8) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) rank += sh.list[j + e] > k;
+      }
+      if (rank < n) out[rank] = k;
+    }
+    for (int i = count + tid; i < n; i += BEAM_T) out[i] = 0;
+    return;
+  }
+  auto next = [&](u64 below) {
+    u64 k = 0;
+#pragma unroll
+    for (int i = 0; i < PT; ++i) {
+      const u64 y = key(i);
+      k = y < below && y > k ? y : k;
+    }
+    return k;
+  };
+  u64 mine = next(~0ull);
+  for (int i = 0; i < n; ++i) {
+    const u64 top = block_max64(mine, sh.best, i & 1);
+    if (tid == 0) out[i] = top;
+    if (top == mine) mine = next(top);
+  }
 }
 
 template <int XT, int VW>
@@ -95,7 +201,7 @@ __device__ __forceinline__ void beam_load(const BeamArgs& a, size_t row, int i, 
 template <int XT, int VW, int PT>
 __global__ __launch_bounds__(BEAM_T) void beam_part_kernel(BeamArgs a) {
   __shared__ float sm[2 * BEAM_W];
-  __shared__ u64 best[2][BEAM_W];
+  __shared__ BeamShared sh;
   const int tid = threadIdx.x, split = blockIdx.x, row = blockIdx.y;
   u64* out = a.cand + ((size_t)row * a.splits + split) * a.n;
   const float score = a.scores[row];
@@ -136,104 +242,26 @@ __global__ __launch_bounds__(BEAM_T) void beam_part_kernel(BeamArgs a) {
     v[i] = beam_value(v[i]);
     m = fmaxf(m, v[i]);
   }
+  const float mine = m;
   m = wave_maxf(m);
   if (lane_id() == 0) sm[wave_id()] = m;
   __syncthreads();
   m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-  float s = 0.f;
-  if (m > -__builtin_inff()) {
-#pragma unroll
-    for (int i = 0; i < PT; ++i) s += beam_exp(v[i], m);
-  }
-  s = wave_sumf(s);
+  const float s = wave_sumf(m > -__builtin_inff() ? beam_exps<PT>(v, m) : 0.f);
   if (lane_id() == 0) sm[BEAM_W + wave_id()] = s;
-  __syncthreads();
-  if (tid == 0) {
+  beam_select<PT>(sh, v, mine, a.n, out, [&](int i) {
+    const int at = c0 + ((i / VW) * BEAM_T + tid) * VW + i % VW;
+    return at < a.V ? beam_key(v[i], at) : 0;
+  });
+  if (tid == 0) {                                    // (behind the selection's barriers)
     a.part[2 * ((size_t)row * a.splits + split)] = m;
     a.part[2 * ((size_t)row * a.splits + split) + 1] = (sm[BEAM_W] + sm[BEAM_W + 1]) + (sm[BEAM_W + 2] + sm[BEAM_W + 3]);
   }
-  // n rounds: each takes the best of the threads' bests, whose owner looks for its next
-  auto index = [&](int i) { return c0 + ((i / VW) * BEAM_T + tid) * VW + i % VW; };
-  auto next = [&](u64 below) {
-    u64 k = 0;
-#pragma unroll
-    for (int i = 0; i < PT; ++i) {
-      const u64 y = index(i) < a.V ? beam_key(v[i], index(i)) : 0;
-      k = y < below && y > k ? y : k;
-    }
-    return k;
-  };
-  u64 mine = next(~0ull);
-  for (int i = 0; i < a.n; ++i) {
-    const u64 top = block_max64(mine, best, i & 1);
-    if (tid == 0) out[i] = top;
-    if (top == mine) mine = next(top);
-  }
 }
 
-// One workgroup a group: the scores of the parts' entries, and the n best of them.
-constexpr int BEAM_PT2 = 8;                     // entries a thread keeps at a time
-__global__ __launch_bounds__(BEAM_T) void beam_join_kernel(BeamArgs a) {
-  __shared__ u64 best[2][BEAM_W];
-  __shared__ u64 kept[BEAM_MAX_N];
-  __shared__ float sM[BEAM_MAX_K], sL[BEAM_MAX_K];
-  const int tid = threadIdx.x, b = blockIdx.x, per = a.splits * a.n;
-  for (int k = wave_id(); k < a.K; k += BEAM_W) {
-    const float* p = a.part + 2 * (size_t)(b * a.K + k) * a.splits;
-    float m = -__builtin_inff(), s = 0.f;
-    for (int i = lane_id(); i < a.splits; i += WAVE) m = fmaxf(m, p[2 * i]);
-    m = wave_maxf(m);
-    for (int i = lane_id(); i < a.splits; i += WAVE)
-      if (p[2 * i] > -__builtin_inff()) s += p[2 * i + 1] * beam_exp(p[2 * i], m);
-    s = wave_sumf(s);
-    if (lane_id() == 0) {
-      sM[k] = m;
-      sL[k] = logf(s);
-    }
-  }
-  for (int i = tid; i < a.n; i += BEAM_T) kept[i] = 0;
-  __syncthreads();
-  const int total = a.K * per;
-  for (int c0 = 0; c0 < total; c0 += BEAM_PT2 * BEAM_T) {
-    u64 key[BEAM_PT2 + 1];
-#pragma unroll
-    for (int i = 0; i < BEAM_PT2; ++i) {
-      const int e = c0 + i * BEAM_T + tid;
-      key[i] = 0;
-      if (e < total) {
-        const int k = e / per;
-        const u64 x = a.cand[(size_t)b * total + e];
-        if (x) {
-          const uint32_t v = beam_key_index(x);
-          const float xv = beam_key_value(x), score = a.scores[b * a.K + k];
-          float c = -__builtin_inff();
-          if (a.finished && a.finished[b * a.K + k]) c = (int)v == a.eos ? beam_value(score) : c;
-          else if (xv > -__builtin_inff() && score > -__builtin_inff())
-            c = beam_value(score + ((xv == sM[k] ? 0.f : xv - sM[k]) - sL[k]));
-          key[i] = beam_key(c, (uint32_t)k * a.V + v);
-        }
-      }
-    }
-    // the best of the entries before, and a finished beam's end token where the parts left it out
-    key[BEAM_PT2] = tid < a.n ? kept[tid] : 0;
-    if (c0 == 0 && a.finished && tid >= a.n && tid - a.n < a.K && a.finished[b * a.K + tid - a.n] && a.eos >= a.n)
-      key[BEAM_PT2] = beam_key(beam_value(a.scores[b * a.K + tid - a.n]), (uint32_t)(tid - a.n) * a.V + a.eos);
-    __syncthreads();
-    u64 mine = 0;
-#pragma unroll
-    for (int i = 0; i <= BEAM_PT2; ++i) mine = key[i] > mine ? key[i] : mine;
-    for (int i = 0; i < a.n; ++i) {
-      const u64 top = block_max64(mine, best, i & 1);
-      if (tid == 0) kept[i] = top;
-      if (top == mine) {
-        mine = 0;
-#pragma unroll
-        for (int j = 0; j <= BEAM_PT2; ++j) mine = key[j] < top && key[j] > mine ? key[j] : mine;
-      }
-    }
-    __syncthreads();
-  }
-  for (int i = tid; i < a.n; i += BEAM_T) {
+// A group's results from its keys
+__device__ __forceinline__ void beam_write(const BeamArgs& a, int b, const u64* kept) {
+  for (int i = threadIdx.x; i < a.n; i += BEAM_T) {
     const u64 x = kept[i];
     const uint32_t at = beam_key_index(x);
     const int k = at / (uint32_t)a.V, v = at - (uint32_t)k * a.V;
@@ -244,6 +272,124 @@ __global__ __launch_bounds__(BEAM_T) void beam_join_kernel(BeamArgs a) {
     if (a.out_finished) a.out_finished[o] = (a.finished && a.finished[b * a.K + k]) || v == a.eos;
   }
 }
+// The score of an entry x of a beam whose logits have the maximum m and ln sum exp(x - m) = ls
+__device__ __forceinline__ float beam_score(float score, float x, float m, float ls) {
+  if (!(x > -__builtin_inff() && score > -__builtin_inff())) return -__builtin_inff();
+  return beam_value(score + ((x == m ? 0.f : x - m) - ls));
+}
+
+// One workgroup a group: the scores of the parts' entries, and the n best of them.
+constexpr int BEAM_PT2 = 8;                     // entries a thread keeps at a time
+__global__ __launch_bounds__(BEAM_T) void beam_join_kernel(BeamArgs a) {
+  __shared__ BeamShared sh;
+  __shared__ u64 kept[BEAM_MAX_N];
+  __shared__ float sM[BEAM_MAX_K], sL[BEAM_MAX_K], sS[BEAM_MAX_K];
+  __shared__ uint8_t sF[BEAM_MAX_K];
+  const int tid = threadIdx.x, b = blockIdx.x, per = a.splits * a.n, total = a.K * per;
+  const u64* cand = a.cand + (size_t)b * total;
+  u64 x[BEAM_PT2];
+  auto fetch = [&](int c0) {
+#pragma unroll
+    for (int i = 0; i < BEAM_PT2; ++i) x[i] = c0 + i * BEAM_T + tid < total ? cand[c0 + i * BEAM_T + tid] : 0;
+  };
+  fetch(0);
+  for (int k = wave_id(); k < a.K; k += BEAM_W) {
+    const float* p = a.part + 2 * (size_t)(b * a.K + k) * a.splits;
+    float m = -__builtin_inff(), s = 0.f;
+    for (int i = lane_id(); i < a.splits; i += WAVE) {
+      const float mi = p[2 * i], si = p[2 * i + 1];
+      if (mi > m) {
+        s = s * beam_exp(m, mi) + si;
+        m = mi;
+      } else if (mi > -__builtin_inff()) {
+        s += si * beam_exp(mi, m);
+      }
+    }
+    const float top = wave_maxf(m);
+    s = wave_sumf(m > -__builtin_inff() ? s * beam_exp(m, top) : 0.f);
+    if (lane_id() == 0) {
+      sM[k] = top;
+      sL[k] = logf(s);
+      sS[k] = a.scores[b * a.K + k];
+      sF[k] = a.finished ? a.finished[b * a.K + k] : 0;
+    }
+  }
+  for (int i = tid; i < a.n; i += BEAM_T) kept[i] = 0;
+  __syncthreads();
+  for (int c0 = 0; c0 < total; c0 += BEAM_PT2 * BEAM_T) {
+    u64 key[BEAM_PT2 + 1];
+    float val[BEAM_PT2 + 1], m = -__builtin_inff();
+    if (c0) fetch(c0);
+#pragma unroll
+    for (int i = 0; i < BEAM_PT2; ++i) {
+      key[i] = 0;
+      if (x[i]) {
+        const int k = (c0 + i * BEAM_T + tid) / per;
+        const uint32_t v = beam_key_index(x[i]);
+        const float c = sF[k] ? ((int)v == a.eos ? beam_value(sS[k]) : -__builtin_inff())
+                              : beam_score(sS[k], beam_key_value(x[i]), sM[k], sL[k]);
+        key[i] = beam_key(c, (uint32_t)k * a.V + v);
+      }
+    }
+    // the best of the entries before, and a finished beam's end token where the parts left it out
+    key[BEAM_PT2] = tid < a.n ? kept[tid] : 0;
+    const int fk = tid - a.n;
+    if (c0 == 0 && fk >= 0 && fk < a.K && sF[fk] && a.eos >= a.n)
+      key[BEAM_PT2] = beam_key(beam_value(sS[fk]), (uint32_t)fk * a.V + a.eos);
+#pragma unroll
+    for (int i = 0; i <= BEAM_PT2; ++i) {
+      val[i] = key[i] ? beam_key_value(key[i]) : -__builtin_inff();
+      m = fmaxf(m, val[i]);
+    }
+    __syncthreads();                                 // (kept is read)
+    beam_select<BEAM_PT2 + 1>(sh, val, m, a.n, kept, [&](int i) { return key[i]; });
+    __syncthreads();
+  }
+  beam_write(a, b, kept);
+}
+
+// A small vocabulary in one launch: one workgroup a group, R rows a wave and PER entries a lane and row,
+// all kept in registers with their scores.
+template <int XT, int R, int PER>
+__global__ __launch_bounds__(BEAM_T) void beam_small_kernel(BeamArgs a) {
+  __shared__ BeamShared sh;
+  __shared__ u64 kept[BEAM_MAX_N];
+  const int l = lane_id(), w = wave_id(), b = blockIdx.x;
+  float v[R * PER], score[R], best = -__builtin_inff();
+  bool done[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int k = w + BEAM_W * r;
+    const size_t row = (size_t)b * a.K + min(k, a.K - 1);
+    score[r] = k < a.K ? a.scores[row] : -__builtin_inff();
+    done[r] = a.finished && a.finished[row];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) beam_load<XT, 1>(a, row, min(j * WAVE + l, a.V - 1), v + r * PER + j);
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    float* x = v + r * PER;
+    float m = -__builtin_inff();
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      x[j] = j * WAVE + l < a.V ? beam_value(x[j]) : -__builtin_inff();
+      m = fmaxf(m, x[j]);
+    }
+    m = wave_maxf(m);
+    const float ls = logf(wave_sumf(m > -__builtin_inff() ? beam_exps<PER>(x, m) : 0.f));
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      x[j] = done[r] ? (j * WAVE + l == a.eos ? beam_value(score[r]) : -__builtin_inff()) : beam_score(score[r], x[j], m, ls);
+      best = fmaxf(best, x[j]);
+    }
+  }
+  beam_select<R * PER>(sh, v, best, a.n, kept, [&](int i) {
+    const int k = w + BEAM_W * (i / PER), at = i % PER * WAVE + l;
+    return k < a.K && at < a.V ? beam_key(v[i], (uint32_t)k * a.V + at) : 0;
+  });
+  __syncthreads();
+  beam_write(a, b, kept);
+}
 
 template <int XT, int VW>
 static void beam_go(const BeamArgs& a, int pt, hipStream_t s) {
@@ -252,14 +398,29 @@ static void beam_go(const BeamArgs& a, int pt, hipStream_t s) {
   else hipLaunchKernelGGL((beam_part_kernel<XT, VW, 32>), grid, dim3(BEAM_T), 0, s, a);
 }
 
+template <int XT>
+static void beam_small_go(const BeamArgs& a, hipStream_t s) {
+  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(a.B), dim3(BEAM_T), 0, s, a); };
+  if (a.K <= 4) a.V <= 256 ? go(beam_small_kernel<XT, 1, 4>) : go(beam_small_kernel<XT, 1, 32>);
+  else if (a.K <= 8) a.V <= 256 ? go(beam_small_kernel<XT, 2, 4>) : go(beam_small_kernel<XT, 2, 16>);
+  else go(beam_small_kernel<XT, 4, 8>);
+}
+
+// Whether a group's logits fit one workgroup's registers: one launch in place of two.
+static bool beam_small(int K, int V) { return K <= 4 ? V <= 2048 : K <= 8 ? V <= 1024 : K <= 16 && V <= 512; }
 // Entries a thread keeps: 32 when that still gives every CU four workgroups, else 8.
-int beam_per_thread(int rows, int V) { return (int64_t)rows * ((V + 32 * BEAM_T - 1) / (32 * BEAM_T)) >= 1024 ? 32 : 8; }
-int beam_splits(int rows, int V) {
+static int beam_per_thread(int rows, int V) { return (int64_t)rows * ((V + 32 * BEAM_T - 1) / (32 * BEAM_T)) >= 1024 ? 32 : 8; }
+int beam_splits(int rows, int K, int V) {
+  if (beam_small(K, V)) return 0;
   const int per = beam_per_thread(rows, V) * BEAM_T;
   return (V + per - 1) / per;
 }
 
 hipError_t launch_beam(int dtype, const BeamArgs& a, hipStream_t s) {
+  if (a.splits == 0) {
+    dtype == W4_F32 ? beam_small_go<W4_F32>(a, s) : dtype == W4_BF16 ? beam_small_go<W4_BF16>(a, s) : beam_small_go<W4_F16>(a, s);
+    return hipGetLastError();
+  }
   const int pt = beam_per_thread(a.B * a.K, a.V);
   if (dtype == W4_F32) a.vec ? beam_go<W4_F32, 4>(a, pt, s) : beam_go<W4_F32, 1>(a, pt, s);
   else if (dtype == W4_BF16) a.vec ? beam_go<W4_BF16, 8>(a, pt, s) : beam_go<W4_BF16, 1>(a, pt, s);

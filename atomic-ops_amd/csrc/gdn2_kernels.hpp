@@ -430,7 +430,7 @@ struct BeamArgs {
   int B, K, V, n, eos, splits, vec;
   size_t ld;
 };
-int beam_splits(int rows, int V);
+int beam_splits(int rows, int K, int V);        // 0: no workspace
 hipError_t launch_beam(int dtype, const BeamArgs& a, hipStream_t s);
 
 // Linear work index of this workgroup such that consecutive indices (workgroups of one

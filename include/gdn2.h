@@ -344,7 +344,7 @@ int gdn2_w4_linear(const gdn2_w4* p, void* workspace, void* stream);
  * continuation, the token eos at the beam's own score (0 <= eos < V).  eos -1: none.
  * tokens, rows (B, n): v and b K + k; out_scores (B, n); out_finished NULL or (B, n) bytes: whether
  * the beam was finished or v is eos.  1 <= n <= 128, n <= K V, K <= 128, K V < 2^31.
- * workspace: gdn2_beam_workspace_bytes, 16-byte aligned. */
+ * workspace: gdn2_beam_workspace_bytes (0: none), 16-byte aligned. */
 typedef struct gdn2_beam {
   int32_t B, K, V, n, eos, dtype;
   int64_t ld;
