@@ -1,6 +1,8 @@
-"""Token generation from the benchmark LM: the steps of beam search on the HIP kernels.
+"""Token generation from the benchmark LM: beam search on the HIP kernels.
 
-* ``beam_step``    of all continuations of a group's beams, the best n (``csrc/gdn2_beam.hip``);
+* ``Generator``    the LM with 4-bit weights (``w4``): prefill of a prompt, one token for a batch of
+                   sequences, and ``beam_search`` over them;
+* ``beam_step``      of all continuations of a group's beams, the best n (``csrc/gdn2_beam.hip``);
 * ``premix_step``  one token of a block's convolutions, gates and norms from the cached projections of
                    the three tokens before it (``csrc/gdn2_lm.hip``).
 
@@ -11,13 +13,15 @@ of a block are taken from the parent's row where a step reads them anyway (``par
 from __future__ import annotations
 
 import ctypes
-from typing import NamedTuple, Optional
+from typing import List, NamedTuple, Optional
 
 import torch
 
-from . import _lib
+from . import _lib, lm_kernels
+from .inference import chunk_forward_inference, decode_step
+from .w4 import quantize_w4, w4_linear
 
-__all__ = ["BeamStep", "PremixStep", "beam_step", "premix_step"]
+__all__ = ["BeamStep", "PremixStep", "beam_step", "premix_step", "Cache", "BeamResult", "Generator"]
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}        # GDN2_F32, GDN2_BF16, GDN2_F16
 _INDEX = {torch.int32: 1, torch.int64: 2}                                # GDN2_FLAG_INT32, GDN2_FLAG_INT64
@@ -179,3 +183,171 @@ def _parent_rows(parents, R):
     if parents.is_floating_point() or parents.is_complex() or parents.dtype == torch.bool:
         raise TypeError(f"parents must be whole numbers, got {parents.dtype}")
     return parents.contiguous() if parents.dtype in _INDEX else parents.to(torch.int64)
+
+
+# ------------------------------------------------------------------------------------------
+# the LM
+# ------------------------------------------------------------------------------------------
+
+class Cache(NamedTuple):
+    """What a batch of R sequences carries to its next token, per block: the recurrence's state
+    (R, H, D, D) and the last three tokens' q | k | v projections (R, 3, 3 H D)."""
+    states: List[torch.Tensor]
+    history: List[torch.Tensor]
+
+
+class BeamResult(NamedTuple):
+    """tokens (B, n_beams, T): the new tokens, the best beam first, eos_id after a beam's end; scores
+    (B, n_beams): their log-probabilities."""
+    tokens: torch.Tensor
+    scores: torch.Tensor
+
+
+class _Block(NamedTuple):
+    w_in: object            # [Wq | Wk | Wv | We | Ww | Wo | Wd], columns to a multiple of 4
+    conv_w: tuple
+    conv_b: tuple
+    gate_b: tuple
+    decay_b: torch.Tensor
+    decay_a: torch.Tensor
+    mix_norm: torch.Tensor
+    w_out: object
+    mlp_norm: torch.Tensor
+    w_gate_up: object
+    w_down: object
+
+
+class Generator:
+    """An ``e2e_lm.LM`` with its matrices in 4 bits, for generation: float32 activations, every product
+    through ``w4_linear``.  The model itself is not changed or kept."""
+
+    def __init__(self, model, group_size: int = 64, op_cfg=None):
+        from . import e2e_lm
+        c = model.cfg
+        dev = model.embed.device
+        if not model.embed.is_cuda:
+            raise ValueError(f"Generator needs a model on a ROCm device, got {dev}")
+        if c.d_head not in (64, 128) or c.d_conv != 4:
+            raise ValueError(f"d_head={c.d_head}, d_conv={c.d_conv}: the HIP kernels support heads of 64 and 128 and 4 taps")
+        if max(c.proj_dim, c.d_model) > lm_kernels._MAX_C or c.d_model % 4 or (c.mlp_mult * c.d_model) % 4:
+            raise ValueError(f"widths up to {lm_kernels._MAX_C}, multiples of 4")
+        self.cfg, self.device = c, dev
+        self.op_cfg = e2e_lm.operator_cfg() if op_cfg is None else op_cfg
+        self.scale = float(c.d_head) ** -0.5
+        f32 = lambda t: t.detach().to(torch.float32).clone()  # noqa: E731
+        q4 = lambda *ws: quantize_w4(torch.cat([w.detach() for w in ws], 1), group_size)  # noqa: E731
+        pad = torch.zeros((c.d_model, -(6 * c.proj_dim + c.n_heads) % 4), device=dev)
+        self.blocks = [_Block(
+            w_in=q4(*(m.weight for m in (b.q_proj, b.k_proj, b.v_proj, b.erase_gate, b.write_gate, b.out_gate, b.decay_proj)), pad),
+            conv_w=tuple(f32(m.weight) for m in (b.q_conv, b.k_conv, b.v_conv)),
+            conv_b=tuple(f32(m.bias) for m in (b.q_conv, b.k_conv, b.v_conv)),
+            gate_b=(f32(b.erase_gate.bias), f32(b.write_gate.bias)),
+            decay_b=f32(b.decay_proj.bias), decay_a=f32(b.decay_a),
+            mix_norm=f32(b.mixer_out_norm.scale), w_out=q4(b.out_proj.weight), mlp_norm=f32(b.mlp_norm.scale),
+            w_gate_up=q4(b.gate_proj.weight, b.up_proj.weight), w_down=q4(b.down_proj.weight)) for b in model.blocks]
+        self.embed, self.final_norm = f32(model.embed), f32(model.final_norm.scale)
+        self.head = q4(model.embed.t())
+
+    def _rest(self, blk, o, gate, x, L):
+        """The block behind the recurrence; o (B, H, L, D), gate and x rows (B L, ...)."""
+        z = lm_kernels._rms(o, blk.mix_norm, gate, (L, self.cfg.d_head))
+        x = w4_linear(z, blk.w_out, residual=x)
+        act = lm_kernels._swiglu(w4_linear(lm_kernels._rms(x, blk.mlp_norm), blk.w_gate_up))
+        return w4_linear(act, blk.w_down, residual=x)
+
+    def _logits(self, x):
+        return w4_linear(lm_kernels._rms(x, self.final_norm), self.head)
+
+    def _ids(self, ids, dim):
+        if ids.dim() != dim or ids.numel() == 0 or ids.is_floating_point() or ids.dtype == torch.bool:
+            raise ValueError(f"token ids must be whole numbers of {dim} dimensions, not empty, got {ids.dtype} {tuple(ids.shape)}")
+        if ids.device != self.device:
+            raise ValueError(f"token ids are on {ids.device}, the model on {self.device}")
+
+    @torch.no_grad()
+    def prefill(self, ids):
+        """Prompts ids (B, L) from an empty cache: the logits (B, V) behind the last token, the cache."""
+        self._ids(ids, 2)
+        (B, L), c, cache = ids.shape, self.cfg, Cache([], [])
+        H, D, C = c.n_heads, c.d_head, c.proj_dim
+        x = self.embed[ids].reshape(B * L, -1)
+        for blk in self.blocks:
+            y = w4_linear(x, blk.w_in)
+            ops = [torch.empty((B, H, L, D), device=self.device) for _ in range(6)]
+            gate = torch.empty((B * L, C), device=self.device)
+            at = lambda ts: (lm_kernels._vp * len(ts))(*(t.data_ptr() for t in ts))  # noqa: E731
+            a = lm_kernels._PremixArgs(B, L, H, D, y.shape[1], float(c.g_max), y.data_ptr(), at(blk.conv_w), at(blk.conv_b),
+                                       at(blk.gate_b), blk.decay_b.data_ptr(), blk.decay_a.data_ptr(), at(ops), gate.data_ptr())
+            lm_kernels._call("gdn2_lm_premix_fwd", self.device, ctypes.byref(a))
+            o, state = chunk_forward_inference(*ops, scale=self.scale, cfg=self.op_cfg)
+            past = y.view(B, L, -1)[:, max(L - 3, 0):, :3 * C]
+            history = torch.zeros((B, 3, 3 * C), device=self.device)
+            history[:, 3 - past.shape[1]:] = past
+            cache.states.append(state)
+            cache.history.append(history)
+            x = self._rest(blk, o, gate, x, L)
+        return self._logits(x.view(B, L, -1)[:, -1].contiguous()), cache
+
+    @torch.no_grad()
+    def step(self, tokens, cache: Cache, rows=None):
+        """One token for each of R sequences: tokens (R,); rows (R,): the row of the cache that each
+        sequence continues (None: its own).  The logits (R, V) and the sequences' cache."""
+        self._ids(tokens, 1)
+        R, c, new = tokens.shape[0], self.cfg, Cache([], [])
+        x = self.embed[tokens]
+        for blk, state, history in zip(self.blocks, cache.states, cache.history):
+            m = premix_step(w4_linear(x, blk.w_in), history, blk.conv_w, blk.conv_b, blk.gate_b, blk.decay_b, blk.decay_a,
+                            n_heads=c.n_heads, g_max=float(c.g_max), parents=rows)
+            o, state = decode_step(m.q, m.k, m.v, m.w, m.b, m.g, state, self.scale, parents=rows)
+            new.states.append(state)
+            new.history.append(m.history)
+            x = self._rest(blk, o.view(R, c.n_heads, 1, c.d_head), m.gate, x, 1)
+        return self._logits(x), new
+
+    @torch.no_grad()
+    def beam_search(self, ids, n_beams: int, max_new_tokens: int, eos_id: Optional[int] = None) -> BeamResult:
+        """The n_beams continuations of each prompt ids (B, L) that beam search keeps, up to
+        max_new_tokens tokens.  With eos_id a beam ends when it takes that token, keeping its score, and the
+        search ends when all have (looked at every 16 tokens: it costs a synchronisation)."""
+        if max_new_tokens < 1:
+            raise ValueError(f"max_new_tokens={max_new_tokens}: at least one is needed")
+        logits, cache = self.prefill(ids)
+        B = ids.shape[0]
+        # the first token's beams all continue the prompt's one row
+        r = beam_step(logits, torch.zeros((B, 1), device=self.device), n=n_beams, eos_id=eos_id)
+        steps = [(r.tokens, torch.zeros_like(r.rows))]
+        base = torch.arange(B, device=self.device)[:, None] * n_beams
+        for t in range(1, max_new_tokens):
+            if eos_id is not None and t % 16 == 0 and bool(r.finished.all()):
+                break
+            logits, cache = self.step(r.tokens.view(-1), cache, r.rows.view(-1))
+            r = beam_step(logits, r.scores, n=n_beams, finished=r.finished, eos_id=eos_id)
+            steps.append((r.tokens, r.rows - base))
+        # back from the last token along the parents
+        out, at = [], torch.arange(n_beams, device=self.device).expand(B, n_beams)
+        for tokens, parent in reversed(steps):
+            out.append(tokens.gather(1, at))
+            at = parent.gather(1, at)
+        return BeamResult(torch.stack(out[::-1], -1), r.scores)
+
+
+def main():
+    """Beam search from the benchmark LM with random weights: tokens and time per token."""
+    import time
+
+    from . import e2e_lm
+    cfg = e2e_lm.LMConfig()
+    gen = Generator(e2e_lm.make_lm(cfg))
+    ids = e2e_lm.synthetic_tokens(cfg, batch=2, length=100)
+    for n in (16, 64):
+        gen.beam_search(ids, 4, n)
+        torch.cuda.synchronize()
+        t0 = time.perf_counter()
+        r = gen.beam_search(ids, 4, n)
+        torch.cuda.synchronize()
+        print(f"2 prompts of 100 tokens, 4 beams, {n} new tokens: {(time.perf_counter() - t0) * 1e3:.1f} ms, "
+              f"best scores {[round(x, 3) for x in r.scores[:, 0].tolist()]}", flush=True)
+
+
+if __name__ == "__main__":
+    main()

@@ -9,13 +9,17 @@
 //   h and o: NaN / +-Inf -> 0;  o stored in the output dtype, the state carried in the state
 //   dtype (rounded after every token, as consecutive decode_step calls store it).
 // The value columns of the state are independent, so a workgroup takes a slice of columns of one
-// (batch, head) -- 32 of them, whole 128-byte lines of a state row; all D with the cap, which needs
-// the head's norm -- and keeps it in registers: the state is read and written once per call.
+// (batch, head) -- whole 128-byte lines of a state row, 32 columns of fp32 or 64 of bf16; all D with the
+// cap, which needs the head's norm -- and keeps it in registers: the state is read and written once per call.
 // Element-wise, no MFMA: 2 D^2 state elements per (batch, head), plus 7 D per token.
 //   one token (decode_step_kernel): memory-bound at serving batches, so a wave reads whole lines:
 //     thread t owns 4 columns (j0 = 4 (t % (CW/4))) of the D/16 key rows of group t / (CW/4); the key
 //     vectors go through LDS and the key sums over the 16 groups too.  B64 H16 D128 fp32: 26.6 us,
-//     0.81 of the copy rate.
+//     0.81 of the copy rate; 256 rows of H16 D128 bf16 47.2 us (5.7 TB/s; with 32 columns a workgroup, half
+//     lines, and a condition at each load 88.9).  With parents, a row's state is read from its parent's
+//     row: the beams of a search are reordered without a copy, and rows of one parent, whose
+//     workgroups follow each other on an XCD, read it from that XCD's L2 (42.7 us where the children of
+//     four beams have two parents).
 //   several tokens (decode_tail_kernel): bound by a token's dependent chain, so nothing on it goes
 //     through memory or a barrier: a lane holds 4 columns of 4 key rows, a key sum is 4 products per
 //     lane and a butterfly over the D/4 lanes of its columns, and the next tokens' operands are loaded
@@ -91,9 +95,13 @@ __global__ __launch_bounds__(CW / 4 * 16) void decode_step_kernel(DecodeArgs a) 
   const size_t sp = ((size_t)from * a.H + hi) * D * D;
 
   float4 h[KPK];
+  if (a.state_in && from >= 0) {      // (one branch for all the loads, which then are in flight together)
 #pragma unroll
-  for (int i = 0; i < KPK; ++i)
-    h[i] = a.state_in && from >= 0 ? ld_quad<SBF>(a.state_in, sp + (size_t)(d0 + i) * D + j0) : make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = 0; i < KPK; ++i) h[i] = ld_quad<SBF>(a.state_in, sp + (size_t)(d0 + i) * D + j0);
+  } else {
+#pragma unroll
+    for (int i = 0; i < KPK; ++i) h[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
 
   const size_t io = (size_t)bh * a.seq_ld * D;
   // this thread's columns of w and v, issued with the key vectors' loads (one round trip)
@@ -354,7 +362,7 @@ void launch_decode_t(const DecodeArgs& a, int n_bh, hipStream_t s) {
     constexpr int CWV = 1024 / D, NWV = CAP ? D / CWV : 32 / CWV;       // columns of a wave, waves
     hipLaunchKernelGGL((decode_tail_kernel<D, NWV, CAP, IBF, SBF>), dim3(n_bh * (D / (CWV * NWV))), dim3(NWV * WAVE), 0, s, a);
   } else {
-    constexpr int CW = CAP ? D : 32;
+    constexpr int CW = CAP ? D : SBF ? 64 : 32;                         // whole lines
     hipLaunchKernelGGL((decode_step_kernel<D, CW, CAP, IBF, SBF>), dim3(n_bh * (D / CW)), dim3(CW / 4 * 16), 0, s, a);
   }
 }

@@ -368,3 +368,129 @@ def test_premix_step_refusals():
         go(ps=ps[:3] + [ps[3][:0]] + ps[4:], parents=par)
     with pytest.raises(ValueError, match="is on cpu"):
         go(parents=par.cpu())
+
+
+# ---------------------------------------------------------------- the LM
+def _small_lm(seed=0, **kw):
+    from atomic_gdn2 import e2e_lm
+    cfg = e2e_lm.LMConfig(**{**dict(vocab_size=61, d_model=128, n_heads=2, d_head=64, n_layers=2), **kw})
+    model = e2e_lm.make_lm(cfg, seed=seed)
+    with torch.no_grad():       # logits that are not all alike, gates and biases that are not all zero
+        gen = torch.Generator().manual_seed(seed + 1)
+        model.embed.mul_(4.0)
+        for n, p in model.named_parameters():
+            if n.endswith(("bias", "decay_a")) or "conv" in n:
+                p.add_(torch.randn(p.shape, generator=gen).to(p) * 0.3)
+    return model
+
+
+def _lm64(model, group):
+    """The LM of the rounded weights in float64 on the CPU, its recurrence token by token."""
+    from atomic_gdn2 import e2e_lm
+    from atomic_gdn2.w4 import quantize_w4
+
+    def rounded(*ws):
+        full = quantize_w4(torch.cat([w.detach() for w in ws], 1), group).dequantize().double().cpu()
+        return full.split([w.shape[1] for w in ws], 1)
+
+    def mixer(q, k, v, w, b, g):                       # (B, L, H, D)
+        B, L, H, D = q.shape
+        h, os_ = torch.zeros((B, H, D, D), dtype=q.dtype), []
+        for t in range(L):
+            h = h * torch.exp(g[:, t])[..., None]
+            new = w[:, t] * v[:, t] - ((b[:, t] * k[:, t])[..., None] * h).sum(-2)
+            h = h + k[:, t][..., None] * new[..., None, :]
+            os_.append((h * q[:, t][..., None]).sum(-2) * D ** -0.5)
+        return torch.stack(os_, 1)
+
+    c = model.cfg
+    ref = e2e_lm.LM(c, mixer).double()
+    ref.load_state_dict({n: p.double().cpu() for n, p in model.state_dict().items()})
+    pad = torch.zeros((c.d_model, -(6 * c.proj_dim + c.n_heads) % 4), device="cuda")
+    with torch.no_grad():
+        for b, r in zip(model.blocks, ref.blocks):
+            names = ("q_proj", "k_proj", "v_proj", "erase_gate", "write_gate", "out_gate", "decay_proj")
+            for n, w in zip(names, rounded(*(getattr(b, n).weight for n in names), pad)):
+                getattr(r, n).weight.copy_(w)
+            for names in (("out_proj",), ("gate_proj", "up_proj"), ("down_proj",)):
+                for n, w in zip(names, rounded(*(getattr(b, n).weight for n in names))):
+                    getattr(r, n).weight.copy_(w)
+    head = rounded(model.embed.t())[0]
+
+    def logits(ids):
+        x = ref.embed[ids]
+        for blk in ref.blocks:
+            x = blk(x)
+        return (ref.final_norm(x) @ head).detach()
+    return logits
+
+
+@pytest.mark.parametrize("L", [1, 2, 5, 64, 70])
+def test_prefill_and_steps_are_the_language_model(L):
+    """Logits of a prompt and of the tokens after it, from caches, against the whole sequence at once.
+    Bound: float32 through two blocks, 2e-4 of the largest logit (the operator's own gate is 2e-3)."""
+    from atomic_gdn2.generation import Generator
+    model = _small_lm()
+    gen, ref = Generator(model, group_size=32), _lm64(model, 32)
+    ids = torch.randint(0, 61, (3, L + 6), generator=torch.Generator().manual_seed(L))
+    want = ref(ids)
+    logits, cache = gen.prefill(ids[:, :L].cuda())
+    tol = 2e-4 * float(want.abs().max())
+    assert float((logits.cpu().double() - want[:, L - 1]).abs().max()) <= tol
+    order = torch.tensor([0, 1, 2])
+    for t in range(L, L + 6):
+        perm = torch.randperm(3, generator=torch.Generator().manual_seed(t))         # rows change their places
+        order = order[perm]
+        logits, cache = gen.step(ids[order, t].cuda(), cache, perm.cuda())
+        assert float((logits.cpu().double() - want[order, t]).abs().max()) <= tol, t
+
+
+@pytest.mark.parametrize("eos", [None, 7])
+def test_beam_search_is_the_search_over_whole_sequences(eos):
+    """Against a search that scores every continuation of every beam by the whole sequence in float64."""
+    from atomic_gdn2.generation import Generator
+    model = _small_lm(seed=3)
+    gen, ref = Generator(model, group_size=32), _lm64(model, 32)
+    B, L, n, T, V = 2, 9, 3, 12, 61
+    ids = torch.randint(0, V, (B, L), generator=torch.Generator().manual_seed(11))
+    r = gen.beam_search(ids.cuda(), n, T, eos_id=eos)
+    assert r.tokens.shape == (B, n, T) and r.scores.shape == (B, n)
+    for b in range(B):
+        beams = [((), 0.0, False)]
+        gap = math.inf
+        for _ in range(T):
+            cand = []
+            for seq, score, done in beams:
+                if done:
+                    cand.append((score, seq + (eos,), True))
+                    continue
+                lp = torch.log_softmax(ref(torch.cat([ids[b], torch.tensor(seq, dtype=torch.long)])[None])[0, -1], -1)
+                cand += [(score + float(lp[v]), seq + (v,), eos is not None and v == eos) for v in range(V)]
+            cand.sort(key=lambda c: -c[0])
+            gap = min([gap] + [x[0] - y[0] for x, y in zip(cand[:n], cand[1:n + 1])])
+            beams = [(seq, score, done) for score, seq, done in cand[:n]]
+        print(f"[gpu-test] smallest gap between candidates {gap:.2g}", flush=True)
+        assert gap > 1e-4, "choose another seed: the reference's own order is in doubt"
+        assert [tuple(x) for x in r.tokens[b].tolist()] == [s for s, _, _ in beams]
+        assert torch.allclose(r.scores[b].cpu().double(), torch.tensor([s for _, s, _ in beams], dtype=torch.float64), atol=2e-3)
+    if eos is not None:
+        ended = (r.tokens == eos).cummax(-1).values
+        assert bool(((r.tokens == eos) == ended).all())
+
+
+def test_generator_refusals():
+    from atomic_gdn2.generation import Generator
+    with pytest.raises(ValueError, match="d_head"):
+        Generator(_small_lm(d_head=32))
+    with pytest.raises(ValueError, match="ROCm device"):
+        Generator(_small_lm().cpu())
+    gen = Generator(_small_lm())
+    ids = torch.zeros((1, 4), dtype=torch.int64, device="cuda")
+    with pytest.raises(ValueError, match="token ids"):
+        gen.prefill(ids[0])
+    with pytest.raises(ValueError, match="token ids"):
+        gen.prefill(ids[:, :0])
+    with pytest.raises(ValueError, match="token ids are on cpu"):
+        gen.prefill(ids.cpu())
+    with pytest.raises(ValueError, match="max_new_tokens"):
+        gen.beam_search(ids, 2, 0)
