@@ -478,6 +478,20 @@ def test_beam_search_is_the_search_over_whole_sequences(eos):
         assert bool(((r.tokens == eos) == ended).all())
 
 
+@pytest.mark.parametrize("eos", [None, 7])
+def test_beam_search_by_graph_replays_gives_the_same(eos):
+    """Every replay works on the caches that the one before left; the searches run eager work and
+    synchronise between them."""
+    from atomic_gdn2.generation import Generator
+    gen = Generator(_small_lm(seed=3), group_size=32)
+    for seed, (B, n, T) in enumerate(((2, 3, 30), (1, 1, 5), (3, 4, 2), (2, 8, 20))):
+        ids = torch.randint(0, 61, (B, 9), generator=torch.Generator().manual_seed(seed)).cuda()
+        a = gen.beam_search(ids, n, T, eos_id=eos, graph=True)
+        torch.cuda.synchronize()
+        b = gen.beam_search(ids, n, T, eos_id=eos, graph=False)
+        assert torch.equal(a.tokens, b.tokens) and torch.equal(a.scores, b.scores)
+
+
 def test_generator_refusals():
     from atomic_gdn2.generation import Generator
     with pytest.raises(ValueError, match="d_head"):
