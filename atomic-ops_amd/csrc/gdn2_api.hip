@@ -847,14 +847,14 @@ int w4_args(const gdn2_w4* p, gdn2::W4Args* a) {
 
 size_t gdn2_w4_workspace_bytes(const gdn2_w4* p) {
   gdn2::W4Args a{};
-  return w4_args(p, &a) ? 0 : gdn2::w4_workspace_bytes(p->dtype, a);
+  return w4_args(p, &a) ? 0 : gdn2::w4_workspace_bytes(p->dtype, p->group, a);
 }
 
 int gdn2_w4_linear(const gdn2_w4* p, void* workspace, void* stream) {
   gdn2::W4Args a{};
   const int st = w4_args(p, &a);
   if (st) return st;
-  if (!aligned16({workspace}) || (!workspace && gdn2::w4_workspace_bytes(p->dtype, a)))
+  if (!aligned16({workspace}) || (!workspace && gdn2::w4_workspace_bytes(p->dtype, p->group, a)))
     return fail(GDN2_ERR_INVALID, "null workspace, or not 16-byte aligned");
   a.part = static_cast<float*>(workspace);
   return lm_done(gdn2::launch_w4(p->dtype, p->group, a, reinterpret_cast<hipStream_t>(stream)), "w4 launch");

@@ -412,7 +412,7 @@ struct W4Args {
   int vec;                     // whole 16-byte accesses of x: alignment, ldx and K allow them
   int wide;                    // four columns at a time of y, bias and res
 };
-size_t w4_workspace_bytes(int dtype, const W4Args& a);
+size_t w4_workspace_bytes(int dtype, int group, const W4Args& a);
 hipError_t launch_w4(int dtype, int group, const W4Args& a, hipStream_t s);
 
 // Beam search's selection (gdn2_beam.hip).  logits (B K, V) rows of ld elements; part: per row and split

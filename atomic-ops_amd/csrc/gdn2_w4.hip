@@ -9,6 +9,7 @@
 // Activations of 16 bits are the other operand as they are, of float32 as three bfloat16 pieces of
 // eight bits each, whose sum is x.  So no product is rounded; sums, group sums of x and the scaling
 // are float32, and y is rounded once.
+#include <stdlib.h>
 #include "gdn2_kernels.hpp"
 
 namespace gdn2 {
@@ -23,6 +24,23 @@ template <bool F16>
 __device__ __forceinline__ void w4_mfma_first(f4& acc, const s8& a, const s8& b) {      // acc = a b
   if constexpr (F16) asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_f16 %0, %1, %2, 0" : "=&v"(acc) : "v"(a), "v"(b));
   else asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %2, 0" : "=&v"(acc) : "v"(a), "v"(b));
+}
+
+// Four products with one left operand; FIRST: results, else added to.
+template <bool F16, bool FIRST>
+__device__ __forceinline__ void w4_mfma4(f4& a0, f4& a1, f4& a2, f4& a3, const s8& x, const s8& b0, const s8& b1, const s8& b2, const s8& b3) {
+#define W4_FOUR(op, c0, c1, c2, c3)                                            \
+  "s_nop 1\n\t" op " %0, %4, %5, " c0 "\n\t" op " %1, %4, %6, " c1 "\n\t" op \
+  " %2, %4, %7, " c2 "\n\t" op " %3, %4, %8, " c3
+  if constexpr (FIRST && F16)
+    asm volatile(W4_FOUR("v_mfma_f32_16x16x32_f16", "0", "0", "0", "0") : "=&v"(a0), "=&v"(a1), "=&v"(a2), "=&v"(a3) : "v"(x), "v"(b0), "v"(b1), "v"(b2), "v"(b3));
+  else if constexpr (FIRST)
+    asm volatile(W4_FOUR("v_mfma_f32_16x16x32_bf16", "0", "0", "0", "0") : "=&v"(a0), "=&v"(a1), "=&v"(a2), "=&v"(a3) : "v"(x), "v"(b0), "v"(b1), "v"(b2), "v"(b3));
+  else if constexpr (F16)
+    asm volatile(W4_FOUR("v_mfma_f32_16x16x32_f16", "%0", "%1", "%2", "%3") : "+v"(a0), "+v"(a1), "+v"(a2), "+v"(a3) : "v"(x), "v"(b0), "v"(b1), "v"(b2), "v"(b3));
+  else
+    asm volatile(W4_FOUR("v_mfma_f32_16x16x32_bf16", "%0", "%1", "%2", "%3") : "+v"(a0), "+v"(a1), "+v"(a2), "+v"(a3) : "v"(x), "v"(b0), "v"(b1), "v"(b2), "v"(b3));
+#undef W4_FOUR
 }
 
 // Eight nibbles as operands: element e of 0 .. 3 is nibble 2 e, of 4 .. 7 nibble 2 (e - 4) + 1.
@@ -125,11 +143,18 @@ __device__ __forceinline__ W4Raw<XT> w4_load_odd(const W4Args& a, int m, int k) 
 // ... and by buffer loads from base + off: an offset past the buffer's end reads zero, without a branch
 constexpr uint32_t W4_OUT = 0x60000000u;             // above any offset of a buffer (at most 2^30)
 typedef unsigned u4v __attribute__((ext_vector_type(4)));
+// (a buffer that the compiler does not know to be uniform costs a loop over the lanes at every load)
+__device__ __forceinline__ int w4_uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t w4_buffer(const void* p, size_t at, int64_t bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(p)) + at, 0, (int)bytes, 0x00027000);
+  const uint64_t u = reinterpret_cast<uint64_t>(p) + at;
+  const uint64_t base = (uint64_t)(uint32_t)w4_uniform((int)(u >> 32)) << 32 | (uint32_t)w4_uniform((int)u);
+  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(base), 0, w4_uniform((int)bytes), 0x00027000);
 }
 __device__ __forceinline__ uint4 w4_buffer16(__amdgpu_buffer_rsrc_t b, uint32_t off, int uniform) {
-  return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(b, (int)off, uniform, 0));
+  return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(b, (int)off, w4_uniform(uniform), 0));
+}
+__device__ __forceinline__ uint32_t w4_buffer4(__amdgpu_buffer_rsrc_t b, uint32_t off, int uniform) {
+  return __builtin_amdgcn_raw_buffer_load_b32(b, (int)off, w4_uniform(uniform), 0);
 }
 
 template <int XT>
@@ -266,7 +291,7 @@ __global__ __launch_bounds__(w4_waves(XT, NB) * WAVE) void w4_rows_kernel(W4Args
       o.q[i] = w4_buffer16(qb, qoff[i], kb * 1024);
 #pragma unroll
       for (int g = 0; g < NG; ++g)
-        o.sz[i][g] = __builtin_amdgcn_raw_buffer_load_b32(sb, (int)(soff[i] + 64 * g), kb * (NG * 64), 0);
+        o.sz[i][g] = w4_buffer4(sb, soff[i] + 64 * g, kb * (NG * 64));
     }
     if (!a.vec) {
 #pragma unroll
@@ -435,7 +460,7 @@ __global__ __launch_bounds__(C::W * WAVE) void w4_tile_kernel(W4Args a) {
       o.q[i] = w4_buffer16(qb, i * a.nkb * 1024 + 16 * l, kw * 1024);
 #pragma unroll
       for (int g = 0; g < NG; ++g)
-        o.sz[i][g] = __builtin_amdgcn_raw_buffer_load_b32(sb, i * a.nkb * (NG * 64) + 64 * g + 4 * r, kw * (NG * 64), 0);
+        o.sz[i][g] = w4_buffer4(sb, i * a.nkb * (NG * 64) + 64 * g + 4 * r, kw * (NG * 64));
     }
     __builtin_amdgcn_sched_barrier(0);               // issued here, not where they are used
   };
@@ -511,7 +536,7 @@ __global__ __launch_bounds__(C::W * WAVE) void w4_tile_kernel(W4Args a) {
               else w4_mfma<F16>(acc[i][t], xt, op[i]);
             }
             if (at + AHEAD < STEPS) x[at % AHEAD] = read(at + AHEAD);
-            __builtin_amdgcn_sched_barrier(0x3ff & ~0x300);      // (reads of LDS stay where they are)
+            __builtin_amdgcn_sched_barrier(0x7f);    // (reads of LDS stay where they are)
           }
       }
       auto sum = [&](int t) __attribute__((always_inline)) { return *reinterpret_cast<const f4*>(sums(buf, u0 + t, g) + 4 * c); };
@@ -607,6 +632,238 @@ __global__ __launch_bounds__(256) void w4_join_kernel(W4Args a, int parts) {
   w4_out4<XT>(a, m, n, v);
 }
 
+// Many rows: bound by the matrix cores and by what the operands cost beside them, so nothing else is left in
+// the loop.  A pass over x first (w4_prep_kernel) writes the groups' sums of x as operands, three
+// bfloat16 pieces each, and where x's own rows cannot be read as they are (float32, odd strides, a last
+// block that ends early) its 16-bit pieces as rows of whole blocks.  Then a workgroup of eight waves takes
+// BM rows and 256 columns, a wave 16 MT rows and 64 columns: x comes into LDS by DMA, a block ahead of
+// its use, the scale is one fma a group and result, and the zeros are a product of their own behind the
+// sum, (sums of x) x (-s z) over the groups, 32 groups a step: s z has 16 bits, two pieces.
+template <int XT_, int GROUP_>
+struct W4Gemm {
+  static constexpr int XT = XT_, GROUP = GROUP_, NP = W4Frag<XT>::NP;
+  static constexpr int WM = 2, WN = 4, MT = XT == W4_F32 ? 2 : 4, NBW = 4;
+  static constexpr int BM = 16 * MT * WM, BN = 16 * NBW * WN, LDO = BN + 4;
+  // a block's x, codes and scales in LDS, NBUF blocks in turn (float32: as many as fit)
+  static constexpr int NBUF = XT == W4_F32 ? 2 : 3, NG = W4_KB / GROUP;
+  static constexpr int XB = NP * BM * W4_KB * 2, QB = BN / 16 * 1024, BUF = XB + QB + NG * 1024;
+  static constexpr int LDS = NBUF * BUF > BM * LDO * 4 ? NBUF * BUF : BM * LDO * 4;
+};
+struct W4GemmArgs {
+  const uint16_t *x, *sums;     // NP planes of rows of ld elements; w4_sums_bytes
+  size_t ld, plane;
+  int ngb;                      // steps of 32 groups
+};
+
+// A wave a row: sums of the groups, and with planes (x's 16-bit pieces, Kp columns, zero past K)
+template <int XT, int GROUP>
+__global__ __launch_bounds__(256) void w4_prep_kernel(W4Args a, uint16_t* planes, uint16_t* sums, int ngb) {
+  constexpr int NP = W4Frag<XT>::NP, LG = GROUP / 8;          // lanes of a group
+  const int l = lane_id(), m = blockIdx.x * 4 + wave_id(), Kp = a.nkb * W4_KB, mt = (a.M + 15) / 16;
+  if (m >= a.M) return;
+  for (int k = 8 * (l + WAVE * (int)blockIdx.y); k < ngb * 32 * GROUP; k += 8 * WAVE * gridDim.y) {
+    W4Raw<XT> x;
+    if (a.vec && k < a.K) {
+      const uint4* p = reinterpret_cast<const uint4*>(static_cast<const char*>(a.x) + ((size_t)m * a.ldx + k) * (XT == W4_F32 ? 4 : 2));
+#pragma unroll
+      for (int v = 0; v < W4Raw<XT>::NV; ++v) x.v[v] = p[v];
+    } else {
+      x = w4_load_odd<XT>(a, k < a.K ? m : a.M, k);
+    }
+    if (planes && k < Kp) {
+      const W4Frag<XT> f = w4_frag<XT>(x);
+#pragma unroll
+      for (int p = 0; p < NP; ++p)                   // (the largest piece last, as in W4Frag)
+        *reinterpret_cast<uint4*>(planes + ((size_t)p * a.M + m) * Kp + k) = __builtin_bit_cast(uint4, f.p[p]);
+    }
+    float s = w4_quad_sum(w4_sum8<XT>(x));
+    if constexpr (LG >= 8) s += w4_dpp<0x141>(s);    // the other quad of eight lanes,
+    if constexpr (LG >= 16) s += w4_dpp<0x128>(s);   // the other eight of sixteen
+    if (l % LG == 0) {
+      const int g = k / GROUP, gb = g / 32, gi = g % 32;
+      const float h = w4_top(s), r = s - h;
+      const uint32_t piece[3] = {__float_as_uint(r - w4_top(r)), __float_as_uint(r), __float_as_uint(h)};
+#pragma unroll
+      for (int p = 0; p < 3; ++p)
+        sums[(((size_t)p * mt + m / 16) * ngb + gb) * 512 + (m % 16 + 16 * (gi / 8)) * 8 + gi % 8] = (uint16_t)(piece[p] >> 16);
+    }
+  }
+}
+
+template <class C>
+__global__ __launch_bounds__(512) void w4_gemm_kernel(W4Args a, W4GemmArgs b) {
+  constexpr int XT = C::XT, GROUP = C::GROUP, MT = C::MT, NBW = C::NBW, WN = C::WN, NP = C::NP;
+  constexpr bool F16 = XT == W4_F16;
+  constexpr int NG = C::NG, SG = GROUP / 32, RO = C::BM / 8, DMA = NP * RO * 2 / 8;     // octets of rows, a wave's DMAs of x
+  extern __shared__ char lds[];
+  const int l = lane_id(), r = l & 15, c = l >> 4, w = wave_id(), wm = w / WN, wn = w % WN;
+  const int tb0 = blockIdx.x * (C::BN / 16), nb0 = tb0 + wn * NBW, m0 = blockIdx.y * C::BM;
+  // A KB of x in LDS holds eight rows' 64 k: lane l's sixteen bytes are row l / 8's chunk (l % 8) ^ (l / 8), so
+  // that rows come as whole lines and a wave's reads of an operand meet no bank twice.  (Rows and columns
+  // past the last: the last again, and not looked at.)
+  const char *src[DMA], *qsrc[2];
+#pragma unroll
+  for (int i = 0; i < DMA; ++i) {
+    const int u = w * DMA + i, p = u / (2 * RO), ro = u / 2 % RO, h = u % 2;
+    const int m = min(m0 + 8 * ro + (l >> 3), a.M - 1);
+    src[i] = reinterpret_cast<const char*>(b.x + p * b.plane + (size_t)m * b.ld + 64 * h + 8 * ((l & 7) ^ (l >> 3)));
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    qsrc[i] = reinterpret_cast<const char*>(a.q) + (size_t)min(tb0 + 2 * w + i, a.nnb - 1) * a.nkb * 1024 + 16 * l;
+  // (sixteen columns' words of a group are 64 bytes; a wave fetches group w % NG of the block)
+  const char* ssrc = reinterpret_cast<const char*>(a.meta) +
+                     ((size_t)min(tb0 + (l >> 2), a.nnb - 1) * a.nkb * NG + w % NG) * 64 + 16 * (l & 3);
+  auto dma = [&](const char* from, int to) __attribute__((always_inline)) {
+    lds_dma16(reinterpret_cast<const float*>(from), reinterpret_cast<float*>(lds + to));
+  };
+  constexpr int DMAS = DMA + 3;
+  auto fetch = [&](int kb, int buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < DMA; ++i) dma(src[i] + (size_t)kb * (2 * W4_KB), buf + (w * DMA + i) * 1024);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) dma(qsrc[i] + (size_t)kb * 1024, buf + C::XB + (2 * w + i) * 1024);
+    dma(ssrc + (size_t)kb * (NG * 64), buf + C::XB + C::QB + w % NG * 1024);
+  };
+  f4 tot[NBW][MT];
+#pragma unroll
+  for (int i = 0; i < NBW; ++i)
+#pragma unroll
+    for (int t = 0; t < MT; ++t) tot[i][t] = f4{0.f, 0.f, 0.f, 0.f};
+  // where the lane's operands lie in a KB, for the steps 0 | 2 and 1 | 3
+  const int at0 = (r & 7) * 128 + (c ^ (r & 7)) * 16, at1 = (r & 7) * 128 + ((c + 4) ^ (r & 7)) * 16;
+  auto add = [&](int buf) __attribute__((always_inline)) {
+    constexpr int STEPS = 4 * NP * MT, AHEAD = 2;
+    static_assert(NBW == 4 && NP * MT >= NBW, "a step of the sum leaves room for the next one's operands");
+    auto read = [&](int i) __attribute__((always_inline)) {
+      const int t = i % MT, p = i / MT % NP, j = i / (MT * NP);
+      return *reinterpret_cast<const s8*>(lds + buf + ((p * RO + 2 * (wm * MT + t) + (r >> 3)) * 2 + j / 2) * 1024 + (j & 1 ? at1 : at0));
+    };
+    uint4 q[NBW];
+#pragma unroll
+    for (int i = 0; i < NBW; ++i) q[i] = *reinterpret_cast<const uint4*>(lds + buf + C::XB + (wn * NBW + i) * 1024 + 16 * l);
+    auto word = [&](int i, int j) __attribute__((always_inline)) {
+      return w4_operand<F16>(j == 0 ? q[i].x : j == 1 ? q[i].y : j == 2 ? q[i].z : q[i].w);
+    };
+    s8 x[AHEAD], op[2][NBW];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) x[i] = read(i);
+#pragma unroll
+    for (int i = 0; i < NBW; ++i) op[0][i] = word(i, 0);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      f4 acc[NBW][MT];
+#pragma unroll
+      for (int s = 0; s < SG; ++s) {
+        const int j = g * SG + s;
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            const int i = p * MT + t, at = j * NP * MT + i;
+            const s8 xt = x[at % AHEAD];
+            const s8* w4 = op[j % 2];
+            if (s == 0 && p == 0) w4_mfma4<F16, true>(acc[0][t], acc[1][t], acc[2][t], acc[3][t], xt, w4[0], w4[1], w4[2], w4[3]);
+            else w4_mfma4<F16, false>(acc[0][t], acc[1][t], acc[2][t], acc[3][t], xt, w4[0], w4[1], w4[2], w4[3]);
+            // beside the products: the operands of the next step of the sum, one column block's at a time
+            if (at + AHEAD < STEPS) x[at % AHEAD] = read(at + AHEAD);
+            if (j < 3 && i < NBW) op[(j + 1) % 2][i] = word(i, j + 1);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+      }
+      drain(acc[0][0]);
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int i = 0; i < NBW; ++i) w4_hold(acc[i][t]);
+#pragma unroll
+      for (int i = 0; i < NBW; ++i) {
+        const float s = __uint_as_float(*reinterpret_cast<const uint32_t*>(lds + buf + C::XB + C::QB + g * 1024 + (wn * NBW + i) * 64 + 4 * r) << 16);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) tot[i][t][e] = fmaf(s, acc[i][t][e], tot[i][t][e]);
+          w4_hold(tot[i][t]);
+        }
+      }
+    }
+  };
+  // Block kb has come when only the DMAs of the NBUF - 2 behind it are under way; then everyone's has.  (Past
+  // the end the last block again, so that the counts stay the same.)
+  constexpr int BEHIND = (C::NBUF - 2) * DMAS;
+  static_assert(BEHIND < 16, "vmcnt's low bits");
+  const int last = a.nkb - 1;
+  int buf = 0, into = (C::NBUF - 1) * C::BUF;
+  auto next = [&](int x) { return x == (C::NBUF - 1) * C::BUF ? 0 : x + C::BUF; };
+#pragma unroll
+  for (int i = 0; i < C::NBUF - 1; ++i) fetch(min(i, last), i * C::BUF);
+  for (int kb = 0; kb <= last; ++kb) {
+    __builtin_amdgcn_s_waitcnt(WAIT_VMCNT0 | BEHIND);
+    __syncthreads();
+    fetch(min(kb + C::NBUF - 1, last), into);
+    add(buf);
+    buf = next(buf);
+    into = next(into);
+  }
+  __builtin_amdgcn_s_waitcnt(WAIT_VMCNT0);           // (LDS is used again below)
+  // the zeros
+  const int mtiles = (a.M + 15) / 16, nbs = max(0, min(NBW, a.nnb - nb0));
+  const __amdgpu_buffer_rsrc_t sb = w4_buffer(a.meta, (size_t)(nbs ? nb0 : 0) * a.nkb * (NG * 64), (int64_t)nbs * a.nkb * (NG * 64));
+  for (int gb = 0; gb < b.ngb; ++gb) {
+    s8 z[NBW][2];
+#pragma unroll
+    for (int i = 0; i < NBW; ++i) {
+      uint32_t lo[8], hi[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        // (groups past the last: meta ends at the columns' last block, and may go on with the next columns')
+        const int g = gb * 32 + 8 * c + e;
+        const uint32_t off = g < a.nkb * NG ? (uint32_t)((i * a.nkb * NG + g) * 64 + 4 * r) : W4_OUT;
+        const uint32_t sz = w4_buffer4(sb, off, 0);
+        const float v = -(bf16_val(sz & 0xffffu) * __uint_as_float(sz & 0xffff0000u));
+        hi[e] = __float_as_uint(v) >> 16;
+        lo[e] = __float_as_uint(v - w4_top(v)) >> 16;
+      }
+      z[i][0] = __builtin_bit_cast(s8, make_uint4(lo[0] | lo[1] << 16, lo[2] | lo[3] << 16, lo[4] | lo[5] << 16, lo[6] | lo[7] << 16));
+      z[i][1] = __builtin_bit_cast(s8, make_uint4(hi[0] | hi[1] << 16, hi[2] | hi[3] << 16, hi[4] | hi[5] << 16, hi[6] | hi[7] << 16));
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      const size_t mt = min(m0 / 16 + wm * MT + t, mtiles - 1);
+#pragma unroll
+      for (int p = 0; p < 3; ++p) {
+        const s8 x = *reinterpret_cast<const s8*>(b.sums + (((size_t)p * mtiles + mt) * b.ngb + gb) * 512 + 8 * l);
+#pragma unroll
+        for (int i = 0; i < NBW; ++i) {
+          w4_mfma<false>(tot[i][t], x, z[i][0]);
+          w4_mfma<false>(tot[i][t], x, z[i][1]);
+        }
+      }
+    }
+  }
+  drain(tot[0][0]);
+#pragma unroll
+  for (int i = 0; i < NBW; ++i)
+#pragma unroll
+    for (int t = 0; t < MT; ++t) w4_hold(tot[i][t]);
+  // results through LDS, so that whole lines are written
+  float* out = reinterpret_cast<float*>(lds);
+  __syncthreads();
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int i = 0; i < NBW; ++i) out[(16 * (wm * MT + t) + 4 * c + e) * C::LDO + 16 * (wn * NBW + i) + r] = tot[i][t][e];
+  __syncthreads();
+  const int n0 = blockIdx.x * C::BN, rows = min(C::BM, a.M - m0);
+  for (int x = threadIdx.x; x < C::BM * C::BN / 4; x += 512) {
+    const int row = x / (C::BN / 4), col = 4 * (x % (C::BN / 4)), n = n0 + col;
+    if (row >= rows || n >= a.N) continue;
+    w4_out4<XT>(a, m0 + row, n, *reinterpret_cast<const float4*>(out + row * C::LDO + col));
+  }
+}
+
 // How a product runs: parts 0: rows; else tiles, the sum in parts.
 //   rows: one launch, x and (over 16 rows) the weights read again by each tile of rows.  Up to 8 rows
 //     always; more where the weights come from the caches again, 2^15 tiles of 16 rows and 128 x 16
@@ -618,10 +875,16 @@ __global__ __launch_bounds__(256) void w4_join_kernel(W4Args a, int parts) {
 //     4096 x 4096, 1 / 2: 21.8, 23.5).
 template <int XT, int GROUP>
 using W4Tiles = W4Tile<XT, GROUP, 2, 2, 1, 4, 2>;
+// (parts -1) many rows: workgroups of w4_gemm_kernel for most of the chip.
+static bool w4_many(int M, int nnb) {
+  static const int many = getenv("W4MANY") ? atoi(getenv("W4MANY")) : 128;
+  return (int64_t)((M + 127) / 128) * ((nnb + 15) / 16) >= many;
+}
 static int w4_parts(int M, int nkb, int nnb) {
   using C = W4Tiles<W4_BF16, 128>;
   if (M <= 8 || (nkb <= 64 && (int64_t)nkb * nnb * ((M + 15) / 16) <= 32768)) return 0;
   const int64_t tiles = (int64_t)((16 * nnb + C::BN - 1) / C::BN) * ((M + C::BM - 1) / C::BM), cus = cu_count();
+  if (w4_many(M, nnb)) return -1;
   const int64_t two = 2 * cus / tiles, one = cus / tiles;
   const int64_t p = two >= 1 && nkb / two >= 14 ? two : one < nkb / 4 ? one : nkb / 4;
   return p < 1 ? 1 : (int)p;
@@ -630,8 +893,14 @@ static int w4_parts(int M, int nkb, int nnb) {
 static size_t w4_align_bytes(int dtype, const W4Args& a) {
   return a.vec ? 0 : ((size_t)a.M * ((a.K + 7) / 8 * 8) * (dtype == W4_F32 ? 4 : 2) + 255) / 256 * 256;
 }
-size_t w4_workspace_bytes(int dtype, const W4Args& a) {
+static int w4_ngb(int group, const W4Args& a) { return (a.nkb * (W4_KB / group) + 31) / 32; }
+static size_t w4_sums_bytes(int group, const W4Args& a) { return (size_t)3 * ((a.M + 15) / 16) * w4_ngb(group, a) * 1024; }
+// whether w4_gemm_kernel can read x's own rows
+static bool w4_direct(int dtype, const W4Args& a) { return dtype != W4_F32 && a.vec && a.K % W4_KB == 0; }
+size_t w4_workspace_bytes(int dtype, int group, const W4Args& a) {
   const int parts = w4_parts(a.M, a.nkb, a.nnb);
+  if (parts < 0)
+    return w4_sums_bytes(group, a) + (w4_direct(dtype, a) ? 0 : (size_t)(dtype == W4_F32 ? 3 : 1) * a.M * a.nkb * W4_KB * 2);
   return parts ? w4_align_bytes(dtype, a) + (parts > 1 ? (size_t)parts * a.M * a.N * 4 : 0) : 0;
 }
 
@@ -653,6 +922,20 @@ static void w4_go(W4Args a, hipStream_t s) {
     if (a.M <= 4) two ? w4_rows<XT, GROUP, 4, 2>(a, s) : w4_rows<XT, GROUP, 4, 1>(a, s);
     else if (a.M <= 8) two ? w4_rows<XT, GROUP, 2, 2>(a, s) : w4_rows<XT, GROUP, 2, 1>(a, s);
     else two ? w4_rows<XT, GROUP, 1, 2>(a, s) : w4_rows<XT, GROUP, 1, 1>(a, s);
+    return;
+  }
+  if (parts < 0) {
+    using C = W4Gemm<XT, GROUP>;
+    W4GemmArgs b{};
+    b.ngb = w4_ngb(GROUP, a);
+    uint16_t* sums = reinterpret_cast<uint16_t*>(a.part);
+    uint16_t* planes = w4_direct(XT, a) ? nullptr : sums + w4_sums_bytes(GROUP, a) / 2;
+    b.sums = sums;
+    b.x = planes ? planes : static_cast<const uint16_t*>(a.x);
+    b.ld = planes ? (size_t)a.nkb * W4_KB : a.ldx;
+    b.plane = (size_t)a.M * b.ld;
+    hipLaunchKernelGGL((w4_prep_kernel<XT, GROUP>), dim3((a.M + 3) / 4, (b.ngb * GROUP + 31) / 32), dim3(256), 0, s, a, planes, sums, b.ngb);
+    hipLaunchKernelGGL((w4_gemm_kernel<C>), dim3((a.N + C::BN - 1) / C::BN, (a.M + C::BM - 1) / C::BM), dim3(512), C::LDS, s, a, b);
     return;
   }
   if (!a.vec) {
