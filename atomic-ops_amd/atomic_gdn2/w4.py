@@ -153,7 +153,8 @@ def w4_linear(x, weight: W4Weight, bias=None, residual=None):
     """y = x W (+ bias) (+ residual): x (..., in) float32, bfloat16 or float16, y (..., out) in x's dtype.
 
     bias (out,) and residual (..., out) are cast to x's dtype.  Rows may be strided (a slice of wider
-    rows); sums are float32.  A row of x that holds an infinity or NaN gives NaN."""
+    rows); sums are float32 (16 K max |x| has to fit).  A row of x that holds an infinity or NaN gives
+    nothing finite, and touches no other row."""
     if type(weight) is W4Weight and isinstance(x, torch.Tensor) and x.is_cuda:
         # plain calls (csrc/bind.cpp) go native; None = not one, and what follows handles it
         y = _lib.bind().w4(x, weight.q, weight.meta, weight.in_features, weight.out_features, weight.group_size, bias, residual)

@@ -823,7 +823,7 @@ int w4_args(const gdn2_w4* p, gdn2::W4Args* a) {
   if (!p) return fail(GDN2_ERR_INVALID, "null argument block");
   if (p->M < 1 || p->K < 1 || p->N < 1) return fail(GDN2_ERR_INVALID, "non-positive shape");
   if (p->dtype < GDN2_F32 || p->dtype > GDN2_F16) return fail(GDN2_ERR_INVALID, "unknown dtype");
-  if (p->M > (1 << 20) || p->K > (1 << 24) || p->N > (1 << 24)) return fail(GDN2_ERR_UNSUPPORTED, "shape too large");
+  if (p->M > (1 << 20) || p->K > (1 << 20) || p->N > (1 << 24)) return fail(GDN2_ERR_UNSUPPORTED, "shape too large");
   if (p->group != 32 && p->group != 64 && p->group != 128) return fail(GDN2_ERR_UNSUPPORTED, "groups of 32, 64 or 128 rows");
   if (p->ldx < p->K || (p->residual && p->ldr < p->N)) return fail(GDN2_ERR_INVALID, "row stride below the row");
   if (!p->x || !p->q || !p->meta || !p->y || !aligned16({p->q, p->meta}))

@@ -9,7 +9,6 @@
 // Activations of 16 bits are the other operand as they are, of float32 as three bfloat16 pieces of
 // eight bits each, whose sum is x.  So no product is rounded; sums, group sums of x and the scaling
 // are float32, and y is rounded once.
-#include <stdlib.h>
 #include "gdn2_kernels.hpp"
 
 namespace gdn2 {
@@ -873,18 +872,19 @@ __global__ __launch_bounds__(512) void w4_gemm_kernel(W4Args a, W4GemmArgs b) {
 //   parts: two workgroups a CU where that leaves 14 blocks of 128 or more to each, else one, with
 //     four blocks at least (64 rows of 14336 x 4096, 1 / 4 / 8 / 16 parts: 74, 25, 21, 27; 256 of
 //     4096 x 4096, 1 / 2: 21.8, 23.5).
+//   -1: many rows, w4_gemm_kernel, from three workgroups for four CUs on (bfloat16, us, against tiles: 2048
+//     rows of 4096 x 4096 77, 103; 1024 72, 55; 512 of 4096 x 14336 73, 92; 512 of 14336 x 4096 228, 95).
 template <int XT, int GROUP>
 using W4Tiles = W4Tile<XT, GROUP, 2, 2, 1, 4, 2>;
-// (parts -1) many rows: workgroups of w4_gemm_kernel for most of the chip.
-static bool w4_many(int M, int nnb) {
-  static const int many = getenv("W4MANY") ? atoi(getenv("W4MANY")) : 128;
-  return (int64_t)((M + 127) / 128) * ((nnb + 15) / 16) >= many;
+static bool w4_many(int dtype, int M, int nnb) {
+  const int bm = dtype == W4_F32 ? W4Gemm<W4_F32, 128>::BM : W4Gemm<W4_BF16, 128>::BM, bn = W4Gemm<W4_BF16, 128>::BN;
+  return (int64_t)((M + bm - 1) / bm) * ((16 * nnb + bn - 1) / bn) * 4 >= (int64_t)cu_count() * 3;
 }
-static int w4_parts(int M, int nkb, int nnb) {
+static int w4_parts(int dtype, int M, int nkb, int nnb) {
   using C = W4Tiles<W4_BF16, 128>;
   if (M <= 8 || (nkb <= 64 && (int64_t)nkb * nnb * ((M + 15) / 16) <= 32768)) return 0;
   const int64_t tiles = (int64_t)((16 * nnb + C::BN - 1) / C::BN) * ((M + C::BM - 1) / C::BM), cus = cu_count();
-  if (w4_many(M, nnb)) return -1;
+  if (w4_many(dtype, M, nnb)) return -1;
   const int64_t two = 2 * cus / tiles, one = cus / tiles;
   const int64_t p = two >= 1 && nkb / two >= 14 ? two : one < nkb / 4 ? one : nkb / 4;
   return p < 1 ? 1 : (int)p;
@@ -898,7 +898,7 @@ static size_t w4_sums_bytes(int group, const W4Args& a) { return (size_t)3 * ((a
 // whether w4_gemm_kernel can read x's own rows
 static bool w4_direct(int dtype, const W4Args& a) { return dtype != W4_F32 && a.vec && a.K % W4_KB == 0; }
 size_t w4_workspace_bytes(int dtype, int group, const W4Args& a) {
-  const int parts = w4_parts(a.M, a.nkb, a.nnb);
+  const int parts = w4_parts(dtype, a.M, a.nkb, a.nnb);
   if (parts < 0)
     return w4_sums_bytes(group, a) + (w4_direct(dtype, a) ? 0 : (size_t)(dtype == W4_F32 ? 3 : 1) * a.M * a.nkb * W4_KB * 2);
   return parts ? w4_align_bytes(dtype, a) + (parts > 1 ? (size_t)parts * a.M * a.N * 4 : 0) : 0;
@@ -914,7 +914,7 @@ static void w4_rows(const W4Args& a, hipStream_t s) {
 
 template <int XT, int GROUP>
 static void w4_go(W4Args a, hipStream_t s) {
-  const int parts = w4_parts(a.M, a.nkb, a.nnb);
+  const int parts = w4_parts(XT, a.M, a.nkb, a.nnb);
   if (parts == 0) {
     // two columns' blocks a wave where two workgroups a CU are left (one row of 4096 x 14336 float32:
     // 14.6 -> 11.8 us, 16 of 4096 x 11008 14.7 -> 12.5; one of 4096 x 4096 4.5 -> 5.1)
@@ -963,7 +963,6 @@ static void w4_go_group(int group, const W4Args& a, hipStream_t s) {
 }
 
 hipError_t launch_w4(int dtype, int group, const W4Args& a, hipStream_t s) {
-
   if (dtype == W4_F32) w4_go_group<W4_F32>(group, a, s);
   else if (dtype == W4_BF16) w4_go_group<W4_BF16>(group, a, s);
   else w4_go_group<W4_F16>(group, a, s);

@@ -325,8 +325,9 @@ int gdn2_lm_premix_step_fwd(const gdn2_lm_premix_step* p, void* stream);
  *         e = 0 .. 7, of column l % 16, element e < 4 in nibble 2 e, e >= 4 in nibble 2 e - 7;
  *   meta  (Np / 16, Kp / group, 16) words, scale | zero << 16 as bfloat16 bits; 0 past K and N.
  * group: 32, 64 or 128 rows of W share a scale and a zero.  q and meta 16-byte aligned; workspace
- * gdn2_w4_workspace_bytes (0: none), 16-byte aligned.  Sums are
- * float32 and products exact; y is rounded once.  A row of x with an infinity or NaN gives NaN. */
+ * gdn2_w4_workspace_bytes (0: none), 16-byte aligned.  M, K <= 2^20, N <= 2^24.  Products are exact and
+ * sums float32 (16 K max |x| has to fit); y is rounded once.  A row of x with an infinity or NaN gives
+ * nothing finite, and touches no other row. */
 enum { GDN2_F32 = 0, GDN2_BF16 = 1, GDN2_F16 = 2 };
 typedef struct gdn2_w4 {
   int32_t M, K, N, group, dtype;

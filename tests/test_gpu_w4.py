@@ -73,6 +73,43 @@ def test_product_matches_the_definition(M, K, N, group, dtype):
         assert torch.equal(y, w4_linear(x, W, bias=bias, residual=res))        # the same bits again
 
 
+# Long sums and many entries: one part, sums in parts, rows that 16-byte accesses cannot take, and tiles of
+# many rows with x read in place (K a multiple of 128) and not, and with groups past a block of 32 of them
+LARGE = [
+    (17, 8321, 40, 32), (40, 9000, 130, 64), (500, 8200, 2040, 64), (520, 500, 4100, 128), (521, 501, 4100, 32),
+    (2100, 100, 4100, 32), (1500, 256, 4100, 128), (1500, 264, 4096, 64), (1537, 301, 4111, 32), (1500, 1152, 4100, 32),
+    (1290, 4229, 4800, 128), (1409, 2176, 4353, 64),
+]
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("M,K,N,group", LARGE)
+def test_large_product_matches_the_definition(M, K, N, group, dtype):
+    test_product_matches_the_definition(M, K, N, group, dtype)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("M,K,N", [(520, 500, 4100), (1500, 300, 4100), (1500, 256, 4100)])
+def test_many_strided_rows_and_one_that_is_not_finite(M, K, N, dtype):
+    from atomic_gdn2.w4 import w4_linear
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    dt, group = TYPES[dtype], 64
+    codes, scales, z, W = _weights(K, N, group, True, gen)
+    wide = torch.randn((M, K + 13), device="cuda", generator=gen).to(dt)
+    print(f"[gpu-test] w4 strided {M}x{K}x{N} {dtype}", flush=True)
+    for x in (wide[:, 8:8 + K], wide[:, 3:3 + K]):
+        y = w4_linear(x, W)
+        _check(y, x, codes, scales, z, group, None, None, dtype)
+        assert torch.equal(y, w4_linear(x.contiguous(), W))
+    x = wide[:, 3:3 + K].contiguous()
+    clean = w4_linear(x, W)
+    x[1, 7], x[M - 1, K - 1] = float("nan"), float("inf")
+    y = w4_linear(x, W)
+    assert not torch.isfinite(y[1]).any() and not torch.isfinite(y[M - 1]).any()
+    keep = [i for i in range(M) if i not in (1, M - 1)]
+    assert torch.equal(y[keep], clean[keep])
+
+
 @pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("M", [1, 9, 40, 200])
 def test_strided_and_misaligned_rows(M, dtype):
