@@ -267,8 +267,9 @@ __global__ __launch_bounds__(w4_waves(XT, NB) * WAVE) void w4_rows_kernel(W4Args
   const __amdgpu_buffer_rsrc_t qb = w4_buffer(a.q, (size_t)nb0 * a.nkb * 1024, (int64_t)nbs * a.nkb * 1024);
   const __amdgpu_buffer_rsrc_t sb = w4_buffer(a.meta, (size_t)nb0 * a.nkb * (NG * 64), (int64_t)nbs * a.nkb * (NG * 64));
   const int xk = 32 * (r % SP) + 8 * c;              // the lane's first k of a load
-  const uint32_t xoff = r / SP < rows ? (uint32_t)(r / SP * a.ldx + xk) * E : W4_OUT;
-  uint32_t qoff[NB], soff[NB];
+  uint32_t xoff[XL], qoff[NB], soff[NB];
+#pragma unroll
+  for (int u = 0; u < XL; ++u) xoff[u] = r / SP < rows ? (uint32_t)(r / SP * a.ldx + 32 * SP * u + xk) * E : W4_OUT;
 #pragma unroll
   for (int i = 0; i < NB; ++i) {                     // (columns past the last: zero codes and scales)
     qoff[i] = (uint32_t)i * a.nkb * 1024 + 16 * l;
@@ -284,31 +285,26 @@ __global__ __launch_bounds__(w4_waves(XT, NB) * WAVE) void w4_rows_kernel(W4Args
     uint32_t sz[NB][NG];
     W4Raw<XT> x[XL];
   };
-  auto load = [&](Block& o, int kb) __attribute__((always_inline)) {
+  // Without a branch, behind which the compiler would wait for all loads, these included: past the last
+  // block offsets go out of range for good (in place, since a register of its own may be one that a load is
+  // still to write), nothing is read and nothing used.
+  auto load = [&](Block& o, int kb, auto vec) __attribute__((always_inline)) {
+    const uint32_t past = kb < a.nkb ? 0u : W4_OUT;
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
-      o.q[i] = w4_buffer16(qb, qoff[i], kb * 1024);
+      o.q[i] = w4_buffer16(qb, qoff[i] |= past, kb * 1024);
+      soff[i] |= past;
 #pragma unroll
-      for (int g = 0; g < NG; ++g)
-        o.sz[i][g] = w4_buffer4(sb, soff[i] + 64 * g, kb * (NG * 64));
+      for (int g = 0; g < NG; ++g) o.sz[i][g] = w4_buffer4(sb, soff[i] + 64 * g, kb * (NG * 64));
     }
-    if (!a.vec) {
 #pragma unroll
-      for (int u = 0; u < XL; ++u)
-          o.x[u] = w4_load_odd<XT>(a, r / SP < rows ? m0 + r / SP : a.M, kb * W4_KB + 32 * SP * u + xk);
-    } else if ((kb + 1) * W4_KB <= a.K) {
+    for (int u = 0; u < XL; ++u) {
+      if constexpr (vec.value) {
+        xoff[u] = kb * W4_KB < a.K - 32 * SP * u - xk ? xoff[u] : W4_OUT;
 #pragma unroll
-      for (int u = 0; u < XL; ++u)
-#pragma unroll
-          for (int v = 0; v < W4Raw<XT>::NV; ++v)
-            o.x[u].v[v] = w4_buffer16(xb, xoff + 32 * SP * u * E + 16 * v, kb * (W4_KB * E));
-    } else {
-#pragma unroll
-      for (int u = 0; u < XL; ++u) {
-        const uint32_t out = kb * W4_KB + 32 * SP * u + xk < a.K ? 0u : W4_OUT;
-#pragma unroll
-        for (int v = 0; v < W4Raw<XT>::NV; ++v)
-          o.x[u].v[v] = w4_buffer16(xb, (xoff + 32 * SP * u * E + 16 * v) | out, kb * (W4_KB * E));
+        for (int v = 0; v < W4Raw<XT>::NV; ++v) o.x[u].v[v] = w4_buffer16(xb, xoff[u] + 16 * v, kb * (W4_KB * E));
+      } else {
+        o.x[u] = w4_load_odd<XT>(a, r / SP < rows ? m0 + r / SP : a.M, kb * W4_KB + 32 * SP * u + xk);
       }
     }
   };
@@ -353,19 +349,22 @@ __global__ __launch_bounds__(w4_waves(XT, NB) * WAVE) void w4_rows_kernel(W4Args
       }
     }
   };
-  if (w < a.nkb) {                                   // (the launch gives every wave a block)
+  auto run = [&](auto vec) __attribute__((always_inline)) {
     Block even, odd;
     int kb = w;
-    load(even, kb);
+    load(even, kb, vec);
     for (;;) {
-      if (kb + W < a.nkb) load(odd, kb + W);
+      load(odd, kb + W, vec);
       add(even);
       if ((kb += W) >= a.nkb) break;
-      if (kb + W < a.nkb) load(even, kb + W);
+      load(even, kb + W, vec);
       add(odd);
       if ((kb += W) >= a.nkb) break;
     }
-  }
+  };
+  // (the launch gives every wave a block)
+  if (a.vec) run(std::true_type{});
+  else run(std::false_type{});
 #pragma unroll
   for (int i = 0; i < NB; ++i)
 #pragma unroll
@@ -433,33 +432,39 @@ __global__ __launch_bounds__(C::W * WAVE) void w4_tile_kernel(W4Args a) {
   W4Raw<XT> xr[NU][4];
   // the wave's own block kb + wk of the weights, and its units of x of the blocks kb .. kb + WK - 1 (past the
   // part's last block: zeros of x); lane l takes rows l / 8 (+ 8) and k 8 (l % 8) (+ 64) of a unit
-  uint32_t xoff[NU][2];
+  uint32_t xoff[NU][4], qoff[NBW], soff[NBW];
 #pragma unroll
   for (int i = 0; i < NU; ++i) {
     const int unit = w + W * i;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int m = 16 * (unit % (MT * WM)) + (l >> 3) + 8 * h;
-      xoff[i][h] = unit < C::UNITS && m < rows ? (uint32_t)(m * a.ldx + unit / (MT * WM) * W4_KB + 8 * (l & 7)) * E : W4_OUT;
+    for (int j = 0; j < 4; ++j) {                    // rows 8 (j / 2) .., k 64 (j % 2) ..
+      const int m = 16 * (unit % (MT * WM)) + (l >> 3) + 8 * (j / 2);
+      xoff[i][j] = unit < C::UNITS && m < rows ? (uint32_t)(m * a.ldx + unit / (MT * WM) * W4_KB + 64 * (j % 2) + 8 * (l & 7)) * E : W4_OUT;
     }
   }
+#pragma unroll
+  for (int i = 0; i < NBW; ++i) {
+    qoff[i] = (uint32_t)i * a.nkb * 1024 + 16 * l;
+    soff[i] = (uint32_t)i * a.nkb * (NG * 64) + 4 * r;
+  }
+  // (past the end: as in w4_rows_kernel)
   auto load = [&](Block& o, int kb) __attribute__((always_inline)) {
-    const int kw = __builtin_amdgcn_readfirstlane(min(kb + wk, a.nkb - 1));
+    const uint32_t past = kb + wk < kb1 ? 0u : W4_OUT;
 #pragma unroll
     for (int i = 0; i < NU; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {                  // rows 8 (j / 2) .., k 64 (j % 2) ..
-        const int k = (kb + (w + W * i) / (MT * WM)) * W4_KB + 64 * (j % 2) + 8 * (l & 7);
-        const uint32_t off = (k < k_end ? xoff[i][j / 2] : W4_OUT) + 64 * (j % 2) * E;
+      for (int j = 0; j < 4; ++j) {
+        const int k = (w + W * i) / (MT * WM) * W4_KB + 64 * (j % 2) + 8 * (l & 7);
+        xoff[i][j] = kb * W4_KB < k_end - k ? xoff[i][j] : W4_OUT;
 #pragma unroll
-        for (int v = 0; v < W4Raw<XT>::NV; ++v) xr[i][j].v[v] = w4_buffer16(xb, off + 16 * v, kb * (W4_KB * E));
+        for (int v = 0; v < W4Raw<XT>::NV; ++v) xr[i][j].v[v] = w4_buffer16(xb, xoff[i][j] + 16 * v, kb * (W4_KB * E));
       }
 #pragma unroll
     for (int i = 0; i < NBW; ++i) {
-      o.q[i] = w4_buffer16(qb, i * a.nkb * 1024 + 16 * l, kw * 1024);
+      o.q[i] = w4_buffer16(qb, qoff[i] |= past, (kb + wk) * 1024);
+      soff[i] |= past;
 #pragma unroll
-      for (int g = 0; g < NG; ++g)
-        o.sz[i][g] = w4_buffer4(sb, i * a.nkb * (NG * 64) + 64 * g + 4 * r, kw * (NG * 64));
+      for (int g = 0; g < NG; ++g) o.sz[i][g] = w4_buffer4(sb, soff[i] + 64 * g, (kb + wk) * (NG * 64));
     }
     __builtin_amdgcn_sched_barrier(0);               // issued here, not where they are used
   };
@@ -505,7 +510,7 @@ __global__ __launch_bounds__(C::W * WAVE) void w4_tile_kernel(W4Args a) {
   auto add = [&](const Block& o, int buf) __attribute__((always_inline)) {
     const int u0 = wk * (MT * WM) + wm * MT, slot = l ^ c;
     // operands of x in the order of their use, read AHEAD of it
-    constexpr int STEPS = 4 * NP * MT, AHEAD = NBW >= 4 ? 2 : 4;
+    constexpr int STEPS = 4 * NP * MT, AHEAD = 4;
     auto read = [&](int i) __attribute__((always_inline)) {
       const int t = i % MT, p = i / MT % NP, j = i / (MT * NP);
       return __builtin_bit_cast(s8, frag(buf, u0 + t, p, j)[j & 1 ? slot ^ 4 : slot]);
@@ -565,12 +570,12 @@ __global__ __launch_bounds__(C::W * WAVE) void w4_tile_kernel(W4Args a) {
   stage(0);
   __syncthreads();
   for (;;) {
-    if (kb + WK < kb1) load(odd, kb + WK);
+    load(odd, kb + WK);
     add(even, buf);
     if ((kb += WK) >= kb1) break;
     stage(buf ^= 1);
     __syncthreads();
-    if (kb + WK < kb1) load(even, kb + WK);
+    load(even, kb + WK);
     add(odd, buf);
     if ((kb += WK) >= kb1) break;
     stage(buf ^= 1);
