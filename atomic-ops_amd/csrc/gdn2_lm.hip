@@ -358,7 +358,8 @@ __global__ __launch_bounds__(256) void lm_premix_bwd_kernel(LmPremixBwdArgs a) {
 // ------------------------------------------------------------------------------------
 // premix of one token from cached projections: the convolutions' window is the row's parent's last
 // three projections and y itself.  One wave a row, head and role (the roles of premix), lanes over the
-// channels, so that rows of any alignment are read whole.
+// channels, so that rows of any alignment are read whole.  Bound by its bytes: 1024 rows of 6 heads of 128
+// in 17.2 us, 5.7 TB/s; 4 rows by a launch, 3.3 us.
 // ------------------------------------------------------------------------------------
 template <int D>
 __global__ __launch_bounds__(256) void lm_premix_step_kernel(LmPremixStepArgs a) {

@@ -244,8 +244,10 @@ __device__ __forceinline__ float w4_quad_sum(float x) {      // over the four la
 // Waves of a workgroup at most
 constexpr int w4_waves(int XT, int NB) { return XT != W4_F32 && NB == 1 ? 16 : 8; }
 
-// Few rows: bound by the bytes of the weights.  A workgroup takes 16 NB columns and 16 / SP rows; its waves take the 128-deep blocks of the sum in turn, the next one's
-// loads issued before the products of this one, and add their parts through LDS in wave order.
+// Few rows: bound by the bytes of the weights (one row of 8192 x 28672 bfloat16, groups of 128: 23.3 us,
+// 5.3 TB/s; a plain read of as much 19.8 us), small matrices by a launch (512 x 4614 float32 3.3 us).  A
+// workgroup takes 16 NB columns and 16 / SP rows; its waves take the 128-deep blocks of the sum in turn, the
+// next one's loads issued before the products of this one, and add their parts through LDS in wave order.
 //   x is the products' left operand, so a lane's results are rows 4 (l / 16) + e of one column and it
 // needs one scale.  With few rows an operand's 16 rows hold SP steps' pieces of each: row m's at rows
 // SP m, SP m + 1, ...: one load then serves SP steps, the later ones after a move by lanes (whose other
@@ -389,6 +391,8 @@ __global__ __launch_bounds__(w4_waves(XT, NB) * WAVE) void w4_rows_kernel(W4Args
 // caches once for all the columns: a CU takes about 34 bytes a nanosecond from the L2, and with x in
 // every wave's registers that was the bound.  The next blocks are loaded while these are multiplied.
 // With several parts the sums go to a.part (part, M, N), which w4_join_kernel adds in order.
+//   32 rows of 14336 x 4096 bfloat16: 14.1 us (32 MB, 2.3 TB/s), of that the join 3: a workgroup has seven
+// rounds of loads, products and a barrier, and the memory's latency in each.  128 rows of 4096 x 4096 15.3.
 template <int XT_, int GROUP_, int MT_, int NBW_, int WM_, int WN_, int WK_>
 struct W4Tile {
   static constexpr int XT = XT_, GROUP = GROUP_, MT = MT_, NBW = NBW_, WM = WM_, WN = WN_, WK = WK_;
@@ -643,6 +647,10 @@ __global__ __launch_bounds__(256) void w4_join_kernel(W4Args a, int parts) {
 // BM rows and 256 columns, a wave 16 MT rows and 64 columns: x comes into LDS by DMA, a block ahead of
 // its use, the scale is one fma a group and result, and the zeros are a product of their own behind the
 // sum, (sums of x) x (-s z) over the groups, 32 groups a step: s z has 16 bits, two pieces.
+//   2048 rows of 4096 x 4096 bfloat16: 76 us, 905 TFLOP/s (a large library product of bfloat16 1219), of that
+// the pass over x 4.  With parts of the loop left out: products alone 55, without the DMA 64, without the
+// scaling 70, without the conversions 74, without the products 59.  Zeros in the scaling instead of a product,
+// x staged through registers as in w4_tile_kernel: 112.
 template <int XT_, int GROUP_>
 struct W4Gemm {
   static constexpr int XT = XT_, GROUP = GROUP_, NP = W4Frag<XT>::NP;
