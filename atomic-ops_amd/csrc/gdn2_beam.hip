@@ -225,16 +225,21 @@ __global__ __launch_bounds__(BEAM_T) void beam_part_kernel(BeamArgs a) {
   }
   float v[PT];
   const int c0 = split * PT * BEAM_T;
+  if (c0 + PT * BEAM_T <= a.V) {                     // (uniform: loads without a branch at each, 58 -> 56.5 us)
 #pragma unroll
-  for (int i = 0; i < PT / VW; ++i) {
-    const int at = c0 + (i * BEAM_T + tid) * VW;
-    if (at + VW <= a.V) {
-      beam_load<XT, VW>(a, row, at, v + i * VW);
-    } else {
+    for (int i = 0; i < PT / VW; ++i) beam_load<XT, VW>(a, row, c0 + (i * BEAM_T + tid) * VW, v + i * VW);
+  } else {
 #pragma unroll
-      for (int e = 0; e < VW; ++e) {
-        v[i * VW + e] = -__builtin_inff();
-        if (at + e < a.V) beam_load<XT, 1>(a, row, at + e, v + i * VW + e);
+    for (int i = 0; i < PT / VW; ++i) {
+      const int at = c0 + (i * BEAM_T + tid) * VW;
+      if (at + VW <= a.V) {
+        beam_load<XT, VW>(a, row, at, v + i * VW);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VW; ++e) {
+          v[i * VW + e] = -__builtin_inff();
+          if (at + e < a.V) beam_load<XT, 1>(a, row, at + e, v + i * VW + e);
+        }
       }
     }
   }
