@@ -392,7 +392,8 @@ __global__ __launch_bounds__(w4_waves(XT, NB) * WAVE) void w4_rows_kernel(W4Args
 // every wave's registers that was the bound.  The next blocks are loaded while these are multiplied.
 // With several parts the sums go to a.part (part, M, N), which w4_join_kernel adds in order.
 //   32 rows of 14336 x 4096 bfloat16: 14.1 us (32 MB, 2.3 TB/s), of that the join 3: a workgroup has seven
-// rounds of loads, products and a barrier, and the memory's latency in each.  128 rows of 4096 x 4096 15.3.
+// rounds of staging, a barrier, products and scaling, one after the other (weights loaded two rounds ahead
+// instead of one: 14.3).  128 rows of 4096 x 4096 15.4.
 template <int XT_, int GROUP_, int MT_, int NBW_, int WM_, int WN_, int WK_>
 struct W4Tile {
   static constexpr int XT = XT_, GROUP = GROUP_, MT = MT_, NBW = NBW_, WM = WM_, WN = WN_, WK = WK_;
@@ -880,8 +881,8 @@ __global__ __launch_bounds__(512) void w4_gemm_kernel(W4Args a, W4GemmArgs b) {
 //   rows: one launch, x and (over 16 rows) the weights read again by each tile of rows.  Up to 8 rows
 //     always; more where the weights come from the caches again, 2^15 tiles of 16 rows and 128 x 16
 //     weights, and the sum is not long beside the columns (bfloat16, us, rows against tiles: 64 rows of
-//     2048 x 2048 5.6, 8.2; 64 of 4096 x 4096 11.6, 12.4; 128 of 4096 x 4096 20, 17; 16 of
-//     14336 x 4096 19, 14.8).
+//     2048 x 2048 5.7, 8.8; 64 of 4096 x 4096 11.8, 11.7; 128 of 4096 x 4096 20.7, 15.1; 16 of
+//     4096 x 14336 12.5, 14.5; 16 of 14336 x 4096 16.8, 13.2).
 //   parts: two workgroups a CU where that leaves 14 blocks of 128 or more to each, else one, with
 //     four blocks at least (64 rows of 14336 x 4096, 1 / 4 / 8 / 16 parts: 74, 25, 21, 27; 256 of
 //     4096 x 4096, 1 / 2: 21.8, 23.5).
