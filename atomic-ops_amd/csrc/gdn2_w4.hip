@@ -292,19 +292,20 @@ __global__ __launch_bounds__(w4_waves(XT, NB) * WAVE) void w4_rows_kernel(W4Args
   // still to write), nothing is read and nothing used.
   auto load = [&](Block& o, int kb, auto vec) __attribute__((always_inline)) {
     const uint32_t past = kb < a.nkb ? 0u : W4_OUT;
+    const int at = min(kb, a.nkb - 1);               // (the uniform part of an offset stays within the buffer)
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
-      o.q[i] = w4_buffer16(qb, qoff[i] |= past, kb * 1024);
+      o.q[i] = w4_buffer16(qb, qoff[i] |= past, at * 1024);
       soff[i] |= past;
 #pragma unroll
-      for (int g = 0; g < NG; ++g) o.sz[i][g] = w4_buffer4(sb, soff[i] + 64 * g, kb * (NG * 64));
+      for (int g = 0; g < NG; ++g) o.sz[i][g] = w4_buffer4(sb, soff[i] + 64 * g, at * (NG * 64));
     }
 #pragma unroll
     for (int u = 0; u < XL; ++u) {
       if constexpr (vec.value) {
         xoff[u] = kb * W4_KB < a.K - 32 * SP * u - xk ? xoff[u] : W4_OUT;
 #pragma unroll
-        for (int v = 0; v < W4Raw<XT>::NV; ++v) o.x[u].v[v] = w4_buffer16(xb, xoff[u] + 16 * v, kb * (W4_KB * E));
+        for (int v = 0; v < W4Raw<XT>::NV; ++v) o.x[u].v[v] = w4_buffer16(xb, xoff[u] + 16 * v, at * (W4_KB * E));
       } else {
         o.x[u] = w4_load_odd<XT>(a, r / SP < rows ? m0 + r / SP : a.M, kb * W4_KB + 32 * SP * u + xk);
       }
@@ -455,6 +456,7 @@ __global__ __launch_bounds__(C::W * WAVE) void w4_tile_kernel(W4Args a) {
   // (past the end: as in w4_rows_kernel)
   auto load = [&](Block& o, int kb) __attribute__((always_inline)) {
     const uint32_t past = kb + wk < kb1 ? 0u : W4_OUT;
+    const int at = min(kb, a.nkb - 1), qat = min(kb + wk, a.nkb - 1);
 #pragma unroll
     for (int i = 0; i < NU; ++i)
 #pragma unroll
@@ -462,14 +464,14 @@ __global__ __launch_bounds__(C::W * WAVE) void w4_tile_kernel(W4Args a) {
         const int k = (w + W * i) / (MT * WM) * W4_KB + 64 * (j % 2) + 8 * (l & 7);
         xoff[i][j] = kb * W4_KB < k_end - k ? xoff[i][j] : W4_OUT;
 #pragma unroll
-        for (int v = 0; v < W4Raw<XT>::NV; ++v) xr[i][j].v[v] = w4_buffer16(xb, xoff[i][j] + 16 * v, kb * (W4_KB * E));
+        for (int v = 0; v < W4Raw<XT>::NV; ++v) xr[i][j].v[v] = w4_buffer16(xb, xoff[i][j] + 16 * v, at * (W4_KB * E));
       }
 #pragma unroll
     for (int i = 0; i < NBW; ++i) {
-      o.q[i] = w4_buffer16(qb, qoff[i] |= past, (kb + wk) * 1024);
+      o.q[i] = w4_buffer16(qb, qoff[i] |= past, qat * 1024);
       soff[i] |= past;
 #pragma unroll
-      for (int g = 0; g < NG; ++g) o.sz[i][g] = w4_buffer4(sb, soff[i] + 64 * g, (kb + wk) * (NG * 64));
+      for (int g = 0; g < NG; ++g) o.sz[i][g] = w4_buffer4(sb, soff[i] + 64 * g, qat * (NG * 64));
     }
     __builtin_amdgcn_sched_barrier(0);               // issued here, not where they are used
   };
