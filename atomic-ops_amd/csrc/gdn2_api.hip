@@ -870,14 +870,12 @@ int beam_shape(int B, int K, int V, int n) {
     return fail(GDN2_ERR_UNSUPPORTED, "shape too large");
   return GDN2_OK;
 }
-size_t beam_cand_bytes(int B, int K, int V, int n) {
-  return align_up((size_t)B * K * gdn2::beam_splits(B * K, K, V) * n * 8);
-}
+size_t beam_pieces(int B, int K, int V) { return (size_t)B * K * gdn2::beam_splits(B * K, K, V); }
 }  // namespace
 
 size_t gdn2_beam_workspace_bytes(int B, int K, int V, int n) {
   if (beam_shape(B, K, V, n)) return 0;
-  return beam_cand_bytes(B, K, V, n) + (size_t)B * K * gdn2::beam_splits(B * K, K, V) * 8;
+  return beam_pieces(B, K, V) * (16 + (size_t)n * 8);
 }
 
 int gdn2_beam_step(const gdn2_beam* p, void* workspace, void* stream) {
@@ -895,11 +893,12 @@ int gdn2_beam_step(const gdn2_beam* p, void* workspace, void* stream) {
   if (reinterpret_cast<uintptr_t>(p->logits) % e) return fail(GDN2_ERR_INVALID, "pointer not aligned to its elements");
   gdn2::BeamArgs a{};
   a.logits = p->logits; a.scores = p->scores; a.finished = p->finished;
-  a.cand = static_cast<unsigned long long*>(workspace);
-  a.part = at<float>(workspace, beam_cand_bytes(p->B, p->K, p->V, p->n));
+  a.part = static_cast<float*>(workspace);
+  a.cand = at<unsigned long long>(workspace, beam_pieces(p->B, p->K, p->V) * 16);
   a.tokens = p->tokens; a.rows = p->rows; a.out_scores = p->out_scores; a.out_finished = p->out_finished;
   a.B = p->B; a.K = p->K; a.V = p->V; a.n = p->n; a.eos = p->eos;
   a.splits = gdn2::beam_splits(p->B * p->K, p->K, p->V);
+  a.piece = gdn2::beam_piece(p->B * p->K, p->V);
   a.ld = (size_t)p->ld;
   a.vec = aligned16({p->logits}) && p->ld * e % 16 == 0;
   return lm_done(gdn2::launch_beam(p->dtype, a, reinterpret_cast<hipStream_t>(stream)), "beam launch");

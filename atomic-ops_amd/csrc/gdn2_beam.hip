@@ -4,11 +4,13 @@
 // a finished beam has one continuation, the end token at its own score; NaN counts as -inf.
 //
 // One pass over the logits, bound by their bytes (beam_part_kernel): a workgroup keeps a piece of a row
-// in registers, forms its maximum and sum, and its n best entries, which are the row's best whatever the
-// row's sum is.  beam_join_kernel then has a few hundred entries a group: it joins the sums, forms the
-// scores in float32 as written above, and selects among them.
-//   64 groups of 8 beams, 131072 float32: 56 us (268 MB; the join 7 of them); 16 of 4, 32000 bfloat16: 13 us,
-// the two launches' latency; with n rounds of a maximum in place of a threshold 112 and 19 us.
+// in registers, forms its maximum and sum, its n best entries by logit, and the best logit that it leaves
+// out.  beam_join_kernel then has a few hundred entries a group: it joins the sums, forms the scores in
+// float32 as written above, and selects among them.  Scores rise with the logits, so what a piece leaves out
+// never scores above the n-th best, but may round to the same score at a lower index: where the best
+// left out scores as much as the n-th best, the join looks through the piece's logits again.
+//   64 groups of 8 beams, 131072 float32: 57 us (268 MB; the join 8 of them); 16 of 4, 32000 bfloat16: 13.7 us,
+// the two launches' latency (56 and 13.2 without a look at what the pieces leave out); with n rounds of a maximum in place of a threshold 112 and 19 us.
 // Selection is by one 64-bit key: the value's bits in an order that compares as integers, then the
 // complement of the index, so the largest key is the highest value at its lowest index.
 #include "gdn2_kernels.hpp"
@@ -98,16 +100,19 @@ __device__ __forceinline__ u64 block_max64(u64 x, u64 (*best)[BEAM_W], int parit
   return y;
 }
 
-// The n best of the workgroup's entries, out[0 .. n) in order (0: no more entries).  key(i), i < PT:
-// a thread's entries, 0 for none; v[i]: their values; m: the largest v of the thread.
+// The n best of the workgroup's entries, put(0, .), ..., put(n - 1, .) in order (0: no more entries), each by
+// some thread, and with NEXT in put(n, .) a key of the next one's value (-inf or 0: none).  key(i), i < PT: a
+// thread's entries, 0 for none; v[i]: their values; m: the largest v of the thread.
 //   Of a wave's lanes' maxima, the n-th largest bounds the n best from below, and so does the least of the
 // four waves' ceil(n / 4)-th largest (n entries at least reach either).  A few times n entries reach the
 // higher of the two; they are gathered and ranked by counting.  Where more than BEAM_LIST reach it (long ties, rows that are almost
 // all masked), n rounds of the largest key of all take their place.
-template <int PT, class Key>
-__device__ __forceinline__ void beam_select(BeamShared& sh, const float* v, float m, int n, u64* out, Key key) {
+//   With NEXT the bound is n + 1's, except where a quarter more of n would reach it for that (n = 8: 52.8 us in
+// place of 50.1 for the parts of 64 x 8 x 131072): there a look at what lies below it finds the next one, if only n reach it.
+template <bool NEXT, int PT, class Key, class Put>
+__device__ __forceinline__ void beam_select(BeamShared& sh, const float* v, float m, int n, Key key, Put put) {
   const int tid = threadIdx.x, l = lane_id();
-  const int share = (n + BEAM_W - 1) / BEAM_W, rounds = n <= 16 ? n : share;
+  const int reach = n + (NEXT && n % BEAM_W != 0), share = (reach + BEAM_W - 1) / BEAM_W, rounds = reach <= 16 ? reach : share;
   float t = 0.f, ts = 0.f;
   for (int i = 0; i < rounds; ++i) {
     t = wave_maxf(m);
@@ -117,7 +122,7 @@ __device__ __forceinline__ void beam_select(BeamShared& sh, const float* v, floa
   }
   if (l == 0) {
     sh.t[wave_id()] = ts;
-    sh.t[BEAM_W + wave_id()] = rounds == n ? t : -__builtin_inff();
+    sh.t[BEAM_W + wave_id()] = rounds == reach ? t : -__builtin_inff();
   }
   if (tid == 0) sh.count = 0;
   __syncthreads();
@@ -149,9 +154,18 @@ __device__ __forceinline__ void beam_select(BeamShared& sh, const float* v, floa
 #pragma unroll
         for (int e = 0; e < 8; ++e) rank += sh.list[j + e] > k;
       }
-      if (rank < n) out[rank] = k;
+      if (rank < n + NEXT) put(rank, k);
     }
-    for (int i = count + tid; i < n; i += BEAM_T) out[i] = 0;
+    for (int i = count + tid; i < n; i += BEAM_T) put(i, (u64)0);
+    if (NEXT && count <= n) {
+      float below = -__builtin_inff();
+#pragma unroll
+      for (int i = 0; i < PT; ++i) below = fmaxf(below, v[i] < t ? v[i] : -__builtin_inff());
+      below = wave_maxf(below);
+      if (l == 0) sh.t[wave_id()] = below;           // (t is read, two barriers ago)
+      __syncthreads();
+      if (tid == 0) put(n, beam_key(fmaxf(fmaxf(sh.t[0], sh.t[1]), fmaxf(sh.t[2], sh.t[3])), 0));
+    }
     return;
   }
   auto next = [&](u64 below) {
@@ -164,9 +178,9 @@ __device__ __forceinline__ void beam_select(BeamShared& sh, const float* v, floa
     return k;
   };
   u64 mine = next(~0ull);
-  for (int i = 0; i < n; ++i) {
+  for (int i = 0; i < n + NEXT; ++i) {
     const u64 top = block_max64(mine, sh.best, i & 1);
-    if (tid == 0) out[i] = top;
+    if (tid == 0) put(i, top);
     if (top == mine) mine = next(top);
   }
 }
@@ -198,29 +212,28 @@ __device__ __forceinline__ void beam_load(const BeamArgs& a, size_t row, int i, 
   }
 }
 
-// Row r = blockIdx.y, entries [split PT T, ...): maximum, sum and n best keys.  VW consecutive
-// entries a thread and load.
+// Row r = blockIdx.y, entries [split PT T, ...): maximum, sum, the n best keys and the next
+// one's logit.  VW consecutive entries a thread and load.
 template <int XT, int VW, int PT>
 __global__ __launch_bounds__(BEAM_T) void beam_part_kernel(BeamArgs a) {
   __shared__ float sm[2 * BEAM_W];
   __shared__ BeamShared sh;
   const int tid = threadIdx.x, split = blockIdx.x, row = blockIdx.y;
-  u64* out = a.cand + ((size_t)row * a.splits + split) * a.n;
+  const size_t piece = (size_t)row * a.splits + split;
+  u64* out = a.cand + piece * a.n;
+  float* part = a.part + 4 * piece;
   const float score = a.scores[row];
   const bool done = a.finished && a.finished[row];
   if (done || !(score > -__builtin_inff())) {
     // no logit of this row matters: -inf at its first entries (the end token's own score apart, which
     // the join forms)
-    if (split == 0 && tid == 0) {
-      a.part[2 * (size_t)row * a.splits] = 0.f;
-      a.part[2 * (size_t)row * a.splits + 1] = 1.f;
+    if (tid == 0) {
+      part[0] = split == 0 ? 0.f : -__builtin_inff();
+      part[1] = split == 0 ? 1.f : 0.f;
+      part[2] = -__builtin_inff();
     }
     for (int i = tid; i < a.n; i += BEAM_T)
       out[i] = split == 0 && i < a.V ? beam_key(-__builtin_inff(), i) : 0;
-    if (split != 0 && tid == 0) {
-      a.part[2 * ((size_t)row * a.splits + split)] = -__builtin_inff();
-      a.part[2 * ((size_t)row * a.splits + split) + 1] = 0.f;
-    }
     return;
   }
   float v[PT];
@@ -256,13 +269,16 @@ __global__ __launch_bounds__(BEAM_T) void beam_part_kernel(BeamArgs a) {
   m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
   const float s = wave_sumf(m > -__builtin_inff() ? beam_exps<PT>(v, m) : 0.f);
   if (lane_id() == 0) sm[BEAM_W + wave_id()] = s;
-  beam_select<PT>(sh, v, mine, a.n, out, [&](int i) {
+  beam_select<true, PT>(sh, v, mine, a.n, [&](int i) {
     const int at = c0 + ((i / VW) * BEAM_T + tid) * VW + i % VW;
     return at < a.V ? beam_key(v[i], at) : 0;
+  }, [&](int i, u64 k) {
+    if (i < a.n) out[i] = k;
+    else part[2] = k ? beam_key_value(k) : -__builtin_inff();
   });
   if (tid == 0) {                                    // (behind the selection's barriers)
-    a.part[2 * ((size_t)row * a.splits + split)] = m;
-    a.part[2 * ((size_t)row * a.splits + split) + 1] = (sm[BEAM_W] + sm[BEAM_W + 1]) + (sm[BEAM_W + 2] + sm[BEAM_W + 3]);
+    part[0] = m;
+    part[1] = (sm[BEAM_W] + sm[BEAM_W + 1]) + (sm[BEAM_W + 2] + sm[BEAM_W + 3]);
   }
 }
 
@@ -284,14 +300,38 @@ __device__ __forceinline__ float beam_score(float score, float x, float m, float
   if (!(x > -__builtin_inff() && score > -__builtin_inff())) return -__builtin_inff();
   return beam_value(score + ((x == m ? 0.f : x - m) - ls));
 }
+// The logits' type's next value above (d = 1) or below (-1) x; nothing lies above +inf, nor below -inf
+template <int XT>
+__device__ __forceinline__ float beam_near(float x, int d) {
+  if (x == 0.f && d < 0) d = -2;                     // (-0 is 0)
+  if constexpr (XT == W4_F32) {
+    const uint32_t u = __float_as_uint(x), o = (u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u)) + d;
+    return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xffffffffu));
+  } else {
+    const uint32_t u = XT == W4_BF16 ? __float_as_uint(x) >> 16 : __builtin_bit_cast(uint16_t, (_Float16)x);
+    const uint32_t o = (u ^ ((u >> 15) ? 0xffffu : 0x8000u)) + d, y = o ^ ((o >> 15) ? 0x8000u : 0xffffu);
+    return XT == W4_BF16 ? bf16_val(y) : (float)__builtin_bit_cast(_Float16, (uint16_t)y);
+  }
+}
+// Whether a piece may have left out entries of the score c that come before others of this score: x is the
+// best logit that it left out, of that score.  Not where all of the row's entries of that score are x, which
+// are kept and left out by their indices.
+template <int XT>
+__device__ __forceinline__ bool beam_unsure(float score, float x, float m, float ls, float c) {
+  return (x < m && beam_score(score, beam_near<XT>(x, 1), m, ls) == c) ||
+         (x > -__builtin_inff() && beam_score(score, beam_near<XT>(x, -1), m, ls) == c);
+}
 
 // One workgroup a group: the scores of the parts' entries, and the n best of them.
 constexpr int BEAM_PT2 = 8;                     // entries a thread keeps at a time
+template <int XT>
 __global__ __launch_bounds__(BEAM_T) void beam_join_kernel(BeamArgs a) {
   __shared__ BeamShared sh;
   __shared__ u64 kept[BEAM_MAX_N];
   __shared__ float sM[BEAM_MAX_K], sL[BEAM_MAX_K], sS[BEAM_MAX_K];
   __shared__ uint8_t sF[BEAM_MAX_K];
+  __shared__ float sAgain[BEAM_W];
+  __shared__ u64 sPieces[BEAM_W];
   const int tid = threadIdx.x, b = blockIdx.x, per = a.splits * a.n, total = a.K * per;
   const u64* cand = a.cand + (size_t)b * total;
   u64 x[BEAM_PT2];
@@ -300,11 +340,16 @@ __global__ __launch_bounds__(BEAM_T) void beam_join_kernel(BeamArgs a) {
     for (int i = 0; i < BEAM_PT2; ++i) x[i] = c0 + i * BEAM_T + tid < total ? cand[c0 + i * BEAM_T + tid] : 0;
   };
   fetch(0);
+  const float4* part = reinterpret_cast<const float4*>(a.part) + (size_t)b * a.K * a.splits;
+  float again = __builtin_nanf("");                  // the wave's rows' highest score that a piece left out
   for (int k = wave_id(); k < a.K; k += BEAM_W) {
-    const float* p = a.part + 2 * (size_t)(b * a.K + k) * a.splits;
-    float m = -__builtin_inff(), s = 0.f;
+    float m = -__builtin_inff(), s = 0.f, next = -__builtin_inff();
+    const float score = a.scores[b * a.K + k];
+    const bool done = a.finished && a.finished[b * a.K + k];
     for (int i = lane_id(); i < a.splits; i += WAVE) {
-      const float mi = p[2 * i], si = p[2 * i + 1];
+      const float4 p = part[k * a.splits + i];
+      const float mi = p.x, si = p.y;
+      next = fmaxf(next, p.z);
       if (mi > m) {
         s = s * beam_exp(m, mi) + si;
         m = mi;
@@ -314,18 +359,37 @@ __global__ __launch_bounds__(BEAM_T) void beam_join_kernel(BeamArgs a) {
     }
     const float top = wave_maxf(m);
     s = wave_sumf(m > -__builtin_inff() ? s * beam_exp(m, top) : 0.f);
+    const float ls = logf(s);
+    next = wave_maxf(next);
+    if (!done && score > -__builtin_inff()) {
+      // (masked tokens alone are left out in order, unless logits above theirs have no score either)
+      const float c = beam_score(score, next, top, ls);
+      if (!(again >= c) && (next > -__builtin_inff() || beam_unsure<XT>(score, next, top, ls, c))) again = c;
+    }
     if (lane_id() == 0) {
       sM[k] = top;
-      sL[k] = logf(s);
-      sS[k] = a.scores[b * a.K + k];
-      sF[k] = a.finished ? a.finished[b * a.K + k] : 0;
+      sL[k] = ls;
+      sS[k] = score;
+      sF[k] = done;
     }
   }
+  if (lane_id() == 0) sAgain[wave_id()] = again;
   for (int i = tid; i < a.n; i += BEAM_T) kept[i] = 0;
   __syncthreads();
+  // the entries of this pass and the n best before them
+  auto select = [&](u64* key) __attribute__((always_inline)) {
+    float val[BEAM_PT2 + 1], m = -__builtin_inff();
+#pragma unroll
+    for (int i = 0; i <= BEAM_PT2; ++i) {
+      val[i] = key[i] ? beam_key_value(key[i]) : -__builtin_inff();
+      m = fmaxf(m, val[i]);
+    }
+    __syncthreads();                                 // (kept is read)
+    beam_select<false, BEAM_PT2 + 1>(sh, val, m, a.n, [&](int i) { return key[i]; }, [&](int i, u64 k) { kept[i] = k; });
+    __syncthreads();
+  };
   for (int c0 = 0; c0 < total; c0 += BEAM_PT2 * BEAM_T) {
     u64 key[BEAM_PT2 + 1];
-    float val[BEAM_PT2 + 1], m = -__builtin_inff();
     if (c0) fetch(c0);
 #pragma unroll
     for (int i = 0; i < BEAM_PT2; ++i) {
@@ -343,14 +407,48 @@ __global__ __launch_bounds__(BEAM_T) void beam_join_kernel(BeamArgs a) {
     const int fk = tid - a.n;
     if (c0 == 0 && fk >= 0 && fk < a.K && sF[fk] && a.eos >= a.n)
       key[BEAM_PT2] = beam_key(beam_value(sS[fk]), (uint32_t)fk * a.V + a.eos);
-#pragma unroll
-    for (int i = 0; i <= BEAM_PT2; ++i) {
-      val[i] = key[i] ? beam_key_value(key[i]) : -__builtin_inff();
-      m = fmaxf(m, val[i]);
+    select(key);
+  }
+  // Equal scores on both sides of a piece's n-th place, the group's n-th score among them: what such pieces
+  // left out of this score, pieces in the order of their indices.
+  const float least = beam_key_value(kept[a.n - 1]);
+  bool more = sAgain[0] == least || sAgain[1] == least || sAgain[2] == least || sAgain[3] == least;
+  const int pieces = a.K * a.splits;
+  for (int p0 = 0; more && p0 < pieces; p0 += BEAM_T) {
+    bool mine = false;
+    if (p0 + tid < pieces) {
+      const int p = p0 + tid, k = p / a.splits;
+      const float x = part[p].z, c = beam_score(sS[k], x, sM[k], sL[k]);
+      mine = !sF[k] && sS[k] > -__builtin_inff() && c == least && beam_unsure<XT>(sS[k], x, sM[k], sL[k], c);
     }
-    __syncthreads();                                 // (kept is read)
-    beam_select<BEAM_PT2 + 1>(sh, val, m, a.n, kept, [&](int i) { return key[i]; });
+    const u64 who = __ballot(mine);
+    __syncthreads();                                 // (the pieces before are read)
+    if (lane_id() == 0) sPieces[wave_id()] = who;
     __syncthreads();
+    for (int i = 0; more && i < BEAM_T; ++i) {
+      if (!(sPieces[i / WAVE] >> (i % WAVE) & 1)) continue;
+      const int p = p0 + i, k = p / a.splits, first = (p - k * a.splits) * a.piece, end = min(first + a.piece, a.V);
+      const u64 last = cand[(size_t)p * a.n + a.n - 1];
+      // (n of this score or above lie before this piece)
+      more = (uint32_t)k * a.V + first <= beam_key_index(kept[a.n - 1]);
+      for (int c0 = first; more && c0 < end; c0 += BEAM_PT2 * BEAM_T) {
+        u64 key[BEAM_PT2 + 1];
+#pragma unroll
+        for (int j = 0; j < BEAM_PT2; ++j) {
+          const int at = c0 + j * BEAM_T + tid;
+          key[j] = 0;
+          if (at < end) {
+            float x;
+            beam_load<XT, 1>(a, (size_t)b * a.K + k, at, &x);
+            x = beam_value(x);
+            if (beam_key(x, at) < last && beam_score(sS[k], x, sM[k], sL[k]) == least)
+              key[j] = beam_key(least, (uint32_t)k * a.V + at);
+          }
+        }
+        key[BEAM_PT2] = tid < a.n ? kept[tid] : 0;
+        select(key);
+      }
+    }
   }
   beam_write(a, b, kept);
 }
@@ -391,10 +489,10 @@ __global__ __launch_bounds__(BEAM_T) void beam_small_kernel(BeamArgs a) {
       best = fmaxf(best, x[j]);
     }
   }
-  beam_select<R * PER>(sh, v, best, a.n, kept, [&](int i) {
+  beam_select<false, R * PER>(sh, v, best, a.n, [&](int i) {
     const int k = w + BEAM_W * (i / PER), at = i % PER * WAVE + l;
     return k < a.K && at < a.V ? beam_key(v[i], (uint32_t)k * a.V + at) : 0;
-  });
+  }, [&](int i, u64 k) { kept[i] = k; });
   __syncthreads();
   beam_write(a, b, kept);
 }
@@ -418,9 +516,10 @@ static void beam_small_go(const BeamArgs& a, hipStream_t s) {
 static bool beam_small(int K, int V) { return K <= 4 ? V <= 2048 : K <= 8 ? V <= 1024 : K <= 16 && V <= 512; }
 // Entries a thread keeps: 32 when that still gives every CU four workgroups, else 8.
 static int beam_per_thread(int rows, int V) { return (int64_t)rows * ((V + 32 * BEAM_T - 1) / (32 * BEAM_T)) >= 1024 ? 32 : 8; }
+int beam_piece(int rows, int V) { return beam_per_thread(rows, V) * BEAM_T; }
 int beam_splits(int rows, int K, int V) {
   if (beam_small(K, V)) return 0;
-  const int per = beam_per_thread(rows, V) * BEAM_T;
+  const int per = beam_piece(rows, V);
   return (V + per - 1) / per;
 }
 
@@ -433,7 +532,8 @@ hipError_t launch_beam(int dtype, const BeamArgs& a, hipStream_t s) {
   if (dtype == W4_F32) a.vec ? beam_go<W4_F32, 4>(a, pt, s) : beam_go<W4_F32, 1>(a, pt, s);
   else if (dtype == W4_BF16) a.vec ? beam_go<W4_BF16, 8>(a, pt, s) : beam_go<W4_BF16, 1>(a, pt, s);
   else a.vec ? beam_go<W4_F16, 8>(a, pt, s) : beam_go<W4_F16, 1>(a, pt, s);
-  hipLaunchKernelGGL(beam_join_kernel, dim3(a.B), dim3(BEAM_T), 0, s, a);
+  auto join = dtype == W4_F32 ? beam_join_kernel<W4_F32> : dtype == W4_BF16 ? beam_join_kernel<W4_BF16> : beam_join_kernel<W4_F16>;
+  hipLaunchKernelGGL(join, dim3(a.B), dim3(BEAM_T), 0, s, a);
   return hipGetLastError();
 }
 

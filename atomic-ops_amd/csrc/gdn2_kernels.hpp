@@ -416,7 +416,7 @@ size_t w4_workspace_bytes(int dtype, int group, const W4Args& a);
 hipError_t launch_w4(int dtype, int group, const W4Args& a, hipStream_t s);
 
 // Beam search's selection (gdn2_beam.hip).  logits (B K, V) rows of ld elements; part: per row and split
-// (maximum, sum of exp); cand: per row and split n keys.
+// (maximum, sum of exp, the next logit behind the n best, -); cand: per row and split n keys.
 constexpr int BEAM_MAX_N = 128, BEAM_MAX_K = 128;
 struct BeamArgs {
   const void* logits;
@@ -427,10 +427,11 @@ struct BeamArgs {
   int64_t *tokens, *rows;
   float* out_scores;
   uint8_t* out_finished;
-  int B, K, V, n, eos, splits, vec;
+  int B, K, V, n, eos, splits, piece, vec;    // splits of piece entries
   size_t ld;
 };
 int beam_splits(int rows, int K, int V);        // 0: no workspace
+int beam_piece(int rows, int V);
 hipError_t launch_beam(int dtype, const BeamArgs& a, hipStream_t s);
 
 // Linear work index of this workgroup such that consecutive indices (workgroups of one
