@@ -119,20 +119,22 @@ def quantize_w4(weight, group_size: int = 128, symmetric: bool = False) -> W4Wei
     _check_group(group_size)
     if weight.dim() != 2 or weight.numel() == 0 or not weight.is_floating_point():
         raise ValueError(f"weight must be a floating-point (in, out) matrix, got {weight.dtype} {tuple(weight.shape)}")
-    if not bool(torch.isfinite(weight).all()):
-        raise ValueError("weight must be finite")
     K, N = weight.shape
     groups = -(-K // group_size)
     w = torch.zeros((groups * group_size, N), dtype=torch.float32, device=weight.device)
     w[:K] = weight.detach()
+    if not bool(torch.isfinite(w).all()):
+        raise ValueError("weight must be finite in float32")
     w = w.view(groups, group_size, N)
     if symmetric:
         scales, zeros = w.abs().amax(1) / 7, None
     else:
         lo, hi = w.amin(1).clamp(max=0), w.amax(1).clamp(min=0)
         scales = (hi - lo) / 15
-    # codes are chosen for the scale as it is kept; a group of zeros has any
-    scales = torch.where(scales > 0, scales, 1.0).to(torch.bfloat16)
+        scales = torch.where(torch.isinf(scales), hi / 15 - lo / 15, scales)         # (hi - lo above float32)
+    # codes are chosen for the scale as it is kept; a group of zeros, or below bfloat16's least scale, has any
+    scales = scales.to(torch.bfloat16)
+    scales = torch.where(scales > 0, scales, torch.ones_like(scales))
     s = scales.float()
     if symmetric:
         offset = torch.full_like(s, 8.0)
