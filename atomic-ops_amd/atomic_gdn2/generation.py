@@ -307,10 +307,13 @@ class Generator:
     def _captured(self, r, cache, n_beams, eos_id):
         """One step and its selection as a HIP graph that works in place on r and cache: its replay.  A step
         of the benchmark LM is 75 launches, bound by the host: 0.66 ms, as a graph 0.33 (8 rows).  The
-        caches are copied back inside the graph."""
+        caches are copied back inside the graph.  The capture is on a stream of the model's device (torch's own
+        one belongs to the device that was current at the process's first capture), and other threads may
+        use the GPU meanwhile."""
         keep = [r.tokens, r.rows, r.scores, *([] if r.finished is None else [r.finished]), *cache.states, *cache.history]
         graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph):
+        with torch.cuda.device(self.device), torch.cuda.graph(graph, stream=torch.cuda.Stream(self.device),
+                                                              capture_error_mode="thread_local"):
             logits, new = self.step(r.tokens.view(-1), cache, r.rows.view(-1))
             s = beam_step(logits, r.scores, n=n_beams, finished=r.finished, eos_id=eos_id)
             for old, t in zip(keep, [s.tokens, s.rows, s.scores, *([] if s.finished is None else [s.finished]),
