@@ -14,6 +14,7 @@ by float32 rounding and one rounding to its own type.  For inference: no gradien
 from __future__ import annotations
 
 import ctypes
+import operator
 
 import torch
 
@@ -27,14 +28,37 @@ _KB, _NB = 128, 16          # rows and columns of a block of the layout
 _NIBBLE = (0, 2, 4, 6, 1, 3, 5, 7)
 
 
+def _int(x):
+    """x as an int where it is a whole number of another type."""
+    return operator.index(x) if hasattr(x, "__index__") else x
+
+
 class W4Weight:
     """A matrix (in_features, out_features) of 4-bit codes with group scales, laid out for the kernels
-    (include/gdn2.h, ``gdn2_w4``)."""
+    (include/gdn2.h, ``gdn2_w4``): q (out / 16, in / 128, 64, 4) and meta (out / 16, in / group_size, 16),
+    int32, sizes rounded up to whole blocks of 128 rows and 16 columns."""
     __slots__ = ("q", "meta", "in_features", "out_features", "group_size")
 
     def __init__(self, q, meta, in_features, out_features, group_size):
         self.q, self.meta = q, meta
-        self.in_features, self.out_features, self.group_size = in_features, out_features, group_size
+        self.in_features, self.out_features, self.group_size = _int(in_features), _int(out_features), _int(group_size)
+        self._check()
+
+    def _check(self):
+        """Raise unless q and meta are what the sizes say: the kernels read by the sizes."""
+        _check_group(self.group_size)
+        for n in ("in_features", "out_features"):
+            if type(getattr(self, n)) is not int or getattr(self, n) < 1:
+                raise ValueError(f"{n} must be a positive int, got {getattr(self, n)!r}")
+        nkb, nnb = -(-self.in_features // _KB), -(-self.out_features // _NB)
+        for t, n, shape in ((self.q, "q", (nnb, nkb, 64, 4)), (self.meta, "meta", (nnb, nkb * _KB // self.group_size, _NB))):
+            if not isinstance(t, torch.Tensor) or t.dtype != torch.int32:
+                raise TypeError(f"{n} must be an int32 tensor, got {getattr(t, 'dtype', type(t).__name__)}")
+            if tuple(t.shape) != shape or not t.is_contiguous():
+                raise ValueError(f"{n} must be contiguous {shape} for a weight of {self.in_features} x {self.out_features} in "
+                                 f"groups of {self.group_size}, got {tuple(t.shape)}")
+        if self.q.device != self.meta.device:
+            raise ValueError(f"meta is on {self.meta.device}, q on {self.q.device}")
 
     @property
     def shape(self):
@@ -72,8 +96,9 @@ class W4Weight:
 
 
 def _check_group(group_size):
-    if group_size not in GROUP_SIZES:
+    if type(group_size) is not int or group_size not in GROUP_SIZES:
         raise ValueError(f"group_size={group_size}: the kernels support groups of {', '.join(map(str, GROUP_SIZES))} rows")
+    return group_size
 
 
 def pack_w4(codes, scales, zeros=None, group_size: int = 128) -> W4Weight:
@@ -81,7 +106,7 @@ def pack_w4(codes, scales, zeros=None, group_size: int = 128) -> W4Weight:
 
     codes (in, out): whole numbers 0 .. 15; scales (groups, out), groups = ceil(in / group_size), kept
     as bfloat16; zeros (groups, out), kept as bfloat16, or None: 8 everywhere."""
-    _check_group(group_size)
+    group_size = _check_group(_int(group_size))
     if codes.dim() != 2 or codes.numel() == 0:
         raise ValueError(f"codes must be (in, out), got {tuple(codes.shape)}")
     if codes.is_floating_point() or codes.is_complex() or codes.dtype == torch.bool:
@@ -116,7 +141,7 @@ def quantize_w4(weight, group_size: int = 128, symmetric: bool = False) -> W4Wei
     """The matrix ``weight`` (in, out) rounded to 4-bit codes, each to the nearest of its group's grid:
     16 levels from the group's least to its largest entry (and 0, which stays exactly 0), or with
     ``symmetric`` 15 levels around 0 and no zeros to choose."""
-    _check_group(group_size)
+    group_size = _check_group(_int(group_size))
     if weight.dim() != 2 or weight.numel() == 0 or not weight.is_floating_point():
         raise ValueError(f"weight must be a floating-point (in, out) matrix, got {weight.dtype} {tuple(weight.shape)}")
     K, N = weight.shape
@@ -164,6 +189,7 @@ def w4_linear(x, weight: W4Weight, bias=None, residual=None):
             return y
     if not isinstance(weight, W4Weight):
         raise TypeError(f"weight must be a W4Weight (pack_w4, quantize_w4), got {type(weight).__name__}")
+    weight._check()
     if x.dtype not in _DTYPES:
         raise TypeError(f"x must be float32, bfloat16 or float16, got {x.dtype}")
     K, N = weight.shape

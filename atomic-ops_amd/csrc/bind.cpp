@@ -467,6 +467,11 @@ PyObject* py_w4(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (kind < 0 || !ldx || !plain(x, dev) || M > INT32_MAX || K > INT32_MAX || N > INT32_MAX) return none();
   for (const Tensor* t : {&q, &meta})
     if (!plain(*t, dev) || t->scalar_type() != at::kInt || !t->is_contiguous()) return none();
+  // (the kernels read by K, N and group: a weight whose tensors have other sizes is not theirs)
+  const int64_t blocks = ((N + 15) / 16) * ((K + 127) / 128);
+  if (K < 1 || N < 1 || (group != 32 && group != 64 && group != 128) || q.numel() != 256 * blocks ||
+      meta.numel() != 16 * (128 / group) * blocks)
+    return none();
   if (bias.defined() && (!plain(bias, dev) || bias.scalar_type() != dt || bias.dim() != 1 || bias.size(0) != N || !bias.is_contiguous()))
     return none();
   int64_t ldr = 0;
