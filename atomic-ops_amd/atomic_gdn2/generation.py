@@ -8,7 +8,8 @@
 
 A beam that is kept continues the sequence of its parent, so its caches are its parent's.  Both caches
 of a block are taken from the parent's row where a step reads them anyway (``parents`` here and in
-``inference.decode_step``): nothing is copied to reorder them.  For inference: no gradients.
+``inference.decode_step``): nothing is copied to reorder them.  For inference: no gradients; asking
+``beam_step`` or ``premix_step`` for one raises.
 """
 from __future__ import annotations
 
@@ -19,7 +20,7 @@ import torch
 
 from . import _lib, lm_kernels
 from .inference import chunk_forward_inference, decode_step
-from .w4 import quantize_w4, w4_linear
+from .w4 import for_inference, quantize_w4, w4_linear
 
 __all__ = ["BeamStep", "PremixStep", "beam_step", "premix_step", "Cache", "BeamResult", "Generator"]
 
@@ -72,6 +73,9 @@ def beam_step(logits, scores, n: Optional[int] = None, finished=None, eos_id: Op
         out = _lib.bind().beam(logits, scores, scores.shape[-1] if n is None else n, finished, -1 if eos_id is None else eos_id)
         if out is not None:
             return BeamStep(*out, None) if eos_id is None else BeamStep(*out)
+    out = for_inference("beam_step", lambda *ts: beam_step(*ts, n=n, finished=finished, eos_id=eos_id), logits, scores)
+    if out is not None:
+        return BeamStep(*out)
     if scores.dim() != 2 or scores.numel() == 0:
         raise ValueError(f"scores must be (B, K), got {tuple(scores.shape)}")
     B, K = scores.shape
@@ -121,10 +125,16 @@ def premix_step(y, history, conv_w, conv_b, gate_b, decay_b, decay_a, n_heads: i
     the convolutions' taps and biases for q, k, v; gate_b two (C,): the erase and write gates' biases;
     decay_b, decay_a (H,).  parents (R,) int32 or int64: the history row that each row continues (one
     outside 0 .. S-1 has none: zeros); None: its own.  All float32 but parents."""
+    n_w, n_b = len(conv_w), len(conv_b)
     if isinstance(y, torch.Tensor) and y.is_cuda and type(n_heads) is int and type(g_max) is float:
         out = _lib.bind().premix_step(y, history, (*conv_w, *conv_b, *gate_b, decay_b, decay_a), n_heads, g_max, parents)
         if out is not None:
             return PremixStep(*out)
+    out = for_inference("premix_step", lambda y, history, *ws: premix_step(
+        y, history, ws[:n_w], ws[n_w:n_w + n_b], ws[n_w + n_b:-2], *ws[-2:], n_heads=n_heads, g_max=g_max, parents=parents),
+        y, history, *conv_w, *conv_b, *gate_b, decay_b, decay_a)
+    if out is not None:
+        return PremixStep(*out)
     H = int(n_heads)
     if y.dim() != 2 or history.dim() != 3 or H < 1 or history.shape[1] != 3 or history.shape[2] % (3 * H) or history.shape[2] == 0:
         raise ValueError(f"y must be (R, columns) and history (S, 3, 3 H D), got {tuple(y.shape)} and {tuple(history.shape)}")

@@ -9,7 +9,8 @@ and a zero for each column and group of ``group_size`` (32, 64 or 128) rows:
 out once, when a model is loaded, in the order in which the kernels read them (``W4Weight``).
 ``w4_linear`` multiplies: float32, bfloat16 or float16 rows, one (a token) or thousands (a prompt).
 Codes enter the products as they are and sums are float32, so a result differs from the definition's
-by float32 rounding and one rounding to its own type.  For inference: no gradients.
+by float32 rounding and one rounding to its own type.  For inference: no gradients, and asking for one
+raises.
 """
 from __future__ import annotations
 
@@ -17,6 +18,7 @@ import ctypes
 import operator
 
 import torch
+import torch.autograd.forward_ad as fwd
 
 from . import _lib
 
@@ -31,6 +33,28 @@ _NIBBLE = (0, 2, 4, 6, 1, 3, 5, 7)
 def _int(x):
     """x as an int where it is a whole number of another type."""
     return operator.index(x) if hasattr(x, "__index__") else x
+
+
+class _Inference(torch.autograd.Function):
+    """fn(*ts) as a node whose gradients raise.  (It has no forward mode either: a tangent raises.)"""
+
+    @staticmethod
+    def forward(ctx, name, fn, *ts):
+        ctx.name = name
+        return fn(*ts)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"{ctx.name} is for inference and has no gradients: call it under torch.no_grad(), or detach its inputs")
+
+
+def for_inference(name, fn, *ts):
+    """fn(*ts) where a gradient or tangent of one of ts is not to be lost in silence, else None."""
+    if (torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in ts)) \
+            or fwd._current_level >= 0 and any(
+                isinstance(t, torch.Tensor) and fwd.unpack_dual(t).tangent is not None for t in ts):
+        return _Inference.apply(name, fn, *ts)
+    return None
 
 
 class W4Weight:
@@ -187,6 +211,9 @@ def w4_linear(x, weight: W4Weight, bias=None, residual=None):
         y = _lib.bind().w4(x, weight.q, weight.meta, weight.in_features, weight.out_features, weight.group_size, bias, residual)
         if y is not None:
             return y
+    y = for_inference("w4_linear", lambda *ts: w4_linear(ts[0], weight, *ts[1:]), x, bias, residual)
+    if y is not None:
+        return y
     if not isinstance(weight, W4Weight):
         raise TypeError(f"weight must be a W4Weight (pack_w4, quantize_w4), got {type(weight).__name__}")
     weight._check()

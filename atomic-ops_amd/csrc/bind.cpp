@@ -431,6 +431,13 @@ int64_t row_stride(const Tensor& t, int64_t n) {
   if (t.is_contiguous()) return n;
   return t.dim() == 2 && t.stride(1) == 1 && (t.stride(0) >= n || t.size(0) == 1) ? std::max(t.stride(0), n) : 0;
 }
+// Whether gradients are recorded of one of ts: Python's path has the error for them.
+bool recorded(std::initializer_list<const Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : ts)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
 PyObject* tuple_of(std::initializer_list<const Tensor*> ts) {
   PyObject* out = PyTuple_New((Py_ssize_t)ts.size());
   Py_ssize_t i = 0;
@@ -481,6 +488,7 @@ PyObject* py_w4(PyObject*, PyObject* const* args, Py_ssize_t n) {
       if (res.size(i) != x.size(i)) return none();
     if (!(ldr = row_stride(res, N))) return none();
   }
+  if (recorded({&x, &bias, &res})) return none();
   gdn2_w4 a{};
   a.M = (int32_t)M; a.K = (int32_t)K; a.N = (int32_t)N; a.group = (int32_t)group;
   a.dtype = kind; a.ldx = ldx; a.ldr = ldr;
@@ -527,6 +535,7 @@ PyObject* py_beam(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
                         !fin.is_contiguous()))
     return none();
   if (B > 65535 || K > 65535 || V > INT32_MAX || n < 1 || n > INT32_MAX || eos < -1 || eos > INT32_MAX) return none();
+  if (recorded({&x, &scores})) return none();
   gdn2_beam a{};
   a.B = (int32_t)B; a.K = (int32_t)K; a.V = (int32_t)V; a.n = (int32_t)n; a.eos = (int32_t)eos;
   a.dtype = kind; a.ld = ld;
@@ -584,8 +593,10 @@ PyObject* py_premix_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int64_t len = i < 8 ? C : H;
     if (!ready(t) || !t.is_contiguous() || t.numel() != (i < 3 ? 4 * C : len) || t.size(0) != len || t.dim() != (i < 3 ? 2 : 1))
       return none();
+    if (recorded({&t})) return none();
     ps[i] = f32_at(t);
   }
+  if (recorded({&y, &past})) return none();
   a.R = (int32_t)R; a.S = (int32_t)S; a.H = (int32_t)H; a.D = (int32_t)D; a.ldy = (int32_t)ldy;
   a.g_max = (float)PyFloat_AS_DOUBLE(args[4]);
   a.y = f32_at(y); a.history = f32_at(past);
