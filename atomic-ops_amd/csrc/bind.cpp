@@ -591,7 +591,7 @@ PyObject* py_premix_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
   for (int i = 0; i < 10; ++i) {
     const Tensor& t = THPVariable_Unpack(PyTuple_GET_ITEM(args[2], i));
     const int64_t len = i < 8 ? C : H;
-    if (!ready(t) || !t.is_contiguous() || t.numel() != (i < 3 ? 4 * C : len) || t.size(0) != len || t.dim() != (i < 3 ? 2 : 1))
+    if (!ready(t) || !t.is_contiguous() || t.dim() != (i < 3 ? 2 : 1) || t.numel() != (i < 3 ? 4 * C : len) || t.size(0) != len)
       return none();
     if (recorded({&t})) return none();
     ps[i] = f32_at(t);
