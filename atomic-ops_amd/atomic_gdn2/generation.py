@@ -125,13 +125,15 @@ def premix_step(y, history, conv_w, conv_b, gate_b, decay_b, decay_a, n_heads: i
     the convolutions' taps and biases for q, k, v; gate_b two (C,): the erase and write gates' biases;
     decay_b, decay_a (H,).  parents (R,) int32 or int64: the history row that each row continues (one
     outside 0 .. S-1 has none: zeros); None: its own.  All float32 but parents."""
-    n_w, n_b = len(conv_w), len(conv_b)
+    conv_w, conv_b, gate_b = tuple(conv_w), tuple(conv_b), tuple(gate_b)
+    if (len(conv_w), len(conv_b), len(gate_b)) != (3, 3, 2):
+        raise ValueError("three convolutions (taps and biases) and two gates are needed")
     if isinstance(y, torch.Tensor) and y.is_cuda and type(n_heads) is int and type(g_max) is float:
         out = _lib.bind().premix_step(y, history, (*conv_w, *conv_b, *gate_b, decay_b, decay_a), n_heads, g_max, parents)
         if out is not None:
             return PremixStep(*out)
     out = for_inference("premix_step", lambda y, history, *ws: premix_step(
-        y, history, ws[:n_w], ws[n_w:n_w + n_b], ws[n_w + n_b:-2], *ws[-2:], n_heads=n_heads, g_max=g_max, parents=parents),
+        y, history, ws[:3], ws[3:6], ws[6:8], *ws[8:], n_heads=n_heads, g_max=g_max, parents=parents),
         y, history, *conv_w, *conv_b, *gate_b, decay_b, decay_a)
     if out is not None:
         return PremixStep(*out)
@@ -150,8 +152,6 @@ def premix_step(y, history, conv_w, conv_b, gate_b, decay_b, decay_a, n_heads: i
     ps.update({f"conv_b[{i}]": (t, (C,)) for i, t in enumerate(conv_b)})
     ps.update({f"gate_b[{i}]": (t, (C,)) for i, t in enumerate(gate_b)})
     ps.update(decay_b=(decay_b, (H,)), decay_a=(decay_a, (H,)))
-    if len(ps) != 10:
-        raise ValueError("three convolutions (taps and biases) and two gates are needed")
     for n, (t, shape) in ps.items():
         if tuple(t.shape) != shape:
             raise ValueError(f"{n} must be {shape}, got {tuple(t.shape)}")

@@ -29,3 +29,13 @@ def test_premix_parameters_without_dimensions(name):
     kw["conv_b"][1] = torch.zeros((), device="cuda")
     with pytest.raises(ValueError, match="conv_b.1. must be"):
         premix_step(**kw)
+
+
+def test_premix_parameters_of_another_count():
+    """Ten tensors in all are not enough: three taps, three biases of theirs, two of the gates."""
+    from atomic_gdn2.generation import premix_step
+    for a, b in (("conv_b", "gate_b"), ("gate_b", "conv_b"), ("conv_w", "conv_b")):
+        kw = _premix()
+        kw[b].append(kw[a].pop())
+        with pytest.raises(ValueError):
+            premix_step(**kw)
