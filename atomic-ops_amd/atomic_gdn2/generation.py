@@ -68,7 +68,7 @@ def beam_step(logits, scores, n: Optional[int] = None, finished=None, eos_id: Op
     continuation, eos_id at its own score; a beam that takes eos_id is finished.  Each group's
     result does not depend on the others, and equal inputs give equal bits."""
     if isinstance(logits, torch.Tensor) and logits.is_cuda and (finished is None or eos_id is not None) \
-            and (eos_id is None or type(eos_id) is int and eos_id >= 0) and (n is None or type(n) is int):
+            and (eos_id is None or type(eos_id) is int and eos_id >= 0) and (n is None or type(n) is int) and scores.dim() == 2:
         # plain calls (csrc/bind.cpp) go native; None = not one, and what follows handles it
         out = _lib.bind().beam(logits, scores, scores.shape[-1] if n is None else n, finished, -1 if eos_id is None else eos_id)
         if out is not None:

@@ -39,3 +39,9 @@ def test_premix_parameters_of_another_count():
         kw[b].append(kw[a].pop())
         with pytest.raises(ValueError):
             premix_step(**kw)
+
+
+def test_beam_scores_without_dimensions():
+    from atomic_gdn2.generation import beam_step
+    with pytest.raises(ValueError, match="scores must be"):
+        beam_step(torch.zeros((1, 10), device="cuda"), torch.tensor(0.0, device="cuda"))
