@@ -534,7 +534,7 @@ PyObject* py_beam(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   if (fin.defined() && (!plain(fin, dev) || fin.scalar_type() != at::kBool || fin.dim() != 2 || fin.size(0) != B || fin.size(1) != K ||
                         !fin.is_contiguous()))
     return none();
-  if (B > 65535 || K > 65535 || V > INT32_MAX || n < 1 || n > INT32_MAX || eos < -1 || eos > INT32_MAX) return none();
+  if (B > 65535 || K > 65535 || V > INT32_MAX || n < 1 || n > std::min<int64_t>(128, K * V) || eos < -1 || eos >= V) return none();
   if (recorded({&x, &scores})) return none();
   gdn2_beam a{};
   a.B = (int32_t)B; a.K = (int32_t)K; a.V = (int32_t)V; a.n = (int32_t)n; a.eos = (int32_t)eos;

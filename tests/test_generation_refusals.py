@@ -45,3 +45,14 @@ def test_beam_scores_without_dimensions():
     from atomic_gdn2.generation import beam_step
     with pytest.raises(ValueError, match="scores must be"):
         beam_step(torch.zeros((1, 10), device="cuda"), torch.tensor(0.0, device="cuda"))
+
+
+def test_beam_count_is_checked_before_memory_is_taken():
+    from atomic_gdn2.generation import beam_step
+    x, s = torch.zeros((64, 9), device="cuda"), torch.zeros((64, 1), device="cuda")
+    torch.cuda.synchronize()
+    before = torch.cuda.max_memory_reserved()
+    for n in (129, 1 << 20, (1 << 31) - 1):
+        with pytest.raises(ValueError, match=f"n={n}"):
+            beam_step(x, s, n=n)
+    assert torch.cuda.max_memory_reserved() == before
