@@ -84,6 +84,8 @@ def beam_step(logits, scores, n: Optional[int] = None, finished=None, eos_id: Op
     if logits.dtype not in _DTYPES:
         raise TypeError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")
     V = logits.shape[-1]
+    if max(B * K, K * V) >= 2 ** 31:
+        raise ValueError(f"{B} groups of {K} beams over {V} tokens: B K and K V must be below 2^31")
     n = K if n is None else int(n)
     if not 1 <= n <= min(128, K * V):
         raise ValueError(f"n={n}: between 1 and min(128, K V) = {min(128, K * V)} continuations can be kept")
@@ -165,7 +167,7 @@ def premix_step(y, history, conv_w, conv_b, gate_b, decay_b, decay_a, n_heads: i
     parents = _parent_rows(parents, R)
     if not y.is_cuda:
         raise ValueError(f"premix_step needs tensors on a ROCm device, got {dev}")
-    if y.stride(1) != 1 or (y.stride(0) < 6 * C + H and R > 1):
+    if y.stride(1) != 1 or (not 6 * C + H <= y.stride(0) < 2 ** 31 and R > 1):      # (a stride has 32 bits)
         y = y.clone(memory_format=torch.contiguous_format)
     history = history.contiguous()
     cw, cb, gb = ([t.contiguous() for t in ts] for ts in (conv_w, conv_b, gate_b))

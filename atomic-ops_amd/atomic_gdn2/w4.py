@@ -222,6 +222,8 @@ def w4_linear(x, weight: W4Weight, bias=None, residual=None):
     K, N = weight.shape
     if x.dim() == 0 or x.shape[-1] != K:
         raise ValueError(f"x must be (..., {K}), got {tuple(x.shape)}")
+    if x.numel() // K >= 2 ** 31:
+        raise ValueError(f"x has {x.numel() // K} rows: fewer than 2^31 are supported")
     if bias is not None and tuple(bias.shape) != (N,):
         raise ValueError(f"bias must be ({N},), got {tuple(bias.shape)}")
     if residual is not None and tuple(residual.shape) != (*x.shape[:-1], N):
