@@ -271,7 +271,7 @@ class Generator:
         return w4_linear(lm_kernels._rms(x, self.final_norm), self.head)
 
     def _ids(self, ids, dim):
-        if ids.dim() != dim or ids.numel() == 0 or ids.is_floating_point() or ids.dtype == torch.bool:
+        if ids.dim() != dim or ids.numel() == 0 or ids.is_floating_point() or ids.is_complex() or ids.dtype == torch.bool:
             raise ValueError(f"token ids must be whole numbers of {dim} dimensions, not empty, got {ids.dtype} {tuple(ids.shape)}")
         if ids.device != self.device:
             raise ValueError(f"token ids are on {ids.device}, the model on {self.device}")
@@ -280,6 +280,10 @@ class Generator:
     def prefill(self, ids):
         """Prompts ids (B, L) from an empty cache: the logits (B, V) behind the last token, the cache."""
         self._ids(ids, 2)
+        ids = ids.long()
+        lo, hi = (int(v) for v in torch.aminmax(ids))
+        if lo < 0 or hi >= self.cfg.vocab_size:
+            raise ValueError(f"token ids must lie in 0 .. {self.cfg.vocab_size - 1}, got {lo} .. {hi}")
         (B, L), c, cache = ids.shape, self.cfg, Cache([], [])
         H, D, C = c.n_heads, c.d_head, c.proj_dim
         x = self.embed[ids].reshape(B * L, -1)
@@ -302,9 +306,13 @@ class Generator:
 
     @torch.no_grad()
     def step(self, tokens, cache: Cache, rows=None):
-        """One token for each of R sequences: tokens (R,); rows (R,): the row of the cache that each
+        """One token for each of R sequences: tokens (R,), one outside the vocabulary counting as the nearest
+        within (the host does not wait for the tokens to look at them); rows (R,): the row of the cache that each
         sequence continues (None: its own).  The logits (R, V) and the sequences' cache."""
         self._ids(tokens, 1)
+        return self._step(tokens.long().clamp(0, self.cfg.vocab_size - 1), cache, rows)
+
+    def _step(self, tokens, cache, rows):
         R, c, new = tokens.shape[0], self.cfg, Cache([], [])
         x = self.embed[tokens]
         for blk, state, history in zip(self.blocks, cache.states, cache.history):
@@ -326,7 +334,7 @@ class Generator:
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.device(self.device), torch.cuda.graph(graph, stream=torch.cuda.Stream(self.device),
                                                               capture_error_mode="thread_local"):
-            logits, new = self.step(r.tokens.view(-1), cache, r.rows.view(-1))
+            logits, new = self._step(r.tokens.view(-1), cache, r.rows.view(-1))
             s = beam_step(logits, r.scores, n=n_beams, finished=r.finished, eos_id=eos_id)
             for old, t in zip(keep, [s.tokens, s.rows, s.scores, *([] if s.finished is None else [s.finished]),
                                      *new.states, *new.history]):
@@ -359,7 +367,7 @@ class Generator:
                 replay()
                 steps.append((r.tokens.clone(), r.rows - base))
                 continue
-            logits, cache = self.step(r.tokens.view(-1), cache, r.rows.view(-1))
+            logits, cache = self._step(r.tokens.view(-1), cache, r.rows.view(-1))
             r = beam_step(logits, r.scores, n=n_beams, finished=r.finished, eos_id=eos_id)
             # (copies: a graph that is captured next works in place on r)
             steps.append((r.tokens.clone(), r.rows - base) if graph else (r.tokens, r.rows - base))

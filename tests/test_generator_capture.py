@@ -36,7 +36,7 @@ def _bare(monkeypatch, device):
 
     for name, fake in (("device", on), ("Stream", Stream), ("graph", capture), ("CUDAGraph", Graph)):
         monkeypatch.setattr(torch.cuda, name, fake)
-    monkeypatch.setattr(gen, "step", lambda tokens, cache, rows=None: (None, generation.Cache([], [])))
+    monkeypatch.setattr(gen, "_step", lambda tokens, cache, rows: (None, generation.Cache([], [])))
     monkeypatch.setattr(generation, "beam_step", lambda *a, **kw: result())
     result = lambda: generation.BeamStep(torch.zeros((1, 2)), torch.zeros((1, 2)), torch.zeros((1, 2)), None)  # noqa: E731
     return gen, seen, result(), generation.Cache([], [])
@@ -58,7 +58,7 @@ def test_capture_beside_a_thread_that_allocates():
     gen = Generator(e2e_lm.make_lm(e2e_lm.LMConfig(vocab_size=61, d_model=128, n_heads=2, d_head=64, n_layers=2)), group_size=32)
     ids = torch.arange(18, device="cuda").view(2, 9)
     want = gen.beam_search(ids, 3, 12, graph=False)
-    plain, errors, held = gen.step, [], []
+    plain, errors, held = gen._step, [], []
 
     def other():
         try:
@@ -73,7 +73,7 @@ def test_capture_beside_a_thread_that_allocates():
             t.join()
         return plain(*a, **kw)
 
-    gen.step = step
+    gen._step = step
     got = gen.beam_search(ids, 3, 12, graph=True)
     assert held and not errors
     assert torch.equal(got.tokens, want.tokens) and torch.equal(got.scores, want.scores)
