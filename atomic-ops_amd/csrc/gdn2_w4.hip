@@ -889,12 +889,14 @@ __global__ __launch_bounds__(512) void w4_gemm_kernel(W4Args a, W4GemmArgs b) {
 //     four blocks at least (64 rows of 14336 x 4096, 1 / 4 / 8 / 16 parts: 74, 25, 21, 27; 256 of
 //     4096 x 4096, 1 / 2: 21.8, 23.5).
 //   -1: many rows, w4_gemm_kernel, from three workgroups for four CUs on (bfloat16, us, against tiles: 2048
-//     rows of 4096 x 4096 77, 103; 1024 72, 55; 512 of 4096 x 14336 73, 92; 512 of 14336 x 4096 228, 95).
+//     rows of 4096 x 4096 77, 103; 1024 72, 55; 512 of 4096 x 14336 73, 92; 512 of 14336 x 4096 228, 95) and
+//     more than half a tile of rows, since it multiplies whole ones (rows of 4096 x 131072: 16 133, 66; 64
+//     138, 131; 96 146, 190; 256 306, 487; float32, tiles of 64, 4096 x 50257: 32 83, 68; 64 89, 133).
 template <int XT, int GROUP>
 using W4Tiles = W4Tile<XT, GROUP, 2, 2, 1, 4, 2>;
 static bool w4_many(int dtype, int M, int nnb) {
   const int bm = dtype == W4_F32 ? W4Gemm<W4_F32, 128>::BM : W4Gemm<W4_BF16, 128>::BM, bn = W4Gemm<W4_BF16, 128>::BN;
-  return (int64_t)((M + bm - 1) / bm) * ((16 * nnb + bn - 1) / bn) * 4 >= (int64_t)cu_count() * 3;
+  return M > bm / 2 && (int64_t)((M + bm - 1) / bm) * ((16 * nnb + bn - 1) / bn) * 4 >= (int64_t)cu_count() * 3;
 }
 static int w4_parts(int dtype, int M, int nkb, int nnb) {
   using C = W4Tiles<W4_BF16, 128>;
