@@ -351,6 +351,11 @@ class Generator:
         if max_new_tokens < 1:
             raise ValueError(f"max_new_tokens={max_new_tokens}: at least one is needed")
         graph = max_new_tokens >= 48 if graph is None else graph
+        # (the graph is dropped as _search returns, which makes its device the current one)
+        with torch.cuda.device(self.device):
+            return self._search(ids, n_beams, max_new_tokens, eos_id, graph)
+
+    def _search(self, ids, n_beams, max_new_tokens, eos_id, graph):
         logits, cache = self.prefill(ids)
         B = ids.shape[0]
         # the first token's beams all continue the prompt's one row
