@@ -31,7 +31,7 @@ _INDEX = {torch.int32: 1, torch.int64: 2}                                # GDN2_
 class BeamStep(NamedTuple):
     """The kept continuations of each group, the best first, all (B, n): the new tokens (int64), the
     rows b K + k of the beams that they continue (int64: ``parents`` of the next steps), their scores
-    (float32), and whether they are finished (None without an end token)."""
+    (float32), and whether they are finished (None without an end token).  They may share one storage."""
     tokens: torch.Tensor
     rows: torch.Tensor
     scores: torch.Tensor
@@ -40,7 +40,7 @@ class BeamStep(NamedTuple):
 
 class PremixStep(NamedTuple):
     """What the recurrence takes for one token, q, k, v, w, b, g (R, H, D); the output gate's logits
-    (R, H D); the history of the next token (R, 3, 3 H D)."""
+    (R, H D); the history of the next token (R, 3, 3 H D).  All but the history may share one storage."""
     q: torch.Tensor
     k: torch.Tensor
     v: torch.Tensor
@@ -65,8 +65,9 @@ def beam_step(logits, scores, n: Optional[int] = None, finished=None, eos_id: Op
     log_softmax(logits[b, k])[v] in float32; equal scores go to the lower k V + v.  NaN counts as -inf
     (a banned token, a beam that is not in use), and with fewer than n continuations above -inf the
     lowest of the others follow, at -inf.  finished (B, K) bool, with eos_id: a finished beam has one
-    continuation, eos_id at its own score; a beam that takes eos_id is finished.  Each group's
-    result does not depend on the others, and equal inputs give equal bits."""
+    continuation, eos_id at its own score; a beam that takes eos_id is finished.  A group's result
+    does not depend on what the others hold (on their number its scores' last bits do), and equal inputs
+    give equal bits."""
     if isinstance(logits, torch.Tensor) and logits.is_cuda and (finished is None or eos_id is not None) \
             and (eos_id is None or type(eos_id) is int and eos_id >= 0) and (n is None or type(n) is int) and scores.dim() == 2:
         # plain calls (csrc/bind.cpp) go native; None = not one, and what follows handles it

@@ -9,7 +9,8 @@ and a zero for each column and group of ``group_size`` (32, 64 or 128) rows:
 out once, when a model is loaded, in the order in which the kernels read them (``W4Weight``).
 ``w4_linear`` multiplies: float32, bfloat16 or float16 rows, one (a token) or thousands (a prompt).
 Codes enter the products as they are and sums are float32, so a result differs from the definition's
-by float32 rounding and one rounding to its own type.  For inference: no gradients, and asking for one
+by float32 rounding (of entries below 1e-33 of a float32 row, by their bits below 2^-133) and one
+rounding to its own type.  For inference: no gradients, and asking for one
 raises.
 """
 from __future__ import annotations

@@ -7,8 +7,9 @@
 // 0 .. 15 read as an fp8 e4m3 number is q 2^-9 (its subnormals and first binade are one even grid), so
 // two masks and four conversions with the scale 2^9 make eight operands of a word of eight nibbles.
 // Activations of 16 bits are the other operand as they are, of float32 as three bfloat16 pieces of
-// eight bits each, whose sum is x.  So no product is rounded; sums, group sums of x and the scaling
-// are float32, and y is rounded once.
+// eight bits each, whose sum is x but for bits below 2^-133, bfloat16's smallest number (so an x below
+// about 1e-33 has fewer than 24 bits).  So no product is rounded; sums, group sums of x and the
+// scaling are float32, and y is rounded once.
 #include "gdn2_kernels.hpp"
 
 namespace gdn2 {
@@ -392,9 +393,10 @@ __global__ __launch_bounds__(w4_waves(XT, NB) * WAVE) void w4_rows_kernel(W4Args
 // caches once for all the columns: a CU takes about 34 bytes a nanosecond from the L2, and with x in
 // every wave's registers that was the bound.  The next blocks are loaded while these are multiplied.
 // With several parts the sums go to a.part (part, M, N), which w4_join_kernel adds in order.
-//   32 rows of 14336 x 4096 bfloat16: 14.1 us (32 MB, 2.3 TB/s), of that the join 3: a workgroup has seven
+//   32 rows of 14336 x 4096: 13.6 us bfloat16, 13.3 float16, 20.7 float32 with the weights (32 MB) in the
+// last-level cache, 14.0, 14.1 and 21.2 from HBM (2.3 TB/s), of that the join 2 to 4: a workgroup has seven
 // rounds of staging, a barrier, products and scaling, one after the other (weights loaded two rounds ahead
-// instead of one: 14.3).  128 rows of 4096 x 4096 15.4.
+// instead of one, bfloat16: 14.5 for 14.3).  128 rows of 4096 x 4096 15.4.
 template <int XT_, int GROUP_, int MT_, int NBW_, int WM_, int WN_, int WK_>
 struct W4Tile {
   static constexpr int XT = XT_, GROUP = GROUP_, MT = MT_, NBW = NBW_, WM = WM_, WN = WN_, WK = WK_;
@@ -650,8 +652,8 @@ __global__ __launch_bounds__(256) void w4_join_kernel(W4Args a, int parts) {
 // BM rows and 256 columns, a wave 16 MT rows and 64 columns: x comes into LDS by DMA, a block ahead of
 // its use, the scale is one fma a group and result, and the zeros are a product of their own behind the
 // sum, (sums of x) x (-s z) over the groups, 32 groups a step: s z has 16 bits, two pieces.
-//   2048 rows of 4096 x 4096 bfloat16: 76 us, 905 TFLOP/s (a large library product of bfloat16 1219), of that
-// the pass over x 4.  With parts of the loop left out: products alone 55, without the DMA 64, without the
+//   2048 rows of 4096 x 4096: 76 us bfloat16 and float16, 905 TFLOP/s (a large library product of bfloat16
+// 1219), of that the pass over x 4; float32, three products each, 188.  With parts of the loop left out: products alone 55, without the DMA 64, without the
 // scaling 70, without the conversions 74, without the products 59.  Zeros in the scaling instead of a product,
 // x staged through registers as in w4_tile_kernel: 112.
 template <int XT_, int GROUP_>
@@ -884,7 +886,8 @@ __global__ __launch_bounds__(512) void w4_gemm_kernel(W4Args a, W4GemmArgs b) {
 //     always; more where the weights come from the caches again, 2^15 tiles of 16 rows and 128 x 16
 //     weights, and the sum is not long beside the columns (bfloat16, us, rows against tiles: 64 rows of
 //     2048 x 2048 5.7, 8.8; 64 of 4096 x 4096 11.8, 11.7; 128 of 4096 x 4096 20.7, 15.1; 16 of
-//     4096 x 14336 12.5, 14.5; 16 of 14336 x 4096 16.8, 13.2).
+//     4096 x 14336 12.5, 14.5; 16 of 14336 x 4096 16.8, 13.2).  Not measured against tiles: float32, and more
+//     than 128 rows of small matrices (2048 float32 rows of 768 x 512 29.8 us, of 1024 x 512 32.6).
 //   parts: two workgroups a CU where that leaves 14 blocks of 128 or more to each, else one, with
 //     four blocks at least (64 rows of 14336 x 4096, 1 / 4 / 8 / 16 parts: 74, 25, 21, 27; 256 of
 //     4096 x 4096, 1 / 2: 21.8, 23.5).

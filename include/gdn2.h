@@ -325,8 +325,8 @@ int gdn2_lm_premix_step_fwd(const gdn2_lm_premix_step* p, void* stream);
  *         e = 0 .. 7, of column l % 16, element e < 4 in nibble 2 e, e >= 4 in nibble 2 e - 7;
  *   meta  (Np / 16, Kp / group, 16) words, scale | zero << 16 as bfloat16 bits; 0 past K and N.
  * group: 32, 64 or 128 rows of W share a scale and a zero.  q and meta 16-byte aligned; workspace
- * gdn2_w4_workspace_bytes (0: none), 16-byte aligned.  M, K <= 2^20, N <= 2^24.  Products are exact and
- * sums float32 (16 K max |x| has to fit); y is rounded once.  A row of x with an infinity or NaN gives
+ * gdn2_w4_workspace_bytes (0: none), 16-byte aligned.  M, K <= 2^20, N <= 2^24.  Products are exact (but
+ * for bits of a float32 x below 2^-133) and sums float32 (16 K max |x| has to fit); y is rounded once.  A row of x with an infinity or NaN gives
  * nothing finite, and touches no other row. */
 enum { GDN2_F32 = 0, GDN2_BF16 = 1, GDN2_F16 = 2 };
 typedef struct gdn2_w4 {
@@ -344,7 +344,8 @@ int gdn2_w4_linear(const gdn2_w4* p, void* workspace, void* stream);
  * beam whose score or whose logits are all -inf.  finished NULL or B*K bytes: a beam with a nonzero one has a single
  * continuation, the token eos at the beam's own score (0 <= eos < V).  eos -1: none.
  * tokens, rows (B, n): v and b K + k; out_scores (B, n); out_finished NULL or (B, n) bytes: whether
- * the beam was finished or v is eos.  1 <= n <= 128, n <= K V, K <= 128, K V < 2^31.
+ * the beam was finished or v is eos.  1 <= n <= 128, n <= K V, K <= 128, K V < 2^31,
+ * B K <= 65535.
  * workspace: gdn2_beam_workspace_bytes (0: none), 16-byte aligned. */
 typedef struct gdn2_beam {
   int32_t B, K, V, n, eos, dtype;
