@@ -71,6 +71,31 @@ class Gdn2Beam(ctypes.Structure):
                     (n, _vp) for n in ("logits", "scores", "finished", "tokens", "rows", "out_scores", "out_finished")]
 
 
+class Gdn2Product(ctypes.Structure):
+    """``struct gdn2_product`` (include/gdn2.h)."""
+    _fields_ = [(n, _c_int) for n in ("M", "K", "N", "form", "dtype", "out_dtype", "bias_dtype", "activation")] + [
+        (n, ctypes.c_int64) for n in ("lda", "ldb", "ldr")] + [(n, _vp) for n in ("a", "b", "bias", "residual", "y", "z")]
+
+
+class Gdn2Slope(ctypes.Structure):
+    """``struct gdn2_slope`` (include/gdn2.h)."""
+    _fields_ = [(n, _c_int) for n in ("M", "N", "dtype", "dy_dtype", "bias_dtype", "activation")] + [
+        (n, _vp) for n in ("dy", "z", "dz", "dbias")]
+
+
+class Gdn2Loss(ctypes.Structure):
+    """``struct gdn2_loss`` (include/gdn2.h)."""
+    _fields_ = [(n, _c_int) for n in ("rows", "V", "dtype", "target_type", "reduction", "upstream_ld")] + [
+        ("smoothing", ctypes.c_float), ("z_loss", ctypes.c_float), ("ld", ctypes.c_int64), ("ignore_index", ctypes.c_int64)] + [
+        (n, _vp) for n in ("logits", "targets", "upstream", "loss", "dlogits")]
+
+
+class Gdn2AdamwTensor(ctypes.Structure):
+    """``struct gdn2_adamw_tensor`` (include/gdn2.h)."""
+    _fields_ = [(n, _vp) for n in ("p", "g", "m", "v", "m_scale", "v_scale", "master", "step")] + [
+        ("numel", ctypes.c_int64), ("ordinal", _c_int), ("dtype", _c_int)] + [(n, _c_dbl) for n in ("lr", "beta1", "beta2", "eps", "weight_decay")]
+
+
 class Gdn2Error(RuntimeError):
     pass
 
@@ -111,6 +136,20 @@ def lib():
         L.gdn2_beam_workspace_bytes.argtypes = [_c_int] * 4
         L.gdn2_beam_workspace_bytes.restype = _c_size
         L.gdn2_beam_step.argtypes = [P(Gdn2Beam), _vp, _vp]
+        L.gdn2_linear_workspace_bytes.argtypes = [P(Gdn2Product)]
+        L.gdn2_linear_workspace_bytes.restype = _c_size
+        L.gdn2_linear.argtypes = [P(Gdn2Product), _vp, _vp]
+        L.gdn2_linear_slope_workspace_bytes.argtypes = [P(Gdn2Slope)]
+        L.gdn2_linear_slope_workspace_bytes.restype = _c_size
+        L.gdn2_linear_slope.argtypes = [P(Gdn2Slope), _vp, _vp]
+        L.gdn2_loss_workspace_bytes.argtypes = [_c_int]
+        L.gdn2_loss_workspace_bytes.restype = _c_size
+        L.gdn2_cross_entropy.argtypes = [P(Gdn2Loss), _vp, _vp]
+        L.gdn2_scale_rows.argtypes = [_vp, _c_int, _c_int, _c_int, _vp, _c_int, _vp]
+        L.gdn2_adamw_workspace_bytes.argtypes = [P(Gdn2AdamwTensor), _c_int]
+        L.gdn2_adamw_workspace_bytes.restype = _c_size
+        L.gdn2_adamw.argtypes = [P(Gdn2AdamwTensor), _c_int, _c_int, _c_dbl, _vp, _vp, _vp]
+        L.gdn2_adamw_unpack.argtypes = [P(Gdn2AdamwTensor), _c_int, P(_vp), P(_vp), _vp]
         L.gdn2_bwd.argtypes = [P(Gdn2Desc)] + [_vp] * 18
         L.gdn2_wy_stage.argtypes = [P(Gdn2Desc)] + [_vp] * 15
         L.gdn2_scores.argtypes = [P(Gdn2Desc)] + [_vp] * 7
@@ -138,6 +177,7 @@ def lib():
                    "gdn2_decode", "gdn2_prefill_prep", "gdn2_decode_flags", "gdn2_bwd", "gdn2_wy_stage", "gdn2_scores", "gdn2_debug_gemm", "gdn2_debug_stream",
                    "gdn2_debug_mfma", "gdn2_lm_premix_fwd", "gdn2_lm_premix_bwd", "gdn2_lm_rms_fwd", "gdn2_lm_rms_bwd",
                    "gdn2_lm_swiglu", "gdn2_lm_columns", "gdn2_decode_from", "gdn2_lm_premix_step_fwd", "gdn2_w4_linear", "gdn2_beam_step",
+                   "gdn2_linear", "gdn2_linear_slope", "gdn2_cross_entropy", "gdn2_scale_rows", "gdn2_adamw", "gdn2_adamw_unpack",
                    "gdn2_prof_begin", "gdn2_prof_end"):
             getattr(L, fn).restype = _c_int
         if L.gdn2_abi_version() != ABI_VERSION:

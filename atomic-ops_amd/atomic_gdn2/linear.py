@@ -1,0 +1,161 @@
+"""Matrix products of a layer, forward and backward, on the HIP kernels of ``csrc/gdn2_linear.hip``.
+
+``linear`` computes y = act(x W + bias) + residual in one pass behind the product: float32, bfloat16 or float16 rows,
+one (a token) or thousands (a batch).  W is (in, out), as ``e2e_lm.Dense`` holds it, or a transposed view of an
+(out, in) matrix (a tied embedding), read as it lies.  Sums are float32 and y is rounded once; float32 operands enter as
+three bfloat16 pieces each (entries below 1e-33 lose their bits below 2^-133), which keeps float32's precision at the
+rate of the 16-bit matrix cores.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .w4 import _rows
+
+__all__ = ["linear"]
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}        # GDN2_F32, GDN2_BF16, GDN2_F16
+_ACTS = {None: 0, "silu": 1, "gelu": 2, "gelu_tanh": 3}                  # GDN2_ACT_*
+_XW, _XWT, _XTW = 0, 1, 2
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _turned(w):
+    """Whether w is the transposed view of a matrix with whole rows."""
+    return w.stride(0) == 1 and w.stride(1) >= w.shape[0] and not (w.stride(1) == 1 and w.shape[1] > 1)
+
+
+def _ld(t):
+    return t.shape[1] if t.shape[0] == 1 else t.stride(0)
+
+
+def _product(form, a, b, M, K, N, out, bias=None, residual=None, act=0, z=None):
+    """out (M, N) = act(A B + bias) + residual; a, b rows of whole elements (include/gdn2.h, gdn2_product)."""
+    p = _lib.Gdn2Product(M, K, N, form, _DTYPES[a.dtype], _DTYPES[out.dtype], 0 if bias is None else _DTYPES[bias.dtype], act,
+                         _ld(a), _ld(b), 0 if residual is None else _ld(residual), a.data_ptr(), b.data_ptr(), _addr(bias),
+                         _addr(residual), out.data_ptr(), _addr(z))
+    L = _lib.lib()
+    ws = torch.empty(L.gdn2_linear_workspace_bytes(ctypes.byref(p)), dtype=torch.uint8, device=out.device)
+    with torch.cuda.device(out.device):
+        _lib.check(L.gdn2_linear(ctypes.byref(p), _lib.ptr(ws), _lib.stream_handle(out.device)), "gdn2_linear")
+    return out
+
+
+def _forward(x, weight, bias, residual, act, out_dtype, keep):
+    """y, and z = x W + bias where keep; x (M, K), residual (M, N) rows."""
+    M, (K, N) = x.shape[0], weight.shape
+    y = torch.empty((M, N), dtype=out_dtype, device=x.device)
+    z = torch.empty((M, N), dtype=x.dtype, device=x.device) if keep else None
+    if M:
+        turned = _turned(weight)
+        _product(_XWT if turned else _XW, x, weight.t() if turned else weight, M, K, N, y, bias, residual, act, z)
+    return y, z
+
+
+def _slope(dy, z, dtype, act, bias_dtype, need_dz):
+    """dz = dy act'(z) (None: dy itself) and the bias' gradient (None: not asked for)."""
+    M, N = dy.shape
+    dz = torch.empty((M, N), dtype=dtype, device=dy.device) if need_dz else None
+    db = None if bias_dtype is None else torch.empty(N, dtype=bias_dtype, device=dy.device)
+    p = _lib.Gdn2Slope(M, N, _DTYPES[dtype], _DTYPES[dy.dtype], 0 if db is None else _DTYPES[bias_dtype], act, dy.data_ptr(), _addr(z),
+                       _addr(dz), _addr(db))
+    L = _lib.lib()
+    ws = torch.empty(L.gdn2_linear_slope_workspace_bytes(ctypes.byref(p)), dtype=torch.uint8, device=dy.device)
+    with torch.cuda.device(dy.device):
+        _lib.check(L.gdn2_linear_slope(ctypes.byref(p), _lib.ptr(ws), _lib.stream_handle(dy.device)), "gdn2_linear_slope")
+    return dz, db
+
+
+def _saved(t, like):
+    """A saved tensor as it was saved; hooks may have changed its strides, type or device."""
+    if t is None:
+        return None
+    t = t if (t.shape, t.dtype, t.device) == like else _lib.restored(t, *like)
+    return t if _turned(t) else _rows(t, t.shape[1])
+
+
+class _Linear(torch.autograd.Function):
+    """(x rows, weight, bias, residual rows) -> y rows.  Once differentiable: a second derivative raises."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act, out_dtype):
+        y, z = _forward(x, weight, bias, residual, act, out_dtype, act != 0)
+        ctx.act, ctx.bias_dtype = act, None if bias is None else bias.dtype
+        ctx.save_for_backward(x, weight, z)
+        ctx.likes = [None if t is None else (t.shape, t.dtype, t.device) for t in (x, weight, z)]
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, z = (_saved(t, like) for t, like in zip(ctx.saved_tensors, ctx.likes))
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+        (M, K), N, dev = x.shape, weight.shape[1], x.device
+        if M == 0:
+            return (torch.zeros_like(x) if need_x else None, torch.zeros_like(weight) if need_w else None,
+                    torch.zeros(N, dtype=ctx.bias_dtype, device=dev) if need_b else None, dy if need_r else None, None, None)
+        dres, dy = dy if need_r else None, dy.contiguous()
+        own = ctx.act != 0 or dy.dtype != x.dtype
+        dz, db = dy, None
+        if (own and (need_x or need_w)) or need_b:
+            dz, db = _slope(dy, z, x.dtype, ctx.act, ctx.bias_dtype if need_b else None, own and (need_x or need_w))
+            dz = dy if dz is None else dz
+        turned, dx, dw = _turned(weight), None, None
+        if need_x:
+            dx = _product(_XW if turned else _XWT, dz, weight.t() if turned else weight, M, N, K,
+                          torch.empty((M, K), dtype=x.dtype, device=dev))
+        if need_w and turned:
+            dw = _product(_XTW, dz, x, N, M, K, torch.empty((N, K), dtype=x.dtype, device=dev)).t()
+        elif need_w:
+            dw = _product(_XTW, x, dz, K, M, N, torch.empty((K, N), dtype=x.dtype, device=dev))
+        return dx, dw, db, dres, None, None
+
+
+def linear(x, weight, bias=None, residual=None, activation=None, out_dtype=None):
+    """y = act(x W + bias) + residual: x (..., in), weight (in, out), y (..., out).
+
+    x and weight share a dtype: float32, bfloat16 or float16.  y has out_dtype, theirs (default) or float32 (a
+    float32 residual stream over 16-bit products).  bias (out,): their dtype or float32; residual (..., out) is cast
+    to out_dtype.  activation: None, "silu", "gelu" (z Phi(z)) or "gelu_tanh".  x and residual may be rows of wider
+    matrices.  Gradients of all four, each summed in float32 and in its tensor's dtype; with an activation
+    z = x W + bias is kept for them in x's dtype, and the gradient of z has x's dtype.  Once differentiable.  A row
+    of x with an infinity or NaN gives nothing finite in float32, and touches no other row."""
+    if activation not in _ACTS:
+        raise ValueError(f"activation must be one of {', '.join(map(repr, _ACTS))}, got {activation!r}")
+    if x.dtype not in _DTYPES:
+        raise TypeError(f"x must be float32, bfloat16 or float16, got {x.dtype}")
+    if weight.dtype != x.dtype:
+        raise TypeError(f"weight must be {x.dtype} as x, got {weight.dtype}")
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    if out_dtype not in (x.dtype, torch.float32):
+        raise TypeError(f"out_dtype must be {x.dtype} or float32, got {out_dtype}")
+    if weight.dim() != 2 or weight.numel() == 0:
+        raise ValueError(f"weight must be (in, out), got {tuple(weight.shape)}")
+    K, N = weight.shape
+    if x.dim() == 0 or x.shape[-1] != K:
+        raise ValueError(f"x must be (..., {K}), got {tuple(x.shape)}")
+    shape = (*x.shape[:-1], N)
+    if bias is not None and tuple(bias.shape) != (N,):
+        raise ValueError(f"bias must be ({N},), got {tuple(bias.shape)}")
+    if bias is not None and bias.dtype not in (x.dtype, torch.float32):
+        raise TypeError(f"bias must be {x.dtype} or float32, got {bias.dtype}")
+    if residual is not None and tuple(residual.shape) != shape:
+        raise ValueError(f"residual must be {shape}, got {tuple(residual.shape)}")
+    dev = x.device
+    for t, n in ((weight, "weight"), (bias, "bias"), (residual, "residual")):
+        if t is not None and t.device != dev:
+            raise ValueError(f"{n} is on {t.device}, x on {dev}")
+    if not x.is_cuda:
+        raise ValueError(f"linear needs tensors on a ROCm device, got {dev}")
+    x = _rows(x, K)
+    weight = weight if _turned(weight) else _rows(weight, N)
+    bias = None if bias is None else bias.contiguous()
+    residual = None if residual is None else _rows(residual.to(out_dtype), N)
+    return _Linear.apply(x, weight, bias, residual, _ACTS[activation], out_dtype).view(shape)

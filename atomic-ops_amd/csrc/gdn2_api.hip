@@ -7,6 +7,7 @@
 
 #include "../../include/gdn2.h"
 #include "gdn2_kernels.hpp"
+#include "gdn2_optim.hpp"
 
 namespace {
 
@@ -902,6 +903,159 @@ int gdn2_beam_step(const gdn2_beam* p, void* workspace, void* stream) {
   a.ld = (size_t)p->ld;
   a.vec = aligned16({p->logits}) && p->ld * e % 16 == 0;
   return lm_done(gdn2::launch_beam(p->dtype, a, reinterpret_cast<hipStream_t>(stream)), "beam launch");
+}
+
+static_assert(GDN2_F32 == gdn2::LIN_F32 && GDN2_BF16 == gdn2::LIN_BF16 && GDN2_F16 == gdn2::LIN_F16 && GDN2_XW == gdn2::LIN_XW &&
+              GDN2_XWT == gdn2::LIN_XWT && GDN2_XTW == gdn2::LIN_XTW && GDN2_ADAMW_BLOCK == 256, "header constants");
+
+namespace {
+constexpr int kMaxSide = 1 << 27;
+bool float_type(int t) { return t >= GDN2_F32 && t <= GDN2_F16; }
+uintptr_t low(const void* p) { return reinterpret_cast<uintptr_t>(p); }
+uintptr_t size_of(int t) { return t == GDN2_F32 ? 4 : 2; }
+
+// the product's arguments, checked
+int product_args(const gdn2_product* p, gdn2::LinProduct* a) {
+  if (!p) return fail(GDN2_ERR_INVALID, "null argument block");
+  if (p->M < 1 || p->K < 1 || p->N < 1) return fail(GDN2_ERR_INVALID, "non-positive shape");
+  if (p->M > kMaxSide || p->K > kMaxSide || p->N > kMaxSide) return fail(GDN2_ERR_UNSUPPORTED, "shape too large");
+  if (((int64_t)p->M / 64 + 1) * ((int64_t)p->N / 64 + 1) >= (int64_t(1) << 31) || ((int64_t)p->M / 64 + 1) * ((int64_t)p->K / 64 + 1) >= (int64_t(1) << 30) ||
+      ((int64_t)p->K / 64 + 1) * ((int64_t)p->N / 64 + 1) >= (int64_t(1) << 30))
+    return fail(GDN2_ERR_UNSUPPORTED, "shape too large");
+  if (p->form < GDN2_XW || p->form > GDN2_XTW) return fail(GDN2_ERR_INVALID, "unknown form");
+  if (!float_type(p->dtype) || (p->out_dtype != p->dtype && p->out_dtype != GDN2_F32) ||
+      (p->bias && p->bias_dtype != p->dtype && p->bias_dtype != GDN2_F32))
+    return fail(GDN2_ERR_INVALID, "unknown dtype");
+  if (p->activation < GDN2_ACT_NONE || p->activation > GDN2_ACT_GELU_TANH) return fail(GDN2_ERR_INVALID, "unknown activation");
+  if (p->form == GDN2_XTW && (p->activation || p->bias || p->z)) return fail(GDN2_ERR_UNSUPPORTED, "bias and activation belong to a layer's own product");
+  const int64_t ca = p->form == GDN2_XTW ? p->M : p->K, cb = p->form == GDN2_XWT ? p->K : p->N;
+  if (p->lda < ca || p->ldb < cb || (p->residual && p->ldr < p->N)) return fail(GDN2_ERR_INVALID, "row stride below the row");
+  if (!p->a || !p->b || !p->y) return fail(GDN2_ERR_INVALID, "null pointer");
+  if ((low(p->a) | low(p->b) | low(p->z)) % size_of(p->dtype) || (low(p->y) | low(p->residual)) % size_of(p->out_dtype) ||
+      low(p->bias) % size_of(p->bias_dtype))
+    return fail(GDN2_ERR_INVALID, "pointer not aligned to its elements");
+  *a = gdn2::LinProduct{p->M, p->K, p->N, p->form, p->dtype, p->out_dtype, p->bias_dtype, p->activation, (size_t)p->lda,
+                        (size_t)p->ldb, p->residual ? (size_t)p->ldr : 0, p->a, p->b, p->bias, p->residual, p->y, p->z};
+  return GDN2_OK;
+}
+int slope_args(const gdn2_slope* p, gdn2::LinSlope* a) {
+  if (!p) return fail(GDN2_ERR_INVALID, "null argument block");
+  if (p->M < 1 || p->N < 1) return fail(GDN2_ERR_INVALID, "non-positive shape");
+  if (p->M > kMaxSide || p->N > kMaxSide || p->M > 65535 * 64) return fail(GDN2_ERR_UNSUPPORTED, "shape too large");
+  if (!float_type(p->dtype) || (p->dy_dtype != p->dtype && p->dy_dtype != GDN2_F32) ||
+      (p->dbias && p->bias_dtype != p->dtype && p->bias_dtype != GDN2_F32))
+    return fail(GDN2_ERR_INVALID, "unknown dtype");
+  if (p->activation < GDN2_ACT_NONE || p->activation > GDN2_ACT_GELU_TANH) return fail(GDN2_ERR_INVALID, "unknown activation");
+  if (!p->dy || (p->activation && !p->z) || (!p->dz && !p->dbias)) return fail(GDN2_ERR_INVALID, "null pointer");
+  if ((low(p->z) | low(p->dz)) % size_of(p->dtype) || low(p->dy) % size_of(p->dy_dtype) || low(p->dbias) % size_of(p->bias_dtype))
+    return fail(GDN2_ERR_INVALID, "pointer not aligned to its elements");
+  *a = gdn2::LinSlope{p->M, p->N, p->dtype, p->dy_dtype, p->bias_dtype, p->activation, p->dy, p->z, p->dz, p->dbias};
+  return GDN2_OK;
+}
+}  // namespace
+
+size_t gdn2_linear_workspace_bytes(const gdn2_product* p) {
+  gdn2::LinProduct a{};
+  return product_args(p, &a) ? 0 : gdn2::linear_workspace_bytes(a);
+}
+
+int gdn2_linear(const gdn2_product* p, void* workspace, void* stream) {
+  gdn2::LinProduct a{};
+  const int st = product_args(p, &a);
+  if (st) return st;
+  if (!aligned16({workspace}) || (!workspace && gdn2::linear_workspace_bytes(a)))
+    return fail(GDN2_ERR_INVALID, "null workspace, or not 16-byte aligned");
+  return lm_done(gdn2::launch_linear(a, workspace, reinterpret_cast<hipStream_t>(stream)), "linear launch");
+}
+
+size_t gdn2_linear_slope_workspace_bytes(const gdn2_slope* p) {
+  gdn2::LinSlope a{};
+  return slope_args(p, &a) ? 0 : gdn2::linear_slope_workspace_bytes(a);
+}
+
+int gdn2_linear_slope(const gdn2_slope* p, void* workspace, void* stream) {
+  gdn2::LinSlope a{};
+  const int st = slope_args(p, &a);
+  if (st) return st;
+  if (!aligned16({workspace}) || (!workspace && gdn2::linear_slope_workspace_bytes(a)))
+    return fail(GDN2_ERR_INVALID, "null workspace, or not 16-byte aligned");
+  return lm_done(gdn2::launch_linear_slope(a, workspace, reinterpret_cast<hipStream_t>(stream)), "linear slope launch");
+}
+
+size_t gdn2_loss_workspace_bytes(int rows) { return rows < 1 ? 0 : gdn2::loss_workspace_bytes(rows); }
+
+int gdn2_cross_entropy(const gdn2_loss* p, void* workspace, void* stream) {
+  if (!p) return fail(GDN2_ERR_INVALID, "null argument block");
+  if (p->rows < 1 || p->V < 1) return fail(GDN2_ERR_INVALID, "non-positive shape");
+  if (p->rows > (1 << 30) || p->V > (1 << 30)) return fail(GDN2_ERR_UNSUPPORTED, "shape too large");
+  if (!float_type(p->dtype)) return fail(GDN2_ERR_INVALID, "unknown dtype");
+  if (p->target_type != GDN2_FLAG_INT32 && p->target_type != GDN2_FLAG_INT64) return fail(GDN2_ERR_INVALID, "targets must be int32 or int64");
+  if (p->reduction < 0 || p->reduction > 2) return fail(GDN2_ERR_INVALID, "unknown reduction");
+  if (p->upstream_ld < 0 || p->upstream_ld > 1 || (p->upstream_ld && p->reduction)) return fail(GDN2_ERR_INVALID, "one upstream gradient for each loss");
+  if (!(p->smoothing >= 0.f && p->smoothing <= 1.f) || !(p->z_loss >= 0.f)) return fail(GDN2_ERR_INVALID, "smoothing in [0, 1], z_loss not negative");
+  if (p->ld < p->V) return fail(GDN2_ERR_INVALID, "row stride below the row");
+  if (!p->logits || !p->targets || (!p->loss && !p->dlogits) || !workspace || !aligned16({workspace}))
+    return fail(GDN2_ERR_INVALID, "null pointer, or workspace not 16-byte aligned");
+  const int tb = p->target_type == GDN2_FLAG_INT64 ? 8 : 4;
+  if ((low(p->logits) | low(p->dlogits)) % size_of(p->dtype) || low(p->targets) % tb || (low(p->loss) | low(p->upstream)) % 4)
+    return fail(GDN2_ERR_INVALID, "pointer not aligned to its elements");
+  gdn2::LossArgs a{};
+  a.rows = p->rows; a.V = p->V; a.dtype = p->dtype; a.target_bytes = tb; a.reduction = p->reduction;
+  a.upstream_ld = p->upstream_ld; a.smoothing = p->smoothing; a.z_loss = p->z_loss; a.ld = (size_t)p->ld; a.ignore = p->ignore_index;
+  a.logits = p->logits; a.targets = p->targets; a.upstream = p->upstream; a.loss = p->loss; a.dlogits = p->dlogits;
+  a.scale = static_cast<float*>(workspace);
+  a.row_loss = !p->loss ? nullptr : p->reduction ? at<float>(workspace, 256) : p->loss;
+  return lm_done(gdn2::launch_cross_entropy(a, reinterpret_cast<hipStream_t>(stream)), "cross entropy launch");
+}
+
+int gdn2_scale_rows(void* x, int dtype, int rows, int V, const float* factor, int factor_ld, void* stream) {
+  if (rows < 1 || V < 1 || !float_type(dtype) || !x || !factor || factor_ld < 0 || factor_ld > 1) return fail(GDN2_ERR_INVALID, "bad argument");
+  if (rows > (1 << 30) || V > (1 << 30)) return fail(GDN2_ERR_UNSUPPORTED, "shape too large");
+  if (low(x) % size_of(dtype) || low(factor) % 4) return fail(GDN2_ERR_INVALID, "pointer not aligned to its elements");
+  return lm_done(gdn2::launch_scale_rows(x, dtype, rows, V, factor, factor_ld, reinterpret_cast<hipStream_t>(stream)), "scale rows launch");
+}
+
+namespace {
+int adamw_check(const gdn2_adamw_tensor* t, int n, int bits, bool step) {
+  if (!t || n < 1) return fail(GDN2_ERR_INVALID, "no tensors");
+  if (bits != 8 && bits != 32) return fail(GDN2_ERR_INVALID, "states of 8 or 32 bits");
+  for (int i = 0; i < n; ++i) {
+    const gdn2_adamw_tensor& x = t[i];
+    if (x.numel < 1 || x.numel >= (int64_t(1) << 43)) return fail(GDN2_ERR_INVALID, "bad tensor size");
+    if (!x.m || !x.v || (bits == 8 && (!x.m_scale || !x.v_scale))) return fail(GDN2_ERR_INVALID, "null state");
+    if (bits == 32 && (low(x.m) | low(x.v)) % 4) return fail(GDN2_ERR_INVALID, "pointer not aligned to its elements");
+    if (bits == 8 && (low(x.m_scale) | low(x.v_scale)) % 4) return fail(GDN2_ERR_INVALID, "pointer not aligned to its elements");
+    if (!step) continue;
+    if (!float_type(x.dtype)) return fail(GDN2_ERR_INVALID, "unknown dtype");
+    if (!x.p || !x.g || !x.step || (x.dtype != GDN2_F32 && !x.master)) return fail(GDN2_ERR_INVALID, "null pointer");
+    if ((low(x.p) | low(x.g)) % size_of(x.dtype) || (low(x.step) | low(x.master)) % 4)
+      return fail(GDN2_ERR_INVALID, "pointer not aligned to its elements");
+    if (!(x.beta1 >= 0.0 && x.beta1 < 1.0 && x.beta2 >= 0.0 && x.beta2 < 1.0 && x.eps >= 0.0 && x.lr >= 0.0 && x.weight_decay >= 0.0))
+      return fail(GDN2_ERR_INVALID, "bad hyperparameter");
+  }
+  return GDN2_OK;
+}
+}  // namespace
+
+size_t gdn2_adamw_workspace_bytes(const gdn2_adamw_tensor* t, int n) {
+  if (!t || n < 1) return 0;
+  return gdn2::adamw_workspace_bytes(t, n);
+}
+
+int gdn2_adamw(const gdn2_adamw_tensor* t, int n, int bits, double max_norm, float* norm, void* workspace, void* stream) {
+  const int st = adamw_check(t, n, bits, true);
+  if (st) return st;
+  if (!workspace || !aligned16({workspace}) || low(norm) % 4) return fail(GDN2_ERR_INVALID, "null workspace, or not aligned");
+  return lm_done(gdn2::launch_adamw(t, n, bits, max_norm, norm, workspace, reinterpret_cast<hipStream_t>(stream)), "adamw launch");
+}
+
+int gdn2_adamw_unpack(const gdn2_adamw_tensor* t, int n, float* const* m_out, float* const* v_out, void* stream) {
+  const int st = adamw_check(t, n, 8, false);
+  if (st) return st;
+  if (!m_out || !v_out) return fail(GDN2_ERR_INVALID, "null pointer");
+  for (int i = 0; i < n; ++i)
+    if (!m_out[i] || !v_out[i] || (low(m_out[i]) | low(v_out[i])) % 4) return fail(GDN2_ERR_INVALID, "null pointer, or not aligned");
+  return lm_done(gdn2::launch_adamw_unpack(t, n, m_out, v_out, reinterpret_cast<hipStream_t>(stream)), "adamw unpack launch");
 }
 
 int gdn2_debug_scan_copies(int n_bh, int D, int nc, int in_place, int cus) {

@@ -472,4 +472,38 @@ __device__ __forceinline__ float piece_col_leg(const Piece& pc, const float* sG,
   return leg_col(pc.kind, sG[j * LD + d], piece_ga(pc, sG, LD, d, ar), piece_gz(pc, sG, LD, d, az));
 }
 
+// Products with an epilogue (gdn2_linear.hip): the argument block of include/gdn2.h's gdn2_product, checked.
+constexpr int LIN_F32 = 0, LIN_BF16 = 1, LIN_F16 = 2;
+constexpr int LIN_XW = 0, LIN_XWT = 1, LIN_XTW = 2;
+struct LinProduct {
+  int M, K, N, form, dtype, out_dtype, bias_dtype, act;
+  size_t lda, ldb, ldr;
+  const void *a, *b, *bias, *residual;
+  void *y, *z;
+};
+size_t linear_workspace_bytes(const LinProduct& p);
+hipError_t launch_linear(const LinProduct& p, void* workspace, hipStream_t s);
+struct LinSlope {
+  int M, N, dtype, dy_dtype, bias_dtype, act;
+  const void *dy, *z;
+  void *dz, *dbias;
+};
+size_t linear_slope_workspace_bytes(const LinSlope& p);
+hipError_t launch_linear_slope(const LinSlope& p, void* workspace, hipStream_t s);
+
+// Cross-entropy (gdn2_loss.hip): gdn2_loss of include/gdn2.h; target_bytes 4 or 8.
+struct LossArgs {
+  int rows, V, dtype, target_bytes, reduction, upstream_ld;
+  float smoothing, z_loss;
+  size_t ld;
+  int64_t ignore;
+  const void *logits, *targets;
+  const float* upstream;
+  float *loss, *row_loss, *scale;     // row_loss (rows): the losses, or workspace; scale: workspace, 1 / count
+  void* dlogits;
+};
+size_t loss_workspace_bytes(int rows);
+hipError_t launch_cross_entropy(const LossArgs& a, hipStream_t s);
+hipError_t launch_scale_rows(void* x, int dtype, int rows, int V, const float* factor, int factor_ld, hipStream_t s);
+
 }  // namespace gdn2

@@ -360,6 +360,91 @@ typedef struct gdn2_beam {
 size_t gdn2_beam_workspace_bytes(int B, int K, int V, int n);
 int gdn2_beam_step(const gdn2_beam* p, void* workspace, void* stream);
 
+/* ---- a training step around the blocks -------------------------------------------------------- */
+
+/* y = act(A B + bias) + residual, sums float32.  y (M, N) contiguous.  How a and b lie in memory, rows of lda and
+ * ldb elements:
+ *   GDN2_XW   a (M, K), b (K, N): a layer, x W;
+ *   GDN2_XWT  a (M, K), b (N, K): a layer whose weight is kept transposed; the input's gradient, dz W^T;
+ *   GDN2_XTW  a (K, M), b (K, N): the weight's gradient, x^T dz.
+ * dtype: of a and b; out_dtype, of y and residual (rows of ldr): dtype or float32; bias (N): bias_dtype, dtype or
+ * float32.  z: NULL, or (M, N) of dtype: A B + bias, rounded.  activation: GDN2_ACT_*; with GDN2_XTW
+ * none, no bias and no z.  Float32 operands enter as three bfloat16 pieces each, whose sum they are but for bits below
+ * 2^-133, in six products of pieces; what is left out is below 2^-22 of |a| |b|.  workspace:
+ * gdn2_linear_workspace_bytes (0: none), 16-byte aligned.  M, K, N <= 2^27. */
+enum { GDN2_XW = 0, GDN2_XWT = 1, GDN2_XTW = 2 };
+enum { GDN2_ACT_NONE = 0, GDN2_ACT_SILU = 1, GDN2_ACT_GELU = 2, GDN2_ACT_GELU_TANH = 3 };
+typedef struct gdn2_product {
+  int32_t M, K, N, form, dtype, out_dtype, bias_dtype, activation;
+  int64_t lda, ldb, ldr;
+  const void *a, *b, *bias, *residual;
+  void *y, *z;
+} gdn2_product;
+size_t gdn2_linear_workspace_bytes(const gdn2_product* p);
+int gdn2_linear(const gdn2_product* p, void* workspace, void* stream);
+
+/* dz = dy act'(z) and dbias[n] = sum_m dz[m][n].  dy (M, N) contiguous, dy_dtype; z (M, N) of dtype (unused
+ * without an activation); dz NULL or (M, N) of dtype; dbias NULL or (N) of bias_dtype.  workspace:
+ * gdn2_linear_slope_workspace_bytes (0: none), 16-byte aligned. */
+typedef struct gdn2_slope {
+  int32_t M, N, dtype, dy_dtype, bias_dtype, activation;
+  const void *dy, *z;
+  void *dz, *dbias;
+} gdn2_slope;
+size_t gdn2_linear_slope_workspace_bytes(const gdn2_slope* p);
+int gdn2_linear_slope(const gdn2_slope* p, void* workspace, void* stream);
+
+/* Cross-entropy of rows of logits, and its gradient.  With p = softmax(x), lse = log sum exp x, t = targets[i]:
+ *   loss_i = lse - (1 - smoothing) x[t] - smoothing mean(x) + z_loss lse^2,   0 where t = ignore_index;
+ * reduction: 0 none: losses (rows) are written; 1 sum and 2 mean over the rows that are not ignored (none: 0): loss[0].
+ *   dlogits[i][j] = s_i (p_j (1 + 2 z_loss lse) - (1 - smoothing) [j = t] - smoothing / V),
+ * s_i = the factor of loss_i in the result, times upstream: NULL (1), or one float, or with reduction 0 one for each
+ * row (upstream_ld 1; 0: one for all).  A target outside 0 .. V-1 makes its row's loss and gradient NaN.  logits
+ * (rows, V) of ld elements, dlogits contiguous of the same dtype, or NULL; loss or losses may be NULL where dlogits is
+ * not.  targets int64 (GDN2_FLAG_INT64) or int32 (GDN2_FLAG_INT32).  workspace: gdn2_loss_workspace_bytes, 16-byte
+ * aligned.  rows, V < 2^31. */
+typedef struct gdn2_loss {
+  int32_t rows, V, dtype, target_type, reduction, upstream_ld;
+  float smoothing, z_loss;
+  int64_t ld, ignore_index;
+  const void *logits, *targets;
+  const float* upstream;
+  float* loss;
+  void* dlogits;
+} gdn2_loss;
+size_t gdn2_loss_workspace_bytes(int rows);
+int gdn2_cross_entropy(const gdn2_loss* p, void* workspace, void* stream);
+/* x *= *factor or, with factor_ld 1, row i *= factor[i]; where a factor is 1 the row is left as it is.  x (rows, V)
+ * contiguous. */
+int gdn2_scale_rows(void* x, int dtype, int rows, int V, const float* factor, int factor_ld, void* stream);
+
+/* One step of AdamW over n tensors.  In 32 bits, each product and sum rounded by itself:
+ *   t = ++*step;  g' = c g;  m = beta1 m + (1 - beta1) g';  v = beta2 v + (1 - beta2) g' g';
+ *   p = p (1 - lr weight_decay) - m / (sqrt(v) / sqrt(1 - beta2^t) + eps) * (lr / (1 - beta1^t)),
+ * c = max_norm / max(norm, max_norm), norm the square root of the sum of the squares of all gradients, summed in 64
+ * bits (max_norm <= 0: c = 1; norm is written only where it is asked for).  A tensor of 16 bits is formed from, and
+ * kept as, its float32 master, and rounded.  bits 32: m and v are float32.  bits 8: m (int8) and v (uint8) are codes of
+ * blocks of 256 elements with a float32 scale each (m_scale, v_scale): m = c |c| s, v = (c^2 s)^2, rounded to one of
+ * the two neighbours at random in proportion, by a hash of element, tensor (its ordinal) and t; a block with an
+ * infinity or NaN has the scale NaN.  workspace: gdn2_adamw_workspace_bytes, 16-byte aligned; the tensors
+ * may have any alignment of their elements.  Tensors must not overlap. */
+typedef struct gdn2_adamw_tensor {
+  void* p;
+  const void* g;
+  void *m, *v;
+  float *m_scale, *v_scale;       /* bits 8 */
+  float* master;                  /* p of 16 bits */
+  float* step;                    /* whole; one for each tensor */
+  int64_t numel;
+  int32_t ordinal, dtype;
+  double lr, beta1, beta2, eps, weight_decay;
+} gdn2_adamw_tensor;
+#define GDN2_ADAMW_BLOCK 256
+size_t gdn2_adamw_workspace_bytes(const gdn2_adamw_tensor* t, int n);
+int gdn2_adamw(const gdn2_adamw_tensor* t, int n, int bits, double max_norm, float* norm, void* workspace, void* stream);
+/* The float32 values of 8-bit states: m_out[i], v_out[i] (numel) of tensor i. */
+int gdn2_adamw_unpack(const gdn2_adamw_tensor* t, int n, float* const* m_out, float* const* v_out, void* stream);
+
 /* Diagnostics: C[M,N] = A[M,K] B[K,N] (row-major float32) through the kernels' MFMA tile
  * routine in the given dot mode.  M, N <= 64, K <= 128, all multiples of 16. */
 int gdn2_debug_gemm(int mode, const float* A, const float* B, float* C, int M, int N, int K,
