@@ -127,6 +127,11 @@ def linear(x, weight, bias=None, residual=None, activation=None, out_dtype=None)
     matrices.  Gradients of all four, each summed in float32 and in its tensor's dtype; with an activation
     z = x W + bias is kept for them in x's dtype, and the gradient of z has x's dtype.  Once differentiable.  A row
     of x with an infinity or NaN gives nothing finite in float32, and touches no other row."""
+    if activation in _ACTS and isinstance(x, torch.Tensor) and x.is_cuda and out_dtype in (None, x.dtype, torch.float32):
+        # plain calls (csrc/bind.cpp) go native; None = not one, and what follows handles it
+        y = _lib.bind().linear(x, weight, bias, residual, _ACTS[activation], out_dtype is torch.float32)
+        if y is not None:
+            return y
     if activation not in _ACTS:
         raise ValueError(f"activation must be one of {', '.join(map(repr, _ACTS))}, got {activation!r}")
     if x.dtype not in _DTYPES:

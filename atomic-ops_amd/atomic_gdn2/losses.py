@@ -74,6 +74,13 @@ def cross_entropy(logits, targets, ignore_index: int = -100, label_smoothing: fl
     is multiplied with before it is rounded in float16, after it in the others).  A target outside 0 .. V-1 makes its
     row's loss and gradient NaN (the host does not wait to look at them).  -inf is a banned token.  Once
     differentiable."""
+    how = _REDUCTIONS.get(reduction)
+    if (isinstance(logits, torch.Tensor) and logits.is_cuda and how is not None and type(label_smoothing) is float and 0.0 <= label_smoothing <= 1.0
+            and type(z_loss) is float and z_loss >= 0.0):
+        # plain calls (csrc/bind.cpp) go native; None = not one, and what follows handles it
+        loss = _lib.bind().cross_entropy(logits, targets, ignore_index, label_smoothing, z_loss, how)
+        if loss is not None:
+            return loss
     if logits.dtype not in _DTYPES:
         raise TypeError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")
     if targets.is_floating_point() or targets.is_complex() or targets.dtype == torch.bool:
@@ -96,7 +103,7 @@ def cross_entropy(logits, targets, ignore_index: int = -100, label_smoothing: fl
         x = x.clone(memory_format=torch.contiguous_format)
     t = targets.reshape(-1)
     t = t.contiguous() if t.dtype in _INDEX else t.to(torch.int64)
-    how = (int(ignore_index), float(label_smoothing), float(z_loss), _REDUCTIONS[reduction])
+    how = (int(ignore_index), float(label_smoothing), float(z_loss), how)
     if (torch.is_grad_enabled() and x.requires_grad) or (fwd._current_level >= 0 and fwd.unpack_dual(x).tangent is not None):
         loss = _CrossEntropy.apply(x, t, how)
     else:

@@ -117,6 +117,11 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        # plain steps (csrc/bind.cpp) go native; None = not one, and what follows handles it
+        done = _lib.bind().adamw(self.param_groups, self.state, self.state_bits, self.max_norm or 0.0)
+        if done is not None:
+            self.norm = None if done is True else done
+            return loss
         todo, ordinal = [], 0
         for group in self.param_groups:
             hyper = self._hyper(group)

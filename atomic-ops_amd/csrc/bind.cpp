@@ -50,6 +50,15 @@ struct Abi {
   decltype(&gdn2_beam_workspace_bytes) beam_ws;
   decltype(&gdn2_beam_step) beam;
   decltype(&gdn2_lm_premix_step_fwd) premix_step;
+  decltype(&gdn2_linear_workspace_bytes) linear_ws;
+  decltype(&gdn2_linear) linear;
+  decltype(&gdn2_linear_slope_workspace_bytes) slope_ws;
+  decltype(&gdn2_linear_slope) slope;
+  decltype(&gdn2_loss_workspace_bytes) loss_ws;
+  decltype(&gdn2_cross_entropy) cross_entropy;
+  decltype(&gdn2_scale_rows) scale_rows;
+  decltype(&gdn2_adamw_workspace_bytes) adamw_ws;
+  decltype(&gdn2_adamw) adamw;
   decltype(&gdn2_last_error) last_error;
 } abi{};
 
@@ -705,6 +714,8 @@ PyObject* py_dense(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+#include "bind_training.hpp"
+
 PyMethodDef methods[] = {
     {"bind", (PyCFunction)(void (*)())py_bind, METH_FASTCALL, "bind(*addresses)"},
     {"op", (PyCFunction)(void (*)())py_op, METH_FASTCALL, "op(desc, segment)"},
@@ -716,6 +727,9 @@ PyMethodDef methods[] = {
     {"w4", (PyCFunction)(void (*)())py_w4, METH_FASTCALL, "w4(x, q, meta, in, out, group, bias, residual)"},
     {"beam", (PyCFunction)(void (*)())py_beam, METH_FASTCALL, "beam(logits, scores, n, finished, eos)"},
     {"premix_step", (PyCFunction)(void (*)())py_premix_step, METH_FASTCALL, "premix_step(y, history, weights, heads, g_max, parents)"},
+    {"linear", (PyCFunction)(void (*)())py_linear, METH_FASTCALL, "linear(x, weight, bias, residual, activation, float32)"},
+    {"cross_entropy", (PyCFunction)(void (*)())py_cross_entropy, METH_FASTCALL, "cross_entropy(logits, targets, ignore, smoothing, z, reduction)"},
+    {"adamw", (PyCFunction)(void (*)())py_adamw, METH_FASTCALL, "adamw(groups, state, bits, max_norm)"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module{PyModuleDef_HEAD_INIT, "_bind", "native call path of the operator", -1, methods};
 
