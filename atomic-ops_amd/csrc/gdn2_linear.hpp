@@ -1,0 +1,596 @@
+// Kernels of gdn2_linear.hip, instantiated for each type in a translation unit of its own (gdn2_linear_*.hip).
+// Products with an epilogue, on gfx950: y = act(A B + bias) + residual, where a layer's forward pass and its two
+// gradients differ in how the operands lie in memory (include/gdn2.h, gdn2_product).
+//
+// The matrix cores take operands whose lanes hold eight consecutive values along the sum.  An operand whose rows run
+// along the sum (x; W and dz for the input's gradient) is read from LDS as it is.  One whose rows run across it (W of a
+// layer; x and dz for the weight's gradient) lies in LDS as in memory and is transposed on its way to the registers
+// (ds_read_b64_tr_b16), so that no pass over memory turns a matrix around.
+#pragma once
+#include "gdn2_kernels.hpp"
+
+namespace gdn2 {
+
+typedef _Float16 h2v __attribute__((ext_vector_type(2)));
+typedef s4 __attribute__((address_space(3)))* lds_s4;
+constexpr int LIN_NONE = 0, LIN_SILU = 1, LIN_GELU = 2, LIN_TANH = 3;
+
+template <int DT>
+struct LinType {
+  using T = std::conditional_t<DT == LIN_F32, float, std::conditional_t<DT == LIN_BF16, uint16_t, _Float16>>;
+  static __device__ __forceinline__ float get(const void* p, size_t i) {
+    if constexpr (DT == LIN_BF16) return bf16_val(static_cast<const uint16_t*>(p)[i]);
+    else return (float)static_cast<const T*>(p)[i];
+  }
+  static __device__ __forceinline__ void put(void* p, size_t i, float v) {
+    if constexpr (DT == LIN_BF16) static_cast<uint16_t*>(p)[i] = (uint16_t)bf16_bits(v);
+    else static_cast<T*>(p)[i] = (T)v;
+  }
+  static __device__ __forceinline__ float4 get4(const void* p, size_t i) {
+    if constexpr (DT == LIN_F32) return *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+    const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
+    if constexpr (DT == LIN_BF16)
+      return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                         __uint_as_float(u.y & 0xffff0000u));
+    const h2v a = __builtin_bit_cast(h2v, u.x), b = __builtin_bit_cast(h2v, u.y);
+    return make_float4((float)a[0], (float)a[1], (float)b[0], (float)b[1]);
+  }
+  static __device__ __forceinline__ void put4(void* p, size_t i, const float4& v) {
+    if constexpr (DT == LIN_F32) *reinterpret_cast<float4*>(static_cast<float*>(p) + i) = v;
+    else if constexpr (DT == LIN_BF16)
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + i) = make_uint2(bf16_pack(v.x, v.y), bf16_pack(v.z, v.w));
+    else {
+      const h2v a = {(_Float16)v.x, (_Float16)v.y}, b = {(_Float16)v.z, (_Float16)v.w};
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + i) = make_uint2(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b));
+    }
+  }
+};
+// by a type known at run time (wave-uniform)
+__device__ __forceinline__ float lin_get(int dt, const void* p, size_t i) {
+  return dt == LIN_F32 ? LinType<LIN_F32>::get(p, i) : dt == LIN_BF16 ? LinType<LIN_BF16>::get(p, i) : LinType<LIN_F16>::get(p, i);
+}
+__device__ __forceinline__ void lin_put(int dt, void* p, size_t i, float v) {
+  if (dt == LIN_F32) LinType<LIN_F32>::put(p, i, v);
+  else if (dt == LIN_BF16) LinType<LIN_BF16>::put(p, i, v);
+  else LinType<LIN_F16>::put(p, i, v);
+}
+__device__ __forceinline__ float4 lin_get4(int dt, const void* p, size_t i) {
+  return dt == LIN_F32 ? LinType<LIN_F32>::get4(p, i) : dt == LIN_BF16 ? LinType<LIN_BF16>::get4(p, i) : LinType<LIN_F16>::get4(p, i);
+}
+__device__ __forceinline__ void lin_put4(int dt, void* p, size_t i, const float4& v) {
+  if (dt == LIN_F32) LinType<LIN_F32>::put4(p, i, v);
+  else if (dt == LIN_BF16) LinType<LIN_BF16>::put4(p, i, v);
+  else LinType<LIN_F16>::put4(p, i, v);
+}
+
+// ---- activations: z s(u), s the logistic function, with u = z, 1.5958 (z + 0.044715 z^3), or gelu's z Phi(z).  The
+// tanh form 0.5 (1 + tanh(u / 2)) is s(u), which does not cancel where tanh goes to -1.
+constexpr float LIN_TANH_C = 1.59576912160573072f;       // 2 sqrt(2 / pi)
+__device__ __forceinline__ float lin_logistic(float u) { return 1.f / (1.f + __builtin_amdgcn_exp2f(u * -1.44269504088896341f)); }
+template <int ACT>
+__device__ __forceinline__ float lin_act(float z) {
+  if constexpr (ACT == LIN_SILU) return z * lin_logistic(z);
+  else if constexpr (ACT == LIN_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+  else if constexpr (ACT == LIN_TANH) return z * lin_logistic(LIN_TANH_C * (z + 0.044715f * z * z * z));
+  else return z;
+}
+template <int ACT>
+__device__ __forceinline__ float lin_slope(float z) {
+  if constexpr (ACT == LIN_SILU) {
+    const float s = lin_logistic(z);
+    return s * (1.f + z * (1.f - s));
+  } else if constexpr (ACT == LIN_GELU) {
+    return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);
+  } else if constexpr (ACT == LIN_TANH) {
+    const float s = lin_logistic(LIN_TANH_C * (z + 0.044715f * z * z * z));
+    return s + z * s * (1.f - s) * (LIN_TANH_C * (1.f + 0.134145f * z * z));
+  } else {
+    return 1.f;
+  }
+}
+
+// ---- the product --------------------------------------------------------------------------------------------------
+
+// Operands of lane l in a 32-deep product: eight values along the sum (group l / 16) of row or column l % 16.
+template <bool F16>
+__device__ __forceinline__ void lin_mfma4(f4& a0, f4& a1, f4& a2, f4& a3, const s8& n0, const s8& n1, const s8& n2, const s8& n3, const s8& m) {
+#define LIN_FOUR(op)                                                                                       \
+  "s_nop 1\n\t" op " %0, %4, %8, %0\n\t" op " %1, %5, %8, %1\n\t" op " %2, %6, %8, %2\n\t" op " %3, %7, %8, %3"
+  if constexpr (F16)
+    asm volatile(LIN_FOUR("v_mfma_f32_16x16x32_f16") : "+v"(a0), "+v"(a1), "+v"(a2), "+v"(a3) : "v"(n0), "v"(n1), "v"(n2), "v"(n3), "v"(m));
+  else
+    asm volatile(LIN_FOUR("v_mfma_f32_16x16x32_bf16") : "+v"(a0), "+v"(a1), "+v"(a2), "+v"(a3) : "v"(n0), "v"(n1), "v"(n2), "v"(n3), "v"(m));
+#undef LIN_FOUR
+}
+__device__ __forceinline__ void lin_hold(f4& a) { asm volatile("" : "+v"(a)); }
+
+// An operand as the kernels read it: 16-bit rows of ld elements, 16-byte aligned; planes of float32's pieces
+struct LinOperand {
+  const uint16_t* p;
+  size_t ld, plane;
+  int rows;              // across the sum: M or N; of a matrix whose rows run across it, a multiple of 8
+};
+struct LinArgs {
+  LinOperand a, b;
+  int M, N, K;           // K: up to the last whole value of the sum
+  int mt, nt, parts, per;        // tiles; parts of the sum, of `per` blocks each
+  int out_dtype, bias_dtype, vec;
+  size_t ldr;
+  const void *bias, *residual;
+  void *y, *z;
+  float* part;
+};
+
+static __device__ uint4 lin_zeros;      // what lies past the end of a sum
+
+// BM x BN results a workgroup of WM x WN waves; blocks of BK along the sum, NBUF of them in LDS; NP planes; AR, BR: rows
+// run across the sum
+template <int DT_, int ACT_, int NP_, bool AR_, bool BR_, int BM_, int BN_, int WM_, int WN_, int BK_, int NBUF_, int GM_>
+struct LinTile {
+  static constexpr int GM = GM_, DT = DT_, ACT = ACT_, NP = NP_, BM = BM_, BN = BN_, WM = WM_, WN = WN_, BK = BK_, NBUF = NBUF_, W = WM * WN;
+  static constexpr bool AR = AR_, BR = BR_;
+  static constexpr int MT = BM / WM / 16, NT = BN / WN / 16;
+  static constexpr int AB = BM * BK * 2, BB = BN * BK * 2, BUF = NP * (AB + BB), LDO = 68;
+  static constexpr int LDS = NBUF * BUF > W * 64 * LDO * 4 ? NBUF * BUF : W * 64 * LDO * 4;      // LDO: a row of a wave's results
+  static constexpr int DA = NP * AB / 1024 / W, DB = NP * BB / 1024 / W;       // a wave's DMAs of a block
+  static_assert(AB % 1024 == 0 && BB % 1024 == 0 && NP * AB % (1024 * W) == 0 && NP * BB % (1024 * W) == 0, "whole DMAs");
+  static_assert(NT == 4 && MT % 4 == 0 && (NP == 1 || (!AR && !BR)) && LDS <= 160 * 1024, "shapes");
+};
+
+// Where a wave's i-th DMA of an operand's block comes from.  Sixteen bytes a lane:
+//   rows along the sum: row q / CH, chunk (q % CH) ^ f(row) of eight values;
+//   rows across it: value q / (ROWS / 8) along the sum, the pair of chunks exchanged by its own f.
+// f spreads what the lanes of a read have in common over LDS's banks.
+template <int BK>
+__device__ __forceinline__ int lin_turn(int row) { return BK == 64 ? row & 7 : (row >> 1) & 3; }
+__device__ __forceinline__ int lin_turn_r(int k) { return (k & 3) | (k >> 1 & 4); }
+
+template <class C, bool R, int ROWS, int D>
+struct LinSource {
+  static constexpr int PLANE = ROWS * C::BK * 2 / 1024;
+  const char* src[D];
+  int k[D];                // along the sum, of the lane's first value
+  size_t step;
+  __device__ __forceinline__ void init(const LinOperand& o, int row0, int kb0) {
+    const int l = lane_id(), w = wave_id();
+    step = (R ? C::BK * o.ld : (size_t)C::BK) * 2;
+#pragma unroll
+    for (int i = 0; i < D; ++i) {
+      const int u = w * D + i, p = u / PLANE, q = u % PLANE * 64 + l;
+      size_t at;
+      if constexpr (R) {
+        k[i] = q / (ROWS / 8);
+        const int c = q % (ROWS / 8), unit = (c >> 1) ^ lin_turn_r(k[i]);
+        at = (size_t)k[i] * o.ld + min(row0 + 16 * unit + 8 * (c & 1), o.rows - 8);
+      } else {
+        constexpr int CH = C::BK / 8;
+        const int row = q / CH;
+        k[i] = 8 * (q % CH ^ lin_turn<C::BK>(row));
+        at = (size_t)min(row0 + row, o.rows - 1) * o.ld + k[i];
+      }
+      src[i] = reinterpret_cast<const char*>(o.p + p * o.plane + at) + (size_t)kb0 * step;
+      k[i] += kb0 * C::BK;
+    }
+  }
+  // the next block into LDS at dst; tail: it may pass the end of the sum
+  __device__ __forceinline__ void fetch(char* dst, int K, bool tail) {
+    const int w = wave_id();
+#pragma unroll
+    for (int i = 0; i < D; ++i) {
+      const char* s = src[i];
+      if (tail) s = k[i] < K ? s : reinterpret_cast<const char*>(&lin_zeros);
+      lds_dma16(reinterpret_cast<const float*>(s), reinterpret_cast<float*>(dst + (w * D + i) * 1024));
+      src[i] += step;
+      k[i] += C::BK;
+    }
+  }
+};
+
+// A lane's operands of tile t (16 rows) and step s (32 values) of a block in LDS
+template <class C, bool R, int ROWS>
+__device__ __forceinline__ s8 lin_read(const char* lds, int t, int s) {
+  const int l = lane_id(), r = l & 15, c = l >> 4;
+  if constexpr (R) {
+    const int k = 8 * c + (r >> 2), at = k * ROWS * 2 + ((t ^ lin_turn_r(k)) << 5) + (r & 3) * 8 + s * 32 * ROWS * 2;
+    const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(lds + at));
+    const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(lds + at + 8 * ROWS));
+    return s8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  } else {
+    const int row = 16 * t + r;
+    return *reinterpret_cast<const s8*>(lds + row * C::BK * 2 + (((4 * s + c) ^ lin_turn<C::BK>(row)) << 4));
+  }
+}
+
+// Results of a row, E of them from column n on: bias, activation, residual
+template <int DT, int ACT, int E>
+__device__ __forceinline__ void lin_out(const LinArgs& a, int m, int n, const float* f) {
+  const size_t at = (size_t)m * a.N + n;
+  if (a.vec) {               // (whole groups of eight columns, and every pointer takes 16 bytes)
+#pragma unroll
+    for (int q = 0; q < E; q += 4) {
+      float4 v = make_float4(f[q], f[q + 1], f[q + 2], f[q + 3]);
+      if (a.bias) {
+        const float4 b = lin_get4(a.bias_dtype, a.bias, n + q);
+        v.x += b.x; v.y += b.y; v.z += b.z; v.w += b.w;
+      }
+      if (a.z) LinType<DT>::put4(a.z, at + q, v);
+      v = make_float4(lin_act<ACT>(v.x), lin_act<ACT>(v.y), lin_act<ACT>(v.z), lin_act<ACT>(v.w));
+      if (a.residual) {
+        const float4 r = lin_get4(a.out_dtype, a.residual, (size_t)m * a.ldr + n + q);
+        v.x += r.x; v.y += r.y; v.z += r.z; v.w += r.w;
+      }
+      lin_put4(a.out_dtype, a.y, at + q, v);
+    }
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    if (n + e >= a.N) break;
+    float z = f[e] + (a.bias ? lin_get(a.bias_dtype, a.bias, n + e) : 0.f);
+    if (a.z) LinType<DT>::put(a.z, at + e, z);
+    z = lin_act<ACT>(z);
+    if (a.residual) z += lin_get(a.out_dtype, a.residual, (size_t)m * a.ldr + n + e);
+    lin_put(a.out_dtype, a.y, at + e, z);
+  }
+}
+// ... or of a part of the sum
+template <int E>
+__device__ __forceinline__ void lin_out_part(const LinArgs& a, int part, int m, int n, const float* f) {
+  float* p = a.part + ((size_t)part * a.M + m) * a.N + n;
+  if (a.vec) {
+#pragma unroll
+    for (int q = 0; q < E; q += 4) *reinterpret_cast<float4*>(p + q) = make_float4(f[q], f[q + 1], f[q + 2], f[q + 3]);
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (n + e < a.N) p[e] = f[e];
+}
+
+// Workgroups go to the 8 dies in turn: each die gets a run of neighbouring tiles (of one part of the sum), GM rows of tiles
+// high, so that what its workgroups read at a time is shared in its L2.
+__device__ __forceinline__ void lin_place(const LinArgs& a, int gm, int& part, int& mi, int& ni) {
+  const int tiles = a.mt * a.nt, total = tiles * a.parts, b = blockIdx.x, x = b & 7, whole = total >> 3, more = total & 7;
+  const int i = x * whole + min(x, more) + (b >> 3);
+  part = i / tiles;
+  const int t = i - part * tiles, group = t / (gm * a.nt), m0 = group * gm, h = min(gm, a.mt - m0), in = t - m0 * a.nt;
+  ni = in / h;
+  mi = m0 + in - ni * h;
+}
+
+template <class C>
+__global__ __launch_bounds__(C::W * WAVE) void lin_tile_kernel(LinArgs a) {
+  constexpr int MT = C::MT, NT = C::NT, NP = C::NP, S = C::BK / 32;
+  constexpr bool F16 = C::DT == LIN_F16;
+  extern __shared__ char lds[];
+  const int l = lane_id(), r = l & 15, c = l >> 4, w = wave_id(), wm = w / C::WN, wn = w % C::WN;
+  int part, mi, ni;
+  lin_place(a, C::GM, part, mi, ni);
+  const int m0 = mi * C::BM, n0 = ni * C::BN;
+  const int blocks = (a.K + C::BK - 1) / C::BK, kb0 = part * a.per, kb1 = min(blocks, kb0 + a.per);
+  LinSource<C, C::AR, C::BM, C::DA> sa;
+  LinSource<C, C::BR, C::BN, C::DB> sb;
+  sa.init(a.a, m0, kb0);
+  sb.init(a.b, n0, kb0);
+  auto fetch = [&](int kb, int buf) __attribute__((always_inline)) {
+    const bool tail = (kb + 1) * C::BK > a.K;
+    sa.fetch(lds + buf, a.K, tail);
+    sb.fetch(lds + buf + NP * C::AB, a.K, tail);
+  };
+  // float32: the products of the leading pieces on their own, so that the small ones are not rounded beside them
+  constexpr int NA = NP > 1 ? 2 : 1;
+  f4 acc[NA][NT][MT];
+#pragma unroll
+  for (int q = 0; q < NA; ++q)
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int t = 0; t < MT; ++t) acc[q][i][t] = f4{0.f, 0.f, 0.f, 0.f};
+  auto add = [&](const char* at) __attribute__((always_inline)) {
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      s8 n[NP][NT];
+#pragma unroll
+      for (int p = 0; p < NP; ++p)
+#pragma unroll
+        for (int i = 0; i < NT; ++i) n[p][i] = lin_read<C, C::BR, C::BN>(at + NP * C::AB + p * C::BB, wn * NT + i, s);
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        s8 m[NP];
+#pragma unroll
+        for (int p = 0; p < NP; ++p) m[p] = lin_read<C, C::AR, C::BM>(at + p * C::AB, wm * MT + t, s);
+#pragma unroll
+        for (int o = NP - 1; o >= 0; --o)
+#pragma unroll
+          for (int p = 0; p <= o; ++p) {
+            auto& x = acc[o ? NA - 1 : 0];
+            lin_mfma4<F16>(x[0][t], x[1][t], x[2][t], x[3][t], n[o - p][0], n[o - p][1], n[o - p][2], n[o - p][3], m[p]);
+          }
+      }
+    }
+  };
+  // Block kb has come when only the DMAs of the NBUF - 2 behind it are under way
+  constexpr int AHEAD = C::NBUF - 1, BEHIND = (C::NBUF - 2) * (C::DA + C::DB);
+  static_assert(BEHIND < 16, "vmcnt's low bits");
+  auto next = [&](int x) { return x == (C::NBUF - 1) * C::BUF ? 0 : x + C::BUF; };
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i)
+    if (kb0 + i < kb1) fetch(kb0 + i, i * C::BUF);
+  int buf = 0, into = AHEAD * C::BUF;
+  for (int kb = kb0; kb < kb1; ++kb) {
+    if (kb + C::NBUF - 2 < kb1) __builtin_amdgcn_s_waitcnt(WAIT_VMCNT0 | BEHIND);
+    else __builtin_amdgcn_s_waitcnt(WAIT_VMCNT0);
+    __syncthreads();
+    if (kb + AHEAD < kb1) fetch(kb + AHEAD, into);
+    add(lds + buf);
+    buf = next(buf);
+    into = next(into);
+  }
+  drain(acc[0][0][0]);
+#pragma unroll
+  for (int q = 0; q < NA; ++q)
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int t = 0; t < MT; ++t) lin_hold(acc[q][i][t]);
+  // Each wave turns its results around in LDS, 64 rows at a time: a lane holds four columns of a row here and takes eight
+  // there, so that whole lines are written (and the epilogue's code stands once, not for every register).
+  __syncthreads();
+  float* own = reinterpret_cast<float*>(lds) + w * (64 * C::LDO);
+#pragma unroll
+  for (int h = 0; h < MT; h += 4) {
+#pragma unroll
+    for (int t = h; t < h + 4; ++t)
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        f4 v = acc[0][i][t];
+        if constexpr (NA == 2) v += acc[1][i][t];
+        *reinterpret_cast<f4*>(own + (16 * (t - h) + r) * C::LDO + 16 * i + 4 * c) = v;
+      }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+    for (int j = 0; j < 8; ++j) {
+      const int row = 8 * j + (l >> 3), col = 8 * (l & 7), m = m0 + 16 * (wm * MT + h) + row, n = n0 + 64 * wn + col;
+      if (m >= a.M || n >= a.N) continue;
+      float f[8];
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) *reinterpret_cast<f4*>(f + e) = *reinterpret_cast<const f4*>(own + row * C::LDO + col + e);
+      if (a.parts > 1) lin_out_part<8>(a, part, m, n, f);
+      else lin_out<C::DT, C::ACT, 8>(a, m, n, f);
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// The parts of a sum, in order, and the epilogue; four columns a thread
+template <int DT, int ACT>
+__global__ __launch_bounds__(256) void lin_join_kernel(LinArgs a) {
+  const int cols = (a.N + 3) / 4;
+  const size_t x = (size_t)blockIdx.x * 256 + threadIdx.x, step = (size_t)a.M * a.N;
+  const int m = (int)(x / cols), n = 4 * (int)(x - (size_t)m * cols);
+  if (m >= a.M) return;
+  const float* p = a.part + (size_t)m * a.N + n;
+  float f[4] = {0.f, 0.f, 0.f, 0.f};
+  if (a.N % 4 == 0) {
+#pragma unroll 8
+    for (int i = 0; i < a.parts; ++i) {
+      const float4 v = *reinterpret_cast<const float4*>(p + i * step);
+      f[0] += v.x; f[1] += v.y; f[2] += v.z; f[3] += v.w;
+    }
+  } else {
+    for (int i = 0; i < a.parts; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n + e < a.N) f[e] += p[i * step + e];
+  }
+  lin_out<DT, ACT, 4>(a, m, n, f);
+}
+
+// ---- few rows -----------------------------------------------------------------------------------------------------
+
+// Few rows are bound by W's bytes, and the matrix cores have nothing to share: every element of W is read once, from memory
+// to registers, and multiplied there, float32 as it is.  MR rows at a time; a.parts parts of `per` values of the sum.
+constexpr int LIN_ROWS_W = 8, LIN_ROWS_COLS = 8;       // waves; lanes along the columns of W
+template <int DT>
+struct LinVec {                                          // 16 bytes
+  static constexpr int E = DT == LIN_F32 ? 4 : 8;
+  static __device__ __forceinline__ void widen(const uint4& u, float* x) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (DT == LIN_F32) x[i] = __uint_as_float(w[i]);
+      else if constexpr (DT == LIN_BF16) {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      } else {
+        const h2v h = __builtin_bit_cast(h2v, w[i]);
+        x[2 * i] = (float)h[0];
+        x[2 * i + 1] = (float)h[1];
+      }
+    }
+  }
+  // N values from p[at] on, those before `end` (VEC: all, 16-byte aligned)
+  template <int N, bool VEC>
+  static __device__ __forceinline__ void load(const void* p, size_t at, int left, float* x) {
+    if constexpr (VEC) {
+#pragma unroll
+      for (int i = 0; i < N; i += E)
+        widen(*reinterpret_cast<const uint4*>(static_cast<const typename LinType<DT>::T*>(p) + at + i), x + i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = i < left ? LinType<DT>::get(p, at + i) : 0.f;
+    }
+  }
+};
+
+// W (K, N): eight lanes take 16 bytes each of a row of W, the workgroup's 64 groups of lanes eight rows each; their sums meet
+// over the wave's lanes and then in LDS.
+template <int DT, int ACT, int MR, bool VEC>
+__global__ __launch_bounds__(LIN_ROWS_W * WAVE) void lin_rows_kernel(LinArgs a) {
+  using V = LinVec<DT>;
+  constexpr int E = V::E, COLS = LIN_ROWS_COLS * E;
+  __shared__ float sums[LIN_ROWS_W][MR][COLS];
+  const int l = lane_id(), w = wave_id(), n = blockIdx.x * COLS + (l & 7) * E, m0 = blockIdx.z * MR;
+  const int k0 = blockIdx.y * a.per, k1 = min(a.K, k0 + a.per);
+  float acc[MR][E];
+#pragma unroll
+  for (int m = 0; m < MR; ++m)
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[m][e] = 0.f;
+  if (n < a.N)
+    for (int k = k0 + 8 * (w * 8 + (l >> 3)); k < k1; k += 64 * LIN_ROWS_W) {
+      float wt[8][E], x[MR][8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) V::template load<E, VEC>(a.b.p, (size_t)(VEC ? k + j : min(k + j, k1 - 1)) * a.b.ld + n, a.N - n, wt[j]);
+#pragma unroll
+      for (int m = 0; m < MR; ++m) V::template load<8, VEC>(a.a.p, (size_t)min(m0 + m, a.M - 1) * a.a.ld + k, k1 - k, x[m]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int m = 0; m < MR; ++m)
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[m][e] = VEC || k + j < k1 ? fmaf(x[m][j], wt[j][e], acc[m][e]) : acc[m][e];
+    }
+#pragma unroll
+  for (int m = 0; m < MR; ++m)
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+#pragma unroll
+      for (int o = 8; o < WAVE; o *= 2) acc[m][e] += __shfl_xor(acc[m][e], o);
+      if (l < 8) sums[w][m][l * E + e] = acc[m][e];
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < MR * COLS / 4; i += LIN_ROWS_W * WAVE) {
+    const int m = i / (COLS / 4), col = 4 * (i % (COLS / 4)), at = blockIdx.x * COLS + col;
+    if (m0 + m >= a.M || at >= a.N) continue;
+    float f[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int v = 0; v < LIN_ROWS_W; ++v)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] += sums[v][m][col + e];
+    if (a.parts > 1) lin_out_part<4>(a, blockIdx.y, m0 + m, at, f);
+    else lin_out<DT, ACT, 4>(a, m0 + m, at, f);
+  }
+}
+
+// W (N, K): a wave takes four rows of W, its lanes along the sum
+template <int DT, int ACT, int MR, bool VEC>
+__global__ __launch_bounds__(256) void lin_dots_kernel(LinArgs a) {
+  using V = LinVec<DT>;
+  constexpr int E = V::E, NR = 4;
+  const int l = lane_id(), n0 = (blockIdx.x * 4 + wave_id()) * NR, m0 = blockIdx.z * MR;
+  if (n0 >= a.N) return;
+  const int k0 = blockIdx.y * a.per, k1 = min(a.K, k0 + a.per);
+  float acc[MR][NR];
+#pragma unroll
+  for (int m = 0; m < MR; ++m)
+#pragma unroll
+    for (int i = 0; i < NR; ++i) acc[m][i] = 0.f;
+#pragma unroll 2
+  for (int k = k0 + E * l; k < k1; k += E * WAVE) {
+    float wt[NR][E], x[MR][E];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) V::template load<E, VEC>(a.b.p, (size_t)min(n0 + i, a.N - 1) * a.b.ld + k, k1 - k, wt[i]);
+#pragma unroll
+    for (int m = 0; m < MR; ++m) V::template load<E, VEC>(a.a.p, (size_t)min(m0 + m, a.M - 1) * a.a.ld + k, k1 - k, x[m]);
+#pragma unroll
+    for (int m = 0; m < MR; ++m)
+#pragma unroll
+      for (int i = 0; i < NR; ++i)
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[m][i] = fmaf(x[m][e], wt[i][e], acc[m][i]);
+  }
+#pragma unroll
+  for (int m = 0; m < MR; ++m) {
+#pragma unroll
+    for (int i = 0; i < NR; ++i)
+#pragma unroll
+      for (int o = 1; o < WAVE; o *= 2) acc[m][i] += __shfl_xor(acc[m][i], o);
+    if (l != m || m0 + m >= a.M) continue;
+    if (a.parts > 1) lin_out_part<4>(a, blockIdx.y, m0 + m, n0, acc[m]);
+    else lin_out<DT, ACT, 4>(a, m0 + m, n0, acc[m]);
+  }
+}
+
+// ---- launches -----------------------------------------------------------------------------------------------------
+
+// How a product runs.
+struct LinPlan {
+  int rows;                  // rows at a time by lin_rows_kernel or lin_dots_kernel; 0: tiles
+  int tile;                  // LIN_SMALL, LIN_MID, LIN_BIG
+  int parts, per;            // parts of the sum, of `per` blocks (rows: values)
+};
+enum { LIN_SMALL, LIN_MID, LIN_BIG };
+constexpr int lin_bk(int dtype) { return dtype == LIN_F32 ? 32 : 64; }
+
+template <int DT, int ACT>
+static void lin_join(const LinArgs& a, hipStream_t s) {
+  if (a.parts == 1) return;
+  const size_t threads = (size_t)a.M * ((a.N + 3) / 4);
+  hipLaunchKernelGGL((lin_join_kernel<DT, ACT>), dim3((threads + 255) / 256), dim3(256), 0, s, a);
+}
+template <class C>
+static void lin_go(LinArgs a, const LinPlan& r, hipStream_t s) {
+  a.mt = (a.M + C::BM - 1) / C::BM;
+  a.nt = (a.N + C::BN - 1) / C::BN;
+  a.parts = r.parts;
+  a.per = r.per;
+  hipLaunchKernelGGL(lin_tile_kernel<C>, dim3(a.mt * a.nt * a.parts), dim3(C::W * WAVE), C::LDS, s, a);
+  lin_join<C::DT, C::ACT>(a, s);
+}
+template <int DT, int ACT, int NP, bool AR, bool BR>
+static void lin_tiles(const LinArgs& a, const LinPlan& r, hipStream_t s) {
+  if (r.tile != LIN_BIG) lin_go<LinTile<DT, ACT, NP, AR, BR, 128, 128, 2, 2, lin_bk(DT), 2, 8>>(a, r, s);
+  else if constexpr (DT == LIN_F32) lin_go<LinTile<DT, ACT, NP, AR, BR, 256, 128, 4, 2, lin_bk(DT), 2, 4>>(a, r, s);
+  else lin_go<LinTile<DT, ACT, NP, AR, BR, 256, 256, 2, 4, lin_bk(DT), 2, 4>>(a, r, s);
+}
+
+// Few rows; whole: every row of x and W takes 16-byte accesses
+template <int DT, int ACT, int MR, bool VEC>
+static void lin_rows_go(const LinArgs& a, bool dots, hipStream_t s) {
+  const int z = (a.M + MR - 1) / MR;
+  if (dots) hipLaunchKernelGGL((lin_dots_kernel<DT, ACT, MR, VEC>), dim3((a.N + 15) / 16, a.parts, z), dim3(256), 0, s, a);
+  else {
+    constexpr int cols = LIN_ROWS_COLS * LinVec<DT>::E;
+    hipLaunchKernelGGL((lin_rows_kernel<DT, ACT, MR, VEC>), dim3((a.N + cols - 1) / cols, a.parts, z), dim3(LIN_ROWS_W * WAVE), 0, s, a);
+  }
+  lin_join<DT, ACT>(a, s);
+}
+template <int DT, int ACT>
+static void lin_rows_act(const LinArgs& a, const LinPlan& r, bool dots, bool whole, hipStream_t s) {
+  auto go = [&](auto mr) {
+    if (whole) lin_rows_go<DT, ACT, decltype(mr)::value, true>(a, dots, s);
+    else lin_rows_go<DT, ACT, decltype(mr)::value, false>(a, dots, s);
+  };
+  if (r.rows == 1) go(std::integral_constant<int, 1>{});
+  else if (r.rows == 2) go(std::integral_constant<int, 2>{});
+  else if (r.rows == 4) go(std::integral_constant<int, 4>{});
+  else go(std::integral_constant<int, 8>{});
+}
+template <int DT>
+void lin_rows(const LinArgs& a, const LinPlan& r, int act, bool dots, bool whole, hipStream_t s) {
+  if (act == LIN_SILU) lin_rows_act<DT, LIN_SILU>(a, r, dots, whole, s);
+  else if (act == LIN_GELU) lin_rows_act<DT, LIN_GELU>(a, r, dots, whole, s);
+  else if (act == LIN_TANH) lin_rows_act<DT, LIN_TANH>(a, r, dots, whole, s);
+  else lin_rows_act<DT, LIN_NONE>(a, r, dots, whole, s);
+}
+template <int DT, int NP, bool AR, bool BR>
+static void lin_acts(const LinArgs& a, const LinPlan& r, int act, hipStream_t s) {
+  if (act == LIN_SILU) lin_tiles<DT, LIN_SILU, NP, AR, BR>(a, r, s);
+  else if (act == LIN_GELU) lin_tiles<DT, LIN_GELU, NP, AR, BR>(a, r, s);
+  else if (act == LIN_TANH) lin_tiles<DT, LIN_TANH, NP, AR, BR>(a, r, s);
+  else lin_tiles<DT, LIN_NONE, NP, AR, BR>(a, r, s);
+}
+template <int DT>
+void lin_forms(const LinArgs& a, const LinPlan& r, int form, int act, hipStream_t s) {
+  if constexpr (DT == LIN_F32) {
+    lin_acts<DT, 3, false, false>(a, r, act, s);
+  } else {
+    if (form == LIN_XW) lin_acts<DT, 1, false, true>(a, r, act, s);
+    else if (form == LIN_XWT) lin_acts<DT, 1, false, false>(a, r, act, s);
+    else lin_tiles<DT, LIN_NONE, 1, true, true>(a, r, s);
+  }
+}
+
+
+}  // namespace gdn2
