@@ -941,7 +941,7 @@ int product_args(const gdn2_product* p, gdn2::LinProduct* a) {
 int slope_args(const gdn2_slope* p, gdn2::LinSlope* a) {
   if (!p) return fail(GDN2_ERR_INVALID, "null argument block");
   if (p->M < 1 || p->N < 1) return fail(GDN2_ERR_INVALID, "non-positive shape");
-  if (p->M > kMaxSide || p->N > kMaxSide || p->M > 65535 * 64) return fail(GDN2_ERR_UNSUPPORTED, "shape too large");
+  if (p->M > kMaxSide || p->N > kMaxSide) return fail(GDN2_ERR_UNSUPPORTED, "shape too large");
   if (!float_type(p->dtype) || (p->dy_dtype != p->dtype && p->dy_dtype != GDN2_F32) ||
       (p->dbias && p->bias_dtype != p->dtype && p->bias_dtype != GDN2_F32))
     return fail(GDN2_ERR_INVALID, "unknown dtype");

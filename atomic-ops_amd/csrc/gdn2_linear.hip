@@ -21,7 +21,7 @@ struct LinPack {
   uint16_t* out;
   size_t lds, ld, plane;
   int rows, cols, turn;      // of src
-  int tr, tc;                // tiles of 64 x 64
+  int tr, tc, vec;           // tiles of 64 x 64; whether four values of src can be read at a time
 };
 struct LinPacks {
   LinPack job[2];
@@ -30,74 +30,122 @@ struct LinPacks {
 __device__ __forceinline__ float lin_top(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
 template <bool F32>
 __global__ __launch_bounds__(256) void lin_pack_kernel(LinPacks js) {
-  constexpr int NP = F32 ? 3 : 1;
+  constexpr int NP = F32 ? 3 : 1, LDT = 72;
   const int which = blockIdx.x >= (unsigned)js.start[1];
   const LinPack& j = js.job[which];
-  const int b = blockIdx.x - js.start[which], r0 = b / j.tc * 64, c0 = b % j.tc * 64, x = threadIdx.x & 63, y = threadIdx.x >> 6;
-  __shared__ uint16_t tile[NP][64][65];
-#pragma unroll 4
-  for (int i = 0; i < 16; ++i) {
-    const int row = r0 + 4 * i + y, col = c0 + x;
-    const bool in = row < j.rows && col < j.cols;
-    uint16_t piece[NP];
-    if constexpr (F32) {
-      const float v = in ? static_cast<const float*>(j.src)[(size_t)row * j.lds + col] : 0.f;
-      const float v1 = v - lin_top(v), v2 = v1 - lin_top(v1);
-      piece[0] = (uint16_t)(__float_as_uint(v) >> 16);
-      piece[1] = (uint16_t)(__float_as_uint(v1) >> 16);
-      piece[2] = (uint16_t)(__float_as_uint(v2) >> 16);
+  const int b = blockIdx.x - js.start[which], r0 = b / j.tc * 64, c0 = b % j.tc * 64;
+  __shared__ __attribute__((aligned(16))) uint16_t tile[NP][64][LDT];       // rows of out
+  // four rows of src a wave at a time, four neighbouring values a lane
+  const int y = threadIdx.x >> 4, x = 4 * (threadIdx.x & 15);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = r0 + 16 * i + y, col = c0 + x, last = j.cols - 1;
+    const size_t at = (size_t)min(row, j.rows - 1) * j.lds;
+    uint32_t v[4];
+    if (j.vec && col + 3 < j.cols) {
+      if constexpr (F32) {
+        const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint32_t*>(j.src) + at + col);
+        v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+      } else {
+        const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(j.src) + at + col);
+        v[0] = u.x & 0xffffu; v[1] = u.x >> 16; v[2] = u.y & 0xffffu; v[3] = u.y >> 16;
+      }
     } else {
-      piece[0] = in ? static_cast<const uint16_t*>(j.src)[(size_t)row * j.lds + col] : (uint16_t)0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (F32) v[e] = static_cast<const uint32_t*>(j.src)[at + min(col + e, last)];
+        else v[e] = static_cast<const uint16_t*>(j.src)[at + min(col + e, last)];
+      }
     }
 #pragma unroll
-    for (int p = 0; p < NP; ++p) {
-      if (j.turn) tile[p][4 * i + y][x] = piece[p];
-      else if (row < j.rows && (size_t)col < j.ld) j.out[p * j.plane + (size_t)row * j.ld + col] = piece[p];
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t u = row < j.rows && col + e < j.cols ? v[e] : 0u;
+      uint16_t piece[NP];
+      if constexpr (F32) {
+        const float f = __uint_as_float(u), f1 = f - lin_top(f), f2 = f1 - lin_top(f1);
+        piece[0] = (uint16_t)(u >> 16);
+        piece[1] = (uint16_t)(__float_as_uint(f1) >> 16);
+        piece[2] = (uint16_t)(__float_as_uint(f2) >> 16);
+      } else {
+        piece[0] = (uint16_t)u;
+      }
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        if (j.turn) tile[p][x + e][16 * i + y] = piece[p];
+        else tile[p][16 * i + y][x + e] = piece[p];
+      }
     }
   }
-  if (!j.turn) return;
   __syncthreads();
-#pragma unroll 4
-  for (int i = 0; i < 16; ++i) {
-    const int row = c0 + 4 * i + y, col = r0 + x;      // of out
-    if (row >= j.cols || (size_t)col >= j.ld) continue;
+  const int ro = j.turn ? c0 : r0, co = j.turn ? r0 : c0, rows = j.turn ? j.cols : j.rows;
 #pragma unroll
-    for (int p = 0; p < NP; ++p) j.out[p * j.plane + (size_t)row * j.ld + col] = tile[p][x][4 * i + y];
+  for (int i = 0; i < 2; ++i) {
+    const int ry = threadIdx.x / 8 + 32 * i, row = ro + ry, col = co + 8 * (threadIdx.x & 7);
+    if (row >= rows || (size_t)col >= j.ld) continue;        // (ld: a multiple of 8)
+#pragma unroll
+    for (int p = 0; p < NP; ++p)
+      *reinterpret_cast<uint4*>(j.out + p * j.plane + (size_t)row * j.ld + col) = *reinterpret_cast<const uint4*>(&tile[p][ry][8 * (threadIdx.x & 7)]);
   }
 }
 
 // ---- dz = dy act'(z) and the bias' gradient ------------------------------------------------------------------------
 
-// A workgroup takes 64 columns of 64 rows; part: sums of its rows, [row block][N]
-constexpr int SLOPE_ROWS = 64;
+// A workgroup takes 256 columns, a wave every fourth of `rows` rows, a lane four columns; part: sums of its rows, [row
+// block][N].  vec: whole groups of four columns, and every pointer takes 16 bytes.
 template <int ACT>
-__global__ __launch_bounds__(256) void lin_slope_kernel(LinSlope a, float* part) {
-  __shared__ float sums[4][64];
-  const int n = blockIdx.x * 64 + (threadIdx.x & 63), y = threadIdx.x >> 6;
+__global__ __launch_bounds__(256) void lin_slope_kernel(LinSlope a, float* part, int rows, int vec) {
+  __shared__ float4 sums[4][64];
+  const int l = lane_id(), w = wave_id(), n = blockIdx.x * 256 + 4 * l;
+  const int64_t first = (int64_t)blockIdx.y * rows, last = min((int64_t)a.M, first + rows);
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  if (n < a.N && vec) {
+#pragma unroll 4
+    for (int64_t m = first + w; m < last; m += 4) {
+      const size_t at = (size_t)m * a.N + n;
+      const float4 d = lin_get4(a.dy_dtype, a.dy, at);
+      float f[4] = {d.x, d.y, d.z, d.w};
+      if constexpr (ACT != LIN_NONE) {
+        const float4 z = lin_get4(a.dtype, a.z, at);
+        f[0] *= lin_slope<ACT>(z.x); f[1] *= lin_slope<ACT>(z.y); f[2] *= lin_slope<ACT>(z.z); f[3] *= lin_slope<ACT>(z.w);
+      }
+      if (a.dz) lin_put4(a.dtype, a.dz, at, make_float4(f[0], f[1], f[2], f[3]));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[e] += f[e];
+    }
+  } else if (n < a.N) {
+    for (int64_t m = first + w; m < last; m += 4)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (n + e >= a.N) break;
+        const size_t at = (size_t)m * a.N + n + e;
+        float d = lin_get(a.dy_dtype, a.dy, at);
+        if constexpr (ACT != LIN_NONE) d *= lin_slope<ACT>(lin_get(a.dtype, a.z, at));
+        if (a.dz) lin_put(a.dtype, a.dz, at, d);
+        s[e] += d;
+      }
+  }
+  if (!part) return;
+  sums[w][l] = make_float4(s[0], s[1], s[2], s[3]);
+  __syncthreads();
+  if (w || n >= a.N) return;
+  const float4 x = sums[0][l], y = sums[1][l], u = sums[2][l], v = sums[3][l];
+  const float f[4] = {(x.x + y.x) + (u.x + v.x), (x.y + y.y) + (u.y + v.y), (x.z + y.z) + (u.z + v.z), (x.w + y.w) + (u.w + v.w)};
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (n + e < a.N) part[(size_t)blockIdx.y * a.N + n + e] = f[e];
+}
+// Sixteen groups of sixteen threads: a group's columns, every sixteenth block each
+__global__ __launch_bounds__(256) void lin_bias_kernel(LinSlope a, const float* part, int blocks) {
+  __shared__ float sums[16][17];
+  const int x = threadIdx.x & 15, y = threadIdx.x >> 4, n = blockIdx.x * 16 + x;
   float s = 0.f;
   if (n < a.N)
-    for (int i = y; i < SLOPE_ROWS; i += 4) {
-      const int64_t m = (int64_t)blockIdx.y * SLOPE_ROWS + i;
-      if (m >= a.M) break;
-      const size_t at = (size_t)m * a.N + n;
-      float d = lin_get(a.dy_dtype, a.dy, at);
-      if constexpr (ACT != LIN_NONE) d *= lin_slope<ACT>(lin_get(a.dtype, a.z, at));
-      if (a.dz) lin_put(a.dtype, a.dz, at, d);
-      s += d;
-    }
-  if (!part) return;
-  sums[y][threadIdx.x & 63] = s;
+#pragma unroll 8
+    for (int i = y; i < blocks; i += 16) s += part[(size_t)i * a.N + n];
+  sums[y][x] = s;
   __syncthreads();
-  if (y == 0 && n < a.N) {
-    const int x = threadIdx.x;
-    part[(size_t)blockIdx.y * a.N + n] = (sums[0][x] + sums[1][x]) + (sums[2][x] + sums[3][x]);
-  }
-}
-__global__ __launch_bounds__(256) void lin_bias_kernel(LinSlope a, const float* part, int blocks) {
-  const int n = blockIdx.x * 256 + threadIdx.x;
-  if (n >= a.N) return;
-  float s = 0.f;
-  for (int i = 0; i < blocks; ++i) s += part[(size_t)i * a.N + n];
+  if (y || n >= a.N) return;
+  for (int i = 1; i < 16; ++i) s += sums[i][x];
   lin_put(a.bias_dtype, a.dbias, n, s);
 }
 
@@ -146,9 +194,16 @@ static LinPlan lin_plan(const LinProduct& p) {
     return r;
   }
   const int64_t blocks = (p.K + lin_bk(p.dtype) - 1) / lin_bk(p.dtype);
-  const int64_t big = p.dtype == LIN_F32 ? tiles(256, 128) : tiles(256, 256), mid = tiles(128, 128);
-  if (big * 4 >= cus * 3) r.tile = LIN_BIG;
-  split(blocks, r.tile == LIN_BIG ? 1 : 2 * cus / mid, blocks / 4);
+  const int64_t big = p.dtype == LIN_F32 ? tiles(256, 128) : tiles(256, 256), mid = tiles(128, 128), small = tiles(64, 64);
+  if (big * 4 >= cus * 3) {
+    r.tile = LIN_BIG;
+    split(blocks, 1, 1);
+  } else if (mid >= cus || blocks * mid >= 16 * cus) {
+    split(blocks, 2 * cus / mid, blocks / 4);
+  } else {
+    r.tile = LIN_SMALL;
+    split(blocks, small * 4 >= cus * 3 ? 1 : 2 * cus / small, blocks / 8);
+  }
   return r;
 }
 static size_t lin_parts_bytes(const LinProduct& p, const LinPlan& r) { return r.parts > 1 ? up((size_t)r.parts * p.M * p.N * 4, 256) : 0; }
@@ -196,6 +251,7 @@ hipError_t launch_linear(const LinProduct& p, void* workspace, hipStream_t s) {
     j.rows = d.rows;
     j.cols = d.cols;
     j.turn = p.dtype == LIN_F32 && d.across;
+    j.vec = low(o.p) % 16 == 0 && o.ld % 4 == 0;
     if (d.across && !j.turn) o.rows = (int)d.ld;
     j.tr = (d.rows + 63) / 64;
     j.tc = (d.cols + 63) / 64;
@@ -216,18 +272,29 @@ hipError_t launch_linear(const LinProduct& p, void* workspace, hipStream_t s) {
   return hipGetLastError();
 }
 
-size_t linear_slope_workspace_bytes(const LinSlope& a) {
-  return a.dbias ? (size_t)((a.M + SLOPE_ROWS - 1) / SLOPE_ROWS) * a.N * 4 : 0;
+// rows of a workgroup: four workgroups a CU and more, 32 rows at least
+static int slope_rows(const LinSlope& a) {
+  const int64_t wide = (a.N + 255) / 256, want = (4 * (int64_t)cu_count() + wide - 1) / wide;
+  int64_t rows = (a.M + want - 1) / want;
+  rows = rows < 32 ? 32 : (rows + 3) / 4 * 4;
+  return (int)(rows > a.M ? a.M : rows);
 }
+static int slope_blocks(const LinSlope& a) {
+  const int rows = slope_rows(a);
+  return (a.M + rows - 1) / rows;
+}
+size_t linear_slope_workspace_bytes(const LinSlope& a) { return a.dbias ? (size_t)slope_blocks(a) * a.N * 4 : 0; }
 hipError_t launch_linear_slope(const LinSlope& a, void* workspace, hipStream_t s) {
-  const int blocks = (a.M + SLOPE_ROWS - 1) / SLOPE_ROWS;
+  const int blocks = slope_blocks(a), rows = slope_rows(a);
   float* part = a.dbias ? static_cast<float*>(workspace) : nullptr;
-  const dim3 grid((a.N + 63) / 64, blocks);
-  if (a.act == LIN_SILU) hipLaunchKernelGGL(lin_slope_kernel<LIN_SILU>, grid, dim3(256), 0, s, a, part);
-  else if (a.act == LIN_GELU) hipLaunchKernelGGL(lin_slope_kernel<LIN_GELU>, grid, dim3(256), 0, s, a, part);
-  else if (a.act == LIN_TANH) hipLaunchKernelGGL(lin_slope_kernel<LIN_TANH>, grid, dim3(256), 0, s, a, part);
-  else hipLaunchKernelGGL(lin_slope_kernel<LIN_NONE>, grid, dim3(256), 0, s, a, part);
-  if (part) hipLaunchKernelGGL(lin_bias_kernel, dim3((a.N + 255) / 256), dim3(256), 0, s, a, part, blocks);
+  auto low = [](const void* q) { return reinterpret_cast<uintptr_t>(q); };
+  const int vec = a.N % 4 == 0 && (low(a.dy) | low(a.z) | low(a.dz)) % 16 == 0;
+  const dim3 grid((a.N + 255) / 256, blocks);
+  if (a.act == LIN_SILU) hipLaunchKernelGGL(lin_slope_kernel<LIN_SILU>, grid, dim3(256), 0, s, a, part, rows, vec);
+  else if (a.act == LIN_GELU) hipLaunchKernelGGL(lin_slope_kernel<LIN_GELU>, grid, dim3(256), 0, s, a, part, rows, vec);
+  else if (a.act == LIN_TANH) hipLaunchKernelGGL(lin_slope_kernel<LIN_TANH>, grid, dim3(256), 0, s, a, part, rows, vec);
+  else hipLaunchKernelGGL(lin_slope_kernel<LIN_NONE>, grid, dim3(256), 0, s, a, part, rows, vec);
+  if (part) hipLaunchKernelGGL(lin_bias_kernel, dim3((a.N + 15) / 16), dim3(256), 0, s, a, part, blocks);
   return hipGetLastError();
 }
 

@@ -45,6 +45,59 @@ struct LinType {
     }
   }
 };
+template <int DT>
+struct LinVec {                                          // 16 bytes
+  static constexpr int E = DT == LIN_F32 ? 4 : 8;
+  static __device__ __forceinline__ void widen(const uint4& u, float* x) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (DT == LIN_F32) x[i] = __uint_as_float(w[i]);
+      else if constexpr (DT == LIN_BF16) {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      } else {
+        const h2v h = __builtin_bit_cast(h2v, w[i]);
+        x[2 * i] = (float)h[0];
+        x[2 * i + 1] = (float)h[1];
+      }
+    }
+  }
+  static __device__ __forceinline__ void store8(void* p, size_t at, const float* x) {
+    if constexpr (DT == LIN_F32) {
+      float4* q = reinterpret_cast<float4*>(static_cast<float*>(p) + at);
+      q[0] = make_float4(x[0], x[1], x[2], x[3]);
+      q[1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (DT == LIN_BF16) w[i] = bf16_pack(x[2 * i], x[2 * i + 1]);
+        else {
+          const h2v h = {(_Float16)x[2 * i], (_Float16)x[2 * i + 1]};
+          w[i] = __builtin_bit_cast(uint32_t, h);
+        }
+      }
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + at) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+  // N values from p[at] on, those before `end` (VEC: all, 16-byte aligned)
+  template <int N, bool VEC>
+  static __device__ __forceinline__ void load(const void* p, size_t at, int left, float* x) {
+    if constexpr (VEC) {
+#pragma unroll
+      for (int i = 0; i < N; i += E)
+        widen(*reinterpret_cast<const uint4*>(static_cast<const typename LinType<DT>::T*>(p) + at + i), x + i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = LinType<DT>::get(p, at + min(i, left - 1));      // (no branch: the loads go together)
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = i < left ? x[i] : 0.f;
+    }
+  }
+};
+
+
 // by a type known at run time (wave-uniform)
 __device__ __forceinline__ float lin_get(int dt, const void* p, size_t i) {
   return dt == LIN_F32 ? LinType<LIN_F32>::get(p, i) : dt == LIN_BF16 ? LinType<LIN_BF16>::get(p, i) : LinType<LIN_F16>::get(p, i);
@@ -130,11 +183,11 @@ struct LinTile {
   static constexpr int GM = GM_, DT = DT_, ACT = ACT_, NP = NP_, BM = BM_, BN = BN_, WM = WM_, WN = WN_, BK = BK_, NBUF = NBUF_, W = WM * WN;
   static constexpr bool AR = AR_, BR = BR_;
   static constexpr int MT = BM / WM / 16, NT = BN / WN / 16;
-  static constexpr int AB = BM * BK * 2, BB = BN * BK * 2, BUF = NP * (AB + BB), LDO = 68;
-  static constexpr int LDS = NBUF * BUF > W * 64 * LDO * 4 ? NBUF * BUF : W * 64 * LDO * 4;      // LDO: a row of a wave's results
+  static constexpr int AB = BM * BK * 2, BB = BN * BK * 2, BUF = NP * (AB + BB), LDO = 68, OUT = 16 * (MT < 4 ? MT : 4) * LDO * 4;
+  static constexpr int LDS = NBUF * BUF > W * OUT ? NBUF * BUF : W * OUT;      // LDO: a row of a wave's results
   static constexpr int DA = NP * AB / 1024 / W, DB = NP * BB / 1024 / W;       // a wave's DMAs of a block
   static_assert(AB % 1024 == 0 && BB % 1024 == 0 && NP * AB % (1024 * W) == 0 && NP * BB % (1024 * W) == 0, "whole DMAs");
-  static_assert(NT == 4 && MT % 4 == 0 && (NP == 1 || (!AR && !BR)) && LDS <= 160 * 1024, "shapes");
+  static_assert(NT == 4 && (MT % 4 == 0 || MT < 4) && (NP == 1 || (!AR && !BR)) && LDS <= 160 * 1024, "shapes");
 };
 
 // Where a wave's i-th DMA of an operand's block comes from.  Sixteen bytes a lane:
@@ -143,7 +196,8 @@ struct LinTile {
 // f spreads what the lanes of a read have in common over LDS's banks.
 template <int BK>
 __device__ __forceinline__ int lin_turn(int row) { return BK == 64 ? row & 7 : (row >> 1) & 3; }
-__device__ __forceinline__ int lin_turn_r(int k) { return (k & 3) | (k >> 1 & 4); }
+template <int ROWS>
+__device__ __forceinline__ int lin_turn_r(int k) { return ROWS == 64 ? k & 3 : (k & 3) | (k >> 1 & 4); }
 
 template <class C, bool R, int ROWS, int D>
 struct LinSource {
@@ -160,7 +214,7 @@ struct LinSource {
       size_t at;
       if constexpr (R) {
         k[i] = q / (ROWS / 8);
-        const int c = q % (ROWS / 8), unit = (c >> 1) ^ lin_turn_r(k[i]);
+        const int c = q % (ROWS / 8), unit = (c >> 1) ^ lin_turn_r<ROWS>(k[i]);
         at = (size_t)k[i] * o.ld + min(row0 + 16 * unit + 8 * (c & 1), o.rows - 8);
       } else {
         constexpr int CH = C::BK / 8;
@@ -191,7 +245,7 @@ template <class C, bool R, int ROWS>
 __device__ __forceinline__ s8 lin_read(const char* lds, int t, int s) {
   const int l = lane_id(), r = l & 15, c = l >> 4;
   if constexpr (R) {
-    const int k = 8 * c + (r >> 2), at = k * ROWS * 2 + ((t ^ lin_turn_r(k)) << 5) + (r & 3) * 8 + s * 32 * ROWS * 2;
+    const int k = 8 * c + (r >> 2), at = k * ROWS * 2 + ((t ^ lin_turn_r<ROWS>(k)) << 5) + (r & 3) * 8 + s * 32 * ROWS * 2;
     const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(lds + at));
     const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(lds + at + 8 * ROWS));
     return s8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
@@ -232,6 +286,52 @@ __device__ __forceinline__ void lin_out(const LinArgs& a, int m, int n, const fl
     if (a.residual) z += lin_get(a.out_dtype, a.residual, (size_t)m * a.ldr + n + e);
     lin_put(a.out_dtype, a.y, at + e, z);
   }
+}
+// The same for eight columns, with the bias loaded once and the residual ahead; as lin_out where a.vec does not hold
+struct LinColumns {
+  float4 b[2];
+  __device__ __forceinline__ void load(const LinArgs& a, int n) {
+    b[0] = b[1] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (!a.bias || !a.vec) return;
+    b[0] = lin_get4(a.bias_dtype, a.bias, n);
+    b[1] = lin_get4(a.bias_dtype, a.bias, n + 4);
+  }
+};
+struct LinResidual {
+  uint4 u[2];              // eight of 16 bits, or of 32
+  __device__ __forceinline__ void load(const LinArgs& a, int m, int n) {
+    if (!a.residual || !a.vec) return;
+    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const char*>(a.residual) + ((size_t)m * a.ldr + n) * (a.out_dtype == LIN_F32 ? 4 : 2));
+    u[0] = p[0];
+    if (a.out_dtype == LIN_F32) u[1] = p[1];
+  }
+};
+template <int DT, int ACT>
+__device__ __forceinline__ void lin_out8(const LinArgs& a, int m, int n, float* f, const LinColumns& cols, const LinResidual& r) {
+  if (!a.vec) {
+    lin_out<DT, ACT, 8>(a, m, n, f);
+    return;
+  }
+  const size_t at = (size_t)m * a.N + n;
+  const float b[8] = {cols.b[0].x, cols.b[0].y, cols.b[0].z, cols.b[0].w, cols.b[1].x, cols.b[1].y, cols.b[1].z, cols.b[1].w};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] += b[e];
+  if (a.z) LinVec<DT>::store8(a.z, at, f);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] = lin_act<ACT>(f[e]);
+  if (a.residual) {
+    float x[8];
+    if (a.out_dtype == LIN_F32) {
+      LinVec<LIN_F32>::widen(r.u[0], x);
+      LinVec<LIN_F32>::widen(r.u[1], x + 4);
+    } else {
+      LinVec<DT == LIN_F32 ? LIN_BF16 : DT>::widen(r.u[0], x);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] += x[e];
+  }
+  if (a.out_dtype == LIN_F32) LinVec<LIN_F32>::store8(a.y, at, f);
+  else LinVec<DT>::store8(a.y, at, f);
 }
 // ... or of a part of the sum
 template <int E>
@@ -333,14 +433,18 @@ __global__ __launch_bounds__(C::W * WAVE) void lin_tile_kernel(LinArgs a) {
     for (int i = 0; i < NT; ++i)
 #pragma unroll
       for (int t = 0; t < MT; ++t) lin_hold(acc[q][i][t]);
-  // Each wave turns its results around in LDS, 64 rows at a time: a lane holds four columns of a row here and takes eight
-  // there, so that whole lines are written (and the epilogue's code stands once, not for every register).
+  // Each wave turns its results around in LDS, up to 64 rows at a time: a lane holds four columns of a row here and takes
+  // eight there, so that whole lines are written (and the epilogue's code stands once, not for every register).
   __syncthreads();
-  float* own = reinterpret_cast<float*>(lds) + w * (64 * C::LDO);
+  constexpr int HT = MT < 4 ? MT : 4;
+  float* own = reinterpret_cast<float*>(lds) + w * (16 * HT * C::LDO);
+  const int col = 8 * (l & 7), n = n0 + 64 * wn + col;
+  LinColumns cols;
+  if (n < a.N) cols.load(a, n);
 #pragma unroll
-  for (int h = 0; h < MT; h += 4) {
+  for (int h = 0; h < MT; h += HT) {
 #pragma unroll
-    for (int t = h; t < h + 4; ++t)
+    for (int t = h; t < h + HT; ++t)
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
         f4 v = acc[0][i][t];
@@ -348,15 +452,30 @@ __global__ __launch_bounds__(C::W * WAVE) void lin_tile_kernel(LinArgs a) {
         *reinterpret_cast<f4*>(own + (16 * (t - h) + r) * C::LDO + 16 * i + 4 * c) = v;
       }
     __builtin_amdgcn_wave_barrier();
+    const int mh = m0 + 16 * (wm * MT + h) + (l >> 3);
 #pragma unroll 1
-    for (int j = 0; j < 8; ++j) {
-      const int row = 8 * j + (l >> 3), col = 8 * (l & 7), m = m0 + 16 * (wm * MT + h) + row, n = n0 + 64 * wn + col;
-      if (m >= a.M || n >= a.N) continue;
-      float f[8];
+    for (int j = 0; j < 2 * HT; j += 2) {
+      // (two rows of a lane at a time: the residual's loads are under way together)
+      const int m1 = mh + 8 * j, m2 = m1 + 8;
+      if (n >= a.N || m1 >= a.M) break;
+      LinResidual r1, r2;
+      if (a.parts == 1) {
+        r1.load(a, m1, n);
+        r2.load(a, min(m2, a.M - 1), n);
+      }
+      float f[2][8];
 #pragma unroll
-      for (int e = 0; e < 8; e += 4) *reinterpret_cast<f4*>(f + e) = *reinterpret_cast<const f4*>(own + row * C::LDO + col + e);
-      if (a.parts > 1) lin_out_part<8>(a, part, m, n, f);
-      else lin_out<C::DT, C::ACT, 8>(a, m, n, f);
+      for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int e = 0; e < 8; e += 4)
+          *reinterpret_cast<f4*>(f[q] + e) = *reinterpret_cast<const f4*>(own + (8 * (j + q) + (l >> 3)) * C::LDO + col + e);
+      if (a.parts > 1) {
+        lin_out_part<8>(a, part, m1, n, f[0]);
+        if (m2 < a.M) lin_out_part<8>(a, part, m2, n, f[1]);
+      } else {
+        lin_out8<C::DT, C::ACT>(a, m1, n, f[0], cols, r1);
+        if (m2 < a.M) lin_out8<C::DT, C::ACT>(a, m2, n, f[1], cols, r2);
+      }
     }
     __builtin_amdgcn_wave_barrier();
   }
@@ -391,38 +510,6 @@ __global__ __launch_bounds__(256) void lin_join_kernel(LinArgs a) {
 // Few rows are bound by W's bytes, and the matrix cores have nothing to share: every element of W is read once, from memory
 // to registers, and multiplied there, float32 as it is.  MR rows at a time; a.parts parts of `per` values of the sum.
 constexpr int LIN_ROWS_W = 8, LIN_ROWS_COLS = 8;       // waves; lanes along the columns of W
-template <int DT>
-struct LinVec {                                          // 16 bytes
-  static constexpr int E = DT == LIN_F32 ? 4 : 8;
-  static __device__ __forceinline__ void widen(const uint4& u, float* x) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (DT == LIN_F32) x[i] = __uint_as_float(w[i]);
-      else if constexpr (DT == LIN_BF16) {
-        x[2 * i] = __uint_as_float(w[i] << 16);
-        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-      } else {
-        const h2v h = __builtin_bit_cast(h2v, w[i]);
-        x[2 * i] = (float)h[0];
-        x[2 * i + 1] = (float)h[1];
-      }
-    }
-  }
-  // N values from p[at] on, those before `end` (VEC: all, 16-byte aligned)
-  template <int N, bool VEC>
-  static __device__ __forceinline__ void load(const void* p, size_t at, int left, float* x) {
-    if constexpr (VEC) {
-#pragma unroll
-      for (int i = 0; i < N; i += E)
-        widen(*reinterpret_cast<const uint4*>(static_cast<const typename LinType<DT>::T*>(p) + at + i), x + i);
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) x[i] = i < left ? LinType<DT>::get(p, at + i) : 0.f;
-    }
-  }
-};
-
 // W (K, N): eight lanes take 16 bytes each of a row of W, the workgroup's 64 groups of lanes eight rows each; their sums meet
 // over the wave's lanes and then in LDS.
 template <int DT, int ACT, int MR, bool VEC>
@@ -540,7 +627,8 @@ static void lin_go(LinArgs a, const LinPlan& r, hipStream_t s) {
 }
 template <int DT, int ACT, int NP, bool AR, bool BR>
 static void lin_tiles(const LinArgs& a, const LinPlan& r, hipStream_t s) {
-  if (r.tile != LIN_BIG) lin_go<LinTile<DT, ACT, NP, AR, BR, 128, 128, 2, 2, lin_bk(DT), 2, 8>>(a, r, s);
+  if (r.tile == LIN_SMALL) lin_go<LinTile<DT, ACT, NP, AR, BR, 64, 64, 4, 1, lin_bk(DT), 3, 8>>(a, r, s);
+  else if (r.tile == LIN_MID) lin_go<LinTile<DT, ACT, NP, AR, BR, 128, 128, 2, 2, lin_bk(DT), 2, 8>>(a, r, s);
   else if constexpr (DT == LIN_F32) lin_go<LinTile<DT, ACT, NP, AR, BR, 256, 128, 4, 2, lin_bk(DT), 2, 4>>(a, r, s);
   else lin_go<LinTile<DT, ACT, NP, AR, BR, 256, 256, 2, 4, lin_bk(DT), 2, 4>>(a, r, s);
 }
