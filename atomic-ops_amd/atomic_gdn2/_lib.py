@@ -191,7 +191,7 @@ _BIND_ABI = ("gdn2_residual_layout", "gdn2_fwd_workspace_bytes", "gdn2_bwd_works
              "gdn2_bwd", "gdn2_decode_from", "gdn2_default_state_ckpt", "gdn2_w4_workspace_bytes", "gdn2_w4_linear", "gdn2_beam_workspace_bytes",
              "gdn2_beam_step", "gdn2_lm_premix_step_fwd", "gdn2_linear_workspace_bytes", "gdn2_linear",
              "gdn2_linear_slope_workspace_bytes", "gdn2_linear_slope", "gdn2_loss_workspace_bytes", "gdn2_cross_entropy",
-             "gdn2_scale_rows", "gdn2_adamw_workspace_bytes", "gdn2_adamw", "gdn2_last_error")
+             "gdn2_scale_rows", "gdn2_adamw_workspace_bytes", "gdn2_adamw", "gdn2_adamw_unpack", "gdn2_last_error")
 
 
 def bind():

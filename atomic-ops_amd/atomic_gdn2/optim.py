@@ -153,6 +153,8 @@ class AdamW(torch.optim.Optimizer):
         groups' order, written into the given tensors or new ones (a parameter without a state has zeros)."""
         if self.state_bits != 8:
             raise ValueError("states of 32 bits are values already")
+        if type(exp_avg) is list and type(exp_avg_sq) is list and _lib.bind().adamw_unpack(self.param_groups, self.state, exp_avg, exp_avg_sq):
+            return exp_avg, exp_avg_sq
         ps = [p for group in self.param_groups for p in group["params"]]
         outs = []
         for given in (exp_avg, exp_avg_sq):
@@ -175,6 +177,7 @@ class AdamW(torch.optim.Optimizer):
             dev = ps[0].device
             with torch.cuda.device(dev):
                 _lib.check(_lib.lib().gdn2_adamw_unpack(ts, len(at), *ptrs, _lib.stream_handle(dev)), "gdn2_adamw_unpack")
+            torch.autograd.graph.increment_version([out[i] for out in outs for i in at])
         return tuple(outs)
 
     def load_state_dict(self, state_dict):

@@ -59,6 +59,7 @@ struct Abi {
   decltype(&gdn2_scale_rows) scale_rows;
   decltype(&gdn2_adamw_workspace_bytes) adamw_ws;
   decltype(&gdn2_adamw) adamw;
+  decltype(&gdn2_adamw_unpack) adamw_unpack;
   decltype(&gdn2_last_error) last_error;
 } abi{};
 
@@ -729,6 +730,7 @@ PyMethodDef methods[] = {
     {"premix_step", (PyCFunction)(void (*)())py_premix_step, METH_FASTCALL, "premix_step(y, history, weights, heads, g_max, parents)"},
     {"linear", (PyCFunction)(void (*)())py_linear, METH_FASTCALL, "linear(x, weight, bias, residual, activation, float32)"},
     {"cross_entropy", (PyCFunction)(void (*)())py_cross_entropy, METH_FASTCALL, "cross_entropy(logits, targets, ignore, smoothing, z, reduction)"},
+    {"adamw_unpack", (PyCFunction)(void (*)())py_adamw_unpack, METH_FASTCALL, "adamw_unpack(groups, state, exp_avg, exp_avg_sq)"},
     {"adamw", (PyCFunction)(void (*)())py_adamw, METH_FASTCALL, "adamw(groups, state, bits, max_norm)"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module{PyModuleDef_HEAD_INIT, "_bind", "native call path of the operator", -1, methods};

@@ -369,3 +369,38 @@ PyObject* py_adamw(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Py_RETURN_TRUE;
   END_HANDLE_TH_ERRORS
 }
+
+// adamw_unpack(groups, state, exp_avg, exp_avg_sq): the values of 8-bit states into lists of a tensor for each parameter;
+// True, or None: not as the kernel takes them
+PyObject* py_adamw_unpack(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 4) return PyErr_Format(PyExc_TypeError, "adamw_unpack takes 4 arguments");
+  std::vector<gdn2_adamw_tensor> ts;
+  std::vector<Tensor> ps;
+  if (!plain_mode() || !PyList_Check(args[2]) || !PyList_Check(args[3]) || !adamw_tensors(args[0], args[1], 8, false, &ts, &ps)) return none();
+  const c10::Device dev = ps[0].device();
+  std::vector<float*> out[2];
+  std::vector<Tensor> held;
+  for (int k = 0; k < 2; ++k) {
+    // (every parameter has a state: then the tensors are the parameters')
+    if ((size_t)PyList_GET_SIZE(args[2 + k]) != ts.size()) return none();
+    for (size_t i = 0; i < ts.size(); ++i) {
+      PyObject* o = PyList_GET_ITEM(args[2 + k], (Py_ssize_t)i);
+      if (!THPVariable_Check(o)) return none();
+      const Tensor& t = THPVariable_Unpack(o);
+      if (!plain(t, dev) || t.scalar_type() != at::kFloat || t.numel() != ts[i].numel || !t.is_contiguous() || recorded({&t})) return none();
+      out[k].push_back(f32_at(t));
+      held.push_back(t);
+    }
+  }
+  int status = 0;
+  unlocked([&] {
+    c10::DeviceGuard guard(dev);
+    status = abi.adamw_unpack(ts.data(), (int)ts.size(), out[0].data(), out[1].data(), stream_of(dev));
+    if (!status)
+      for (const Tensor& t : held) t.unsafeGetTensorImpl()->bump_version();
+  });
+  if (status) return none();
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}

@@ -22,9 +22,10 @@
 namespace gdn2 {
 
 constexpr int OPT_CHUNK = 8192;            // elements of a workgroup of the update
-constexpr int OPT_NORM_CHUNK = 32768;      // ... of the norm
+constexpr int OPT_CHUNK8 = 2048;           // ... with states of 8 bits (bound by what it computes: many small ones)
+constexpr int OPT_NORM_CHUNK = 16384;      // ... of the norm
 constexpr int OPT_BLOCK = 256;             // elements of a scale
-constexpr int OPT_TENSORS = 48, OPT_GRADS = 160, OPT_STEPS = 56;
+constexpr int OPT_TENSORS = 200, OPT_GRADS = 200, OPT_STEPS = 200;
 
 // What a tensor's update needs beside it; written by opt_begin_kernel
 struct OptHyper {
@@ -57,7 +58,7 @@ struct OptTensors {
   } t[OPT_TENSORS];
   int tensors;
 };
-static_assert(sizeof(OptGrads) < 4000 && sizeof(OptSteps) < 4000 && sizeof(OptTensors) < 4000, "argument blocks");
+static_assert(sizeof(OptGrads) < 16000 && sizeof(OptSteps) < 16000 && sizeof(OptTensors) < 16000, "argument blocks");
 
 template <int DT>
 struct OptType {
@@ -115,15 +116,19 @@ __global__ __launch_bounds__(256) void opt_norm_kernel(OptGrads a, double* part)
   const int64_t at = (int64_t)(b - a.start[i]) * OPT_NORM_CHUNK, n = min((int64_t)OPT_NORM_CHUNK, a.n[i] - at);
   const T* g = static_cast<const T*>(a.g[i]) + at;
   double s = 0.0;
-  const int whole = (reinterpret_cast<uintptr_t>(g) & (4 * sizeof(T) - 1)) ? 0 : (int)(n / 4);
-#pragma unroll 4
+  constexpr int E = 16 / sizeof(T);
+  const int whole = (reinterpret_cast<uintptr_t>(g) & 15) ? 0 : (int)(n / E);
+#pragma unroll 8
   for (int j = threadIdx.x; j < whole; j += 256) {
-    float x[4];
-    O::get4(g + 4 * j, x);
+    const uint4 u = *reinterpret_cast<const uint4*>(g + E * j);
+    const T* x = reinterpret_cast<const T*>(&u);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s = fma((double)x[e], (double)x[e], s);
+    for (int e = 0; e < E; ++e) {
+      const double v = O::get(x + e);
+      s = fma(v, v, s);
+    }
   }
-  for (int j = 4 * whole + threadIdx.x; j < n; j += 256) {
+  for (int j = E * whole + threadIdx.x; j < n; j += 256) {
     const double x = O::get(g + j);
     s = fma(x, x, s);
   }
@@ -172,12 +177,14 @@ __global__ __launch_bounds__(1024) void opt_begin_kernel(OptSteps a, const doubl
 struct OptState {
   float m, v;
 };
-__device__ __forceinline__ float opt_one(const OptHyper& h, float c, float g, float p, OptState& x) {
+__device__ __forceinline__ float opt_one(const OptHyper& h, float c, float g, float p, OptState& x, float* root = nullptr) {
 #pragma clang fp contract(off)
   g = g * c;
   x.m = x.m * h.b1 + g * h.nb1;
   x.v = x.v * h.b2 + (g * g) * h.nb2;
-  return p * h.keep - (x.m / (sqrtf(x.v) * h.root + h.eps)) * h.size;
+  const float u = sqrtf(x.v);
+  if (root) *root = u;
+  return p * h.keep - (x.m / (u * h.root + h.eps)) * h.size;
 }
 
 template <int DT>
@@ -240,22 +247,24 @@ __device__ __forceinline__ uint32_t opt_hash(uint32_t x) {
   return x ^ (x >> 16);
 }
 __device__ __forceinline__ float opt_dither(uint32_t bits) { return ((float)bits + 0.5f) * (1.f / 65536.f); }
-__device__ __forceinline__ int opt_m_code(float m, float s, float r) {
+// The codes below and above a value are found by the hardware's square root (error below 2^-22, 3e-5 of a code): where that
+// takes the neighbour below a code's own value, the value lies at the very end of the interval, and the comparison gives the
+// same code from either side (the dither keeps 7e-6 from 0 and 1).  inv: 1 / s, or 0 where there is no code.  (A scale whose
+// inverse is no float32 number is divided by.)
+__device__ __forceinline__ int opt_m_code(float m, float s, float inv, float r) {
 #pragma clang fp contract(off)
-  if (!(s > 0.f)) return 0;
-  const float a = fabsf(m), c = fminf(floorf(sqrtf(a / s)), 126.f), low = c * c * s, high = (c + 1.f) * (c + 1.f) * s;
-  const int k = (int)c + (a - low > r * (high - low));
+  const float a = fabsf(m), q = inv < INFINITY ? a * inv : a / s, c = fminf(floorf(__builtin_amdgcn_sqrtf(q)), 126.f), low = c * c * s, high = (c + 1.f) * (c + 1.f) * s;
+  const int k = inv > 0.f ? (int)c + (a - low > r * (high - low)) : 0;
   return m < 0.f ? -k : k;
 }
-__device__ __forceinline__ int opt_v_code(float v, float s, float r) {
+__device__ __forceinline__ int opt_v_code(float v, float u, float s, float inv, float r) {
 #pragma clang fp contract(off)
-  if (!(s > 0.f)) return 0;
-  const float c = fminf(floorf(sqrtf(sqrtf(v) / s)), 254.f);
+  const float q = inv < INFINITY ? u * inv : u / s, c = fminf(floorf(__builtin_amdgcn_sqrtf(q)), 254.f);
   float low = c * c * s, high = (c + 1.f) * (c + 1.f) * s;
   low = low * low;
   high = high * high;
-  const int k = (int)c + (v - low > r * (high - low));
-  return v > 0.f && k < 1 ? 1 : k;
+  const int k = inv > 0.f ? (int)c + (v - low > r * (high - low)) : 0;
+  return inv > 0.f && v > 0.f && k < 1 ? 1 : k;
 }
 // largest of a wave; NaN where one of it is not finite
 __device__ __forceinline__ float opt_wave_max(float x) {
@@ -275,8 +284,8 @@ __global__ __launch_bounds__(256) void opt_update8_kernel(OptTensors a, const fl
   const auto& t = a.t[i];
   const OptHyper h = hyper[t.hyper];
   const float c = coef ? *coef : 1.f;
-  const int64_t first = (int64_t)(b - t.start) * OPT_CHUNK;
-  for (int k = wave_id(); k < OPT_CHUNK / OPT_BLOCK; k += 4) {
+  const int64_t first = (int64_t)(b - t.start) * OPT_CHUNK8;
+  for (int k = wave_id(); k < OPT_CHUNK8 / OPT_BLOCK; k += 4) {
     const int64_t at = first + k * OPT_BLOCK;
     if (at >= t.n) break;
     const int64_t block = at / OPT_BLOCK, j = at + 4 * lane_id();
@@ -310,16 +319,16 @@ __global__ __launch_bounds__(256) void opt_update8_kernel(OptTensors a, const fl
         }
     }
     const float s_m = t.ms[block], s_v = t.vs[block];
-    float mx[4], vx[4], m_top = 0.f, v_top = 0.f;
+    float mx[4], vx[4], ux[4], m_top = 0.f, v_top = 0.f;
     bool bad = false;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       if (e >= n) {
-        mx[e] = vx[e] = 0.f;
+        mx[e] = vx[e] = ux[e] = 0.f;
         continue;
       }
       OptState x{opt_m_value(cm[e], s_m), opt_v_value(cv[e], s_v)};
-      px[e] = opt_one(h, c, gx[e], px[e], x);
+      px[e] = opt_one(h, c, gx[e], px[e], x, &ux[e]);
       mx[e] = x.m;
       vx[e] = x.v;
       bad |= !(fabsf(x.m) < INFINITY);
@@ -330,11 +339,12 @@ __global__ __launch_bounds__(256) void opt_update8_kernel(OptTensors a, const fl
     m_top = opt_wave_max(bad ? INFINITY : m_top);
     v_top = opt_wave_max(v_top);
     const float new_m = m_top * (1.f / 16129.f), new_v = sqrtf(v_top) * (1.f / 65025.f);
+    const float inv_m = new_m > 0.f ? 1.f / new_m : 0.f, inv_v = new_v > 0.f ? 1.f / new_v : 0.f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const uint32_t r = opt_hash((uint32_t)(j + e) * 0x9E3779B1u + h.hash);
-      cm[e] = opt_m_code(mx[e], new_m, opt_dither(r & 0xffffu));
-      cv[e] = opt_v_code(vx[e], new_v, opt_dither(r >> 16));
+      cm[e] = opt_m_code(mx[e], new_m, inv_m, opt_dither(r & 0xffffu));
+      cv[e] = opt_v_code(vx[e], ux[e], new_v, inv_v, opt_dither(r >> 16));
     }
     if (vec) {
       if constexpr (DT != LIN_F32) OptType<LIN_F32>::put4(w, px);
@@ -368,8 +378,8 @@ __global__ __launch_bounds__(256) void opt_update8_kernel(OptTensors a, const fl
 __global__ __launch_bounds__(256) void opt_unpack_kernel(OptTensors a) {
   const int b = blockIdx.x, i = opt_find(a.tensors, b, [&](int k) { return a.t[k].start; });
   const auto& t = a.t[i];
-  const int64_t first = (int64_t)(b - t.start) * OPT_CHUNK;
-  const int n = (int)min((int64_t)OPT_CHUNK, t.n - first);
+  const int64_t first = (int64_t)(b - t.start) * OPT_CHUNK8;
+  const int n = (int)min((int64_t)OPT_CHUNK8, t.n - first);
   const int8_t* mc = static_cast<const int8_t*>(t.m) + first;
   const uint8_t* vc = static_cast<const uint8_t*>(t.v) + first;
   float *m = static_cast<float*>(t.p) + first, *v = t.master + first;
@@ -407,7 +417,7 @@ size_t adamw_workspace_bytes(const gdn2_adamw_tensor* t, int n) { return opt_hyp
 // The tensors of a type, as many to a launch as an argument block holds: go(block, workgroups)
 template <class F>
 static void opt_each(const gdn2_adamw_tensor* t, int n, int dtype, int bits, F go) {
-  const int size = dtype == LIN_F32 ? 4 : 2;
+  const int size = dtype == LIN_F32 ? 4 : 2, chunk = bits == 8 ? OPT_CHUNK8 : OPT_CHUNK;
   OptTensors a{};
   int64_t blocks = 0;
   int first = 0;
@@ -419,7 +429,7 @@ static void opt_each(const gdn2_adamw_tensor* t, int n, int dtype, int bits, F g
   for (int i = 0; i < n; ++i) {
     const gdn2_adamw_tensor& x = t[i];
     if (x.dtype != dtype) continue;
-    const int64_t b = (x.numel + OPT_CHUNK - 1) / OPT_CHUNK;
+    const int64_t b = (x.numel + chunk - 1) / chunk;
     if (a.tensors == OPT_TENSORS || blocks + b > 0x7fffffff || (a.tensors && i - first > 0x7fff)) flush();
     if (a.tensors == 0) first = i;
     auto& o = a.t[a.tensors++];
