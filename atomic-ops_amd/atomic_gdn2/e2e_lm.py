@@ -15,7 +15,9 @@ The training step follows ``PAYLOAD['candidate_e2e.py']`` L15-29: mean cross-ent
 next-token logits, ``clip_by_global_norm(1.0)`` then AdamW (lr 1e-3, weight decay 0.01, the
 optax defaults b1 0.9, b2 0.999, eps 1e-8; decay applied to every parameter).  Inputs are
 uniform tokens in [0, vocab).  Matmuls run in fp32 (the reference sets
-``jax_default_matmul_precision='highest'``).
+``jax_default_matmul_precision='highest'``); ``LMConfig(products="bfloat16")`` rounds their operands to
+bfloat16 and runs them on ``linear``'s kernels, and ``TrainStep(fused=True)`` takes the loss from
+``losses.cross_entropy`` and the update from ``optim.AdamW``.
 
 This module is the operator's caller, written with torch (no flax / optax in this image); the
 operator itself is ``make_blr_trainable`` on the HIP kernels.  On the GPU in float32 a block's
@@ -31,8 +33,10 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
-from . import lm_kernels
+from . import lm_kernels, losses
 from .config import make_cfg
+from .linear import linear
+from .optim import AdamW
 from .pipeline import make_blr_trainable
 
 
@@ -47,6 +51,11 @@ class LMConfig:
     d_conv: int = 4
     g_max: float = 160.0 / 128
     decay_init: float = 0.05
+    products: str = "float32"       # or "bfloat16": what the matrix products' operands are rounded to
+
+    def __post_init__(self):
+        if self.products not in ("float32", "bfloat16"):
+            raise ValueError(f"products={self.products!r}: 'float32' or 'bfloat16'")
 
     @property
     def proj_dim(self):
@@ -152,6 +161,9 @@ class GDN2Block(nn.Module):
         if ws is not None:
             return lm_kernels.block_forward(self, x, ws)
         cfg = self.cfg
+        if cfg.products != "float32":
+            raise ValueError("products in bfloat16 run on the HIP kernels only: float32 weights and inputs on the GPU, the HIP "
+                             "operator as the mixer, no hooks, transforms or autocast")
         B, L, _ = x.shape
         H, D = cfg.n_heads, cfg.d_head
         eps = 1e-6
@@ -184,7 +196,10 @@ class LM(nn.Module):
             x = blk(x)
         if (len(self.blocks) and lm_kernels.operator_of(self.blocks[-1].kernel_fn) is not None
                 and lm_kernels.norm_usable(self.final_norm, x, RMSNorm)):
-            return lm_kernels.rms_norm(self.final_norm, x) @ self.embed.t()
+            h = lm_kernels.rms_norm(self.final_norm, x)
+            if self.cfg.products == "bfloat16":
+                return linear(h.bfloat16(), self.embed.bfloat16().t(), out_dtype=torch.float32)
+            return h @ self.embed.t()
         return self.final_norm(x) @ self.embed.t()
 
 
@@ -192,8 +207,11 @@ def n_params(model: nn.Module) -> int:
     return sum(p.numel() for p in model.parameters())
 
 
-def lm_loss(model, ids):
+def lm_loss(model, ids, fused=False):
+    """Mean cross-entropy of the next tokens; fused: by ``losses.cross_entropy``, on the logits as they lie."""
     logits = model(ids)
+    if fused:
+        return losses.cross_entropy(logits, F.pad(ids[:, 1:], (0, 1), value=-100))
     V = logits.shape[-1]
     return F.cross_entropy(logits[:, :-1].reshape(-1, V), ids[:, 1:].reshape(-1))
 
@@ -206,19 +224,29 @@ def clip_by_global_norm_(grads, max_norm):
 
 
 class TrainStep:
-    """One optimisation step: loss and gradients, clip_by_global_norm(max_norm), AdamW."""
+    """One optimisation step: loss and gradients, clip_by_global_norm(max_norm), AdamW.  fused: the loss,
+    the clipping and the update on their HIP kernels, with states of state_bits (32 or 8)."""
 
-    def __init__(self, model, lr=1e-3, weight_decay=0.01, max_norm=1.0):
-        self.model = model
+    def __init__(self, model, lr=1e-3, weight_decay=0.01, max_norm=1.0, fused=False, state_bits=32):
+        self.model, self.fused = model, fused
         self.params = [p for p in model.parameters()]
+        if fused:
+            self.opt = AdamW(self.params, lr=lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=weight_decay, max_norm=max_norm,
+                             state_bits=state_bits)
+            return
+        if state_bits != 32:
+            raise ValueError(f"state_bits={state_bits}: fewer than 32 need fused=True")
         self.opt = torch.optim.AdamW(self.params, lr=lr, betas=(0.9, 0.999), eps=1e-8,
                                      weight_decay=weight_decay, foreach=True)
         self.max_norm = max_norm
 
     def __call__(self, ids):
         self.opt.zero_grad(set_to_none=True)
-        loss = lm_loss(self.model, ids)
+        loss = lm_loss(self.model, ids, self.fused)
         loss.backward()
+        if self.fused:
+            self.opt.step()
+            return loss.detach()
         clip_by_global_norm_([p.grad for p in self.params], self.max_norm)
         self.opt.step()
         return loss.detach()

@@ -13,6 +13,10 @@ itself to be differentiated (``create_graph``) recomputes the step from ``_premi
 ``_postmix_ref`` / ``_mlp_ref``, the same in torch operations; the operator between them is
 differentiable once, and a second derivative through it raises.
 
+With ``LMConfig.products = "bfloat16"`` the products' operands are rounded to bfloat16 and multiplied by
+the kernels of ``linear`` (``_half`` and ``_product`` below); sums, their results, everything between the
+products, the residual stream and all gradients stay float32.
+
 ``usable`` says where this path stands in for the module's own forward: float32 on the GPU, the
 block's own submodule types without hooks, the HIP operator as the mixer.  Everywhere else (the CPU,
 other dtypes, autocast, function transforms, forward mode, dispatch modes, tracing, hooked, patched or
@@ -30,6 +34,7 @@ import torch.overrides
 import torch.utils._device
 
 from . import _lib
+from .linear import _XTW, _XW, _XWT, _product as _linear_product
 
 _i32, _f32c, _vp = ctypes.c_int32, ctypes.c_float, ctypes.c_void_p
 _EPS = 1e-6
@@ -127,6 +132,22 @@ def _scatter(wide, like):
     out = [torch.empty(t.shape, dtype=torch.float32, device=wide.device) for t in like]
     _columns(1, out, wide)
     return out
+
+
+def _half(t):
+    return t.to(torch.bfloat16, memory_format=torch.contiguous_format)
+
+
+def _product(form, a, b, residual=None):
+    """float32 a b (_XW, plus residual), a b^T (_XWT) or a^T b (_XTW) of bfloat16 matrices."""
+    M, K = a.shape if form != _XTW else a.shape[::-1]
+    N = b.shape[0] if form == _XWT else b.shape[1]
+    return _linear_product(form, a, b, M, K, N, torch.empty((M, N), dtype=torch.float32, device=a.device), residual=residual)
+
+
+def _once(half):
+    if half and torch.is_grad_enabled():
+        raise RuntimeError("a block with products in bfloat16 is once differentiable")
 
 
 def _weight_grad(x, dy):
@@ -247,48 +268,59 @@ class _PreMix(torch.autograd.Function):
     q, k, v, w, b, g (B, H, L, D), output-gate logits (B L, C)."""
 
     @staticmethod
-    def forward(ctx, H, D, g_max, x, *ps):
+    def forward(ctx, H, D, g_max, x, *ps, half=False):
         B, L, d = x.shape
         C, dev = H * D, x.device
         ws = ps[:7]
         ldy = -(-(6 * C + H) // 64) * 64
         wide = _gather(ws, ldy)
-        y = x.reshape(B * L, d) @ wide
+        x2 = x.reshape(B * L, d)
+        if half:
+            wide, x2 = _half(wide), _half(x2)
+        y = _product(_XW, x2, wide) if half else x2 @ wide
         outs = [torch.empty((B, H, L, D), dtype=torch.float32, device=dev) for _ in range(6)]
         og = torch.empty((B * L, C), dtype=torch.float32, device=dev)
-        a = _PreMix._args(H, D, g_max, x, ps, y, outs, og)
+        a = _PreMix._args(H, D, g_max, B, L, ps, y, outs, og)
         _call("gdn2_lm_premix_fwd", dev, ctypes.byref(a))
-        ctx.dims = (H, D, g_max)
-        _save(ctx, x, *ps, wide, y, *outs, og)
+        ctx.dims = (H, D, g_max, half, B)
+        _save(ctx, x2 if half else x, *ps, wide, y, *outs, og)
         return (*outs, og)
 
     @staticmethod
-    def _args(H, D, g_max, x, ps, y, outs, og):
+    def _args(H, D, g_max, B, L, ps, y, outs, og):
         cqw, cqb, ckw, ckb, cvw, cvb, be, bw, bd, da = (t.data_ptr() for t in ps[7:])
-        return _PremixArgs(x.shape[0], x.shape[1], H, D, y.shape[1], float(g_max), y.data_ptr(), (_vp * 3)(cqw, ckw, cvw),
+        return _PremixArgs(B, L, H, D, y.shape[1], float(g_max), y.data_ptr(), (_vp * 3)(cqw, ckw, cvw),
                            (_vp * 3)(cqb, ckb, cvb), (_vp * 2)(be, bw), bd, da, (_vp * 6)(*(t.data_ptr() for t in outs)),
                            og.data_ptr())
 
     @staticmethod
     def backward(ctx, *gs):
-        H, D, g_max = ctx.dims
+        H, D, g_max, half, B = ctx.dims
         saved = _saved(ctx)
         x, ps, wide, y, outs, og = saved[0], saved[1:18], saved[18], saved[19], saved[20:26], saved[26]
+        _once(half)
         if torch.is_grad_enabled():
             return (None, None, None) + _vjp_through(_premix_ref(H, D, g_max), (x,) + ps, ctx.needs_input_grad[3:], gs)
-        B, L, d = x.shape
-        C, dev, N = H * D, x.device, x.shape[0] * x.shape[1]
+        N, d = y.shape[0], x.shape[-1]
+        C, dev, L = H * D, x.device, N // B
         like = list(outs) + [og]
         ds = [torch.zeros_like(t) if g is None else _dense(g) for g, t in zip(gs, like)]
         dy = torch.empty_like(y)
         dparam = torch.empty(17 * C + 2 * H, dtype=torch.float32, device=dev)
         ws = torch.empty(_lib.lib().gdn2_lm_premix_workspace_bytes(B, L, H, D), dtype=torch.uint8, device=dev)
-        a = _PreMix._args(H, D, g_max, x, ps, y, outs, og)
+        a = _PreMix._args(H, D, g_max, B, L, ps, y, outs, og)
         _call("gdn2_lm_premix_bwd", dev, ctypes.byref(a), (_vp * 6)(*(t.data_ptr() for t in ds[:6])), _addr(ds[6]),
               _addr(dy), _addr(dparam), _addr(ws))
         need = ctx.needs_input_grad[3:]
-        dx = _input_grad(dy, wide, 2, 32).reshape(B, L, d) if need[0] else None
         x2, dws = x.reshape(N, d), [None] * 7
+        if half:
+            dy = _half(dy)
+            dx = _product(_XWT, dy, wide).reshape(B, L, d) if need[0] else None
+            if any(need[1:8]):
+                dws = _scatter(_product(_XTW, x2, dy), ps[:7])
+            dps = _scatter(dparam.view(1, -1), ps[7:]) if any(need[8:]) else [None] * 10
+            return (None, None, None) + tuple(g if n else None for g, n in zip([dx, *dws, *dps], need))
+        dx = _input_grad(dy, wide, 2, 32).reshape(B, L, d) if need[0] else None
         if any(need[1:7]):
             dws[:6] = _scatter(_weight_grad(x2, dy[:, :6 * C]), ps[:6])
         if need[7]:
@@ -301,24 +333,33 @@ class _PostMix(torch.autograd.Function):
     """(o (B, H, L, D), output-gate logits, x, norm scale, Wout) -> x + (rms(o) scale silu(og)) Wout."""
 
     @staticmethod
-    def forward(ctx, o, og, x, scale, wo):
+    def forward(ctx, o, og, x, scale, wo, half=False):
         B, H, L, D = o.shape
         z = _rms(o, scale, og, (L, D))
+        ctx.half = half
+        if half:
+            z, wo = _half(z), _half(wo)
+            _save(ctx, o, og, scale, wo, z)
+            return _product(_XW, z, wo, x.reshape(B * L, -1)).reshape(x.shape)
         _save(ctx, o, og, x, scale, wo, z)
         return torch.addmm(x.reshape(B * L, -1), z, wo).reshape(x.shape)
 
     @staticmethod
     def backward(ctx, dy):
-        o, og, x, scale, wo, z = _saved(ctx)
+        saved, need = _saved(ctx), ctx.needs_input_grad
+        o, og, scale, wo, z = saved if ctx.half else (*saved[:2], *saved[3:])
+        _once(ctx.half)
         if torch.is_grad_enabled():
-            return _vjp_through(_postmix_ref, (o, og, x, scale, wo), ctx.needs_input_grad, (dy,))
-        need = ctx.needs_input_grad
+            return _vjp_through(_postmix_ref, (o, og, saved[2], scale, wo), need, (dy,))
         B, H, L, D = o.shape
         d2 = dy.reshape(B * L, -1)
+        db = _half(d2) if ctx.half else None
         do = dog = dscale = None
         if need[0] or need[1] or need[3]:
-            do, dscale, dog = _rms_bwd(o, scale, d2 @ wo.t(), og, (L, D))
-        dwo = _weight_grad(z, d2.contiguous()) if need[4] else None
+            do, dscale, dog = _rms_bwd(o, scale, _product(_XWT, db, wo) if ctx.half else d2 @ wo.t(), og, (L, D))
+        dwo = None
+        if need[4]:
+            dwo = _product(_XTW, z, db) if ctx.half else _weight_grad(z, d2.contiguous())
         return tuple(g if n else None for g, n in zip((do, dog, dy, dscale, dwo), need))
 
 
@@ -326,10 +367,17 @@ class _Mlp(torch.autograd.Function):
     """(x, norm scale, Wgate, Wup, Wdown) -> x + (silu(h Wgate) (h Wup)) Wdown, h = rms(x) scale."""
 
     @staticmethod
-    def forward(ctx, x, scale, wg, wu, wd):
+    def forward(ctx, x, scale, wg, wu, wd, half=False):
         x2 = x.reshape(-1, x.shape[-1])
         h = _rms(x2, scale)
         wide = _gather((wg, wu), 2 * wg.shape[1])
+        ctx.half = half
+        if half:
+            h, wide, wd = _half(h), _half(wide), _half(wd)
+            gu = _product(_XW, h, wide)
+            act = _half(_swiglu(gu))
+            _save(ctx, x, scale, wg, wu, wd, h, wide, gu, act)
+            return _product(_XW, act, wd, x2).reshape(x.shape)
         gu = h @ wide
         act = _swiglu(gu)
         _save(ctx, x, scale, wg, wu, wd, h, wide, gu, act)
@@ -338,15 +386,41 @@ class _Mlp(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         x, scale, wg, wu, wd, h, wide, gu, act = _saved(ctx)
-        if torch.is_grad_enabled():
-            return _vjp_through(_mlp_ref, (x, scale, wg, wu, wd), ctx.needs_input_grad, (dy,))
         need = ctx.needs_input_grad
+        _once(ctx.half)
+        if torch.is_grad_enabled():
+            return _vjp_through(_mlp_ref, (x, scale, wg, wu, wd), need, (dy,))
         d2 = _dense(dy.reshape(-1, dy.shape[-1]))
+        if ctx.half:
+            db = _half(d2)
+            dgu = _half(_swiglu(gu, _product(_XWT, db, wd)))
+            dwd = _product(_XTW, act, db) if need[4] else None
+            dwg, dwu = _scatter(_product(_XTW, h, dgu), (wg, wu)) if need[2] or need[3] else (None, None)
+            dx, dscale, _ = _rms_bwd(x.reshape(d2.shape), scale, _product(_XWT, dgu, wide), res=d2)
+            return tuple(g if n else None for g, n in zip((dx.reshape(x.shape), dscale, dwg, dwu, dwd), need))
         dgu = _swiglu(gu, d2 @ wd.t())
         dwd = act.t() @ d2 if need[4] else None
         dwg, dwu = _scatter(h.t() @ dgu, (wg, wu)) if need[2] or need[3] else (None, None)
         dx, dscale, _ = _rms_bwd(x.reshape(d2.shape), scale, _input_grad(dgu, wide, 4, 8), res=d2)
         return tuple(g if n else None for g, n in zip((dx.reshape(x.shape), dscale, dwg, dwu, dwd), need))
+
+
+class _HalfPreMix(_PreMix):
+    @staticmethod
+    def forward(ctx, *args):
+        return _PreMix.forward(ctx, *args, half=True)
+
+
+class _HalfPostMix(_PostMix):
+    @staticmethod
+    def forward(ctx, *args):
+        return _PostMix.forward(ctx, *args, half=True)
+
+
+class _HalfMlp(_Mlp):
+    @staticmethod
+    def forward(ctx, *args):
+        return _Mlp.forward(ctx, *args, half=True)
 
 
 class _RmsNorm(torch.autograd.Function):
@@ -480,7 +554,8 @@ def rms_norm(module, x):
 
 def block_forward(m, x, ws):
     c = m.cfg
-    *ops, og = _PreMix.apply(c.n_heads, c.d_head, c.g_max, x, *ws[:17])
+    premix, postmix, mlp = (_HalfPreMix, _HalfPostMix, _HalfMlp) if c.products == "bfloat16" else (_PreMix, _PostMix, _Mlp)
+    *ops, og = premix.apply(c.n_heads, c.d_head, c.g_max, x, *ws[:17])
     o, _ = operator_of(m.kernel_fn)(*ops)
-    x = _PostMix.apply(o, og, x, *ws[17:19])
-    return _Mlp.apply(x, *ws[19:])
+    x = postmix.apply(o, og, x, *ws[17:19])
+    return mlp.apply(x, *ws[19:])
