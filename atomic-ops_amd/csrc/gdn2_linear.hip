@@ -176,6 +176,21 @@ static LinSide lin_side(const LinProduct& p, bool b) {
   return s;
 }
 
+// float32 on the matrix cores' own float32 up to this many operations, as pieces beyond (us, own, pieces: 2048 x 768 x 512
+// 22.7, 31.5; 2048 x 1024 x 768 46, 42; 4096 x 1024 x 512 45, 55; 2048 x 2048 x 1024 82, 78; 4096 x 2048 x 1024 159, 126)
+constexpr double LIN_DIRECT_MOST = 6e9;
+// Few rows: whether every row of x and W takes 16-byte accesses
+static bool lin_whole(const LinProduct& p) {
+  const size_t e = p.dtype == LIN_F32 ? 4 : 8;
+  return (reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b)) % 16 == 0 && p.lda % e == 0 && p.ldb % e == 0 &&
+         p.K % 8 == 0 && (p.form == LIN_XWT || p.N % e == 0);
+}
+// float32: whether lin_direct_kernel can read the operands
+static bool lin_float(const LinProduct& p) {
+  const int ca = p.form == LIN_XTW ? p.M : p.K, cb = p.form == LIN_XWT ? p.K : p.N;
+  return p.dtype == LIN_F32 && (reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b)) % 16 == 0 && p.lda % 4 == 0 &&
+         p.ldb % 4 == 0 && ca % 4 == 0 && cb % 4 == 0;
+}
 static LinPlan lin_plan(const LinProduct& p) {
   LinPlan r{0, LIN_MID, 1, 0};
   const int64_t cus = cu_count();
@@ -185,17 +200,25 @@ static LinPlan lin_plan(const LinProduct& p) {
     r.per = (int)((units + (parts < 1 ? 1 : parts) - 1) / (parts < 1 ? 1 : parts));
     r.parts = (int)((units + r.per - 1) / r.per);
   };
-  if (p.form != LIN_XTW && p.M <= (p.dtype == LIN_F32 ? 32 : 8)) {
+  if (p.form != LIN_XTW && p.M <= 8 && p.K <= (1 << 25)) {     // (parts are a grid's y)
     r.rows = p.M == 1 ? 1 : p.M == 2 ? 2 : p.M <= 4 ? 4 : 8;
-    const int64_t e = p.dtype == LIN_F32 ? 4 : 8, wide = p.form == LIN_XW ? LIN_ROWS_COLS * e : 16;
+    const int64_t e = p.dtype == LIN_F32 ? 4 : 8, wide = p.form == LIN_XWT ? 16 : lin_whole(p) ? LIN_ROWS_COLS * e : 64;
     const int64_t wgs = (p.N + wide - 1) / wide * ((p.M + r.rows - 1) / r.rows), eights = (p.K + 7) / 8;
-    split(eights, (p.form == LIN_XW ? cus : 4 * cus) / wgs, p.K / 1024);
+    if (p.form == LIN_XW && !lin_whole(p)) {       // (by columns: 128 values a part and more, 1024 at most)
+      const int64_t least = (p.K + LIN_COLUMNS_K - 1) / LIN_COLUMNS_K, most = (p.K + 127) / 128, parts = 2 * cus / wgs;
+      split(eights, parts < least ? least : parts, most);
+    } else {
+      split(eights, (p.form == LIN_XW ? cus : 4 * cus) / wgs, p.K / 1024);
+    }
     r.per *= 8;
     return r;
   }
   const int64_t blocks = (p.K + lin_bk(p.dtype) - 1) / lin_bk(p.dtype);
   const int64_t big = p.dtype == LIN_F32 ? tiles(256, 128) : tiles(256, 256), mid = tiles(128, 128), small = tiles(64, 64);
-  if (big * 4 >= cus * 3) {
+  if (lin_float(p) && 2.0 * p.M * p.N * p.K <= LIN_DIRECT_MOST) {
+    r.tile = LIN_DIRECT;
+    split(blocks, small * 4 >= cus * 3 ? 1 : 2 * cus / small, blocks / 4);
+  } else if (big * 4 >= cus * 3) {
     r.tile = LIN_BIG;
     split(blocks, 1, 1);
   } else if (mid >= cus || blocks * mid >= 16 * cus) {
@@ -210,7 +233,7 @@ static size_t lin_parts_bytes(const LinProduct& p, const LinPlan& r) { return r.
 
 size_t linear_workspace_bytes(const LinProduct& p) {
   const LinPlan r = lin_plan(p);
-  return (r.rows ? 0 : lin_side(p, false).bytes + lin_side(p, true).bytes) + lin_parts_bytes(p, r);
+  return (r.rows || r.tile == LIN_DIRECT ? 0 : lin_side(p, false).bytes + lin_side(p, true).bytes) + lin_parts_bytes(p, r);
 }
 
 hipError_t launch_linear(const LinProduct& p, void* workspace, hipStream_t s) {
@@ -229,8 +252,7 @@ hipError_t launch_linear(const LinProduct& p, void* workspace, hipStream_t s) {
   if (r.rows) {
     a.part = reinterpret_cast<float*>(ws);
     const bool dots = p.form == LIN_XWT;
-    const size_t e = p.dtype == LIN_F32 ? 4 : 8;
-    const bool whole = (low(p.a) | low(p.b)) % 16 == 0 && p.lda % e == 0 && p.ldb % e == 0 && p.K % 8 == 0 && (dots || p.N % e == 0);
+    const bool whole = lin_whole(p);
     if (p.dtype == LIN_F32) lin_rows<LIN_F32>(a, r, p.act, dots, whole, s);
     else if (p.dtype == LIN_BF16) lin_rows<LIN_BF16>(a, r, p.act, dots, whole, s);
     else lin_rows<LIN_F16>(a, r, p.act, dots, whole, s);
@@ -241,7 +263,7 @@ hipError_t launch_linear(const LinProduct& p, void* workspace, hipStream_t s) {
   for (int b = 0; b < 2; ++b) {
     const LinSide d = lin_side(p, b);
     LinOperand& o = b ? a.b : a.a;
-    if (!d.pack) continue;
+    if (!d.pack || r.tile == LIN_DIRECT) continue;
     LinPack& j = js.job[jobs];
     j.src = o.p;
     j.lds = o.ld;

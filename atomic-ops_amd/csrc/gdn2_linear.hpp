@@ -260,8 +260,10 @@ template <int DT, int ACT, int E>
 __device__ __forceinline__ void lin_out(const LinArgs& a, int m, int n, const float* f) {
   const size_t at = (size_t)m * a.N + n;
   if (a.vec) {               // (whole groups of eight columns, and every pointer takes 16 bytes)
+    static_assert(E % 4 == 0 || E == 1, "columns");
+    if constexpr (E == 1) return;          // (whole rows come by fours)
 #pragma unroll
-    for (int q = 0; q < E; q += 4) {
+    for (int q = 0; q + 3 < E; q += 4) {
       float4 v = make_float4(f[q], f[q + 1], f[q + 2], f[q + 3]);
       if (a.bias) {
         const float4 b = lin_get4(a.bias_dtype, a.bias, n + q);
@@ -481,28 +483,165 @@ __global__ __launch_bounds__(C::W * WAVE) void lin_tile_kernel(LinArgs a) {
   }
 }
 
-// The parts of a sum, in order, and the epilogue; four columns a thread
-template <int DT, int ACT>
+// The parts of a sum, in order, and the epilogue; four columns a thread, or (E 1) one where rows are not whole
+template <int DT, int ACT, int E>
 __global__ __launch_bounds__(256) void lin_join_kernel(LinArgs a) {
-  const int cols = (a.N + 3) / 4;
+  const int cols = (a.N + E - 1) / E;
   const size_t x = (size_t)blockIdx.x * 256 + threadIdx.x, step = (size_t)a.M * a.N;
-  const int m = (int)(x / cols), n = 4 * (int)(x - (size_t)m * cols);
+  const int m = (int)(x / cols), n = E * (int)(x - (size_t)m * cols);
   if (m >= a.M) return;
   const float* p = a.part + (size_t)m * a.N + n;
-  float f[4] = {0.f, 0.f, 0.f, 0.f};
-  if (a.N % 4 == 0) {
+  float f[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) f[e] = 0.f;
 #pragma unroll 8
-    for (int i = 0; i < a.parts; ++i) {
+  for (int i = 0; i < a.parts; ++i) {
+    if constexpr (E == 4) {
       const float4 v = *reinterpret_cast<const float4*>(p + i * step);
       f[0] += v.x; f[1] += v.y; f[2] += v.z; f[3] += v.w;
+    } else {
+      f[0] += p[i * step];
     }
-  } else {
-    for (int i = 0; i < a.parts; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (n + e < a.N) f[e] += p[i * step + e];
   }
-  lin_out<DT, ACT, 4>(a, m, n, f);
+  lin_out<DT, ACT, E>(a, m, n, f);
+}
+
+// ---- float32 as it is ---------------------------------------------------------------------------------------------
+
+// Small float32 products on the matrix cores' own float32 (a sixteenth of bfloat16's rate, a third of that of six products
+// of pieces): no pass over the operands before it.  Tiles of 64 x 64, a wave 32 x 32 and, so that two waves a SIMD cover
+// each other's waits where there is one workgroup a CU, half of each block of 32 along the sum; four blocks in LDS.  A lane
+// takes four values along the sum at a time, 4 c .. 4 c + 3 of sixteen (c = lane / 16), one for each of four
+// 4-deep products, of both operands: rows along the sum by 16 bytes, rows across it by four single values, their chunks
+// exchanged by 64 bytes for each c.
+template <int ACT_, bool AR_, bool BR_>
+struct LinDirect {
+  static constexpr int ACT = ACT_, BM = 64, BN = 64, BK = 32, NBUF = 4, AB = BM * BK * 4, BUF = 2 * AB, LDS = NBUF * BUF, LDO = 36;
+  static constexpr bool AR = AR_, BR = BR_;
+};
+template <bool R>
+struct LinDirectSource {
+  const char* src;
+  int k;
+  size_t step;
+  __device__ __forceinline__ void init(const LinOperand& o, int row0, int kb0) {
+    const float* p = reinterpret_cast<const float*>(o.p);
+    step = (R ? 32 * o.ld : (size_t)32) * 4;
+    const int q = wave_id() * 64 + lane_id();
+    size_t at;
+    if constexpr (R) {
+      k = q >> 4;
+      const int chunk = (q & 15) ^ ((k >> 2 & 3) << 2);
+      at = (size_t)k * o.ld + min(row0 + 4 * chunk, o.rows - 4);
+    } else {
+      const int row = q >> 3;
+      k = 4 * ((q & 7) ^ (row & 7));
+      at = (size_t)min(row0 + row, o.rows - 1) * o.ld + k;
+    }
+    src = reinterpret_cast<const char*>(p + at) + (size_t)kb0 * step;
+    k += kb0 * 32;
+  }
+  __device__ __forceinline__ void fetch(char* dst, int K, bool tail) {
+    const char* s = src;
+    if (tail) s = k < K ? s : reinterpret_cast<const char*>(&lin_zeros);
+    lds_dma16(reinterpret_cast<const float*>(s), reinterpret_cast<float*>(dst + wave_id() * 1024));
+    src += step;
+    k += 32;
+  }
+};
+// A lane's values of tile t and of sixteen along the sum, s of two
+template <bool R>
+__device__ __forceinline__ float4 lin_direct_read(const char* lds, int t, int s) {
+  const int l = lane_id(), r = l & 15, c = l >> 4;
+  if constexpr (R) {
+    const float* p = reinterpret_cast<const float*>(lds) + (16 * s + 4 * c) * 64 + 16 * (t ^ c) + r;
+    return make_float4(p[0], p[64], p[128], p[192]);
+  } else {
+    const int row = 16 * t + r;
+    return *reinterpret_cast<const float4*>(lds + row * 128 + (((4 * s + c) ^ (row & 7)) << 4));
+  }
+}
+template <class C>
+__global__ __launch_bounds__(512) void lin_direct_kernel(LinArgs a) {
+  extern __shared__ char lds[];
+  const int l = lane_id(), r = l & 15, c = l >> 4, w = wave_id(), half = w >> 2, wm = w >> 1 & 1, wn = w & 1;
+  int part, mi, ni;
+  lin_place(a, 8, part, mi, ni);
+  const int m0 = mi * C::BM, n0 = ni * C::BN;
+  const int blocks = (a.K + C::BK - 1) / C::BK, kb0 = part * a.per, kb1 = min(blocks, kb0 + a.per);
+  LinDirectSource<C::AR> sa;
+  LinDirectSource<C::BR> sb;
+  sa.init(a.a, m0, kb0);
+  sb.init(a.b, n0, kb0);
+  auto fetch = [&](int kb, int buf) __attribute__((always_inline)) {
+    const bool tail = (kb + 1) * C::BK > a.K;
+    sa.fetch(lds + buf, a.K, tail);
+    sb.fetch(lds + buf + C::AB, a.K, tail);
+  };
+  f4 acc[2][2];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) acc[q >> 1][q & 1] = f4{0.f, 0.f, 0.f, 0.f};
+  constexpr int AHEAD = C::NBUF - 1, BEHIND = (C::NBUF - 2) * 2;
+  auto next = [&](int x) { return x == (C::NBUF - 1) * C::BUF ? 0 : x + C::BUF; };
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i)
+    if (kb0 + i < kb1) fetch(kb0 + i, i * C::BUF);
+  int buf = 0, into = AHEAD * C::BUF;
+  for (int kb = kb0; kb < kb1; ++kb) {
+    if (kb + C::NBUF - 2 < kb1) __builtin_amdgcn_s_waitcnt(WAIT_VMCNT0 | BEHIND);
+    else __builtin_amdgcn_s_waitcnt(WAIT_VMCNT0);
+    __syncthreads();
+    if (kb + AHEAD < kb1) fetch(kb + AHEAD, into);
+    const char* at = lds + buf;
+    float4 m[2], n[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      m[i] = lin_direct_read<C::AR>(at, wm * 2 + i, half);
+      n[i] = lin_direct_read<C::BR>(at + C::AB, wn * 2 + i, half);
+    }
+    // (the four tiles in turn: a product that waits for the one before it costs an eighth more)
+    auto four = [&](float n0, float n1, float m0, float m1) __attribute__((always_inline)) {
+      asm volatile(
+          "s_nop 1\n\tv_mfma_f32_16x16x4_f32 %0, %4, %6, %0\n\tv_mfma_f32_16x16x4_f32 %1, %4, %7, %1\n\t"
+          "v_mfma_f32_16x16x4_f32 %2, %5, %6, %2\n\tv_mfma_f32_16x16x4_f32 %3, %5, %7, %3"
+          : "+v"(acc[0][0]), "+v"(acc[0][1]), "+v"(acc[1][0]), "+v"(acc[1][1])
+          : "v"(n0), "v"(n1), "v"(m0), "v"(m1));
+    };
+    four(n[0].x, n[1].x, m[0].x, m[1].x);
+    four(n[0].y, n[1].y, m[0].y, m[1].y);
+    four(n[0].z, n[1].z, m[0].z, m[1].z);
+    four(n[0].w, n[1].w, m[0].w, m[1].w);
+    buf = next(buf);
+    into = next(into);
+  }
+  drain(acc[0][0]);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) lin_hold(acc[q >> 1][q & 1]);
+  __syncthreads();
+  // both halves' sums through LDS, each wave then a half of the tile's rows
+  float* own = reinterpret_cast<float*>(lds) + w * (32 * C::LDO);
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) *reinterpret_cast<f4*>(own + (16 * t + r) * C::LDO + 16 * i + 4 * c) = acc[i][t];
+  __syncthreads();
+  const float* low = reinterpret_cast<const float*>(lds) + (w & 3) * (32 * C::LDO);
+  const int col = 8 * (l & 3), n = n0 + 32 * wn + col;
+  if (n >= a.N) return;
+  LinColumns cols;
+  cols.load(a, n);
+  const int row = 16 * half + (l >> 2), m = m0 + 32 * wm + row;
+  if (m >= a.M) return;
+  LinResidual res;
+  if (a.parts == 1) res.load(a, m, n);
+  float f[8];
+#pragma unroll
+  for (int e = 0; e < 8; e += 4) {
+    const float* q = low + row * C::LDO + col + e;
+    *reinterpret_cast<f4*>(f + e) = *reinterpret_cast<const f4*>(q) + *reinterpret_cast<const f4*>(q + 4 * 32 * C::LDO);
+  }
+  if (a.parts > 1) lin_out_part<8>(a, part, m, n, f);
+  else lin_out8<LIN_F32, C::ACT>(a, m, n, f, cols, res);
 }
 
 // ---- few rows -----------------------------------------------------------------------------------------------------
@@ -512,7 +651,7 @@ __global__ __launch_bounds__(256) void lin_join_kernel(LinArgs a) {
 constexpr int LIN_ROWS_W = 8, LIN_ROWS_COLS = 8;       // waves; lanes along the columns of W
 // W (K, N): eight lanes take 16 bytes each of a row of W, the workgroup's 64 groups of lanes eight rows each; their sums meet
 // over the wave's lanes and then in LDS.
-template <int DT, int ACT, int MR, bool VEC>
+template <int DT, int ACT, int MR>
 __global__ __launch_bounds__(LIN_ROWS_W * WAVE) void lin_rows_kernel(LinArgs a) {
   using V = LinVec<DT>;
   constexpr int E = V::E, COLS = LIN_ROWS_COLS * E;
@@ -528,15 +667,15 @@ __global__ __launch_bounds__(LIN_ROWS_W * WAVE) void lin_rows_kernel(LinArgs a) 
     for (int k = k0 + 8 * (w * 8 + (l >> 3)); k < k1; k += 64 * LIN_ROWS_W) {
       float wt[8][E], x[MR][8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) V::template load<E, VEC>(a.b.p, (size_t)(VEC ? k + j : min(k + j, k1 - 1)) * a.b.ld + n, a.N - n, wt[j]);
+      for (int j = 0; j < 8; ++j) V::template load<E, true>(a.b.p, (size_t)(k + j) * a.b.ld + n, E, wt[j]);
 #pragma unroll
-      for (int m = 0; m < MR; ++m) V::template load<8, VEC>(a.a.p, (size_t)min(m0 + m, a.M - 1) * a.a.ld + k, k1 - k, x[m]);
+      for (int m = 0; m < MR; ++m) V::template load<8, true>(a.a.p, (size_t)min(m0 + m, a.M - 1) * a.a.ld + k, 8, x[m]);
 #pragma unroll
       for (int j = 0; j < 8; ++j)
 #pragma unroll
         for (int m = 0; m < MR; ++m)
 #pragma unroll
-          for (int e = 0; e < E; ++e) acc[m][e] = VEC || k + j < k1 ? fmaf(x[m][j], wt[j][e], acc[m][e]) : acc[m][e];
+          for (int e = 0; e < E; ++e) acc[m][e] = fmaf(x[m][j], wt[j][e], acc[m][e]);
     }
 #pragma unroll
   for (int m = 0; m < MR; ++m)
@@ -557,6 +696,55 @@ __global__ __launch_bounds__(LIN_ROWS_W * WAVE) void lin_rows_kernel(LinArgs a) 
       for (int e = 0; e < 4; ++e) f[e] += sums[v][m][col + e];
     if (a.parts > 1) lin_out_part<4>(a, blockIdx.y, m0 + m, at, f);
     else lin_out<DT, ACT, 4>(a, m0 + m, at, f);
+  }
+}
+
+// The same for a W (or x) whose rows are not whole 16 bytes: a lane takes one column, so that a wave's loads are whole lines
+// all the same, the four waves a quarter of the part each (at most 1024 values), x from LDS.
+constexpr int LIN_COLUMNS_K = 1024;
+template <int DT, int ACT, int MR>
+__global__ __launch_bounds__(256) void lin_columns_kernel(LinArgs a) {
+  __shared__ float x[MR][LIN_COLUMNS_K], sums[4][MR][64];
+  const int l = lane_id(), w = wave_id(), n = blockIdx.x * 64 + l, m0 = blockIdx.z * MR;
+  const int k0 = blockIdx.y * a.per, k1 = min(a.K, k0 + a.per), ks = k1 - k0;
+#pragma unroll
+  for (int m = 0; m < MR; ++m) {
+    const size_t row = (size_t)min(m0 + m, a.M - 1) * a.a.ld + k0;
+#pragma unroll 4
+    for (int k = threadIdx.x; k < ks; k += 256) x[m][k] = LinType<DT>::get(a.a.p, row + k);
+  }
+  __syncthreads();
+  const int quarter = (ks + 3) / 4, b = w * quarter, e = min(ks, b + quarter);
+  float acc[MR];
+#pragma unroll
+  for (int m = 0; m < MR; ++m) acc[m] = 0.f;
+  const size_t at = (size_t)k0 * a.b.ld + min(n, a.N - 1);
+  int k = b;
+  for (; k + 8 <= e; k += 8) {
+    float wt[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) wt[j] = LinType<DT>::get(a.b.p, at + (size_t)(k + j) * a.b.ld);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int m = 0; m < MR; ++m) acc[m] = fmaf(x[m][k + j], wt[j], acc[m]);
+  }
+  for (; k < e; ++k) {
+    const float wt = LinType<DT>::get(a.b.p, at + (size_t)k * a.b.ld);
+#pragma unroll
+    for (int m = 0; m < MR; ++m) acc[m] = fmaf(x[m][k], wt, acc[m]);
+  }
+#pragma unroll
+  for (int m = 0; m < MR; ++m) sums[w][m][l] = acc[m];
+  __syncthreads();
+  for (int i = threadIdx.x; i < MR * 16; i += 256) {
+    const int m = i / 16, col = 4 * (i % 16), to = blockIdx.x * 64 + col;
+    if (m0 + m >= a.M || to >= a.N) continue;
+    float f[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) f[q] = (sums[0][m][col + q] + sums[1][m][col + q]) + (sums[2][m][col + q] + sums[3][m][col + q]);
+    if (a.parts > 1) lin_out_part<4>(a, blockIdx.y, m0 + m, to, f);
+    else lin_out<DT, ACT, 4>(a, m0 + m, to, f);
   }
 }
 
@@ -604,17 +792,19 @@ __global__ __launch_bounds__(256) void lin_dots_kernel(LinArgs a) {
 // How a product runs.
 struct LinPlan {
   int rows;                  // rows at a time by lin_rows_kernel or lin_dots_kernel; 0: tiles
-  int tile;                  // LIN_SMALL, LIN_MID, LIN_BIG
+  int tile;                  // LIN_SMALL, LIN_MID, LIN_BIG; LIN_DIRECT: lin_direct_kernel
   int parts, per;            // parts of the sum, of `per` blocks (rows: values)
 };
-enum { LIN_SMALL, LIN_MID, LIN_BIG };
+enum { LIN_SMALL, LIN_MID, LIN_BIG, LIN_DIRECT };
 constexpr int lin_bk(int dtype) { return dtype == LIN_F32 ? 32 : 64; }
 
 template <int DT, int ACT>
 static void lin_join(const LinArgs& a, hipStream_t s) {
   if (a.parts == 1) return;
-  const size_t threads = (size_t)a.M * ((a.N + 3) / 4);
-  hipLaunchKernelGGL((lin_join_kernel<DT, ACT>), dim3((threads + 255) / 256), dim3(256), 0, s, a);
+  const size_t threads = (size_t)a.M * (a.vec ? a.N / 4 : a.N);
+  const dim3 grid((threads + 255) / 256);
+  if (a.vec) hipLaunchKernelGGL((lin_join_kernel<DT, ACT, 4>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((lin_join_kernel<DT, ACT, 1>), grid, dim3(256), 0, s, a);
 }
 template <class C>
 static void lin_go(LinArgs a, const LinPlan& r, hipStream_t s) {
@@ -638,9 +828,11 @@ template <int DT, int ACT, int MR, bool VEC>
 static void lin_rows_go(const LinArgs& a, bool dots, hipStream_t s) {
   const int z = (a.M + MR - 1) / MR;
   if (dots) hipLaunchKernelGGL((lin_dots_kernel<DT, ACT, MR, VEC>), dim3((a.N + 15) / 16, a.parts, z), dim3(256), 0, s, a);
-  else {
+  else if constexpr (VEC) {
     constexpr int cols = LIN_ROWS_COLS * LinVec<DT>::E;
-    hipLaunchKernelGGL((lin_rows_kernel<DT, ACT, MR, VEC>), dim3((a.N + cols - 1) / cols, a.parts, z), dim3(LIN_ROWS_W * WAVE), 0, s, a);
+    hipLaunchKernelGGL((lin_rows_kernel<DT, ACT, MR>), dim3((a.N + cols - 1) / cols, a.parts, z), dim3(LIN_ROWS_W * WAVE), 0, s, a);
+  } else {
+    hipLaunchKernelGGL((lin_columns_kernel<DT, ACT, MR>), dim3((a.N + 63) / 64, a.parts, z), dim3(256), 0, s, a);
   }
   lin_join<DT, ACT>(a, s);
 }
@@ -669,10 +861,32 @@ static void lin_acts(const LinArgs& a, const LinPlan& r, int act, hipStream_t s)
   else if (act == LIN_TANH) lin_tiles<DT, LIN_TANH, NP, AR, BR>(a, r, s);
   else lin_tiles<DT, LIN_NONE, NP, AR, BR>(a, r, s);
 }
+template <int ACT, bool AR, bool BR>
+static void lin_direct_go(LinArgs a, const LinPlan& r, hipStream_t s) {
+  using C = LinDirect<ACT, AR, BR>;
+  a.mt = (a.M + C::BM - 1) / C::BM;
+  a.nt = (a.N + C::BN - 1) / C::BN;
+  hipLaunchKernelGGL(lin_direct_kernel<C>, dim3(a.mt * a.nt * a.parts), dim3(512), C::LDS, s, a);
+  lin_join<LIN_F32, ACT>(a, s);
+}
+template <bool AR, bool BR>
+static void lin_direct_act(const LinArgs& a, const LinPlan& r, int act, hipStream_t s) {
+  if (act == LIN_SILU) lin_direct_go<LIN_SILU, AR, BR>(a, r, s);
+  else if (act == LIN_GELU) lin_direct_go<LIN_GELU, AR, BR>(a, r, s);
+  else if (act == LIN_TANH) lin_direct_go<LIN_TANH, AR, BR>(a, r, s);
+  else lin_direct_go<LIN_NONE, AR, BR>(a, r, s);
+}
+static inline void lin_direct(const LinArgs& a, const LinPlan& r, int form, int act, hipStream_t s) {
+  if (form == LIN_XW) lin_direct_act<false, true>(a, r, act, s);
+  else if (form == LIN_XWT) lin_direct_act<false, false>(a, r, act, s);
+  else lin_direct_go<LIN_NONE, true, true>(a, r, s);
+}
+
 template <int DT>
 void lin_forms(const LinArgs& a, const LinPlan& r, int form, int act, hipStream_t s) {
   if constexpr (DT == LIN_F32) {
-    lin_acts<DT, 3, false, false>(a, r, act, s);
+    if (r.tile == LIN_DIRECT) lin_direct(a, r, form, act, s);
+    else lin_acts<DT, 3, false, false>(a, r, act, s);
   } else {
     if (form == LIN_XW) lin_acts<DT, 1, false, true>(a, r, act, s);
     else if (form == LIN_XWT) lin_acts<DT, 1, false, false>(a, r, act, s);

@@ -99,7 +99,7 @@ def test_epilogues(dtype, act, bias, residual):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("M,K,N", [(1, 4096, 1024), (4, 2048, 4096), (9, 4100, 520), (16, 1024, 2048), (40, 8192, 256), (2048, 768, 512),
-                                   (4096, 256, 128), (1000, 2000, 1500), (64, 64, 8192)])
+                                   (4096, 256, 128), (1000, 2000, 1500), (64, 64, 8192), (8, 9000, 515), (30, 2052, 4100), (33, 1100, 260)])
 def test_large(dtype, M, K, N):
     check(M, K, N, DTYPES[dtype], act="gelu", bias=True, residual=True, seed=3)
 
