@@ -35,45 +35,54 @@ __global__ __launch_bounds__(256) void lin_pack_kernel(LinPacks js) {
   const LinPack& j = js.job[which];
   const int b = blockIdx.x - js.start[which], r0 = b / j.tc * 64, c0 = b % j.tc * 64;
   __shared__ __attribute__((aligned(16))) uint16_t tile[NP][64][LDT];       // rows of out
-  // four rows of src a wave at a time, four neighbouring values a lane
-  const int y = threadIdx.x >> 4, x = 4 * (threadIdx.x & 15);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = r0 + 16 * i + y, col = c0 + x, last = j.cols - 1;
-    const size_t at = (size_t)min(row, j.rows - 1) * j.lds;
-    uint32_t v[4];
-    if (j.vec && col + 3 < j.cols) {
-      if constexpr (F32) {
-        const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint32_t*>(j.src) + at + col);
-        v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
-      } else {
-        const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(j.src) + at + col);
-        v[0] = u.x & 0xffffu; v[1] = u.x >> 16; v[2] = u.y & 0xffffu; v[3] = u.y >> 16;
-      }
+  auto split = [&](uint32_t u, int ry, int cx) __attribute__((always_inline)) {
+    uint16_t piece[NP];
+    if constexpr (F32) {
+      const float f = __uint_as_float(u), f1 = f - lin_top(f), f2 = f1 - lin_top(f1);
+      piece[0] = (uint16_t)(u >> 16);
+      piece[1] = (uint16_t)(__float_as_uint(f1) >> 16);
+      piece[2] = (uint16_t)(__float_as_uint(f2) >> 16);
     } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if constexpr (F32) v[e] = static_cast<const uint32_t*>(j.src)[at + min(col + e, last)];
-        else v[e] = static_cast<const uint16_t*>(j.src)[at + min(col + e, last)];
-      }
+      piece[0] = (uint16_t)u;
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint32_t u = row < j.rows && col + e < j.cols ? v[e] : 0u;
-      uint16_t piece[NP];
+    for (int p = 0; p < NP; ++p) {
+      if (j.turn) tile[p][cx][ry] = piece[p];
+      else tile[p][ry][cx] = piece[p];
+    }
+  };
+  if (j.vec && c0 + 64 <= j.cols) {
+    // four rows of src a wave at a time, four neighbouring values a lane
+    const int y = threadIdx.x >> 4, x = 4 * (threadIdx.x & 15);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = r0 + 16 * i + y;
+      const size_t at = (size_t)min(row, j.rows - 1) * j.lds + c0 + x;
+      uint32_t v[4];
       if constexpr (F32) {
-        const float f = __uint_as_float(u), f1 = f - lin_top(f), f2 = f1 - lin_top(f1);
-        piece[0] = (uint16_t)(u >> 16);
-        piece[1] = (uint16_t)(__float_as_uint(f1) >> 16);
-        piece[2] = (uint16_t)(__float_as_uint(f2) >> 16);
+        const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint32_t*>(j.src) + at);
+        v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
       } else {
-        piece[0] = (uint16_t)u;
+        const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(j.src) + at);
+        v[0] = u.x & 0xffffu; v[1] = u.x >> 16; v[2] = u.y & 0xffffu; v[3] = u.y >> 16;
       }
 #pragma unroll
-      for (int p = 0; p < NP; ++p) {
-        if (j.turn) tile[p][x + e][16 * i + y] = piece[p];
-        else tile[p][16 * i + y][x + e] = piece[p];
+      for (int e = 0; e < 4; ++e) split(row < j.rows ? v[e] : 0u, 16 * i + y, x + e);
+    }
+  } else {
+    // a row of src a wave at a time, a value a lane
+    const int y = threadIdx.x >> 6, x = threadIdx.x & 63, col = c0 + x;
+#pragma unroll
+    for (int g = 0; g < 16; g += 8) {
+      uint32_t v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const size_t at = (size_t)min(r0 + 4 * (g + i) + y, j.rows - 1) * j.lds + min(col, j.cols - 1);
+        if constexpr (F32) v[i] = static_cast<const uint32_t*>(j.src)[at];
+        else v[i] = static_cast<const uint16_t*>(j.src)[at];
       }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) split(r0 + 4 * (g + i) + y < j.rows && col < j.cols ? v[i] : 0u, 4 * (g + i) + y, x);
     }
   }
   __syncthreads();
@@ -215,10 +224,16 @@ static LinPlan lin_plan(const LinProduct& p) {
   }
   const int64_t blocks = (p.K + lin_bk(p.dtype) - 1) / lin_bk(p.dtype);
   const int64_t big = p.dtype == LIN_F32 ? tiles(256, 128) : tiles(256, 256), mid = tiles(128, 128), small = tiles(64, 64);
+  // The large tiles are faster where they fill the chip (16 bits 1090 TFLOP/s against 850 to 1000, one workgroup a CU against
+  // two; float32 233 against 190, one each), but the last round of them may be nearly empty: rounds, in units of a tile of
+  // 128 x 128 a CU (7199 x 8996 x 3131 bfloat16: two rounds of 256 x 256 666 us, three of 128 x 128 588).
+  auto rounds = [&](int64_t tiles, int64_t at_once) { return (tiles + at_once - 1) / at_once; };
+  const double big_rounds = p.dtype == LIN_F32 ? rounds(big, cus) * 2 * 0.82 : rounds(big, cus) * 4 * 0.86;
+  const double mid_rounds = p.dtype == LIN_F32 ? rounds(mid, cus) : rounds(mid, 2 * cus) * 2;
   if (lin_float(p) && 2.0 * p.M * p.N * p.K <= LIN_DIRECT_MOST) {
     r.tile = LIN_DIRECT;
     split(blocks, small * 4 >= cus * 3 ? 1 : 2 * cus / small, blocks / 4);
-  } else if (big * 4 >= cus * 3) {
+  } else if (big * 4 >= cus * 3 && big_rounds <= mid_rounds) {
     r.tile = LIN_BIG;
     split(blocks, 1, 1);
   } else if (mid >= cus || blocks * mid >= 16 * cus) {

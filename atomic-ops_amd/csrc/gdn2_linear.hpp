@@ -349,6 +349,39 @@ __device__ __forceinline__ void lin_out_part(const LinArgs& a, int part, int m, 
     if (n + e < a.N) p[e] = f[e];
 }
 
+// A wave's results in LDS (rows of ldo floats; more: a second part of their sum, or NULL) where rows are not whole groups of
+// eight columns: a lane takes one column of COLS, so that what a wave writes at a time is whole lines all the same.
+template <int DT, int ACT, int COLS>
+__device__ __forceinline__ void lin_out_odd(const LinArgs& a, int part, const float* own, const float* more, int ldo, int rows, int m0, int n0) {
+  const int l = lane_id(), col = l % COLS, n = n0 + col;
+  constexpr int STEP = WAVE / COLS, U = 8;
+  if (n >= a.N) return;
+  const float bias = a.bias ? lin_get(a.bias_dtype, a.bias, n) : 0.f;
+  for (int r = l / COLS; r < rows && m0 + r < a.M; r += STEP * U) {
+    float res[U];
+    if (a.residual && a.parts == 1)
+#pragma unroll
+      for (int u = 0; u < U; ++u) res[u] = lin_get(a.out_dtype, a.residual, (size_t)min(m0 + r + u * STEP, a.M - 1) * a.ldr + n);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int row = r + u * STEP, m = m0 + row;
+      if (row >= rows || m >= a.M) break;
+      float f = own[row * ldo + col];
+      if (more) f += more[row * ldo + col];
+      if (a.parts > 1) {
+        a.part[((size_t)part * a.M + m) * a.N + n] = f;
+        continue;
+      }
+      f += bias;
+      const size_t at = (size_t)m * a.N + n;
+      if (a.z) LinType<DT>::put(a.z, at, f);
+      f = lin_act<ACT>(f);
+      if (a.residual) f += res[u];
+      lin_put(a.out_dtype, a.y, at, f);
+    }
+  }
+}
+
 // Workgroups go to the 8 dies in turn: each die gets a run of neighbouring tiles (of one part of the sum), GM rows of tiles
 // high, so that what its workgroups read at a time is shared in its L2.
 __device__ __forceinline__ void lin_place(const LinArgs& a, int gm, int& part, int& mi, int& ni) {
@@ -454,6 +487,11 @@ __global__ __launch_bounds__(C::W * WAVE) void lin_tile_kernel(LinArgs a) {
         *reinterpret_cast<f4*>(own + (16 * (t - h) + r) * C::LDO + 16 * i + 4 * c) = v;
       }
     __builtin_amdgcn_wave_barrier();
+    if (!a.vec) {
+      lin_out_odd<C::DT, C::ACT, 64>(a, part, own, nullptr, C::LDO, 16 * HT, m0 + 16 * (wm * MT + h), n0 + 64 * wn);
+      __builtin_amdgcn_wave_barrier();
+      continue;
+    }
     const int mh = m0 + 16 * (wm * MT + h) + (l >> 3);
 #pragma unroll 1
     for (int j = 0; j < 2 * HT; j += 2) {
@@ -626,6 +664,11 @@ __global__ __launch_bounds__(512) void lin_direct_kernel(LinArgs a) {
     for (int i = 0; i < 2; ++i) *reinterpret_cast<f4*>(own + (16 * t + r) * C::LDO + 16 * i + 4 * c) = acc[i][t];
   __syncthreads();
   const float* low = reinterpret_cast<const float*>(lds) + (w & 3) * (32 * C::LDO);
+  if (!a.vec) {
+    const float* first = low + 16 * half * C::LDO;
+    lin_out_odd<LIN_F32, C::ACT, 32>(a, part, first, first + 4 * 32 * C::LDO, C::LDO, 16, m0 + 32 * wm + 16 * half, n0 + 32 * wn);
+    return;
+  }
   const int col = 8 * (l & 3), n = n0 + 32 * wn + col;
   if (n >= a.N) return;
   LinColumns cols;
