@@ -421,27 +421,40 @@ __global__ __launch_bounds__(C::W * WAVE) void lin_tile_kernel(LinArgs a) {
     for (int i = 0; i < NT; ++i)
 #pragma unroll
       for (int t = 0; t < MT; ++t) acc[q][i][t] = f4{0.f, 0.f, 0.f, 0.f};
+  // Operands are read ahead of their use, those of A by AHEAD tiles, those of B by one step of the sum, a few beside each
+  // group of products (8192 x 4096 x 4096 bfloat16: 225 us, 1224 TFLOP/s; read where they are used 248)
   auto add = [&](const char* at) __attribute__((always_inline)) {
+    constexpr int STEPS = S * MT, AHEAD = NP == 1 ? 2 : 1, RING = AHEAD + 1;
+    s8 n[2][NP][NT], m[RING][NP];
+    auto read_n = [&](int s, int i) __attribute__((always_inline)) {
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-      s8 n[NP][NT];
+      for (int p = 0; p < NP; ++p) n[s & 1][p][i] = lin_read<C, C::BR, C::BN>(at + NP * C::AB + p * C::BB, wn * NT + i, s);
+    };
+    auto read_m = [&](int x) __attribute__((always_inline)) {
 #pragma unroll
-      for (int p = 0; p < NP; ++p)
+      for (int p = 0; p < NP; ++p) m[x % RING][p] = lin_read<C, C::AR, C::BM>(at + p * C::AB, wm * MT + x % MT, x / MT);
+    };
 #pragma unroll
-        for (int i = 0; i < NT; ++i) n[p][i] = lin_read<C, C::BR, C::BN>(at + NP * C::AB + p * C::BB, wn * NT + i, s);
+    for (int i = 0; i < NT; ++i) read_n(0, i);
 #pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        s8 m[NP];
+    for (int x = 0; x < (AHEAD < STEPS ? AHEAD : STEPS); ++x) read_m(x);
 #pragma unroll
-        for (int p = 0; p < NP; ++p) m[p] = lin_read<C, C::AR, C::BM>(at + p * C::AB, wm * MT + t, s);
+    for (int x = 0; x < STEPS; ++x) {
+      const int s = x / MT, t = x % MT;
+      if (x + AHEAD < STEPS) read_m(x + AHEAD);
+      if (s + 1 < S)
 #pragma unroll
-        for (int o = NP - 1; o >= 0; --o)
+        for (int i = t * NT / MT; i < (t + 1) * NT / MT; ++i) read_n(s + 1, i);
+      // (float32: the smallest pieces' products first)
 #pragma unroll
-          for (int p = 0; p <= o; ++p) {
-            auto& x = acc[o ? NA - 1 : 0];
-            lin_mfma4<F16>(x[0][t], x[1][t], x[2][t], x[3][t], n[o - p][0], n[o - p][1], n[o - p][2], n[o - p][3], m[p]);
-          }
-      }
+      for (int o = NP - 1; o >= 0; --o)
+#pragma unroll
+        for (int p = 0; p <= o; ++p) {
+          auto& c4 = acc[o ? NA - 1 : 0];
+          const auto& b4 = n[s & 1][o - p];
+          lin_mfma4<F16>(c4[0][t], c4[1][t], c4[2][t], c4[3][t], b4[0], b4[1], b4[2], b4[3], m[x % RING][p]);
+        }
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
   // Block kb has come when only the DMAs of the NBUF - 2 behind it are under way
