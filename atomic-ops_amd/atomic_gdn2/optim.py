@@ -23,7 +23,8 @@ class AdamW(torch.optim.Optimizer):
     """AdamW with decoupled weight decay, clipped by the global norm of all gradients.
 
     params: tensors or groups, float32, bfloat16 or float16 in any mixture, contiguous, on one ROCm device; 16-bit ones
-    are updated as a float32 ``master`` in their state and rounded.  max_norm: every gradient times max_norm /
+    are updated as a float32 ``master`` in their state and rounded (values written into one between steps count, and
+    its master starts anew from them).  max_norm: every gradient times max_norm /
     max(norm, max_norm) (None: as it is); ``norm`` is then the last step's norm, a float32 scalar on the GPU.
     state_bits: 32, or 8: ``exp_avg`` and ``exp_avg_sq`` as codes of one byte, with a scale for each 256 elements
     (include/gdn2.h, gdn2_adamw); ``unpack_states`` gives the values that they stand for.  A NaN or infinity in a
@@ -37,6 +38,9 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"max_norm={max_norm}: positive, or None")
         self.max_norm, self.state_bits, self.norm = None if max_norm is None else float(max_norm), state_bits, None
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+
+    def __getstate__(self):
+        return {**super().__getstate__(), "max_norm": self.max_norm, "state_bits": self.state_bits, "norm": None}
 
     def add_param_group(self, param_group):
         super().add_param_group(param_group)

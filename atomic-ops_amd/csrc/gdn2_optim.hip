@@ -9,6 +9,9 @@
 // Products and sums of the update are rounded one by one (no fma): what an 8-bit state becomes turns on a value's last
 // bit, and an update is the same numbers however a compiler would fuse it.
 //
+// A 16-bit parameter is kept as a float32 master as well; where the parameter is no longer the master's rounding (a checkpoint
+// was loaded into it), the parameter counts.
+//
 // States of 8 bits: blocks of 256 elements share a float32 scale.  m = c |c| s with c in -127 .. 127; v = (c^2 s)^2 with c
 // in 0 .. 255: squares put the codes closer together towards 0, so that elements a hundred times below their block's
 // largest keep codes of their own (m 12.7, sqrt(v) 25.5).  A value between two codes takes the upper one with the
@@ -70,6 +73,18 @@ struct OptType {
   static __device__ __forceinline__ void put(T* p, float v) {
     if constexpr (DT == LIN_BF16) *p = (uint16_t)bf16_bits(v);
     else *p = (T)v;
+  }
+  // The master of a 16-bit parameter: w, unless something else than an update has been written into p since
+  static __device__ __forceinline__ float master(float w, T p) {
+    T r;
+    put(&r, w);
+    return __builtin_bit_cast(uint16_t, r) == __builtin_bit_cast(uint16_t, p) ? w : get(&p);
+  }
+  static __device__ __forceinline__ void master4(const float* w, const T* p, float* x) {
+    const float4 v = *reinterpret_cast<const float4*>(w);
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    const T* e = reinterpret_cast<const T*>(&u);
+    x[0] = master(v.x, e[0]); x[1] = master(v.y, e[1]); x[2] = master(v.z, e[2]); x[3] = master(v.w, e[3]);
   }
   static __device__ __forceinline__ void get4(const T* p, float* x) {
     if constexpr (DT == LIN_F32) {
@@ -171,7 +186,7 @@ __global__ __launch_bounds__(1024) void opt_begin_kernel(OptSteps a, const doubl
   s = sqrt(s);
   if (norm) *norm = (float)s;
   // (a norm that is not a number is not below max_norm)
-  *coef = max_norm > 0.0 ? (float)(max_norm / (s < max_norm ? max_norm : s)) : 1.f;
+  *coef = max_norm > 0.0 && !(s < max_norm) ? (float)(max_norm / s) : 1.f;
 }
 
 struct OptState {
@@ -205,7 +220,7 @@ __global__ __launch_bounds__(256) void opt_update_kernel(OptTensors a, const flo
     float gx[4], px[4], mx[4], vx[4];
     O::get4(g + j, gx);
     if constexpr (DT == LIN_F32) O::get4(p + j, px);
-    else OptType<LIN_F32>::get4(w + j, px);
+    else O::master4(w + j, p + j, px);
     OptType<LIN_F32>::get4(m + j, mx);
     OptType<LIN_F32>::get4(v + j, vx);
 #pragma unroll
@@ -222,7 +237,10 @@ __global__ __launch_bounds__(256) void opt_update_kernel(OptTensors a, const flo
   }
   for (int j = 4 * whole + threadIdx.x; j < n; j += 256) {
     OptState x{m[j], v[j]};
-    const float q = opt_one(h, c, O::get(g + j), DT == LIN_F32 ? O::get(p + j) : w[j], x);
+    float start;
+    if constexpr (DT == LIN_F32) start = p[j];
+    else start = O::master(w[j], p[j]);
+    const float q = opt_one(h, c, O::get(g + j), start, x);
     if constexpr (DT != LIN_F32) w[j] = q;
     O::put(p + j, q);
     m[j] = x.m;
@@ -301,7 +319,7 @@ __global__ __launch_bounds__(256) void opt_update8_kernel(OptTensors a, const fl
     if (vec) {
       O::get4(g, gx);
       if constexpr (DT == LIN_F32) O::get4(p, px);
-      else OptType<LIN_F32>::get4(w, px);
+      else O::master4(w, p, px);
       const uint32_t um = *reinterpret_cast<const uint32_t*>(mc), uv = *reinterpret_cast<const uint32_t*>(vc);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -313,7 +331,8 @@ __global__ __launch_bounds__(256) void opt_update8_kernel(OptTensors a, const fl
       for (int e = 0; e < 4; ++e)
         if (e < n) {
           gx[e] = O::get(g + e);
-          px[e] = DT == LIN_F32 ? O::get(p + e) : w[e];
+          if constexpr (DT == LIN_F32) px[e] = p[e];
+          else px[e] = O::master(w[e], p[e]);
           cm[e] = mc[e];
           cv[e] = vc[e];
         }

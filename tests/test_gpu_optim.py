@@ -305,3 +305,84 @@ def test_captured_step(bits):
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(ps, qs)) and torch.equal(one.norm, two.norm), k
         assert all(torch.equal(one.state[p]["exp_avg"], two.state[q]["exp_avg"]) for p, q in zip(ps, qs))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_values_written_into_a_parameter_count(dtype, bits):
+    """A checkpoint loaded into the model between steps is what the next step updates, its master with it."""
+    p, = _params([1000], DTYPES[dtype], seed=11)
+    opt, plain = _opt([p], state_bits=bits), Plain(p, bits, 0)
+    for k in range(3):
+        p.grad, = _grads([p], k)
+        if k == 1:
+            p.data.copy_(torch.linspace(-2, 2, 1000, device="cuda"))
+            keep = torch.arange(1000, device="cuda") % 3 == 0           # (and some that stay as they were)
+            p.data[keep] = plain.w.to(p.dtype)[keep]
+            plain.w = torch.where(plain.w.to(p.dtype) == p.detach(), plain.w, p.detach().float())
+        opt.step()
+        assert torch.equal(p.detach(), plain.step(p.grad)) and torch.equal(opt.state[p]["master"], plain.w), k
+
+
+def test_norm_without_clipping():
+    """max_norm inf: the norm is formed, nothing is scaled."""
+    p, = _params([5000], torch.float32, seed=12)
+    opt, plain = _opt([p], max_norm=math.inf), Plain(p, 32, 0)
+    p.grad = torch.randn_like(p) * 100
+    opt.step()
+    assert torch.equal(p.detach(), plain.step(p.grad))
+    assert abs(opt.norm.item() - p.grad.double().norm().item()) <= 2.0 ** -23 * opt.norm.item()
+
+
+def test_copied_and_pickled():
+    import copy
+    import pickle
+    p, = _params([300], torch.float32, seed=13)
+    opt = _opt([p], state_bits=8, max_norm=2.0)
+    p.grad = torch.randn_like(p)
+    opt.step()
+    for other in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        q = other.param_groups[0]["params"][0]
+        q.grad = torch.ones_like(q)
+        other.step()
+        assert other.state_bits == 8 and other.max_norm == 2.0 and other.state[q]["step"].item() == 2
+    assert opt.state[p]["step"].item() == 1
+
+
+def test_unpacked_states_of_tensors_without_one_are_zero():
+    ps = _params([300, 50], torch.float32, seed=14)
+    opt = _opt(ps, state_bits=8)
+    m, v = opt.unpack_states()
+    assert not any(t.any() for t in (*m, *v))
+    ps[1].grad = torch.randn_like(ps[1])
+    opt.step()
+    outs = [[torch.full_like(p, 7.0) for p in ps] for _ in range(2)]
+    opt.unpack_states(*outs)
+    assert not outs[0][0].any() and outs[0][1].any() and not outs[1][0].any() and outs[1][1].any()
+    with pytest.raises(ValueError):
+        opt.unpack_states([outs[0][0]], outs[1])
+    with pytest.raises(ValueError):
+        opt.unpack_states(outs[0], [t.half() for t in outs[1]])
+    with pytest.raises(ValueError):
+        _opt(ps).unpack_states()
+
+
+def test_states_that_do_not_fit_are_refused():
+    p, = _params([300], torch.float32, seed=15)
+    for key, bad in (("exp_avg", torch.zeros(299, device="cuda")), ("exp_avg", torch.zeros(300, device="cuda").half()),
+                     ("exp_avg_sq", torch.zeros(300)), ("step", torch.zeros(2, device="cuda")), ("exp_avg", torch.zeros(600, device="cuda")[::2])):
+        opt = _opt([p])
+        p.grad = torch.ones_like(p)
+        opt.step()
+        opt.state[p][key] = bad
+        before = p.detach().clone()
+        with pytest.raises(ValueError, match=key):
+            opt.step()
+        assert torch.equal(p.detach(), before)
+    opt = _opt([p])
+    opt.param_groups[0]["lr"] = torch.tensor(1e-3, device="cuda")
+    with pytest.raises(TypeError, match="lr"):
+        opt.step()
+    opt.param_groups[0]["lr"] = -1.0
+    with pytest.raises(ValueError, match="lr"):
+        opt.step()
