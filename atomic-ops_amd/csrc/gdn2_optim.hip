@@ -20,8 +20,6 @@
 // uses m and v as formed, in 32 bits.
 #include "gdn2_optim.hpp"
 
-#include <vector>
-
 namespace gdn2 {
 
 constexpr int OPT_CHUNK = 8192;            // elements of a workgroup of the update
@@ -433,9 +431,9 @@ static int64_t opt_parts(const gdn2_adamw_tensor* t, int n) {
 static size_t opt_hyper_bytes(int n) { return 256 + ((size_t)n * sizeof(OptHyper) + 255) / 256 * 256; }
 size_t adamw_workspace_bytes(const gdn2_adamw_tensor* t, int n) { return opt_hyper_bytes(n) + 8 * (size_t)opt_parts(t, n); }
 
-// The tensors of a type, as many to a launch as an argument block holds: go(block, workgroups)
-template <class F>
-static void opt_each(const gdn2_adamw_tensor* t, int n, int dtype, int bits, F go) {
+// The tensors of a type, at(i), as many to a launch as an argument block holds: go(block, the first's place, workgroups)
+template <class A, class F>
+static void opt_each(int n, int dtype, int bits, A at, F go) {
   const int size = dtype == LIN_F32 ? 4 : 2, chunk = bits == 8 ? OPT_CHUNK8 : OPT_CHUNK;
   OptTensors a{};
   int64_t blocks = 0;
@@ -446,7 +444,7 @@ static void opt_each(const gdn2_adamw_tensor* t, int n, int dtype, int bits, F g
     blocks = 0;
   };
   for (int i = 0; i < n; ++i) {
-    const gdn2_adamw_tensor& x = t[i];
+    const gdn2_adamw_tensor x = at(i);
     if (x.dtype != dtype) continue;
     const int64_t b = (x.numel + chunk - 1) / chunk;
     if (a.tensors == OPT_TENSORS || blocks + b > 0x7fffffff || (a.tensors && i - first > 0x7fff)) flush();
@@ -502,7 +500,7 @@ hipError_t launch_adamw(const gdn2_adamw_tensor* t, int n, int bits, double max_
     hipLaunchKernelGGL(opt_begin_kernel, dim3(1), dim3(1024), 0, s, a, part, i ? 0 : (int)parts, max_norm, coef, norm, hyper + i);
   }
   for (int dtype = LIN_F32; dtype <= LIN_F16; ++dtype)
-    opt_each(t, n, dtype, bits, [&](const OptTensors& a, int from, int blocks) {
+    opt_each(n, dtype, bits, [&](int i) { return t[i]; }, [&](const OptTensors& a, int from, int blocks) {
       auto go = [&](auto k) { hipLaunchKernelGGL(k, dim3(blocks), dim3(256), 0, s, a, clip ? coef : nullptr, hyper + from); };
       if (bits == 8) dtype == LIN_F32 ? go(opt_update8_kernel<LIN_F32>) : dtype == LIN_BF16 ? go(opt_update8_kernel<LIN_BF16>) : go(opt_update8_kernel<LIN_F16>);
       else dtype == LIN_F32 ? go(opt_update_kernel<LIN_F32>) : dtype == LIN_BF16 ? go(opt_update_kernel<LIN_BF16>) : go(opt_update_kernel<LIN_F16>);
@@ -511,16 +509,15 @@ hipError_t launch_adamw(const gdn2_adamw_tensor* t, int n, int bits, double max_
 }
 
 hipError_t launch_adamw_unpack(const gdn2_adamw_tensor* t, int n, float* const* m_out, float* const* v_out, hipStream_t s) {
-  std::vector<gdn2_adamw_tensor> x(t, t + n);
-  for (int i = 0; i < n; ++i) {            // (as parameters of float32 whose place m takes, with v for a master)
-    x[i].dtype = LIN_F32;
-    x[i].p = m_out[i];
-    x[i].g = nullptr;
-    x[i].master = v_out[i];
-  }
-  opt_each(x.data(), n, LIN_F32, 8, [&](const OptTensors& a, int, int blocks) {
-    hipLaunchKernelGGL(opt_unpack_kernel, dim3(blocks), dim3(256), 0, s, a);
-  });
+  auto at = [&](int i) {                   // (as a float32 parameter whose place m takes, with v for a master)
+    gdn2_adamw_tensor x = t[i];
+    x.dtype = LIN_F32;
+    x.p = m_out[i];
+    x.g = nullptr;
+    x.master = v_out[i];
+    return x;
+  };
+  opt_each(n, LIN_F32, 8, at, [&](const OptTensors& a, int, int blocks) { hipLaunchKernelGGL(opt_unpack_kernel, dim3(blocks), dim3(256), 0, s, a); });
   return hipGetLastError();
 }
 
