@@ -52,8 +52,8 @@ __global__ __launch_bounds__(256) void lin_pack_kernel(LinPacks js) {
     }
   };
   if (j.vec && c0 + 64 <= j.cols) {
-    // four rows of src a wave at a time, four neighbouring values a lane
-    const int y = threadIdx.x >> 4, x = 4 * (threadIdx.x & 15);
+    // four neighbouring values a lane, sixteen lanes to a row of src, or to a row of out (so that their writes meet no bank twice)
+    const int y = j.turn ? threadIdx.x & 15 : threadIdx.x >> 4, x = 4 * (j.turn ? threadIdx.x >> 4 : threadIdx.x & 15);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int row = r0 + 16 * i + y;
@@ -133,7 +133,6 @@ __global__ __launch_bounds__(256) void lin_slope_kernel(LinSlope a, float* part,
         s[e] += d;
       }
   }
-  if (!part) return;
   sums[w][l] = make_float4(s[0], s[1], s[2], s[3]);
   __syncthreads();
   if (w || n >= a.N) return;
@@ -142,6 +141,26 @@ __global__ __launch_bounds__(256) void lin_slope_kernel(LinSlope a, float* part,
 #pragma unroll
   for (int e = 0; e < 4; ++e)
     if (n + e < a.N) part[(size_t)blockIdx.y * a.N + n + e] = f[e];
+}
+// Without a bias the rows do not matter: dy, z and dz are arrays of `total` values, whatever a row's width.  vec: every
+// pointer takes 16 bytes.
+template <int ACT>
+__global__ __launch_bounds__(256) void lin_slope_flat_kernel(LinSlope a, size_t total, int vec) {
+  const size_t x = (size_t)blockIdx.x * 256 + threadIdx.x, step = (size_t)gridDim.x * 256, whole = vec ? total / 4 : 0;
+#pragma unroll 4
+  for (size_t i = x; i < whole; i += step) {
+    float4 d = lin_get4(a.dy_dtype, a.dy, 4 * i);
+    if constexpr (ACT != LIN_NONE) {
+      const float4 z = lin_get4(a.dtype, a.z, 4 * i);
+      d.x *= lin_slope<ACT>(z.x); d.y *= lin_slope<ACT>(z.y); d.z *= lin_slope<ACT>(z.z); d.w *= lin_slope<ACT>(z.w);
+    }
+    lin_put4(a.dtype, a.dz, 4 * i, d);
+  }
+  for (size_t i = 4 * whole + x; i < total; i += step) {
+    float d = lin_get(a.dy_dtype, a.dy, i);
+    if constexpr (ACT != LIN_NONE) d *= lin_slope<ACT>(lin_get(a.dtype, a.z, i));
+    lin_put(a.dtype, a.dz, i, d);
+  }
 }
 // Sixteen groups of sixteen threads: a group's columns, every sixteenth block each
 __global__ __launch_bounds__(256) void lin_bias_kernel(LinSlope a, const float* part, int blocks) {
@@ -321,17 +340,25 @@ static int slope_blocks(const LinSlope& a) {
   return (a.M + rows - 1) / rows;
 }
 size_t linear_slope_workspace_bytes(const LinSlope& a) { return a.dbias ? (size_t)slope_blocks(a) * a.N * 4 : 0; }
-hipError_t launch_linear_slope(const LinSlope& a, void* workspace, hipStream_t s) {
-  const int blocks = slope_blocks(a), rows = slope_rows(a);
-  float* part = a.dbias ? static_cast<float*>(workspace) : nullptr;
+template <int ACT>
+static void slope_go(const LinSlope& a, float* part, hipStream_t s) {
   auto low = [](const void* q) { return reinterpret_cast<uintptr_t>(q); };
-  const int vec = a.N % 4 == 0 && (low(a.dy) | low(a.z) | low(a.dz)) % 16 == 0;
-  const dim3 grid((a.N + 255) / 256, blocks);
-  if (a.act == LIN_SILU) hipLaunchKernelGGL(lin_slope_kernel<LIN_SILU>, grid, dim3(256), 0, s, a, part, rows, vec);
-  else if (a.act == LIN_GELU) hipLaunchKernelGGL(lin_slope_kernel<LIN_GELU>, grid, dim3(256), 0, s, a, part, rows, vec);
-  else if (a.act == LIN_TANH) hipLaunchKernelGGL(lin_slope_kernel<LIN_TANH>, grid, dim3(256), 0, s, a, part, rows, vec);
-  else hipLaunchKernelGGL(lin_slope_kernel<LIN_NONE>, grid, dim3(256), 0, s, a, part, rows, vec);
-  if (part) hipLaunchKernelGGL(lin_bias_kernel, dim3((a.N + 15) / 16), dim3(256), 0, s, a, part, blocks);
+  const bool wide = (low(a.dy) | low(a.z) | low(a.dz)) % 16 == 0;
+  if (!part) {
+    const size_t total = (size_t)a.M * a.N, wgs = (total + 4095) / 4096;
+    hipLaunchKernelGGL(lin_slope_flat_kernel<ACT>, dim3(wgs < 16384 ? wgs : 16384), dim3(256), 0, s, a, total, wide);
+    return;
+  }
+  const int rows = slope_rows(a), blocks = slope_blocks(a);
+  hipLaunchKernelGGL(lin_slope_kernel<ACT>, dim3((a.N + 255) / 256, blocks), dim3(256), 0, s, a, part, rows, a.N % 4 == 0 && wide);
+  hipLaunchKernelGGL(lin_bias_kernel, dim3((a.N + 15) / 16), dim3(256), 0, s, a, part, blocks);
+}
+hipError_t launch_linear_slope(const LinSlope& a, void* workspace, hipStream_t s) {
+  float* part = a.dbias ? static_cast<float*>(workspace) : nullptr;
+  if (a.act == LIN_SILU) slope_go<LIN_SILU>(a, part, s);
+  else if (a.act == LIN_GELU) slope_go<LIN_GELU>(a, part, s);
+  else if (a.act == LIN_TANH) slope_go<LIN_TANH>(a, part, s);
+  else slope_go<LIN_NONE>(a, part, s);
   return hipGetLastError();
 }
 

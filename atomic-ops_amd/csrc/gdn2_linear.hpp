@@ -875,7 +875,7 @@ static void lin_go(LinArgs a, const LinPlan& r, hipStream_t s) {
 template <int DT, int ACT, int NP, bool AR, bool BR>
 static void lin_tiles(const LinArgs& a, const LinPlan& r, hipStream_t s) {
   if (r.tile == LIN_SMALL) lin_go<LinTile<DT, ACT, NP, AR, BR, 64, 64, 4, 1, lin_bk(DT), 3, 8>>(a, r, s);
-  else if (r.tile == LIN_MID) lin_go<LinTile<DT, ACT, NP, AR, BR, 128, 128, 2, 2, lin_bk(DT), 2, 8>>(a, r, s);
+  else if (r.tile == LIN_MID) lin_go<LinTile<DT, ACT, NP, AR, BR, 128, 128, DT == LIN_F32 ? 4 : 2, 2, lin_bk(DT), 2, 8>>(a, r, s);
   else if constexpr (DT == LIN_F32) lin_go<LinTile<DT, ACT, NP, AR, BR, 256, 128, 4, 2, lin_bk(DT), 2, 4>>(a, r, s);
   else lin_go<LinTile<DT, ACT, NP, AR, BR, 256, 256, 2, 4, lin_bk(DT), 2, 4>>(a, r, s);
 }
