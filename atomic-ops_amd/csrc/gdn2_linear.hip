@@ -278,6 +278,7 @@ hipError_t launch_linear(const LinProduct& p, void* workspace, hipStream_t s) {
   a.out_dtype = p.out_dtype; a.bias_dtype = p.bias_dtype;
   a.ldr = p.ldr; a.bias = p.bias; a.residual = p.residual; a.y = p.y; a.z = p.z;
   a.vec = p.N % 8 == 0 && p.ldr % 8 == 0 && (low(p.bias) | low(p.residual) | low(p.y) | low(p.z)) % 16 == 0;
+  a.pairs = r.parts == 1 && p.dtype != LIN_F32 && p.out_dtype == p.dtype && (low(p.y) | low(p.z)) % 4 == 0;
   a.parts = r.parts;
   a.per = r.per;
   a.a = LinOperand{static_cast<const uint16_t*>(p.a), p.lda, 0, p.M};

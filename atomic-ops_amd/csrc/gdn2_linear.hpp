@@ -168,7 +168,7 @@ struct LinArgs {
   LinOperand a, b;
   int M, N, K;           // K: up to the last whole value of the sum
   int mt, nt, parts, per;        // tiles; parts of the sum, of `per` blocks each
-  int out_dtype, bias_dtype, vec;
+  int out_dtype, bias_dtype, vec, pairs;       // how results are written: lin_out8, lin_out_pairs
   size_t ldr;
   const void *bias, *residual;
   void *y, *z;
@@ -383,6 +383,70 @@ __device__ __forceinline__ void lin_out_odd(const LinArgs& a, int part, const fl
   }
 }
 
+// The same for results of 16 bits, which would be half a line at a time: half a wave takes a row, a lane two neighbouring
+// columns from an even place in memory on (rows of odd width start at an odd one every other time: then the last lane has the
+// two that are left over).  y and z take 4-byte accesses.
+template <int DT, int ACT>
+__device__ __forceinline__ void lin_out_pairs(const LinArgs& a, const float* own, int ldo, int rows, int m0, int n0) {
+  using L = LinType<DT>;
+  const int l = lane_id(), hl = l & 31;
+  constexpr int U = 4;
+  const int left = a.N - n0;                 // columns from here on
+  if (left <= 0) return;
+  float b[4] = {0.f, 0.f, 0.f, 0.f};         // of columns 2 hl .. 2 hl + 2, and 0
+  if (a.bias) {
+#pragma unroll
+    for (int e = 0; e < 3; ++e) b[e] = lin_get(a.bias_dtype, a.bias, n0 + min(2 * hl + e, left - 1));
+    b[3] = lin_get(a.bias_dtype, a.bias, n0);
+  }
+  for (int r = l >> 5; r < rows && m0 + r < a.M; r += 2 * U) {
+    float res[U][2];
+    int col[U][2];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int m = min(m0 + r + 2 * u, a.M - 1), odd = (int)(((size_t)m * a.N + n0) & 1);
+      const bool over = odd && hl == 31;
+      col[u][0] = over ? 63 : 2 * hl + odd;
+      col[u][1] = over ? 0 : 2 * hl + odd + 1;
+      if (a.residual)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) res[u][e] = lin_get(a.out_dtype, a.residual, (size_t)m * a.ldr + n0 + min(col[u][e], left - 1));
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int row = r + 2 * u, m = m0 + row, odd = col[u][0] & 1;
+      if (row >= rows || m >= a.M) break;
+      const bool over = col[u][1] < col[u][0];
+      float f[2], z[2];
+      z[0] = own[row * ldo + col[u][0]] + (odd ? b[1] : b[0]);
+      z[1] = own[row * ldo + col[u][1]] + (over ? b[3] : odd ? b[2] : b[1]);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        f[e] = lin_act<ACT>(z[e]);
+        if (a.residual) f[e] += res[u][e];
+      }
+      const size_t at = (size_t)m * a.N + n0;
+      auto two = [&](void* p, const float* v) __attribute__((always_inline)) {
+        if (!over && col[u][1] < left) {
+          uint32_t w;
+          if constexpr (DT == LIN_BF16) w = bf16_pack(v[0], v[1]);
+          else {
+            const h2v h = {(_Float16)v[0], (_Float16)v[1]};
+            w = __builtin_bit_cast(uint32_t, h);
+          }
+          *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p) + at + col[u][0]) = w;
+          return;
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (col[u][e] < left) L::put(p, at + col[u][e], v[e]);
+      };
+      if (a.z) two(a.z, z);
+      two(a.y, f);
+    }
+  }
+}
+
 // Workgroups go to the 8 dies in turn: each die gets a run of neighbouring tiles (of one part of the sum), GM rows of tiles
 // high, so that what its workgroups read at a time is shared in its L2.
 __device__ __forceinline__ void lin_place(const LinArgs& a, int gm, int& part, int& mi, int& ni) {
@@ -502,7 +566,10 @@ __global__ __launch_bounds__(C::W * WAVE) void lin_tile_kernel(LinArgs a) {
       }
     __builtin_amdgcn_wave_barrier();
     if (!a.vec) {
-      lin_out_odd<C::DT, C::ACT, 64>(a, part, own, nullptr, C::LDO, 16 * HT, m0 + 16 * (wm * MT + h), n0 + 64 * wn);
+      const int mf = m0 + 16 * (wm * MT + h), nf = n0 + 64 * wn;
+      if constexpr (C::DT == LIN_F32) lin_out_odd<C::DT, C::ACT, 64>(a, part, own, nullptr, C::LDO, 16 * HT, mf, nf);
+      else if (a.pairs) lin_out_pairs<C::DT, C::ACT>(a, own, C::LDO, 16 * HT, mf, nf);
+      else lin_out_odd<C::DT, C::ACT, 64>(a, part, own, nullptr, C::LDO, 16 * HT, mf, nf);
       __builtin_amdgcn_wave_barrier();
       continue;
     }

@@ -84,7 +84,7 @@ def check(M, K, N, dt, act=None, bias=False, residual=False, grad=True, out_dtyp
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("M,K,N", [(1, 1, 1), (1, 64, 8), (2, 7, 3), (3, 200, 130), (17, 33, 65), (128, 64, 128), (129, 72, 136),
-                                   (130, 127, 257), (300, 512, 264), (64, 1000, 777)])
+                                   (130, 127, 257), (70, 40, 1), (66, 48, 62), (300, 40, 191), (77, 16, 127), (270, 33, 129), (300, 512, 264), (64, 1000, 777)])
 def test_sizes(dtype, M, K, N):
     check(M, K, N, DTYPES[dtype], act="silu", bias=True, residual=True)
 
