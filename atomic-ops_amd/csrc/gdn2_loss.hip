@@ -3,7 +3,8 @@
 //   dx_j = s (p_j (1 + 2 z lse) - (1 - e) [j = t] - e / V),  p_j = exp(x_j - m) / sum
 // A row's maximum and sum come from one pass (each thread rescales its sum where its maximum grows); the gradient's p
 // is formed from them, not from lse, whose rounding (2^-24 |lse|) would be an error of every p.  Statistics are
-// float32, the sum over the rows 64 bits, in a fixed order.  Bound by memory.
+// float32, the sum over the rows 64 bits, in a fixed order.  Bound by memory, two exponentials an element close behind: 8192 x
+// 131072 bfloat16 971 us, 4.4 TB/s of reads and writes (a copy 5.2); 16384 x 256 float32 11 us, 2.9 TB/s.
 #include "gdn2_kernels.hpp"
 
 namespace gdn2 {
