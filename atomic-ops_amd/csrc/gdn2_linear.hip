@@ -204,23 +204,28 @@ static LinSide lin_side(const LinProduct& p, bool b) {
   return s;
 }
 
-// float32 on the matrix cores' own float32 up to this many operations, as pieces beyond (us, own, pieces: 2048 x 768 x 512
-// 22.7, 31.5; 2048 x 1024 x 768 46, 42; 4096 x 1024 x 512 45, 55; 2048 x 2048 x 1024 82, 78; 4096 x 2048 x 1024 159, 126)
-constexpr double LIN_DIRECT_MOST = 6e9;
+// float32, up to this many operations on the matrix cores' own float32, beyond as pieces that each wave cuts (us, own, cut:
+// 512^3 10.6, 16.3; 2048 x 768 x 512 21.2, 29.0; 1024^3 28, 33; 2048 x 1024 x 768 46.5, 37.4; 4096 x 2048 x 1024 160, 103); in rows
+// that 16-byte accesses do not take 300 x 677 x 811 17.9, 22.0; 500 x 999 x 1001 24.9, 27.0; 2047 x 767 x 513 43.8, 33.3
+constexpr double LIN_DIRECT_MOST = 2.5e9, LIN_DIRECT_ODD = 1.2e9;
+// float32 as pieces that a pass over memory has cut before (cut by each wave, by the pass): large tiles over a long sum, 4096^3
+// 698, 667, but 4096 x 2048 x 1024 103, 128; odd rows, where an operand is used often enough, which M N / (M + N) says: 2048 x
+// 4095 x 4097 754, 535 (1365); 16383 x 255 x 513 75, 69 (497); 2047 x 767 x 513 33.3, 34.9 (410); 218 x 8190 x 7626 265, 358 (212)
+constexpr int64_t LIN_PACK_K = 4096, LIN_PACK_USE = 450;
 // Few rows: whether every row of x and W takes 16-byte accesses
 static bool lin_whole(const LinProduct& p) {
   const size_t e = p.dtype == LIN_F32 ? 4 : 8;
   return (reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b)) % 16 == 0 && p.lda % e == 0 && p.ldb % e == 0 &&
          p.K % 8 == 0 && (p.form == LIN_XWT || p.N % e == 0);
 }
-// float32: whether lin_direct_kernel can read the operands
+// float32: whether every row of the operands takes 16-byte accesses
 static bool lin_float(const LinProduct& p) {
   const int ca = p.form == LIN_XTW ? p.M : p.K, cb = p.form == LIN_XWT ? p.K : p.N;
   return p.dtype == LIN_F32 && (reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b)) % 16 == 0 && p.lda % 4 == 0 &&
          p.ldb % 4 == 0 && ca % 4 == 0 && cb % 4 == 0;
 }
 static LinPlan lin_plan(const LinProduct& p) {
-  LinPlan r{0, LIN_MID, 1, 0};
+  LinPlan r{0, LIN_MID, 1, 0, lin_float(p)};
   const int64_t cus = cu_count();
   auto tiles = [&](int64_t bm, int64_t bn) { return ((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
   auto split = [&](int64_t units, int64_t parts, int64_t most) {
@@ -249,10 +254,15 @@ static LinPlan lin_plan(const LinProduct& p) {
   auto rounds = [&](int64_t tiles, int64_t at_once) { return (tiles + at_once - 1) / at_once; };
   const double big_rounds = p.dtype == LIN_F32 ? rounds(big, cus) * 2 * 0.82 : rounds(big, cus) * 4 * 0.86;
   const double mid_rounds = p.dtype == LIN_F32 ? rounds(mid, cus) : rounds(mid, 2 * cus) * 2;
-  if (lin_float(p) && 2.0 * p.M * p.N * p.K <= LIN_DIRECT_MOST) {
+  const bool large = big * 4 >= cus * 3 && big_rounds <= mid_rounds;
+  const bool pack = r.wide ? large && p.K >= LIN_PACK_K : (int64_t)p.M * p.N >= LIN_PACK_USE * ((int64_t)p.M + p.N);
+  if (p.dtype == LIN_F32 && 2.0 * p.M * p.N * p.K <= (r.wide ? LIN_DIRECT_MOST : LIN_DIRECT_ODD)) {
     r.tile = LIN_DIRECT;
     split(blocks, small * 4 >= cus * 3 ? 1 : 2 * cus / small, blocks / 4);
-  } else if (big * 4 >= cus * 3 && big_rounds <= mid_rounds) {
+  } else if (p.dtype == LIN_F32 && !pack) {
+    r.tile = LIN_CUT;      // (two workgroups a CU of four waves; one of eight, whose addresses take more registers)
+    split(blocks, (r.wide ? 2 : 1) * cus / mid, blocks / 4);
+  } else if (large) {
     r.tile = LIN_BIG;
     split(blocks, 1, 1);
   } else if (mid >= cus || blocks * mid >= 16 * cus) {
@@ -267,7 +277,7 @@ static size_t lin_parts_bytes(const LinProduct& p, const LinPlan& r) { return r.
 
 size_t linear_workspace_bytes(const LinProduct& p) {
   const LinPlan r = lin_plan(p);
-  return (r.rows || r.tile == LIN_DIRECT ? 0 : lin_side(p, false).bytes + lin_side(p, true).bytes) + lin_parts_bytes(p, r);
+  return (r.rows || r.tile >= LIN_DIRECT ? 0 : lin_side(p, false).bytes + lin_side(p, true).bytes) + lin_parts_bytes(p, r);
 }
 
 hipError_t launch_linear(const LinProduct& p, void* workspace, hipStream_t s) {
@@ -298,7 +308,7 @@ hipError_t launch_linear(const LinProduct& p, void* workspace, hipStream_t s) {
   for (int b = 0; b < 2; ++b) {
     const LinSide d = lin_side(p, b);
     LinOperand& o = b ? a.b : a.a;
-    if (!d.pack || r.tile == LIN_DIRECT) continue;
+    if (!d.pack || r.tile >= LIN_DIRECT) continue;
     LinPack& j = js.job[jobs];
     j.src = o.p;
     j.lds = o.ld;

@@ -12,9 +12,11 @@
 //                       their use, sums in parts where there are few tiles; float32 as three bfloat16 pieces, six
 //                       products.  Bound by the matrix cores: 8192 x 4096 x 4096 bfloat16 225 us, 1.22 PFLOP/s;
 //                       4096^3 float32 660 us, 208 TFLOP/s (a library product on the float32 matrix cores 911).  Each
-//                       tile's epilogue waits for its products: with bias, activation, z and residual 296.
-//   lin_direct_kernel   small float32 products: 2048 x 768 x 512 22.5 us (the library's 18), bound by the waits of 24
-//                       blocks one after the other;
+//                       tile's epilogue waits for its products: with bias, activation, z and residual 296.  CUT:
+//                       float32 stays as it is up to LDS and each wave cuts what it reads, no pass over memory before it:
+//                       218 x 8192 x 7680 197 us (by a pass 357, the library 237), 4096 x 2048 x 1024 103 (128, 119);
+//   lin_direct_kernel   small float32 products: 2048 x 768 x 512 21 us (the library's 18), 512^3 10.6 (17), bound by what
+//                       its small tiles draw from the caches;
 //   lin_rows_kernel, lin_columns_kernel, lin_dots_kernel   up to 8 rows, bound by W's bytes: one row of 4096 x 14336 bfloat16
 //                       21.8 us, 5.4 TB/s.
 #pragma once
@@ -188,18 +190,103 @@ struct LinArgs {
 
 static __device__ uint4 lin_zeros;      // what lies past the end of a sum
 
+// s_waitcnt: all but the last n of the wave's DMAs
+constexpr int lin_wait(int n) { return WAIT_VMCNT0 | (n & 15) | n >> 4 << 14; }
+// lds_dma16 for four bytes a lane (global_load_lds_dword), at dst + i floats
+__device__ __forceinline__ void lin_dma4(const float* src, float* dst) {
+  const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) float*)dst;
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" : : "v"(src), "s"(lds) : "memory", "m0");
+}
+// float32 as it is: blocks of 32 along the sum, by W waves' DMAs of 16 bytes a lane (WIDE: rows that take them) or of 4.
+// In LDS, in chunks of four values:
+//   rows along the sum (8 chunks): chunk c of row r at c ^ (r & 7);
+//   rows across it (ROWS / 4): chunk c of value k at c ^ 4 (k / 4 & 3), so that the lanes of a read, which take k = 4 c + j
+//   for c = 0 .. 3 of sixteen rows each, meet no bank twice.
+template <bool R, int ROWS, int W, bool WIDE>
+struct LinFloats {
+  static constexpr int E = WIDE ? 4 : 1, D = ROWS * 32 / (64 * E * W);
+  const char* src[D];
+  int k[D];
+  size_t step;
+  __device__ __forceinline__ void init(const LinOperand& o, int row0, int kb0) {
+    const float* p = reinterpret_cast<const float*>(o.p);
+    step = (R ? 32 * o.ld : (size_t)32) * 4;
+#pragma unroll
+    for (int i = 0; i < D; ++i) {
+      const int f = ((wave_id() * D + i) * 64 + lane_id()) * E, q = f >> 2, e = f & 3;
+      size_t at;
+      if constexpr (R) {
+        k[i] = q / (ROWS / 4);
+        const int chunk = (q & (ROWS / 4 - 1)) ^ ((k[i] >> 2 & 3) << 2);
+        at = (size_t)k[i] * o.ld + min(row0 + 4 * chunk + e, o.rows - E);
+      } else {
+        const int row = q >> 3;
+        k[i] = 4 * ((q & 7) ^ (row & 7)) + e;
+        at = (size_t)min(row0 + row, o.rows - 1) * o.ld + k[i];
+      }
+      src[i] = reinterpret_cast<const char*>(p + at) + (size_t)kb0 * step;
+      k[i] += kb0 * 32;
+    }
+  }
+  __device__ __forceinline__ void fetch(char* dst, int K, bool tail) {
+#pragma unroll
+    for (int i = 0; i < D; ++i) {
+      const char* s = src[i];
+      if (tail) s = k[i] < K ? s : reinterpret_cast<const char*>(&lin_zeros);
+      float* to = reinterpret_cast<float*>(dst) + (wave_id() * D + i) * 64 * E;
+      if constexpr (WIDE) lds_dma16(reinterpret_cast<const float*>(s), to);
+      else lin_dma4(reinterpret_cast<const float*>(s), to);
+      src[i] += step;
+      k[i] += 32;
+    }
+  }
+};
+// A lane's values of tile t (16 rows) and of sixteen along the sum, s of two: 4 c .. 4 c + 3, c = lane / 16
+template <bool R, int ROWS>
+__device__ __forceinline__ float4 lin_floats(const char* lds, int t, int s) {
+  const int l = lane_id(), r = l & 15, c = l >> 4;
+  if constexpr (R) {
+    const float* p = reinterpret_cast<const float*>(lds) + (16 * s + 4 * c) * ROWS + 16 * (t ^ c) + r;
+    return make_float4(p[0], p[ROWS], p[2 * ROWS], p[3 * ROWS]);
+  } else {
+    const int row = 16 * t + r;
+    return *reinterpret_cast<const float4*>(lds + row * 128 + (((4 * s + c) ^ (row & 7)) << 4));
+  }
+}
+// Both s of a tile as the three pieces of the whole block's operand
+template <bool R, int ROWS>
+__device__ __forceinline__ void lin_cut(const char* lds, int t, s8& hi, s8& mid, s8& lo) {
+  const float4 x = lin_floats<R, ROWS>(lds, t, 0), y = lin_floats<R, ROWS>(lds, t, 1);
+  float f[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+  uint32_t piece[3][4];
+#pragma unroll
+  for (int p = 0; p < 3; ++p)
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const uint32_t a = __float_as_uint(f[e]), b = __float_as_uint(f[e + 1]);
+      piece[p][e / 2] = __builtin_amdgcn_perm(b, a, 0x07060302);
+      f[e] -= __uint_as_float(a & 0xffff0000u);
+      f[e + 1] -= __uint_as_float(b & 0xffff0000u);
+    }
+  hi = __builtin_bit_cast(s8, piece[0]);
+  mid = __builtin_bit_cast(s8, piece[1]);
+  lo = __builtin_bit_cast(s8, piece[2]);
+}
+
 // BM x BN results a workgroup of WM x WN waves; blocks of BK along the sum, NBUF of them in LDS; NP planes; AR, BR: rows
 // run across the sum
-template <int DT_, int ACT_, int NP_, bool AR_, bool BR_, int BM_, int BN_, int WM_, int WN_, int BK_, int NBUF_, int GM_>
+// CUT: operands are float32 in LDS, and each wave cuts what it reads (1: fetched by 16 bytes, 2: by 4)
+template <int DT_, int ACT_, int NP_, bool AR_, bool BR_, int BM_, int BN_, int WM_, int WN_, int BK_, int NBUF_, int GM_, int CUT_ = 0>
 struct LinTile {
   static constexpr int GM = GM_, DT = DT_, ACT = ACT_, NP = NP_, BM = BM_, BN = BN_, WM = WM_, WN = WN_, BK = BK_, NBUF = NBUF_, W = WM * WN;
   static constexpr bool AR = AR_, BR = BR_;
+  static constexpr int CUT = CUT_, LP = CUT ? 1 : NP, ES = CUT ? 4 : 2;        // planes in LDS, of elements of ES bytes
   static constexpr int MT = BM / WM / 16, NT = BN / WN / 16;
-  static constexpr int AB = BM * BK * 2, BB = BN * BK * 2, BUF = NP * (AB + BB), LDO = 68, OUT = 16 * (MT < 4 ? MT : 4) * LDO * 4;
+  static constexpr int AB = BM * BK * ES, BB = BN * BK * ES, BUF = LP * (AB + BB), LDO = 68, OUT = 16 * (MT < 4 ? MT : 4) * LDO * 4;
   static constexpr int LDS = NBUF * BUF > W * OUT ? NBUF * BUF : W * OUT;      // LDO: a row of a wave's results
-  static constexpr int DA = NP * AB / 1024 / W, DB = NP * BB / 1024 / W;       // a wave's DMAs of a block
-  static_assert(AB % 1024 == 0 && BB % 1024 == 0 && NP * AB % (1024 * W) == 0 && NP * BB % (1024 * W) == 0, "whole DMAs");
-  static_assert(NT == 4 && (MT % 4 == 0 || MT < 4) && (NP == 1 || (!AR && !BR)) && LDS <= 160 * 1024, "shapes");
+  static constexpr int DA = LP * AB / 1024 / W * (CUT == 2 ? 4 : 1), DB = LP * BB / 1024 / W * (CUT == 2 ? 4 : 1);       // a wave's DMAs of a block
+  static_assert(AB % 1024 == 0 && BB % 1024 == 0 && LP * AB % (1024 * W) == 0 && LP * BB % (1024 * W) == 0, "whole DMAs");
+  static_assert(NT == 4 && (MT % 4 == 0 || MT < 4) && (CUT ? NP == 3 && BK == 32 : NP == 1 || (!AR && !BR)) && LDS <= 160 * 1024, "shapes");
 };
 
 // Where a wave's i-th DMA of an operand's block comes from.  Sixteen bytes a lane:
@@ -479,14 +566,14 @@ __global__ __launch_bounds__(C::W * WAVE) void lin_tile_kernel(LinArgs a) {
   lin_place(a, C::GM, part, mi, ni);
   const int m0 = mi * C::BM, n0 = ni * C::BN;
   const int blocks = (a.K + C::BK - 1) / C::BK, kb0 = part * a.per, kb1 = min(blocks, kb0 + a.per);
-  LinSource<C, C::AR, C::BM, C::DA> sa;
-  LinSource<C, C::BR, C::BN, C::DB> sb;
+  std::conditional_t<C::CUT != 0, LinFloats<C::AR, C::BM, C::W, C::CUT == 1>, LinSource<C, C::AR, C::BM, C::DA>> sa;
+  std::conditional_t<C::CUT != 0, LinFloats<C::BR, C::BN, C::W, C::CUT == 1>, LinSource<C, C::BR, C::BN, C::DB>> sb;
   sa.init(a.a, m0, kb0);
   sb.init(a.b, n0, kb0);
   auto fetch = [&](int kb, int buf) __attribute__((always_inline)) {
     const bool tail = (kb + 1) * C::BK > a.K;
     sa.fetch(lds + buf, a.K, tail);
-    sb.fetch(lds + buf + NP * C::AB, a.K, tail);
+    sb.fetch(lds + buf + C::LP * C::AB, a.K, tail);
   };
   // float32: the products of the leading pieces on their own, so that the small ones are not rounded beside them
   constexpr int NA = NP > 1 ? 2 : 1;
@@ -499,6 +586,30 @@ __global__ __launch_bounds__(C::W * WAVE) void lin_tile_kernel(LinArgs a) {
       for (int t = 0; t < MT; ++t) acc[q][i][t] = f4{0.f, 0.f, 0.f, 0.f};
   // Operands are read ahead of their use, those of A by AHEAD tiles, those of B by one step of the sum, a few beside each
   // group of products (8192 x 4096 x 4096 bfloat16: 225 us, 1224 TFLOP/s; read where they are used 248)
+  auto products = [&](int t, const s8 (&n)[NP][NT], const s8 (&m)[NP]) __attribute__((always_inline)) {
+    // (float32: the smallest pieces' products first)
+#pragma unroll
+    for (int o = NP - 1; o >= 0; --o)
+#pragma unroll
+      for (int p = 0; p <= o; ++p) {
+        auto& c4 = acc[o ? NA - 1 : 0];
+        const auto& b4 = n[o - p];
+        lin_mfma4<F16>(c4[0][t], c4[1][t], c4[2][t], c4[3][t], b4[0], b4[1], b4[2], b4[3], m[p]);
+      }
+  };
+  // (8 values a lane cost 44 instructions beside the products: a tile of B serves four of A and the other way round)
+  auto add_cut = [&](const char* at) __attribute__((always_inline)) {
+    if constexpr (C::CUT) {
+      s8 n[3][NT], m[3];
+#pragma unroll
+      for (int i = 0; i < NT; ++i) lin_cut<C::BR, C::BN>(at + C::AB, wn * NT + i, n[0][i], n[1][i], n[2][i]);
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        lin_cut<C::AR, C::BM>(at, wm * MT + t, m[0], m[1], m[2]);
+        products(t, n, m);
+      }
+    }
+  };
   auto add = [&](const char* at) __attribute__((always_inline)) {
     constexpr int STEPS = S * MT, AHEAD = NP == 1 ? 2 : 1, RING = AHEAD + 1;
     s8 n[2][NP][NT], m[RING][NP];
@@ -521,32 +632,25 @@ __global__ __launch_bounds__(C::W * WAVE) void lin_tile_kernel(LinArgs a) {
       if (s + 1 < S)
 #pragma unroll
         for (int i = t * NT / MT; i < (t + 1) * NT / MT; ++i) read_n(s + 1, i);
-      // (float32: the smallest pieces' products first)
-#pragma unroll
-      for (int o = NP - 1; o >= 0; --o)
-#pragma unroll
-        for (int p = 0; p <= o; ++p) {
-          auto& c4 = acc[o ? NA - 1 : 0];
-          const auto& b4 = n[s & 1][o - p];
-          lin_mfma4<F16>(c4[0][t], c4[1][t], c4[2][t], c4[3][t], b4[0], b4[1], b4[2], b4[3], m[x % RING][p]);
-        }
+      products(t, n[s & 1], m[x % RING]);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
   // Block kb has come when only the DMAs of the NBUF - 2 behind it are under way
   constexpr int AHEAD = C::NBUF - 1, BEHIND = (C::NBUF - 2) * (C::DA + C::DB);
-  static_assert(BEHIND < 16, "vmcnt's low bits");
+  static_assert(BEHIND < 64, "vmcnt");
   auto next = [&](int x) { return x == (C::NBUF - 1) * C::BUF ? 0 : x + C::BUF; };
 #pragma unroll
   for (int i = 0; i < AHEAD; ++i)
     if (kb0 + i < kb1) fetch(kb0 + i, i * C::BUF);
   int buf = 0, into = AHEAD * C::BUF;
   for (int kb = kb0; kb < kb1; ++kb) {
-    if (kb + C::NBUF - 2 < kb1) __builtin_amdgcn_s_waitcnt(WAIT_VMCNT0 | BEHIND);
+    if (kb + C::NBUF - 2 < kb1) __builtin_amdgcn_s_waitcnt(lin_wait(BEHIND));
     else __builtin_amdgcn_s_waitcnt(WAIT_VMCNT0);
     __syncthreads();
     if (kb + AHEAD < kb1) fetch(kb + AHEAD, into);
-    add(lds + buf);
+    if constexpr (C::CUT) add_cut(lds + buf);
+    else add(lds + buf);
     buf = next(buf);
     into = next(into);
   }
@@ -644,53 +748,11 @@ __global__ __launch_bounds__(256) void lin_join_kernel(LinArgs a) {
 // takes four values along the sum at a time, 4 c .. 4 c + 3 of sixteen (c = lane / 16), one for each of four
 // 4-deep products, of both operands: rows along the sum by 16 bytes, rows across it by four single values, their chunks
 // exchanged by 64 bytes for each c.
-template <int ACT_, bool AR_, bool BR_>
+template <int ACT_, bool AR_, bool BR_, bool WIDE_>
 struct LinDirect {
   static constexpr int ACT = ACT_, BM = 64, BN = 64, BK = 32, NBUF = 4, AB = BM * BK * 4, BUF = 2 * AB, LDS = NBUF * BUF, LDO = 36;
-  static constexpr bool AR = AR_, BR = BR_;
+  static constexpr bool AR = AR_, BR = BR_, WIDE = WIDE_;
 };
-template <bool R>
-struct LinDirectSource {
-  const char* src;
-  int k;
-  size_t step;
-  __device__ __forceinline__ void init(const LinOperand& o, int row0, int kb0) {
-    const float* p = reinterpret_cast<const float*>(o.p);
-    step = (R ? 32 * o.ld : (size_t)32) * 4;
-    const int q = wave_id() * 64 + lane_id();
-    size_t at;
-    if constexpr (R) {
-      k = q >> 4;
-      const int chunk = (q & 15) ^ ((k >> 2 & 3) << 2);
-      at = (size_t)k * o.ld + min(row0 + 4 * chunk, o.rows - 4);
-    } else {
-      const int row = q >> 3;
-      k = 4 * ((q & 7) ^ (row & 7));
-      at = (size_t)min(row0 + row, o.rows - 1) * o.ld + k;
-    }
-    src = reinterpret_cast<const char*>(p + at) + (size_t)kb0 * step;
-    k += kb0 * 32;
-  }
-  __device__ __forceinline__ void fetch(char* dst, int K, bool tail) {
-    const char* s = src;
-    if (tail) s = k < K ? s : reinterpret_cast<const char*>(&lin_zeros);
-    lds_dma16(reinterpret_cast<const float*>(s), reinterpret_cast<float*>(dst + wave_id() * 1024));
-    src += step;
-    k += 32;
-  }
-};
-// A lane's values of tile t and of sixteen along the sum, s of two
-template <bool R>
-__device__ __forceinline__ float4 lin_direct_read(const char* lds, int t, int s) {
-  const int l = lane_id(), r = l & 15, c = l >> 4;
-  if constexpr (R) {
-    const float* p = reinterpret_cast<const float*>(lds) + (16 * s + 4 * c) * 64 + 16 * (t ^ c) + r;
-    return make_float4(p[0], p[64], p[128], p[192]);
-  } else {
-    const int row = 16 * t + r;
-    return *reinterpret_cast<const float4*>(lds + row * 128 + (((4 * s + c) ^ (row & 7)) << 4));
-  }
-}
 template <class C>
 __global__ __launch_bounds__(512) void lin_direct_kernel(LinArgs a) {
   extern __shared__ char lds[];
@@ -699,8 +761,8 @@ __global__ __launch_bounds__(512) void lin_direct_kernel(LinArgs a) {
   lin_place(a, 8, part, mi, ni);
   const int m0 = mi * C::BM, n0 = ni * C::BN;
   const int blocks = (a.K + C::BK - 1) / C::BK, kb0 = part * a.per, kb1 = min(blocks, kb0 + a.per);
-  LinDirectSource<C::AR> sa;
-  LinDirectSource<C::BR> sb;
+  LinFloats<C::AR, C::BM, 8, C::WIDE> sa;
+  LinFloats<C::BR, C::BN, 8, C::WIDE> sb;
   sa.init(a.a, m0, kb0);
   sb.init(a.b, n0, kb0);
   auto fetch = [&](int kb, int buf) __attribute__((always_inline)) {
@@ -711,14 +773,14 @@ __global__ __launch_bounds__(512) void lin_direct_kernel(LinArgs a) {
   f4 acc[2][2];
 #pragma unroll
   for (int q = 0; q < 4; ++q) acc[q >> 1][q & 1] = f4{0.f, 0.f, 0.f, 0.f};
-  constexpr int AHEAD = C::NBUF - 1, BEHIND = (C::NBUF - 2) * 2;
+  constexpr int AHEAD = C::NBUF - 1, BEHIND = (C::NBUF - 2) * (sa.D + sb.D);
   auto next = [&](int x) { return x == (C::NBUF - 1) * C::BUF ? 0 : x + C::BUF; };
 #pragma unroll
   for (int i = 0; i < AHEAD; ++i)
     if (kb0 + i < kb1) fetch(kb0 + i, i * C::BUF);
   int buf = 0, into = AHEAD * C::BUF;
   for (int kb = kb0; kb < kb1; ++kb) {
-    if (kb + C::NBUF - 2 < kb1) __builtin_amdgcn_s_waitcnt(WAIT_VMCNT0 | BEHIND);
+    if (kb + C::NBUF - 2 < kb1) __builtin_amdgcn_s_waitcnt(lin_wait(BEHIND));
     else __builtin_amdgcn_s_waitcnt(WAIT_VMCNT0);
     __syncthreads();
     if (kb + AHEAD < kb1) fetch(kb + AHEAD, into);
@@ -726,8 +788,8 @@ __global__ __launch_bounds__(512) void lin_direct_kernel(LinArgs a) {
     float4 m[2], n[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      m[i] = lin_direct_read<C::AR>(at, wm * 2 + i, half);
-      n[i] = lin_direct_read<C::BR>(at + C::AB, wn * 2 + i, half);
+      m[i] = lin_floats<C::AR, C::BM>(at, wm * 2 + i, half);
+      n[i] = lin_floats<C::BR, C::BN>(at + C::AB, wn * 2 + i, half);
     }
     // (the four tiles in turn: a product that waits for the one before it costs an eighth more)
     auto four = [&](float n0, float n1, float m0, float m1) __attribute__((always_inline)) {
@@ -927,10 +989,11 @@ __global__ __launch_bounds__(256) void lin_dots_kernel(LinArgs a) {
 // How a product runs.
 struct LinPlan {
   int rows;                  // rows at a time by lin_rows_kernel or lin_dots_kernel; 0: tiles
-  int tile;                  // LIN_SMALL, LIN_MID, LIN_BIG; LIN_DIRECT: lin_direct_kernel
+  int tile;                  // LIN_SMALL, LIN_MID, LIN_BIG; float32 as it is: LIN_DIRECT, LIN_CUT, wide: by 16-byte accesses
   int parts, per;            // parts of the sum, of `per` blocks (rows: values)
+  bool wide;
 };
-enum { LIN_SMALL, LIN_MID, LIN_BIG, LIN_DIRECT };
+enum { LIN_SMALL, LIN_MID, LIN_BIG, LIN_DIRECT, LIN_CUT };      // the last two: no workspace but for the parts
 constexpr int lin_bk(int dtype) { return dtype == LIN_F32 ? 32 : 64; }
 
 template <int DT, int ACT>
@@ -996,31 +1059,34 @@ static void lin_acts(const LinArgs& a, const LinPlan& r, int act, hipStream_t s)
   else if (act == LIN_TANH) lin_tiles<DT, LIN_TANH, NP, AR, BR>(a, r, s);
   else lin_tiles<DT, LIN_NONE, NP, AR, BR>(a, r, s);
 }
-template <int ACT, bool AR, bool BR>
-static void lin_direct_go(LinArgs a, const LinPlan& r, hipStream_t s) {
-  using C = LinDirect<ACT, AR, BR>;
+// float32 as it is in memory; wide: in rows that 16-byte accesses take
+template <int ACT, bool AR, bool BR, bool WIDE>
+static void lin_floats_go(LinArgs a, const LinPlan& r, hipStream_t s) {
+  if (r.tile == LIN_CUT) return lin_go<LinTile<LIN_F32, ACT, 3, AR, BR, 128, 128, WIDE ? 2 : 4, 2, 32, 2, 8, WIDE ? 1 : 2>>(a, r, s);
+  using C = LinDirect<ACT, AR, BR, WIDE>;
   a.mt = (a.M + C::BM - 1) / C::BM;
   a.nt = (a.N + C::BN - 1) / C::BN;
   hipLaunchKernelGGL(lin_direct_kernel<C>, dim3(a.mt * a.nt * a.parts), dim3(512), C::LDS, s, a);
   lin_join<LIN_F32, ACT>(a, s);
 }
-template <bool AR, bool BR>
-static void lin_direct_act(const LinArgs& a, const LinPlan& r, int act, hipStream_t s) {
-  if (act == LIN_SILU) lin_direct_go<LIN_SILU, AR, BR>(a, r, s);
-  else if (act == LIN_GELU) lin_direct_go<LIN_GELU, AR, BR>(a, r, s);
-  else if (act == LIN_TANH) lin_direct_go<LIN_TANH, AR, BR>(a, r, s);
-  else lin_direct_go<LIN_NONE, AR, BR>(a, r, s);
+template <bool AR, bool BR, bool WIDE>
+static void lin_floats_act(const LinArgs& a, const LinPlan& r, int act, hipStream_t s) {
+  if (act == LIN_SILU) lin_floats_go<LIN_SILU, AR, BR, WIDE>(a, r, s);
+  else if (act == LIN_GELU) lin_floats_go<LIN_GELU, AR, BR, WIDE>(a, r, s);
+  else if (act == LIN_TANH) lin_floats_go<LIN_TANH, AR, BR, WIDE>(a, r, s);
+  else lin_floats_go<LIN_NONE, AR, BR, WIDE>(a, r, s);
 }
-static inline void lin_direct(const LinArgs& a, const LinPlan& r, int form, int act, hipStream_t s) {
-  if (form == LIN_XW) lin_direct_act<false, true>(a, r, act, s);
-  else if (form == LIN_XWT) lin_direct_act<false, false>(a, r, act, s);
-  else lin_direct_go<LIN_NONE, true, true>(a, r, s);
+template <bool WIDE>
+static void lin_floats_form(const LinArgs& a, const LinPlan& r, int form, int act, hipStream_t s) {
+  if (form == LIN_XW) lin_floats_act<false, true, WIDE>(a, r, act, s);
+  else if (form == LIN_XWT) lin_floats_act<false, false, WIDE>(a, r, act, s);
+  else lin_floats_go<LIN_NONE, true, true, WIDE>(a, r, s);
 }
 
 template <int DT>
 void lin_forms(const LinArgs& a, const LinPlan& r, int form, int act, hipStream_t s) {
   if constexpr (DT == LIN_F32) {
-    if (r.tile == LIN_DIRECT) lin_direct(a, r, form, act, s);
+    if (r.tile >= LIN_DIRECT) r.wide ? lin_floats_form<true>(a, r, form, act, s) : lin_floats_form<false>(a, r, form, act, s);
     else lin_acts<DT, 3, false, false>(a, r, act, s);
   } else {
     if (form == LIN_XW) lin_acts<DT, 1, false, true>(a, r, act, s);

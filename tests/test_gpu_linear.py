@@ -245,3 +245,38 @@ def test_equal_calls_give_equal_bits():
             y = linear(x, w, activation="silu")
             runs.append((y, *torch.autograd.grad(y, (x, w), torch.ones_like(y))))
         assert all(torch.equal(a, b) for run in runs[1:] for a, b in zip(run, runs[0]))
+
+
+# float32 in each of its ways: on the float32 matrix cores, as pieces that a wave or a pass cuts, rows of whole and odd widths
+@pytest.mark.parametrize("M,K,N", [(45, 131, 77), (640, 2052, 1028), (300, 8196, 612), (301, 7001, 331), (300, 1501, 1403),
+                                   (1025, 1027, 1001), (2050, 1000, 1030), (9, 12001, 6007)])
+def test_float32_ways(M, K, N):
+    check(M, K, N, torch.float32, act="gelu", bias=True, residual=True, seed=M)
+
+
+@pytest.mark.parametrize("lead", [1, 4])
+@pytest.mark.parametrize("M,K,N", [(64, 132, 80), (300, 4100, 1200)])
+def test_float32_views(M, K, N, lead):
+    """Rows of a wider tensor, from its column `lead` on; what lies beside them is not a number and stays unread."""
+    def view(t):
+        wide = t.new_full((t.shape[0], t.shape[1] + 2 * lead), float("nan"))
+        wide[:, lead:-lead] = t
+        return wide[:, lead:-lead]
+    check(M, K, N, torch.float32, act="silu", bias=True, seed=M + lead, make=view)
+
+
+def test_float32_equal_bits_and_captured():
+    from atomic_gdn2.linear import linear
+    for M, K, N in [(640, 2052, 1028), (301, 7001, 331)]:
+        x, w = torch.randn(M, K, device="cuda"), torch.randn(K, N, device="cuda")
+        y = linear(x, w)
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            z = linear(x, w)
+        for i in range(3):
+            z.zero_()
+            graph.replay()
+            assert torch.equal(linear(x, w), y) and torch.equal(z, y), (M, K, N, i)
+            torch.cuda.synchronize()
