@@ -131,7 +131,7 @@ __device__ __forceinline__ void lin_put4(int dt, void* p, size_t i, const float4
 
 // ---- activations: z s(u), s the logistic function, with u = z, 1.5958 (z + 0.044715 z^3), or gelu's z Phi(z).  The
 // tanh form 0.5 (1 + tanh(u / 2)) is s(u), which does not cancel where tanh goes to -1.
-constexpr float LIN_TANH_C = 1.59576912160573072f;       // 2 sqrt(2 / pi)
+constexpr float LIN_TANH_C = 1.5957691216f;       // 2 sqrt(2 / pi)
 // (the hardware's reciprocal: an error of one unit of the last place, and a sixth of a division)
 __device__ __forceinline__ float lin_logistic(float u) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(u * -1.44269504088896341f)); }
 template <int ACT>
