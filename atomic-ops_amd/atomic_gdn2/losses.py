@@ -32,6 +32,12 @@ def _run(x, targets, how, loss, dlogits, upstream=None, upstream_ld=0):
         _lib.check(L.gdn2_cross_entropy(ctypes.byref(a), _lib.ptr(ws), _lib.stream_handle(dev)), "gdn2_cross_entropy")
 
 
+def _saved(t, like):
+    """A saved tensor as it was saved: the kernels take its address, and hooks may have changed its strides, type or device."""
+    rows = t.is_contiguous() or (t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= t.shape[1])
+    return t if rows and (t.shape, t.dtype, t.device) == like else _lib.restored(t, *like)
+
+
 class _CrossEntropy(torch.autograd.Function):
     """(rows of logits, targets) -> loss.  Once differentiable: a second derivative raises."""
 
@@ -41,15 +47,14 @@ class _CrossEntropy(torch.autograd.Function):
         # float16 gradients are formed when the factor of a scaled loss is known: without it they would underflow
         d = torch.empty(x.shape, dtype=x.dtype, device=x.device) if x.dtype != torch.float16 and ctx.needs_input_grad[0] else None
         _run(x, targets, how, loss, d)
-        ctx.how, ctx.grad, ctx.like = how, d, (x.shape, x.dtype, x.device)
+        ctx.how, ctx.grad, ctx.likes = how, d, [(t.shape, t.dtype, t.device) for t in (x, targets)]
         ctx.save_for_backward(x, targets)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        x, targets = ctx.saved_tensors
-        x = x if (x.shape, x.dtype, x.device) == ctx.like and x.stride(1) == 1 else _lib.restored(x, *ctx.like)
+        x, targets = (_saved(t, like) for t, like in zip(ctx.saved_tensors, ctx.likes))
         g = g.contiguous()
         ld = 1 if ctx.how[3] == 0 else 0
         d, ctx.grad = ctx.grad, None
