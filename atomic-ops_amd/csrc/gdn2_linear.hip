@@ -21,7 +21,7 @@ struct LinPack {
   uint16_t* out;
   size_t lds, ld, plane;
   int rows, cols, turn;      // of src
-  int tr, tc, vec;           // tiles of 64 x 64; whether four values of src can be read at a time
+  int tr, tc;                // tiles of 64 x 64
 };
 struct LinPacks {
   LinPack job[2];
@@ -51,7 +51,7 @@ __global__ __launch_bounds__(256) void lin_pack_kernel(LinPacks js) {
       else tile[p][ry][cx] = piece[p];
     }
   };
-  if (j.vec && c0 + 64 <= j.cols) {
+  if (c0 + 64 <= j.cols) {
     // four neighbouring values a lane, sixteen lanes to a row of src, or to a row of out (so that their writes meet no bank twice)
     const int y = j.turn ? threadIdx.x & 15 : threadIdx.x >> 4, x = 4 * (j.turn ? threadIdx.x >> 4 : threadIdx.x & 15);
 #pragma unroll
@@ -59,13 +59,7 @@ __global__ __launch_bounds__(256) void lin_pack_kernel(LinPacks js) {
       const int row = r0 + 16 * i + y;
       const size_t at = (size_t)min(row, j.rows - 1) * j.lds + c0 + x;
       uint32_t v[4];
-      if constexpr (F32) {
-        const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint32_t*>(j.src) + at);
-        v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
-      } else {
-        const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(j.src) + at);
-        v[0] = u.x & 0xffffu; v[1] = u.x >> 16; v[2] = u.y & 0xffffu; v[3] = u.y >> 16;
-      }
+      lin_four<F32>(j.src, at, v);
 #pragma unroll
       for (int e = 0; e < 4; ++e) split(row < j.rows ? v[e] : 0u, 16 * i + y, x + e);
     }
@@ -318,7 +312,6 @@ hipError_t launch_linear(const LinProduct& p, void* workspace, hipStream_t s) {
     j.rows = d.rows;
     j.cols = d.cols;
     j.turn = p.dtype == LIN_F32 && d.across;
-    j.vec = low(o.p) % 16 == 0 && o.ld % 4 == 0;
     if (d.across && !j.turn) o.rows = (int)d.ld;
     j.tr = (d.rows + 63) / 64;
     j.tc = (d.cols + 63) / 64;

@@ -109,7 +109,20 @@ struct LinVec {                                          // 16 bytes
     }
   }
 };
-
+// Four neighbouring values of a matrix as they are, aligned to themselves alone (a row of an odd stride starts anywhere): the
+// types say so, and gfx950 reads 16 or 8 bytes from such places at once.
+typedef uint32_t lin_u4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t lin_u2 __attribute__((ext_vector_type(2), aligned(2)));
+template <bool F32>
+__host__ __device__ __forceinline__ void lin_four(const void* src, size_t at, uint32_t* v) {
+  if constexpr (F32) {
+    const lin_u4 u = *reinterpret_cast<const lin_u4*>(static_cast<const uint32_t*>(src) + at);
+    v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+  } else {
+    const lin_u2 u = *reinterpret_cast<const lin_u2*>(static_cast<const uint16_t*>(src) + at);
+    v[0] = u.x & 0xffffu; v[1] = u.x >> 16; v[2] = u.y & 0xffffu; v[3] = u.y >> 16;
+  }
+}
 
 // by a type known at run time (wave-uniform)
 __device__ __forceinline__ float lin_get(int dt, const void* p, size_t i) {
