@@ -46,12 +46,22 @@ class AdamW(torch.optim.Optimizer):
         super().add_param_group(param_group)
         group = self.param_groups[-1]
         try:
+            self._minimises(group)
             self._hyper(group)
             for p in group["params"]:
                 self._check(p)
         except (TypeError, ValueError):
             self.param_groups.pop()
             raise
+
+    @staticmethod
+    def _minimises(group):
+        """torch.optim's groups may ask for steps that are not formed here."""
+        for key in ("maximize", "amsgrad"):
+            if group.get(key):
+                raise ValueError(f"a group with {key}={group[key]}: AdamW has no {key}")
+        if not group.get("decoupled_weight_decay", True) and group["weight_decay"]:
+            raise ValueError("a group of Adam's weight decay: AdamW's is decoupled from the gradient")
 
     @staticmethod
     def _hyper(group):
@@ -186,7 +196,10 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """As in torch.optim, but states keep their own dtypes (there they take the parameter's); states of
-        torch.optim.AdamW are taken over with state_bits 32.  The states must fit state_bits."""
+        torch.optim.AdamW are taken over with state_bits 32, but for those of one that maximises or is amsgrad (or of
+        Adam's weight decay), which are refused.  The states must fit state_bits."""
+        for group in state_dict["param_groups"]:
+            self._minimises(group)
         ps = [p for group in self.param_groups for p in group["params"]]
         ids = list(chain.from_iterable(g["params"] for g in state_dict["param_groups"]))
         new = {}
