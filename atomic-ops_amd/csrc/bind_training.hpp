@@ -275,7 +275,9 @@ PyObject* py_cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 // The tensors of an optimizer's groups (dicts as torch.optim's) with their states; step: those with a gradient, else
 // those with a state.  False: something is not as the kernels take it (Python makes states, casts, validates and raises).
-bool adamw_tensors(PyObject* groups, PyObject* state, int64_t bits, bool step, std::vector<gdn2_adamw_tensor>* out, std::vector<Tensor>* params) {
+// all: how many parameters the groups have.
+bool adamw_tensors(PyObject* groups, PyObject* state, int64_t bits, bool step, std::vector<gdn2_adamw_tensor>* out, std::vector<Tensor>* params,
+                   int32_t* all = nullptr) {
   static PyObject *const kAvg = PyUnicode_InternFromString("exp_avg"), *const kSq = PyUnicode_InternFromString("exp_avg_sq"),
                          *const kAvgScale = PyUnicode_InternFromString("exp_avg_scale"),
                          *const kSqScale = PyUnicode_InternFromString("exp_avg_sq_scale"),
@@ -340,6 +342,7 @@ bool adamw_tensors(PyObject* groups, PyObject* state, int64_t bits, bool step, s
       params->push_back(p);
     }
   }
+  if (all) *all = ordinal;
   return !out->empty();
 }
 
@@ -377,12 +380,13 @@ PyObject* py_adamw_unpack(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (n != 4) return PyErr_Format(PyExc_TypeError, "adamw_unpack takes 4 arguments");
   std::vector<gdn2_adamw_tensor> ts;
   std::vector<Tensor> ps;
-  if (!plain_mode() || !PyList_Check(args[2]) || !PyList_Check(args[3]) || !adamw_tensors(args[0], args[1], 8, false, &ts, &ps)) return none();
+  int32_t all = 0;
+  if (!plain_mode() || !PyList_Check(args[2]) || !PyList_Check(args[3]) || !adamw_tensors(args[0], args[1], 8, false, &ts, &ps, &all)) return none();
+  if (ts.size() != (size_t)all) return none();       // (parameters without a state)
   const c10::Device dev = ps[0].device();
   std::vector<float*> out[2];
   std::vector<Tensor> held;
   for (int k = 0; k < 2; ++k) {
-    // (every parameter has a state: then the tensors are the parameters')
     if ((size_t)PyList_GET_SIZE(args[2 + k]) != ts.size()) return none();
     for (size_t i = 0; i < ts.size(); ++i) {
       PyObject* o = PyList_GET_ITEM(args[2 + k], (Py_ssize_t)i);
