@@ -315,7 +315,20 @@ static void loss_go(const LossArgs& a, hipStream_t s) {
   const int vecs = (a.V + E - 1) / E;
   auto low = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
   const bool aligned = (low(a.logits) | low(a.dlogits)) % 16 == 0 && a.ld % E == 0 && a.V % E == 0;
-  auto wave = [&](auto k) { hipLaunchKernelGGL(k, dim3((a.rows + 3) / 4), dim3(256), 0, s, a); };
+  // (a grid has fewer than 2^32 threads, 64 of them a row: what goes beyond would be left out without an error)
+  auto wave = [&](auto k) {
+    constexpr int MOST = 1 << 25;
+    for (int r = 0; r < a.rows; r += MOST) {
+      LossArgs b = a;
+      b.rows = a.rows - r < MOST ? a.rows - r : MOST;
+      b.logits = static_cast<const typename LossVec<DT>::T*>(a.logits) + (size_t)r * a.ld;
+      b.targets = static_cast<const char*>(a.targets) + (size_t)r * a.target_bytes;
+      if (a.upstream && a.upstream_ld) b.upstream = a.upstream + r;
+      if (a.row_loss) b.row_loss = a.row_loss + r;
+      if (a.dlogits) b.dlogits = static_cast<typename LossVec<DT>::T*>(a.dlogits) + (size_t)r * a.V;
+      hipLaunchKernelGGL(k, dim3((b.rows + 3) / 4), dim3(256), 0, s, b);
+    }
+  };
   auto rows = [&](auto k, int threads) { hipLaunchKernelGGL(k, dim3(a.rows < 65536 ? a.rows : 65536), dim3(threads), 0, s, a); };
   if (aligned && vecs <= 256) {
     if (vecs <= 64) wave(loss_waves_kernel<DT, 1>);

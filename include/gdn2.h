@@ -402,7 +402,7 @@ int gdn2_linear_slope(const gdn2_slope* p, void* workspace, void* stream);
  * row (upstream_ld 1; 0: one for all).  A target outside 0 .. V-1 makes its row's loss and gradient NaN.  logits
  * (rows, V) of ld elements, dlogits contiguous of the same dtype, or NULL; loss or losses may be NULL where dlogits is
  * not.  targets int64 (GDN2_FLAG_INT64) or int32 (GDN2_FLAG_INT32).  workspace: gdn2_loss_workspace_bytes, 16-byte
- * aligned.  rows, V < 2^31. */
+ * aligned.  rows, V <= 2^30. */
 typedef struct gdn2_loss {
   int32_t rows, V, dtype, target_type, reduction, upstream_ld;
   float smoothing, z_loss;
