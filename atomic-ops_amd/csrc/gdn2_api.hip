@@ -936,6 +936,7 @@ int product_args(const gdn2_product* p, gdn2::LinProduct* a) {
     return fail(GDN2_ERR_INVALID, "pointer not aligned to its elements");
   *a = gdn2::LinProduct{p->M, p->K, p->N, p->form, p->dtype, p->out_dtype, p->bias_dtype, p->activation, (size_t)p->lda,
                         (size_t)p->ldb, p->residual ? (size_t)p->ldr : 0, p->a, p->b, p->bias, p->residual, p->y, p->z};
+  if (!gdn2::linear_fits(*a)) return fail(GDN2_ERR_UNSUPPORTED, "shape too large");
   return GDN2_OK;
 }
 int slope_args(const gdn2_slope* p, gdn2::LinSlope* a) {
@@ -1021,7 +1022,7 @@ int adamw_check(const gdn2_adamw_tensor* t, int n, int bits, bool step) {
   if (bits != 8 && bits != 32) return fail(GDN2_ERR_INVALID, "states of 8 or 32 bits");
   for (int i = 0; i < n; ++i) {
     const gdn2_adamw_tensor& x = t[i];
-    if (x.numel < 1 || x.numel >= (int64_t(1) << 43)) return fail(GDN2_ERR_INVALID, "bad tensor size");
+    if (x.numel < 1 || x.numel >= (int64_t(1) << 34)) return fail(GDN2_ERR_INVALID, "bad tensor size");
     if (!x.m || !x.v || (bits == 8 && (!x.m_scale || !x.v_scale))) return fail(GDN2_ERR_INVALID, "null state");
     if (bits == 32 && (low(x.m) | low(x.v)) % 4) return fail(GDN2_ERR_INVALID, "pointer not aligned to its elements");
     if (bits == 8 && (low(x.m_scale) | low(x.v_scale)) % 4) return fail(GDN2_ERR_INVALID, "pointer not aligned to its elements");

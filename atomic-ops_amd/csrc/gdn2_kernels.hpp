@@ -481,6 +481,7 @@ struct LinProduct {
   const void *a, *b, *bias, *residual;
   void *y, *z;
 };
+bool linear_fits(const LinProduct& p);     // whether its launches take so large a product
 size_t linear_workspace_bytes(const LinProduct& p);
 hipError_t launch_linear(const LinProduct& p, void* workspace, hipStream_t s);
 struct LinSlope {

@@ -267,6 +267,17 @@ static LinPlan lin_plan(const LinProduct& p) {
   }
   return r;
 }
+// What copies operands: a grid has fewer than 2^32 threads, 256 of them a tile of 64 x 64
+static bool lin_packs_fit(const LinProduct& p, const LinPlan& r) {
+  int64_t tiles = 0;
+  for (int b = 0; b < 2 && !r.rows && r.tile < LIN_DIRECT; ++b)
+    if (const LinSide d = lin_side(p, b); d.pack) tiles += ((int64_t)d.rows + 63) / 64 * (((int64_t)d.cols + 63) / 64);
+  return tiles < (int64_t)1 << 24;
+}
+bool linear_fits(const LinProduct& p) {
+  const int64_t m = p.M / 64 + 1, k = p.K / 64 + 1, n = p.N / 64 + 1;
+  return (m + n) * k < (int64_t)1 << 24 || lin_packs_fit(p, lin_plan(p));
+}
 static size_t lin_parts_bytes(const LinProduct& p, const LinPlan& r) { return r.parts > 1 ? up((size_t)r.parts * p.M * p.N * 4, 256) : 0; }
 
 size_t linear_workspace_bytes(const LinProduct& p) {

@@ -27,6 +27,7 @@ constexpr int OPT_CHUNK = 8192;            // elements of a workgroup of the upd
 constexpr int OPT_CHUNK8 = 2048;           // ... with states of 8 bits (bound by what it computes: many small ones)
 constexpr int OPT_NORM_CHUNK = 16384;      // ... of the norm
 constexpr int OPT_BLOCK = 256;             // elements of a scale
+constexpr int64_t OPT_GRID = (1 << 24) - 1;            // workgroups of 256 threads in a grid, which has fewer than 2^32
 constexpr int OPT_TENSORS = 200, OPT_GRADS = 200, OPT_STEPS = 200;
 
 // What a tensor's update needs beside it; written by opt_begin_kernel
@@ -448,7 +449,7 @@ static void opt_each(int n, int dtype, int bits, A at, F go) {
     const gdn2_adamw_tensor x = at(i);
     if (x.dtype != dtype) continue;
     const int64_t b = (x.numel + chunk - 1) / chunk;
-    if (a.tensors == OPT_TENSORS || blocks + b > 0x7fffffff || (a.tensors && i - first > 0x7fff)) flush();
+    if (a.tensors == OPT_TENSORS || blocks + b > OPT_GRID || (a.tensors && i - first > 0x7fff)) flush();
     if (a.tensors == 0) first = i;
     auto& o = a.t[a.tensors++];
     o.p = x.p; o.g = x.g; o.m = x.m; o.v = x.v; o.ms = x.m_scale; o.vs = x.v_scale; o.master = x.master;
@@ -482,7 +483,7 @@ hipError_t launch_adamw(const gdn2_adamw_tensor* t, int n, int bits, double max_
     for (int i = 0; i < n; ++i) {
       if (t[i].dtype != dtype) continue;
       const int64_t b = (t[i].numel + OPT_NORM_CHUNK - 1) / OPT_NORM_CHUNK;
-      if (a.tensors == OPT_GRADS || blocks + b > 0x7fffffff) flush();
+      if (a.tensors == OPT_GRADS || blocks + b > OPT_GRID) flush();
       a.g[a.tensors] = t[i].g;
       a.n[a.tensors] = t[i].numel;
       a.start[a.tensors++] = (int)blocks;

@@ -371,7 +371,8 @@ int gdn2_beam_step(const gdn2_beam* p, void* workspace, void* stream);
  * float32.  z: NULL, or (M, N) of dtype: A B + bias, rounded.  activation: GDN2_ACT_*; with GDN2_XTW
  * none, no bias and no z.  Float32 operands enter as three bfloat16 pieces each, whose sum they are but for bits below
  * 2^-133, in six products of pieces; what is left out is below 2^-22 of |a| |b|.  workspace:
- * gdn2_linear_workspace_bytes (0: none), 16-byte aligned.  M, K, N <= 2^27. */
+ * gdn2_linear_workspace_bytes (0: none), 16-byte aligned.  M, K, N <= 2^27, and operands that have to be copied (float32 ones
+ * for large tiles, rows that 16-byte accesses do not take) of fewer than 2^24 tiles of 64 x 64. */
 enum { GDN2_XW = 0, GDN2_XWT = 1, GDN2_XTW = 2 };
 enum { GDN2_ACT_NONE = 0, GDN2_ACT_SILU = 1, GDN2_ACT_GELU = 2, GDN2_ACT_GELU_TANH = 3 };
 typedef struct gdn2_product {
@@ -427,7 +428,7 @@ int gdn2_scale_rows(void* x, int dtype, int rows, int V, const float* factor, in
  * blocks of 256 elements with a float32 scale each (m_scale, v_scale): m = c |c| s, v = (c^2 s)^2, rounded to one of
  * the two neighbours at random in proportion, by a hash of element, tensor (its ordinal) and t; a block with an
  * infinity or NaN has the scale NaN.  workspace: gdn2_adamw_workspace_bytes, 16-byte aligned; the tensors
- * may have any alignment of their elements.  Tensors must not overlap. */
+ * may have any alignment of their elements, and fewer than 2^34 of them.  Tensors must not overlap. */
 typedef struct gdn2_adamw_tensor {
   void* p;
   const void* g;
