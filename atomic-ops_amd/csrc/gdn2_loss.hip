@@ -291,6 +291,7 @@ __global__ __launch_bounds__(1024) void loss_sum_kernel(LossArgs a) {
   *a.loss = (float)(a.reduction == 2 ? s / (double)max(n, 1) : s);
 }
 
+// (zeros stay zeros: a row without a gradient has none, whatever its factor, an infinity or NaN of a padded row among them)
 template <int DT>
 __global__ __launch_bounds__(256) void scale_rows_kernel(typename LossVec<DT>::T* x, int rows, int V, const float* factor, int ld) {
   using L = LossVec<DT>;
@@ -301,7 +302,10 @@ __global__ __launch_bounds__(256) void scale_rows_kernel(typename LossVec<DT>::T
       continue;
     }
     auto* p = x + (size_t)row * V;
-    for (int j = threadIdx.x; j < V; j += 256) L::put(p + j, L::one(p + j) * f);
+    for (int j = threadIdx.x; j < V; j += 256) {
+      const float v = L::one(p + j);
+      L::put(p + j, v == 0.f ? v : v * f);
+    }
   }
 }
 

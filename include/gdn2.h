@@ -415,8 +415,8 @@ typedef struct gdn2_loss {
 } gdn2_loss;
 size_t gdn2_loss_workspace_bytes(int rows);
 int gdn2_cross_entropy(const gdn2_loss* p, void* workspace, void* stream);
-/* x *= *factor or, with factor_ld 1, row i *= factor[i]; where a factor is 1 the row is left as it is.  x (rows, V)
- * contiguous. */
+/* x *= *factor or, with factor_ld 1, row i *= factor[i]; where a factor is 1 the row is left as it is, and zeros stay
+ * zeros whatever the factor.  x (rows, V) contiguous. */
 int gdn2_scale_rows(void* x, int dtype, int rows, int V, const float* factor, int factor_ld, void* stream);
 
 /* One step of AdamW over n tensors.  In 32 bits, each product and sum rounded by itself:
