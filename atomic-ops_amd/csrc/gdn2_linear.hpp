@@ -154,8 +154,12 @@ __device__ __forceinline__ float lin_act(float z) {
   else if constexpr (ACT == LIN_TANH) return z * lin_logistic(LIN_TANH_C * (z + 0.044715f * z * z * z));
   else return z;
 }
+// (far out a slope is 0 or 1 and its terms are 0 times an infinity: z goes no further than where that is so.  float16 keeps a
+// z beyond 65504 as an infinity.  NaN stays NaN.)
 template <int ACT>
 __device__ __forceinline__ float lin_slope(float z) {
+  constexpr float FAR = 1e18f;
+  z = z > FAR ? FAR : z < -FAR ? -FAR : z;
   if constexpr (ACT == LIN_SILU) {
     const float s = lin_logistic(z);
     return s * (1.f + z * (1.f - s));
