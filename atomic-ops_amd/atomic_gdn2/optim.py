@@ -2,7 +2,7 @@
 
 ``AdamW`` is a ``torch.optim.Optimizer``: parameter groups, state_dict and schedulers as there.  A step forms the
 gradients' global norm, clips by it and updates every tensor, without waiting for the GPU, so it can be captured into
-a graph (the step counts live on the GPU; lr and the others are those of the capture).
+a graph once every parameter has taken a step (the step counts live on the GPU; lr and the others are those of the capture).
 """
 from __future__ import annotations
 
@@ -89,6 +89,8 @@ class AdamW(torch.optim.Optimizer):
         """p's state, made at its first step."""
         s = self.state[p]
         if not s:
+            if torch.cuda.is_current_stream_capturing():        # (each replay would begin with the states anew)
+                raise RuntimeError("a parameter's first step makes its state: take one before a step is captured")
             f32 = lambda n: torch.zeros(n, dtype=torch.float32, device=p.device)  # noqa: E731
             s["step"] = f32(())
             if self.state_bits == 32:

@@ -30,3 +30,29 @@ def test_states_are_unpacked_into_a_tensor_for_each_parameter():
     opt.step()
     opt.unpack_states(*outs)
     assert all(torch.equal(a, b) for got, want in zip(outs, opt.unpack_states()) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_first_step_is_not_captured(bits):
+    """Its states would be made anew, as zeros, by every replay."""
+    ps, opt = _opt([300, 50], dt=torch.bfloat16, state_bits=bits, max_norm=1.0)
+    ps[0].grad = torch.randn_like(ps[0])
+    opt.step()
+    ps[1].grad = torch.randn_like(ps[1])
+    before = [p.detach().clone() for p in ps]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with pytest.raises(RuntimeError, match="first step"):
+        with torch.cuda.stream(s), torch.cuda.graph(torch.cuda.CUDAGraph(), stream=s):
+            opt.step()
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(before, ps)) and opt.state[ps[0]]["step"].item() == 1 and not opt.state[ps[1]]
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(s), torch.cuda.graph(graph, stream=s):
+        opt.step()
+    torch.cuda.current_stream().wait_stream(s)
+    for _ in range(3):
+        graph.replay()
+    assert [opt.state[p]["step"].item() for p in ps] == [5, 4]
