@@ -81,7 +81,7 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"AdamW needs dense tensors on a ROCm device, got {p.layout} on {p.device}")
         if not p.is_contiguous():
             raise ValueError(f"parameters must be contiguous, got strides {p.stride()} for {tuple(p.shape)}")
-        dev = self.param_groups[0]["params"][0].device
+        dev = next(q.device for group in self.param_groups for q in group["params"])       # (a group may be empty)
         if p.device != dev:
             raise ValueError(f"parameters must be on one device, got {p.device} and {dev}")
 

@@ -56,3 +56,24 @@ def test_a_first_step_is_not_captured(bits):
     for _ in range(3):
         graph.replay()
     assert [opt.state[p]["step"].item() for p in ps] == [5, 4]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_an_empty_group_comes_first(bits):
+    """(as where parameters are split by their decay and one side has none)"""
+    from atomic_gdn2.optim import AdamW
+    ps, one = _opt([300, 50], seed=1, state_bits=bits)
+    qs, _ = _opt([300, 50], seed=1)
+    two = AdamW([{"params": [], "weight_decay": 0.0}, {"params": qs}], lr=1e-2, state_bits=bits)
+    for p, q in zip(ps, qs):
+        p.grad = torch.randn_like(p)
+        q.grad = p.grad.clone()
+    one.step(), two.step(), two.step(), one.step()
+    assert all(torch.equal(p, q) for p, q in zip(ps, qs))
+    if bits == 8:
+        assert all(torch.equal(a, b) for got, want in zip(two.unpack_states(), one.unpack_states()) for a, b in zip(got, want))
+    with pytest.raises(ValueError, match="device"):
+        two.add_param_group({"params": [torch.nn.Parameter(torch.zeros(3))]})
+    assert len(two.param_groups) == 2
+    three = AdamW([{"params": []}])
+    three.add_param_group({"params": qs})
