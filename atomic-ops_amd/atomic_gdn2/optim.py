@@ -25,7 +25,8 @@ class AdamW(torch.optim.Optimizer):
     params: tensors or groups, float32, bfloat16 or float16 in any mixture, contiguous, on one ROCm device; 16-bit ones
     are updated as a float32 ``master`` in their state and rounded (values written into one between steps count, and
     its master starts anew from them).  max_norm: every gradient times max_norm /
-    max(norm, max_norm) (None: as it is); ``norm`` is then the last step's norm, a float32 scalar on the GPU.
+    max(norm, max_norm) (None: as it is); ``norm`` is then the last step's norm, a float32 scalar on the GPU (0 where
+    there was no gradient).
     state_bits: 32, or 8: ``exp_avg`` and ``exp_avg_sq`` as codes of one byte, with a scale for each 256 elements
     (include/gdn2.h, gdn2_adamw); ``unpack_states`` gives the values that they stand for.  A NaN or infinity in a
     gradient goes into what is formed from it, with max_norm into everything."""
@@ -149,6 +150,8 @@ class AdamW(torch.optim.Optimizer):
                     todo.append((p, p.grad.to(p.dtype).contiguous(), self._state(p), ordinal, hyper))
                 ordinal += 1
         if not todo:
+            dev = next((p.device for group in self.param_groups for p in group["params"]), None)
+            self.norm = None if self.max_norm is None or dev is None else torch.zeros((), dtype=torch.float32, device=dev)
             return loss
         dev = todo[0][0].device
         ts = (_lib.Gdn2AdamwTensor * len(todo))()

@@ -77,3 +77,23 @@ def test_an_empty_group_comes_first(bits):
     assert len(two.param_groups) == 2
     three = AdamW([{"params": []}])
     three.add_param_group({"params": qs})
+
+
+def test_norm_of_no_gradients():
+    """A step without a gradient has the norm 0, not that of the step before."""
+    ps, opt = _opt([300, 50], max_norm=1.0)
+    ps[0].grad = torch.ones_like(ps[0])
+    opt.step()
+    assert opt.norm.item() > 17
+    opt.zero_grad()
+    before = [p.detach().clone() for p in ps]
+    opt.step()
+    assert opt.norm.item() == 0.0 and opt.norm.dtype == torch.float32 and opt.norm.shape == () and opt.norm.is_cuda
+    assert all(torch.equal(a, b) for a, b in zip(before, ps)) and opt.state[ps[0]]["step"].item() == 1
+    qs, other = _opt([300])
+    other.step()
+    assert other.norm is None
+    from atomic_gdn2.optim import AdamW
+    empty = AdamW([{"params": []}], max_norm=1.0)
+    empty.step()
+    assert empty.norm is None
