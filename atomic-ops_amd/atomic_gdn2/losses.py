@@ -57,8 +57,13 @@ class _CrossEntropy(torch.autograd.Function):
         x, targets = (_saved(t, like) for t, like in zip(ctx.saved_tensors, ctx.likes))
         g = g.contiguous()
         ld = 1 if ctx.how[3] == 0 else 0
-        d, ctx.grad = ctx.grad, None
-        if d is None:           # float16, or a second pass over a kept graph
+        d = ctx.grad
+        if d is not None:
+            # (multiplied where it lies: a graph of the backward pass alone would do so at every replay)
+            with torch.cuda.device(x.device):
+                captured = torch.cuda.is_current_stream_capturing()
+            d, ctx.grad = (None, d) if captured else (d, None)
+        if d is None:           # float16, a second pass over a kept graph, or a captured one
             d = torch.empty(x.shape, dtype=x.dtype, device=x.device)
             _run(x, targets, ctx.how, None, d, g, ld)
             return d, None, None

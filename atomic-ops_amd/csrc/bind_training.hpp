@@ -194,6 +194,17 @@ Tensor loss_forward(const Tensor& x, const Tensor& targets, const LossHow& how, 
   return loss;
 }
 
+// The capture that a stream is in (0: none)
+int64_t capture_of(void* stream) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (hipStreamGetCaptureInfo(static_cast<hipStream_t>(stream), &status, &id) != hipSuccess) {
+    (void)hipGetLastError();
+    return 0;
+  }
+  return status == hipStreamCaptureStatusNone ? 0 : (int64_t)id + 1;
+}
+
 struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& targets, int64_t ignore, double e, double z, int64_t reduction) {
     // float16 gradients are formed when the factor of a scaled loss is known: without it they would underflow
@@ -201,7 +212,8 @@ struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
     const Tensor loss = loss_forward(x, targets, LossHow{ignore, e, z, reduction}, x.scalar_type() == at::kHalf ? nullptr : &d);
     ctx->save_for_backward({x, targets});
     if (d.defined()) ctx->saved_data["grad"] = d;
-    ctx->saved_data["how"] = std::vector<int64_t>{ignore, reduction, (int64_t)x.scalar_type(), (int64_t)targets.scalar_type()};
+    ctx->saved_data["how"] = std::vector<int64_t>{ignore, reduction, (int64_t)x.scalar_type(), (int64_t)targets.scalar_type(),
+                                                  capture_of(stream_of(x.device()))};
     ctx->saved_data["terms"] = std::vector<double>{e, z};
     ctx->saved_data["size"] = x.sizes().vec();
     ctx->saved_data["device"] = x.device();
@@ -216,13 +228,14 @@ struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
     const Tensor g = gs[0].contiguous();
     c10::DeviceGuard guard(dev);
     Tensor d;
-    if (const auto it = ctx->saved_data.find("grad"); it != ctx->saved_data.end()) {
+    // (the kept gradient is multiplied where it lies: a graph of the backward pass alone would do so at every replay)
+    if (const auto it = ctx->saved_data.find("grad"); it != ctx->saved_data.end() && capture_of(stream_of(dev)) == how[4]) {
       d = it->second.toTensor();
       ctx->saved_data.erase(it);
       const int64_t V = size.back();
       TORCH_CHECK(abi.scale_rows(d.data_ptr(), float_kind(dt), (int)(d.numel() / V), (int)V, f32_at(g), how[1] == 0, stream_of(dev)) == 0,
                   "gdn2_scale_rows: ", abi.last_error());
-    } else {                 // float16, or a second pass over a kept graph
+    } else {                 // float16, a second pass over a kept graph, or another capture than the forward pass's
       Tensor x = saved[0], t = saved[1];
       if (!x.defined() || x.sizes() != at::IntArrayRef(size) || x.device() != dev || x.scalar_type() != dt || !row_stride(x, size.back()))
         x = restored(x, size, dt, dev);
