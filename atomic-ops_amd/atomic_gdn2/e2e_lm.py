@@ -139,6 +139,10 @@ class CausalDepthwiseConv(nn.Module):
 lm_kernels.register_modules(Dense, CausalDepthwiseConv, RMSNorm)
 
 
+_HALF_ONLY = ("products in bfloat16 run on the HIP kernels only: float32 weights and inputs on the GPU, the HIP "
+              "operator as the mixer, no hooks, transforms or autocast")
+
+
 class GDN2Block(nn.Module):
     def __init__(self, cfg: LMConfig, kernel_fn):
         super().__init__()
@@ -162,8 +166,7 @@ class GDN2Block(nn.Module):
             return lm_kernels.block_forward(self, x, ws)
         cfg = self.cfg
         if cfg.products != "float32":
-            raise ValueError("products in bfloat16 run on the HIP kernels only: float32 weights and inputs on the GPU, the HIP "
-                             "operator as the mixer, no hooks, transforms or autocast")
+            raise ValueError(_HALF_ONLY)
         B, L, _ = x.shape
         H, D = cfg.n_heads, cfg.d_head
         eps = 1e-6
@@ -200,6 +203,8 @@ class LM(nn.Module):
             if self.cfg.products == "bfloat16":
                 return linear(h.bfloat16(), self.embed.bfloat16().t(), out_dtype=torch.float32)
             return h @ self.embed.t()
+        if self.cfg.products != "float32":
+            raise ValueError(_HALF_ONLY)
         return self.final_norm(x) @ self.embed.t()
 
 
