@@ -42,8 +42,8 @@ def _product(form, a, b, M, K, N, out, bias=None, residual=None, act=0, z=None):
                          _ld(a), _ld(b), 0 if residual is None else _ld(residual), a.data_ptr(), b.data_ptr(), _addr(bias),
                          _addr(residual), out.data_ptr(), _addr(z))
     L = _lib.lib()
-    ws = torch.empty(L.gdn2_linear_workspace_bytes(ctypes.byref(p)), dtype=torch.uint8, device=out.device)
-    with torch.cuda.device(out.device):
+    with torch.cuda.device(out.device):         # (its CUs say how a product is split)
+        ws = torch.empty(L.gdn2_linear_workspace_bytes(ctypes.byref(p)), dtype=torch.uint8, device=out.device)
         _lib.check(L.gdn2_linear(ctypes.byref(p), _lib.ptr(ws), _lib.stream_handle(out.device)), "gdn2_linear")
     return out
 
@@ -67,8 +67,8 @@ def _slope(dy, z, dtype, act, bias_dtype, need_dz):
     p = _lib.Gdn2Slope(M, N, _DTYPES[dtype], _DTYPES[dy.dtype], 0 if db is None else _DTYPES[bias_dtype], act, dy.data_ptr(), _addr(z),
                        _addr(dz), _addr(db))
     L = _lib.lib()
-    ws = torch.empty(L.gdn2_linear_slope_workspace_bytes(ctypes.byref(p)), dtype=torch.uint8, device=dy.device)
     with torch.cuda.device(dy.device):
+        ws = torch.empty(L.gdn2_linear_slope_workspace_bytes(ctypes.byref(p)), dtype=torch.uint8, device=dy.device)
         _lib.check(L.gdn2_linear_slope(ctypes.byref(p), _lib.ptr(ws), _lib.stream_handle(dy.device)), "gdn2_linear_slope")
     return dz, db
 
