@@ -73,12 +73,11 @@ def _slope(dy, z, dtype, act, bias_dtype, need_dz):
     return dz, db
 
 
-def _saved(t, like):
-    """A saved tensor as it was saved; hooks may have changed its strides, type or device."""
-    if t is None:
-        return None
-    t = t if (t.shape, t.dtype, t.device) == like else _lib.restored(t, *like)
-    return t if _turned(t) else _rows(t, t.shape[1])
+def _saved(ctx):
+    """x of whole rows, the weight of whole rows or turned, z as one array; hooks may have changed strides, types or devices."""
+    x, weight, z = (t if t is None or (t.shape, t.dtype, t.device) == like else _lib.restored(t, *like)
+                    for t, like in zip(ctx.saved_tensors, ctx.likes))
+    return _rows(x, x.shape[1]), weight if _turned(weight) else _rows(weight, weight.shape[1]), None if z is None else z.contiguous()
 
 
 class _Linear(torch.autograd.Function):
@@ -95,7 +94,7 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, weight, z = (_saved(t, like) for t, like in zip(ctx.saved_tensors, ctx.likes))
+        x, weight, z = _saved(ctx)
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
         (M, K), N, dev = x.shape, weight.shape[1], x.device
         if M == 0:
