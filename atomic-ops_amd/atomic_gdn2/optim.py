@@ -25,11 +25,12 @@ class AdamW(torch.optim.Optimizer):
     params: tensors or groups, float32, bfloat16 or float16 in any mixture, contiguous, on one ROCm device; 16-bit ones
     are updated as a float32 ``master`` in their state and rounded (values written into one between steps count, and
     its master starts anew from them).  max_norm: every gradient times max_norm /
-    max(norm, max_norm) (None: as it is); ``norm`` is then the last step's norm, a float32 scalar on the GPU (0 where
+    max(norm, max_norm) (None, or infinite: as it is); ``norm`` is then the last step's norm, a float32 scalar on the GPU (0 where
     there was no gradient).
     state_bits: 32, or 8: ``exp_avg`` and ``exp_avg_sq`` as codes of one byte, with a scale for each 256 elements
     (include/gdn2.h, gdn2_adamw); ``unpack_states`` gives the values that they stand for.  A NaN or infinity in a
-    gradient goes into what is formed from it, with max_norm into everything."""
+    gradient goes into what is formed from it (in 8 bits its block); with a finite max_norm a NaN goes into everything, and an
+    infinity makes the factor 0: NaN where it is, a step of no gradient elsewhere."""
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *,
                  max_norm=None, state_bits: int = 32):

@@ -185,8 +185,8 @@ __global__ __launch_bounds__(1024) void opt_begin_kernel(OptSteps a, const doubl
   for (int w = 1; w < 16; ++w) s += sums[w];
   s = sqrt(s);
   if (norm) *norm = (float)s;
-  // (a norm that is not a number is not below max_norm)
-  *coef = max_norm > 0.0 && !(s < max_norm) ? (float)(max_norm / s) : 1.f;
+  // (a norm that is not a number is not below max_norm; an infinite max_norm scales nothing, whatever the norm)
+  *coef = max_norm > 0.0 && max_norm < INFINITY && !(s < max_norm) ? (float)(max_norm / s) : 1.f;
 }
 
 struct OptState {

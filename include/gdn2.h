@@ -423,7 +423,8 @@ int gdn2_scale_rows(void* x, int dtype, int rows, int V, const float* factor, in
  *   t = ++*step;  g' = c g;  m = beta1 m + (1 - beta1) g';  v = beta2 v + (1 - beta2) g' g';
  *   p = p (1 - lr weight_decay) - m / (sqrt(v) / sqrt(1 - beta2^t) + eps) * (lr / (1 - beta1^t)),
  * c = max_norm / max(norm, max_norm), norm the square root of the sum of the squares of all gradients, summed in 64
- * bits (max_norm <= 0: c = 1; norm is written only where it is asked for).  A tensor of 16 bits is formed from, and
+ * bits (max_norm <= 0 or infinite: c = 1; norm is written only where it is asked for; an infinite one makes c 0, a NaN makes c
+ * NaN).  A tensor of 16 bits is formed from, and
  * kept as, its float32 master, and rounded (where p is not the master's rounding, p itself is what is updated).  bits 32: m and v are float32.  bits 8: m (int8) and v (uint8) are codes of
  * blocks of 256 elements with a float32 scale each (m_scale, v_scale): m = c |c| s, v = (c^2 s)^2, rounded to one of
  * the two neighbours at random in proportion, by a hash of element, tensor (its ordinal) and t; a block with an

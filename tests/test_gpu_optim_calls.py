@@ -97,3 +97,52 @@ def test_norm_of_no_gradients():
     empty = AdamW([{"params": []}], max_norm=1.0)
     empty.step()
     assert empty.norm is None
+
+
+def _set_bad(p, at, value):
+    p.grad = torch.linspace(-1, 1, p.numel(), device="cuda")
+    p.grad[at] = value
+
+
+def _bad(n, at, bits):
+    want = torch.zeros(n, dtype=torch.bool, device="cuda")
+    want[slice(at // 256 * 256, at // 256 * 256 + 256) if bits == 8 else at] = True
+    return want
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_an_infinite_gradient_makes_the_factor_0(bits):
+    """max_norm / infinity: NaN where 0 times the infinity is, a step of no gradient everywhere else."""
+    ps, opt = _opt([1000, 700], max_norm=1.0, state_bits=bits)
+    qs, ref = _opt([1000, 700], max_norm=1.0, state_bits=bits)
+    _set_bad(ps[0], 600, float("inf"))
+    ps[1].grad = torch.ones_like(ps[1])
+    for q in qs:
+        q.grad = torch.zeros_like(q)
+    opt.step(), ref.step()
+    assert opt.norm.item() == float("inf")
+    one = torch.zeros(1000, dtype=torch.bool, device="cuda")
+    one[600] = True
+    assert torch.equal(torch.isnan(ps[0].detach()), one)
+    assert torch.equal(ps[0].detach()[~one], qs[0].detach()[~one]) and torch.equal(ps[1], qs[1])
+    _set_bad(ps[0], 600, 0.0)
+    opt.step()
+    assert torch.equal(torch.isnan(ps[0].detach()), _bad(1000, 600, bits)) and torch.isfinite(ps[1].detach()).all()
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_an_infinite_max_norm_scales_nothing(bits, value):
+    """The norm is formed, infinite or not a number, and every other element steps as without max_norm."""
+    ps, opt = _opt([1000, 700], max_norm=float("inf"), state_bits=bits)
+    qs, ref = _opt([1000, 700], state_bits=bits)
+    for a, b in (ps, qs):
+        _set_bad(a, 600, value)
+        b.grad = torch.ones_like(b)
+    for _ in range(2):
+        opt.step(), ref.step()
+    assert str(opt.norm.item()) == str(value)
+    for p, q in zip(ps, qs):
+        assert torch.equal(torch.isnan(p.detach()), torch.isnan(q.detach()))
+        assert torch.equal(p.detach().nan_to_num(), q.detach().nan_to_num())
+    assert torch.equal(~torch.isfinite(ps[0].detach()), _bad(1000, 600, bits)) and torch.isfinite(ps[1].detach()).all()
