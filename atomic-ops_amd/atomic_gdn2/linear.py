@@ -2,9 +2,9 @@
 
 ``linear`` computes y = act(x W + bias) + residual in one pass behind the product: float32, bfloat16 or float16 rows,
 one (a token) or thousands (a batch).  W is (in, out), as ``e2e_lm.Dense`` holds it, or a transposed view of an
-(out, in) matrix (a tied embedding), read as it lies.  Sums are float32 and y is rounded once; float32 operands enter as
-three bfloat16 pieces each (entries below 1e-33 lose their bits below 2^-133), which keeps float32's precision at the
-rate of the 16-bit matrix cores.
+(out, in) matrix (a tied embedding), read as it lies.  Sums are float32 and y is rounded once.  float32 operands of
+larger products enter as three bfloat16 pieces each (entries below 1e-33 lose their bits below 2^-133): what the six
+products of pieces leave out is below 2^-21 of |x| |W|, towards zero, at the rate of the 16-bit matrix cores.
 """
 from __future__ import annotations
 
@@ -125,7 +125,8 @@ def linear(x, weight, bias=None, residual=None, activation=None, out_dtype=None)
     to out_dtype.  activation: None, "silu", "gelu" (z Phi(z)) or "gelu_tanh".  x and residual may be rows of wider
     matrices.  Gradients of all four, each summed in float32 and in its tensor's dtype; with an activation
     z = x W + bias is kept for them in x's dtype, and the gradient of z has x's dtype.  Once differentiable.  A row
-    of x with an infinity or NaN gives nothing finite in float32, and touches no other row."""
+    of x with an infinity or NaN gives nothing finite in float32 (an infinity may come out as NaN: larger float32 products
+    take it in pieces), and touches no other row."""
     if activation in _ACTS and isinstance(x, torch.Tensor) and x.is_cuda and out_dtype in (None, x.dtype, torch.float32):
         # plain calls (csrc/bind.cpp) go native; None = not one, and what follows handles it
         y = _lib.bind().linear(x, weight, bias, residual, _ACTS[activation], out_dtype is torch.float32)

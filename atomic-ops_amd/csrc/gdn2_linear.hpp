@@ -270,7 +270,9 @@ __device__ __forceinline__ float4 lin_floats(const char* lds, int t, int s) {
     return *reinterpret_cast<const float4*>(lds + row * 128 + (((4 * s + c) ^ (row & 7)) << 4));
   }
 }
-// Both s of a tile as the three pieces of the whole block's operand
+// Both s of a tile as the three pieces of the whole block's operand, each the next eight bits.  The pieces behind the first are
+// below 2^-7 and 2^-15 of the value, so the three products of pieces that are not formed are below 2^-21 of a product, and of its
+// sign.  (An infinity leaves NaN.)
 template <bool R, int ROWS>
 __device__ __forceinline__ void lin_cut(const char* lds, int t, s8& hi, s8& mid, s8& lo) {
   const float4 x = lin_floats<R, ROWS>(lds, t, 0), y = lin_floats<R, ROWS>(lds, t, 1);

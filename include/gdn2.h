@@ -369,8 +369,9 @@ int gdn2_beam_step(const gdn2_beam* p, void* workspace, void* stream);
  *   GDN2_XTW  a (K, M), b (K, N): the weight's gradient, x^T dz.
  * dtype: of a and b; out_dtype, of y and residual (rows of ldr): dtype or float32; bias (N): bias_dtype, dtype or
  * float32.  z: NULL, or (M, N) of dtype: A B + bias, rounded.  activation: GDN2_ACT_*; with GDN2_XTW
- * none, no bias and no z.  Float32 operands enter as three bfloat16 pieces each, whose sum they are but for bits below
- * 2^-133, in six products of pieces; what is left out is below 2^-22 of |a| |b|.  workspace:
+ * none, no bias and no z.  Float32 operands of small products and of up to 8 rows enter as they are; larger products take
+ * each as three bfloat16 pieces, whose sum it is but for bits below 2^-133, in six products of pieces: what is left out is
+ * below 2^-21 of |a| |b|, always towards zero, and an infinity becomes NaN.  workspace:
  * gdn2_linear_workspace_bytes (0: none), 16-byte aligned.  M, K, N <= 2^27, and operands that have to be copied (float32 ones
  * for large tiles, rows that 16-byte accesses do not take) of fewer than 2^24 tiles of 64 x 64. */
 enum { GDN2_XW = 0, GDN2_XWT = 1, GDN2_XTW = 2 };
