@@ -146,6 +146,8 @@ def linear(x, weight, bias=None, residual=None, activation=None, out_dtype=None)
     K, N = weight.shape
     if x.dim() == 0 or x.shape[-1] != K:
         raise ValueError(f"x must be (..., {K}), got {tuple(x.shape)}")
+    if max(x.numel() // K, K, N) > 2 ** 27:
+        raise ValueError(f"a product of {x.numel() // K} x {K} x {N}: up to 2^27 each are supported")
     shape = (*x.shape[:-1], N)
     if bias is not None and tuple(bias.shape) != (N,):
         raise ValueError(f"bias must be ({N},), got {tuple(bias.shape)}")

@@ -97,6 +97,8 @@ def cross_entropy(logits, targets, ignore_index: int = -100, label_smoothing: fl
         raise TypeError(f"targets must be whole numbers, got {targets.dtype}")
     if logits.dim() < 1 or logits.numel() == 0 or tuple(targets.shape) != tuple(logits.shape[:-1]):
         raise ValueError(f"logits must be (..., V), not empty, and targets (...), got {tuple(logits.shape)} and {tuple(targets.shape)}")
+    if max(targets.numel(), logits.shape[-1]) > 2 ** 30:
+        raise ValueError(f"{targets.numel()} rows of {logits.shape[-1]}: up to 2^30 each are supported")
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {', '.join(map(repr, _REDUCTIONS))}, got {reduction!r}")
     if not 0.0 <= label_smoothing <= 1.0:
