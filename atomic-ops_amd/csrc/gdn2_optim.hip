@@ -18,7 +18,8 @@
 // largest keep codes of their own (m 12.7, sqrt(v) 25.5).  A value between two codes takes the upper one with the
 // probability that keeps its mean: rounded to the nearest, v would never decay, since a step takes 0.1 % of it, less than
 // half of any code's distance.  (v above 0 takes code 1 at least: with 0 the update would be m / eps.)  The step itself
-// uses m and v as formed, in 32 bits.  Bound by what it computes: 4.2 M elements 25 us, 2.7 TB/s.
+// uses m and v as formed, in 32 bits.  Bound by what it computes: 4.2 M elements 27 us, 2.5 TB/s (25 with codes off by one beside
+// a border, from the hardware's quotient and root alone; 30 with correctly rounded ones formed where they are near).
 #include "gdn2_optim.hpp"
 
 namespace gdn2 {
@@ -265,19 +266,40 @@ __device__ __forceinline__ uint32_t opt_hash(uint32_t x) {
   return x ^ (x >> 16);
 }
 __device__ __forceinline__ float opt_dither(uint32_t bits) { return ((float)bits + 0.5f) * (1.f / 65536.f); }
-// The codes below and above a value are found by the hardware's square root (error below 2^-22, 3e-5 of a code): where that
-// takes the neighbour below a code's own value, the value lies at the very end of the interval, and the comparison gives the
-// same code from either side (the dither keeps 7e-6 from 0 and 1).  inv: 1 / s, or 0 where there is no code.  (A scale whose
-// inverse is no float32 number is divided by.)
-__device__ __forceinline__ int opt_m_code(float m, float s, float inv, float r) {
+// floor(sqrt(x / s)) as correctly rounded division and root give it: a code turns on it where a value lies at a code's own, and
+// most do, since a step moves v by a thousandth and its scale with it.  The quotient by the inverse is within two units of the
+// last place; its remainder (exact) corrects it, twice, and it is the rounded one.  Its root rounds to the whole number n or beyond
+// where it is above n^2 - n u, u the distance of the number below n ((n - u / 2)^2 is between the two, and no quotient).
+__device__ __forceinline__ float opt_floor_root(float x, float s, float inv) {
 #pragma clang fp contract(off)
-  const float a = fabsf(m), q = inv < INFINITY ? a * inv : a / s, c = fminf(floorf(__builtin_amdgcn_sqrtf(q)), 126.f), low = c * c * s, high = (c + 1.f) * (c + 1.f) * s;
+  float q = x * inv;
+  q = fmaf(fmaf(-q, s, x), inv, q);
+  q = fmaf(fmaf(-q, s, x), inv, q);
+  const float n = fmaxf(rintf(__builtin_amdgcn_sqrtf(q)), 1.f), u = __uint_as_float((__float_as_uint(n) - 1) & 0x7f800000u) * 0x1p-23f;
+  return fmaf(n, u, fmaf(-n, n, q)) > 0.f ? n : n - 1.f;
+}
+// ... of four values; inv: 1 / s, or 0 where there is no code
+__device__ __forceinline__ void opt_roots(const float* x, float s, float inv, float* root) {
+#pragma clang fp contract(off)
+  const float all = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(s)));      // (the wave's)
+  if (all < 0x1p-100f) {                   // (remainders would be cut)
+#pragma unroll 1
+    for (int e = 0; e < 4; ++e) root[e] = floorf(sqrtf(x[e] / s));
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) root[e] = opt_floor_root(x[e], s, inv);
+}
+// root: floor(sqrt(|m| / s)), floor(sqrt(u / s))
+__device__ __forceinline__ int opt_m_code(float m, float s, float inv, float root, float r) {
+#pragma clang fp contract(off)
+  const float a = fabsf(m), c = fminf(root, 126.f), low = c * c * s, high = (c + 1.f) * (c + 1.f) * s;
   const int k = inv > 0.f ? (int)c + (a - low > r * (high - low)) : 0;
   return m < 0.f ? -k : k;
 }
-__device__ __forceinline__ int opt_v_code(float v, float u, float s, float inv, float r) {
+__device__ __forceinline__ int opt_v_code(float v, float s, float inv, float root, float r) {
 #pragma clang fp contract(off)
-  const float q = inv < INFINITY ? u * inv : u / s, c = fminf(floorf(__builtin_amdgcn_sqrtf(q)), 254.f);
+  const float c = fminf(root, 254.f);
   float low = c * c * s, high = (c + 1.f) * (c + 1.f) * s;
   low = low * low;
   high = high * high;
@@ -359,11 +381,16 @@ __global__ __launch_bounds__(256) void opt_update8_kernel(OptTensors a, const fl
     v_top = opt_wave_max(v_top);
     const float new_m = m_top * (1.f / 16129.f), new_v = sqrtf(v_top) * (1.f / 65025.f);
     const float inv_m = new_m > 0.f ? 1.f / new_m : 0.f, inv_v = new_v > 0.f ? 1.f / new_v : 0.f;
+    float am[4], rm[4], rv[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) am[e] = fabsf(mx[e]);
+    opt_roots(am, new_m, inv_m, rm);
+    opt_roots(ux, new_v, inv_v, rv);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const uint32_t r = opt_hash((uint32_t)(j + e) * 0x9E3779B1u + h.hash);
-      cm[e] = opt_m_code(mx[e], new_m, inv_m, opt_dither(r & 0xffffu));
-      cv[e] = opt_v_code(vx[e], ux[e], new_v, inv_v, opt_dither(r >> 16));
+      cm[e] = opt_m_code(mx[e], new_m, inv_m, rm[e], opt_dither(r & 0xffffu));
+      cv[e] = opt_v_code(vx[e], new_v, inv_v, rv[e], opt_dither(r >> 16));
     }
     if (vec) {
       if constexpr (DT != LIN_F32) OptType<LIN_F32>::put4(w, px);
