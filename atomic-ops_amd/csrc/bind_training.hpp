@@ -37,12 +37,21 @@ bool product(int form, int64_t M, int64_t K, int64_t N, const Tensor& a, int64_t
   p.dtype = float_kind(a.scalar_type());
   p.out_dtype = float_kind(y.scalar_type());
   p.bias_dtype = bias.defined() ? float_kind(bias.scalar_type()) : 0;
-  p.activation = act; p.lda = lda; p.ldb = ldb; p.ldr = ldr;
+  p.activation = act | (z.defined() && z.scalar_type() == at::kFloat ? GDN2_Z_F32 : 0); p.lda = lda; p.ldb = ldb; p.ldr = ldr;
   p.a = a.data_ptr(); p.b = b.data_ptr(); p.bias = at_of(bias); p.residual = at_of(res);
   p.y = y.data_ptr(); p.z = at_of(z);
   const int64_t bytes = (int64_t)abi.linear_ws(&p);
   const Tensor ws = bytes ? empty_on(y, {bytes}, at::kByte) : Tensor();
   return abi.linear(&p, at_of(ws), stream_of(y.device())) == 0;
+}
+
+// Whether the gradients of a product of 16 bits are formed from dz and what its rounding leaves out, and what z is kept in
+// (linear.py, _fine and _z_dtype)
+bool fine_gradients(int64_t M, int64_t K, int64_t N, at::ScalarType dt) {
+  return dt != at::kFloat && 2.0 * (double)M * (double)K * (double)N <= GDN2_LINEAR_FINE;
+}
+at::ScalarType z_type(int64_t M, int64_t K, int64_t N, at::ScalarType dt) {
+  return fine_gradients(M, K, N, dt) || M * N <= GDN2_LINEAR_Z ? at::kFloat : dt;
 }
 
 // x (..., in) of whole rows, w (in, out) of whole rows or turned; throws Refused
@@ -52,7 +61,7 @@ Tensor linear_forward(const Tensor& x, const Tensor& w, const Tensor& bias, cons
   at::DimVector size(x.sizes());
   size.back() = N;
   const Tensor y = empty_on(x, size, f32 ? at::kFloat : x.scalar_type());
-  if (z) *z = empty_on(x, {M, N}, x.scalar_type());
+  if (z) *z = empty_on(x, {M, N}, z_type(M, K, N, x.scalar_type()));
   const bool t = turned(w);
   if (!product(t ? GDN2_XWT : GDN2_XW, M, K, N, x, row_stride(x, K), w, t ? ld_of(w.t()) : ld_of(w), y, (int)act, bias, res,
                res.defined() ? row_stride(res, N) : 0, z ? *z : Tensor()))
@@ -80,25 +89,26 @@ struct Linear : torch::autograd::Function<Linear> {
     const int64_t act = conf[0], K = wsz[0], N = wsz[1];
     const at::ScalarType dt = (at::ScalarType)conf[3];
     Tensor x = saved[0], w = saved[1], z = saved[2];
-    auto kept = [&](const Tensor& t, at::IntArrayRef size) { return t.defined() && t.sizes() == size && t.device() == dev && t.scalar_type() == dt; };
-    if (!kept(x, xs) || !row_stride(x, K)) x = restored(x, xs, dt, dev);
-    if (!kept(w, wsz) || !(turned(w) || whole_rows(w))) w = restored(w, wsz, dt, dev);
+    auto kept = [&](const Tensor& t, at::IntArrayRef size, at::ScalarType dt) { return t.defined() && t.sizes() == size && t.device() == dev && t.scalar_type() == dt; };
+    if (!kept(x, xs, dt) || !row_stride(x, K)) x = restored(x, xs, dt, dev);
+    if (!kept(w, wsz, dt) || !(turned(w) || whole_rows(w))) w = restored(w, wsz, dt, dev);
     const int64_t M = x.numel() / K;
-    if (act && (!kept(z, {M, N}) || !z.is_contiguous())) z = restored(z, {M, N}, dt, dev);
+    const at::ScalarType zt = z_type(M, K, N, dt);
+    if (act && (!kept(z, {M, N}, zt) || !z.is_contiguous())) z = restored(z, {M, N}, zt, dev);
     size_t edge = 2;
     const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
     const bool need_b = conf[1] >= 0 && ctx->needs_input_grad(edge++), need_r = conf[2] && ctx->needs_input_grad(edge);
     const Tensor dy = gs[0].contiguous();
     c10::DeviceGuard guard(dev);
     Tensor dz = dy, dx, dw, db;
-    const bool own = (act || dy.scalar_type() != dt) && (need_x || need_w);
+    const bool own = (act || dy.scalar_type() != dt) && (need_x || need_w), fine = own && fine_gradients(M, K, N, dt);
     if (own || need_b) {
-      if (own) dz = empty_on(x, {M, N}, dt);
+      if (own) dz = empty_on(x, {fine ? 2 * M : M, N}, dt);
       if (need_b) db = empty_on(x, {N}, (at::ScalarType)conf[1]);
       gdn2_slope s{};
       s.M = (int32_t)M; s.N = (int32_t)N; s.dtype = float_kind(dt); s.dy_dtype = float_kind(dy.scalar_type());
       s.bias_dtype = need_b ? float_kind((at::ScalarType)conf[1]) : 0;
-      s.activation = (int32_t)act;
+      s.activation = (int32_t)act | (zt == at::kFloat ? GDN2_Z_F32 : 0) | (fine ? GDN2_DZ_LOW : 0);
       s.dy = dy.data_ptr(); s.z = act ? z.data_ptr() : nullptr; s.dz = own ? dz.data_ptr() : nullptr; s.dbias = at_of(db);
       const int64_t bytes = (int64_t)abi.slope_ws(&s);
       const Tensor ws = bytes ? empty_on(x, {bytes}, at::kByte) : Tensor();
@@ -108,11 +118,18 @@ struct Linear : torch::autograd::Function<Linear> {
     bool ok = true;
     if (need_x) {
       dx = empty_on(x, x.sizes(), dt);
-      ok = product(t ? GDN2_XW : GDN2_XWT, M, N, K, dz, N, w, t ? ld_of(w.t()) : ld_of(w), dx);
+      ok = product((t ? GDN2_XW : GDN2_XWT) | (fine ? GDN2_HALVES : 0), M, N, K, dz, N, w, t ? ld_of(w.t()) : ld_of(w), dx);
     }
     if (ok && need_w) {
       dw = empty_on(x, t ? at::IntArrayRef{N, K} : at::IntArrayRef{K, N}, dt);
-      ok = t ? product(GDN2_XTW, N, M, K, dz, N, x, row_stride(x, K), dw) : product(GDN2_XTW, K, M, N, x, row_stride(x, K), dz, N, dw);
+      int64_t rows = M;
+      if (fine) {            // (x^T dz is a sum over the rows: over those of both)
+        at::NoGradGuard off;
+        const Tensor r = x.dim() == 2 ? x : x.view({M, K});
+        x = at::cat({r, r});
+        rows = 2 * M;
+      }
+      ok = t ? product(GDN2_XTW, N, rows, K, dz, N, x, row_stride(x, K), dw) : product(GDN2_XTW, K, rows, N, x, row_stride(x, K), dz, N, dw);
       if (t) dw = dw.t();
     }
     TORCH_CHECK(ok, "gdn2_linear: ", abi.last_error());

@@ -918,24 +918,27 @@ uintptr_t size_of(int t) { return t == GDN2_F32 ? 4 : 2; }
 int product_args(const gdn2_product* p, gdn2::LinProduct* a) {
   if (!p) return fail(GDN2_ERR_INVALID, "null argument block");
   if (p->M < 1 || p->K < 1 || p->N < 1) return fail(GDN2_ERR_INVALID, "non-positive shape");
-  if (p->M > kMaxSide || p->K > kMaxSide || p->N > kMaxSide) return fail(GDN2_ERR_UNSUPPORTED, "shape too large");
-  if (((int64_t)p->M / 64 + 1) * ((int64_t)p->N / 64 + 1) >= (int64_t(1) << 31) || ((int64_t)p->M / 64 + 1) * ((int64_t)p->K / 64 + 1) >= (int64_t(1) << 30) ||
+  const bool halves = p->form == (GDN2_XW | GDN2_HALVES) || p->form == (GDN2_XWT | GDN2_HALVES), z_f32 = p->activation & GDN2_Z_F32;
+  const int form = halves ? p->form & ~GDN2_HALVES : p->form, act = p->activation & ~GDN2_Z_F32;
+  if (p->M > (halves ? kMaxSide / 2 : kMaxSide) || p->K > kMaxSide || p->N > kMaxSide) return fail(GDN2_ERR_UNSUPPORTED, "shape too large");
+  const int M = halves ? 2 * p->M : p->M;
+  if (((int64_t)M / 64 + 1) * ((int64_t)p->N / 64 + 1) >= (int64_t(1) << 31) || ((int64_t)M / 64 + 1) * ((int64_t)p->K / 64 + 1) >= (int64_t(1) << 30) ||
       ((int64_t)p->K / 64 + 1) * ((int64_t)p->N / 64 + 1) >= (int64_t(1) << 30))
     return fail(GDN2_ERR_UNSUPPORTED, "shape too large");
-  if (p->form < GDN2_XW || p->form > GDN2_XTW) return fail(GDN2_ERR_INVALID, "unknown form");
+  if (form < GDN2_XW || form > GDN2_XTW) return fail(GDN2_ERR_INVALID, "unknown form");
   if (!float_type(p->dtype) || (p->out_dtype != p->dtype && p->out_dtype != GDN2_F32) ||
       (p->bias && p->bias_dtype != p->dtype && p->bias_dtype != GDN2_F32))
     return fail(GDN2_ERR_INVALID, "unknown dtype");
-  if (p->activation < GDN2_ACT_NONE || p->activation > GDN2_ACT_GELU_TANH) return fail(GDN2_ERR_INVALID, "unknown activation");
-  if (p->form == GDN2_XTW && (p->activation || p->bias || p->z)) return fail(GDN2_ERR_UNSUPPORTED, "bias and activation belong to a layer's own product");
-  const int64_t ca = p->form == GDN2_XTW ? p->M : p->K, cb = p->form == GDN2_XWT ? p->K : p->N;
+  if (act < GDN2_ACT_NONE || act > GDN2_ACT_GELU_TANH) return fail(GDN2_ERR_INVALID, "unknown activation");
+  if (form == GDN2_XTW && (act || p->bias || p->z)) return fail(GDN2_ERR_UNSUPPORTED, "bias and activation belong to a layer's own product");
+  const int64_t ca = form == GDN2_XTW ? p->M : p->K, cb = form == GDN2_XWT ? p->K : p->N;
   if (p->lda < ca || p->ldb < cb || (p->residual && p->ldr < p->N)) return fail(GDN2_ERR_INVALID, "row stride below the row");
   if (!p->a || !p->b || !p->y) return fail(GDN2_ERR_INVALID, "null pointer");
-  if ((low(p->a) | low(p->b) | low(p->z)) % size_of(p->dtype) || (low(p->y) | low(p->residual)) % size_of(p->out_dtype) ||
-      low(p->bias) % size_of(p->bias_dtype))
+  if ((low(p->a) | low(p->b)) % size_of(p->dtype) || low(p->z) % (z_f32 ? 4 : size_of(p->dtype)) ||
+      (low(p->y) | low(p->residual)) % size_of(p->out_dtype) || low(p->bias) % size_of(p->bias_dtype))
     return fail(GDN2_ERR_INVALID, "pointer not aligned to its elements");
-  *a = gdn2::LinProduct{p->M, p->K, p->N, p->form, p->dtype, p->out_dtype, p->bias_dtype, p->activation, (size_t)p->lda,
-                        (size_t)p->ldb, p->residual ? (size_t)p->ldr : 0, p->a, p->b, p->bias, p->residual, p->y, p->z};
+  *a = gdn2::LinProduct{M, p->K, p->N, form, p->dtype, p->out_dtype, p->bias_dtype, act, (size_t)p->lda,
+                        (size_t)p->ldb, p->residual ? (size_t)p->ldr : 0, p->a, p->b, p->bias, p->residual, p->y, p->z, z_f32, halves};
   if (!gdn2::linear_fits(*a)) return fail(GDN2_ERR_UNSUPPORTED, "shape too large");
   return GDN2_OK;
 }
@@ -946,11 +949,16 @@ int slope_args(const gdn2_slope* p, gdn2::LinSlope* a) {
   if (!float_type(p->dtype) || (p->dy_dtype != p->dtype && p->dy_dtype != GDN2_F32) ||
       (p->dbias && p->bias_dtype != p->dtype && p->bias_dtype != GDN2_F32))
     return fail(GDN2_ERR_INVALID, "unknown dtype");
-  if (p->activation < GDN2_ACT_NONE || p->activation > GDN2_ACT_GELU_TANH) return fail(GDN2_ERR_INVALID, "unknown activation");
-  if (!p->dy || (p->activation && !p->z) || (!p->dz && !p->dbias)) return fail(GDN2_ERR_INVALID, "null pointer");
-  if ((low(p->z) | low(p->dz)) % size_of(p->dtype) || low(p->dy) % size_of(p->dy_dtype) || low(p->dbias) % size_of(p->bias_dtype))
+  const int act = p->activation & ~(GDN2_Z_F32 | GDN2_DZ_LOW);
+  const int z_dtype = p->activation & GDN2_Z_F32 ? (int)GDN2_F32 : p->dtype;
+  const bool rest = p->activation & GDN2_DZ_LOW;
+  if (act < GDN2_ACT_NONE || act > GDN2_ACT_GELU_TANH) return fail(GDN2_ERR_INVALID, "unknown activation");
+  if (!p->dy || (act && !p->z) || (!p->dz && !p->dbias)) return fail(GDN2_ERR_INVALID, "null pointer");
+  if (rest && (!p->dz || p->dtype == GDN2_F32)) return fail(GDN2_ERR_INVALID, "what rounding leaves out of a dz of 16 bits");
+  if (low(p->z) % size_of(z_dtype) || low(p->dz) % size_of(p->dtype) || low(p->dy) % size_of(p->dy_dtype) ||
+      low(p->dbias) % size_of(p->bias_dtype))
     return fail(GDN2_ERR_INVALID, "pointer not aligned to its elements");
-  *a = gdn2::LinSlope{p->M, p->N, p->dtype, p->dy_dtype, p->bias_dtype, p->activation, p->dy, p->z, p->dz, p->dbias};
+  *a = gdn2::LinSlope{p->M, p->N, p->dtype, p->dy_dtype, p->bias_dtype, act, p->dy, p->z, p->dz, p->dbias, z_dtype, rest};
   return GDN2_OK;
 }
 }  // namespace

@@ -480,6 +480,7 @@ struct LinProduct {
   size_t lda, ldb, ldr;
   const void *a, *b, *bias, *residual;
   void *y, *z;
+  bool z_f32, halves;        // (halves: M counts a's rows, twice those of y)
 };
 bool linear_fits(const LinProduct& p);     // whether its launches take so large a product
 size_t linear_workspace_bytes(const LinProduct& p);
@@ -488,6 +489,8 @@ struct LinSlope {
   int M, N, dtype, dy_dtype, bias_dtype, act;
   const void *dy, *z;
   void *dz, *dbias;
+  int z_dtype;
+  bool low;                  // dz: M rows more, of what rounding left out
 };
 size_t linear_slope_workspace_bytes(const LinSlope& p);
 hipError_t launch_linear_slope(const LinSlope& p, void* workspace, hipStream_t s);

@@ -93,6 +93,21 @@ __global__ __launch_bounds__(256) void lin_pack_kernel(LinPacks js) {
 
 // ---- dz = dy act'(z) and the bias' gradient ------------------------------------------------------------------------
 
+// dz = v, and what its rounding leaves out in dz's second half (nothing of what is infinite or not a number there)
+__device__ __forceinline__ float lin_left(int dt, float v) {
+  const float r = dt == LIN_BF16 ? bf16_val((uint16_t)bf16_bits(v)) : (float)(_Float16)v;
+  return fabsf(r) < INFINITY ? v - r : 0.f;
+}
+__device__ __forceinline__ void lin_dz4(const LinSlope& a, size_t at, const float4& v) {
+  lin_put4(a.dtype, a.dz, at, v);
+  if (a.low)
+    lin_put4(a.dtype, a.dz, (size_t)a.M * a.N + at, make_float4(lin_left(a.dtype, v.x), lin_left(a.dtype, v.y), lin_left(a.dtype, v.z), lin_left(a.dtype, v.w)));
+}
+__device__ __forceinline__ void lin_dz(const LinSlope& a, size_t at, float v) {
+  lin_put(a.dtype, a.dz, at, v);
+  if (a.low) lin_put(a.dtype, a.dz, (size_t)a.M * a.N + at, lin_left(a.dtype, v));
+}
+
 // A workgroup takes 256 columns, a wave every fourth of `rows` rows, a lane four columns; part: sums of its rows, [row
 // block][N].  vec: whole groups of four columns, and every pointer takes 16 bytes.
 template <int ACT>
@@ -108,10 +123,10 @@ __global__ __launch_bounds__(256) void lin_slope_kernel(LinSlope a, float* part,
       const float4 d = lin_get4(a.dy_dtype, a.dy, at);
       float f[4] = {d.x, d.y, d.z, d.w};
       if constexpr (ACT != LIN_NONE) {
-        const float4 z = lin_get4(a.dtype, a.z, at);
+        const float4 z = lin_get4(a.z_dtype, a.z, at);
         f[0] *= lin_slope<ACT>(z.x); f[1] *= lin_slope<ACT>(z.y); f[2] *= lin_slope<ACT>(z.z); f[3] *= lin_slope<ACT>(z.w);
       }
-      if (a.dz) lin_put4(a.dtype, a.dz, at, make_float4(f[0], f[1], f[2], f[3]));
+      if (a.dz) lin_dz4(a, at, make_float4(f[0], f[1], f[2], f[3]));
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[e] += f[e];
     }
@@ -122,8 +137,8 @@ __global__ __launch_bounds__(256) void lin_slope_kernel(LinSlope a, float* part,
         if (n + e >= a.N) break;
         const size_t at = (size_t)m * a.N + n + e;
         float d = lin_get(a.dy_dtype, a.dy, at);
-        if constexpr (ACT != LIN_NONE) d *= lin_slope<ACT>(lin_get(a.dtype, a.z, at));
-        if (a.dz) lin_put(a.dtype, a.dz, at, d);
+        if constexpr (ACT != LIN_NONE) d *= lin_slope<ACT>(lin_get(a.z_dtype, a.z, at));
+        if (a.dz) lin_dz(a, at, d);
         s[e] += d;
       }
   }
@@ -145,15 +160,15 @@ __global__ __launch_bounds__(256) void lin_slope_flat_kernel(LinSlope a, size_t 
   for (size_t i = x; i < whole; i += step) {
     float4 d = lin_get4(a.dy_dtype, a.dy, 4 * i);
     if constexpr (ACT != LIN_NONE) {
-      const float4 z = lin_get4(a.dtype, a.z, 4 * i);
+      const float4 z = lin_get4(a.z_dtype, a.z, 4 * i);
       d.x *= lin_slope<ACT>(z.x); d.y *= lin_slope<ACT>(z.y); d.z *= lin_slope<ACT>(z.z); d.w *= lin_slope<ACT>(z.w);
     }
-    lin_put4(a.dtype, a.dz, 4 * i, d);
+    lin_dz4(a, 4 * i, d);
   }
   for (size_t i = 4 * whole + x; i < total; i += step) {
     float d = lin_get(a.dy_dtype, a.dy, i);
-    if constexpr (ACT != LIN_NONE) d *= lin_slope<ACT>(lin_get(a.dtype, a.z, i));
-    lin_put(a.dtype, a.dz, i, d);
+    if constexpr (ACT != LIN_NONE) d *= lin_slope<ACT>(lin_get(a.z_dtype, a.z, i));
+    lin_dz(a, i, d);
   }
 }
 // Sixteen groups of sixteen threads: a group's columns, every sixteenth block each
@@ -278,7 +293,7 @@ bool linear_fits(const LinProduct& p) {
   const int64_t m = p.M / 64 + 1, k = p.K / 64 + 1, n = p.N / 64 + 1;
   return (m + n) * k < (int64_t)1 << 24 || lin_packs_fit(p, lin_plan(p));
 }
-static size_t lin_parts_bytes(const LinProduct& p, const LinPlan& r) { return r.parts > 1 ? up((size_t)r.parts * p.M * p.N * 4, 256) : 0; }
+static size_t lin_parts_bytes(const LinProduct& p, const LinPlan& r) { return r.parts > 1 || p.halves ? up((size_t)r.parts * p.M * p.N * 4, 256) : 0; }
 
 size_t linear_workspace_bytes(const LinProduct& p) {
   const LinPlan r = lin_plan(p);
@@ -293,7 +308,10 @@ hipError_t launch_linear(const LinProduct& p, void* workspace, hipStream_t s) {
   a.out_dtype = p.out_dtype; a.bias_dtype = p.bias_dtype;
   a.ldr = p.ldr; a.bias = p.bias; a.residual = p.residual; a.y = p.y; a.z = p.z;
   a.vec = p.N % 8 == 0 && p.ldr % 8 == 0 && (low(p.bias) | low(p.residual) | low(p.y) | low(p.z)) % 16 == 0;
-  a.pairs = r.parts == 1 && p.dtype != LIN_F32 && p.out_dtype == p.dtype && (low(p.y) | low(p.z)) % 4 == 0;
+  a.z_dtype = p.z_f32 ? LIN_F32 : p.dtype;
+  a.sums = r.parts > 1 || p.halves;
+  a.halves = p.halves;
+  a.pairs = !a.sums && !(p.z && p.z_f32) && p.dtype != LIN_F32 && p.out_dtype == p.dtype && (low(p.y) | low(p.z)) % 4 == 0;
   a.parts = r.parts;
   a.per = r.per;
   a.a = LinOperand{static_cast<const uint16_t*>(p.a), p.lda, 0, p.M};
@@ -361,7 +379,7 @@ static void slope_go(const LinSlope& a, float* part, hipStream_t s) {
   const bool wide = (low(a.dy) | low(a.z) | low(a.dz)) % 16 == 0;
   if (!part) {
     const size_t total = (size_t)a.M * a.N, wgs = (total + 4095) / 4096;
-    hipLaunchKernelGGL(lin_slope_flat_kernel<ACT>, dim3(wgs < 16384 ? wgs : 16384), dim3(256), 0, s, a, total, wide);
+    hipLaunchKernelGGL(lin_slope_flat_kernel<ACT>, dim3(wgs < 16384 ? wgs : 16384), dim3(256), 0, s, a, total, wide && (!a.low || total % 4 == 0));
     return;
   }
   const int rows = slope_rows(a), blocks = slope_blocks(a);

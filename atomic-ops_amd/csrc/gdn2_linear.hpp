@@ -198,7 +198,8 @@ struct LinArgs {
   LinOperand a, b;
   int M, N, K;           // K: up to the last whole value of the sum
   int mt, nt, parts, per;        // tiles; parts of the sum, of `per` blocks each
-  int out_dtype, bias_dtype, vec, pairs;       // how results are written: lin_out8, lin_out_pairs
+  int out_dtype, bias_dtype, z_dtype, vec, pairs;       // how results are written: lin_out8, lin_out_pairs
+  int sums, halves;        // float32 sums go to `part`, to be joined: of parts, or of the two halves of a's rows
   size_t ldr;
   const void *bias, *residual;
   void *y, *z;
@@ -387,7 +388,7 @@ __device__ __forceinline__ void lin_out(const LinArgs& a, int m, int n, const fl
         const float4 b = lin_get4(a.bias_dtype, a.bias, n + q);
         v.x += b.x; v.y += b.y; v.z += b.z; v.w += b.w;
       }
-      if (a.z) LinType<DT>::put4(a.z, at + q, v);
+      if (a.z) lin_put4(a.z_dtype, a.z, at + q, v);
       v = make_float4(lin_act<ACT>(v.x), lin_act<ACT>(v.y), lin_act<ACT>(v.z), lin_act<ACT>(v.w));
       if (a.residual) {
         const float4 r = lin_get4(a.out_dtype, a.residual, (size_t)m * a.ldr + n + q);
@@ -401,7 +402,7 @@ __device__ __forceinline__ void lin_out(const LinArgs& a, int m, int n, const fl
   for (int e = 0; e < E; ++e) {
     if (n + e >= a.N) break;
     float z = f[e] + (a.bias ? lin_get(a.bias_dtype, a.bias, n + e) : 0.f);
-    if (a.z) LinType<DT>::put(a.z, at + e, z);
+    if (a.z) lin_put(a.z_dtype, a.z, at + e, z);
     z = lin_act<ACT>(z);
     if (a.residual) z += lin_get(a.out_dtype, a.residual, (size_t)m * a.ldr + n + e);
     lin_put(a.out_dtype, a.y, at + e, z);
@@ -436,7 +437,8 @@ __device__ __forceinline__ void lin_out8(const LinArgs& a, int m, int n, float* 
   const float b[8] = {cols.b[0].x, cols.b[0].y, cols.b[0].z, cols.b[0].w, cols.b[1].x, cols.b[1].y, cols.b[1].z, cols.b[1].w};
 #pragma unroll
   for (int e = 0; e < 8; ++e) f[e] += b[e];
-  if (a.z) LinVec<DT>::store8(a.z, at, f);
+  if (a.z && a.z_dtype == LIN_F32) LinVec<LIN_F32>::store8(a.z, at, f);
+  else if (a.z) LinVec<DT>::store8(a.z, at, f);
 #pragma unroll
   for (int e = 0; e < 8; ++e) f[e] = lin_act<ACT>(f[e]);
   if (a.residual) {
@@ -477,7 +479,7 @@ __device__ __forceinline__ void lin_out_odd(const LinArgs& a, int part, const fl
   const float bias = a.bias ? lin_get(a.bias_dtype, a.bias, n) : 0.f;
   for (int r = l / COLS; r < rows && m0 + r < a.M; r += STEP * U) {
     float res[U];
-    if (a.residual && a.parts == 1)
+    if (a.residual && !a.sums)
 #pragma unroll
       for (int u = 0; u < U; ++u) res[u] = lin_get(a.out_dtype, a.residual, (size_t)min(m0 + r + u * STEP, a.M - 1) * a.ldr + n);
 #pragma unroll
@@ -486,13 +488,13 @@ __device__ __forceinline__ void lin_out_odd(const LinArgs& a, int part, const fl
       if (row >= rows || m >= a.M) break;
       float f = own[row * ldo + col];
       if (more) f += more[row * ldo + col];
-      if (a.parts > 1) {
+      if (a.sums) {
         a.part[((size_t)part * a.M + m) * a.N + n] = f;
         continue;
       }
       f += bias;
       const size_t at = (size_t)m * a.N + n;
-      if (a.z) LinType<DT>::put(a.z, at, f);
+      if (a.z) lin_put(a.z_dtype, a.z, at, f);
       f = lin_act<ACT>(f);
       if (a.residual) f += res[u];
       lin_put(a.out_dtype, a.y, at, f);
@@ -714,7 +716,7 @@ __global__ __launch_bounds__(C::W * WAVE) void lin_tile_kernel(LinArgs a) {
       const int m1 = mh + 8 * j, m2 = m1 + 8;
       if (n >= a.N || m1 >= a.M) break;
       LinResidual r1, r2;
-      if (a.parts == 1) {
+      if (!a.sums) {
         r1.load(a, m1, n);
         r2.load(a, min(m2, a.M - 1), n);
       }
@@ -724,7 +726,7 @@ __global__ __launch_bounds__(C::W * WAVE) void lin_tile_kernel(LinArgs a) {
 #pragma unroll
         for (int e = 0; e < 8; e += 4)
           *reinterpret_cast<f4*>(f[q] + e) = *reinterpret_cast<const f4*>(own + (8 * (j + q) + (l >> 3)) * C::LDO + col + e);
-      if (a.parts > 1) {
+      if (a.sums) {
         lin_out_part<8>(a, part, m1, n, f[0]);
         if (m2 < a.M) lin_out_part<8>(a, part, m2, n, f[1]);
       } else {
@@ -849,14 +851,14 @@ __global__ __launch_bounds__(512) void lin_direct_kernel(LinArgs a) {
   const int row = 16 * half + (l >> 2), m = m0 + 32 * wm + row;
   if (m >= a.M) return;
   LinResidual res;
-  if (a.parts == 1) res.load(a, m, n);
+  if (!a.sums) res.load(a, m, n);
   float f[8];
 #pragma unroll
   for (int e = 0; e < 8; e += 4) {
     const float* q = low + row * C::LDO + col + e;
     *reinterpret_cast<f4*>(f + e) = *reinterpret_cast<const f4*>(q) + *reinterpret_cast<const f4*>(q + 4 * 32 * C::LDO);
   }
-  if (a.parts > 1) lin_out_part<8>(a, part, m, n, f);
+  if (a.sums) lin_out_part<8>(a, part, m, n, f);
   else lin_out8<LIN_F32, C::ACT>(a, m, n, f, cols, res);
 }
 
@@ -910,7 +912,7 @@ __global__ __launch_bounds__(LIN_ROWS_W * WAVE) void lin_rows_kernel(LinArgs a) 
     for (int v = 0; v < LIN_ROWS_W; ++v)
 #pragma unroll
       for (int e = 0; e < 4; ++e) f[e] += sums[v][m][col + e];
-    if (a.parts > 1) lin_out_part<4>(a, blockIdx.y, m0 + m, at, f);
+    if (a.sums) lin_out_part<4>(a, blockIdx.y, m0 + m, at, f);
     else lin_out<DT, ACT, 4>(a, m0 + m, at, f);
   }
 }
@@ -959,7 +961,7 @@ __global__ __launch_bounds__(256) void lin_columns_kernel(LinArgs a) {
     float f[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) f[q] = (sums[0][m][col + q] + sums[1][m][col + q]) + (sums[2][m][col + q] + sums[3][m][col + q]);
-    if (a.parts > 1) lin_out_part<4>(a, blockIdx.y, m0 + m, to, f);
+    if (a.sums) lin_out_part<4>(a, blockIdx.y, m0 + m, to, f);
     else lin_out<DT, ACT, 4>(a, m0 + m, to, f);
   }
 }
@@ -998,7 +1000,7 @@ __global__ __launch_bounds__(256) void lin_dots_kernel(LinArgs a) {
 #pragma unroll
       for (int o = 1; o < WAVE; o *= 2) acc[m][i] += __shfl_xor(acc[m][i], o);
     if (l != m || m0 + m >= a.M) continue;
-    if (a.parts > 1) lin_out_part<4>(a, blockIdx.y, m0 + m, n0, acc[m]);
+    if (a.sums) lin_out_part<4>(a, blockIdx.y, m0 + m, n0, acc[m]);
     else lin_out<DT, ACT, 4>(a, m0 + m, n0, acc[m]);
   }
 }
@@ -1016,8 +1018,12 @@ enum { LIN_SMALL, LIN_MID, LIN_BIG, LIN_DIRECT, LIN_CUT };      // the last two:
 constexpr int lin_bk(int dtype) { return dtype == LIN_F32 ? 32 : 64; }
 
 template <int DT, int ACT>
-static void lin_join(const LinArgs& a, hipStream_t s) {
-  if (a.parts == 1) return;
+static void lin_join(LinArgs a, hipStream_t s) {
+  if (!a.sums) return;
+  if (a.halves) {
+    a.M /= 2;
+    a.parts *= 2;
+  }
   const size_t threads = (size_t)a.M * (a.vec ? a.N / 4 : a.N);
   const dim3 grid((threads + 255) / 256);
   if (a.vec) hipLaunchKernelGGL((lin_join_kernel<DT, ACT, 4>), grid, dim3(256), 0, s, a);

@@ -375,7 +375,18 @@ int gdn2_beam_step(const gdn2_beam* p, void* workspace, void* stream);
  * gdn2_linear_workspace_bytes (0: none), 16-byte aligned.  M, K, N <= 2^27, and operands that have to be copied (float32 ones
  * for large tiles, rows that 16-byte accesses do not take) of fewer than 2^24 tiles of 64 x 64. */
 enum { GDN2_XW = 0, GDN2_XWT = 1, GDN2_XTW = 2 };
+/* With GDN2_XW and GDN2_XWT: a holds 2 M rows, and row m of A is the sum of its rows m and M + m, in float32 (dz and what its
+ * rounding left out: GDN2_DZ_LOW). */
+enum { GDN2_HALVES = 4 };
 enum { GDN2_ACT_NONE = 0, GDN2_ACT_SILU = 1, GDN2_ACT_GELU = 2, GDN2_ACT_GELU_TANH = 3 };
+/* Added to an activation.  GDN2_Z_F32: z is float32.  GDN2_DZ_LOW (gdn2_linear_slope, 16 bits): dz holds 2 M rows, and row M + m
+ * what the rounding of row m left out, rounded. */
+enum { GDN2_Z_F32 = 16, GDN2_DZ_LOW = 32 };
+/* The gradients of a product of 16 bits with 2 M K N up to GDN2_LINEAR_FINE operations are formed from both of dz's numbers, and
+ * z is kept in float32 for them, and for other results of up to GDN2_LINEAR_Z elements: there it costs little, and few numbers
+ * average a rounding out. */
+#define GDN2_LINEAR_FINE 1073741824
+#define GDN2_LINEAR_Z 2097152
 typedef struct gdn2_product {
   int32_t M, K, N, form, dtype, out_dtype, bias_dtype, activation;
   int64_t lda, ldb, ldr;

@@ -30,7 +30,7 @@ def test_what_the_backward_pass_hands_to_the_kernels(monkeypatch, hook):
         seen.extend((a, b))
         return out.zero_()
 
-    def slope(dy, z, dtype, act, bias_dtype, need_dz):
+    def slope(dy, z, dtype, act, bias_dtype, need_dz, fine):
         assert z.is_contiguous() and torch.equal(z, kept) and z.dtype == dtype
         return torch.ones_like(dy), None
 
