@@ -22,7 +22,7 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}        # GDN2_
 _ACTS = {None: 0, "silu": 1, "gelu": 2, "gelu_tanh": 3}                  # GDN2_ACT_*
 _XW, _XWT, _XTW = 0, 1, 2
 _HALVES, _Z_F32, _DZ_LOW = 4, 16, 32                                     # GDN2_*
-_FINE, _FINE_Z = 2 ** 30, 2 ** 21                                        # GDN2_LINEAR_FINE, GDN2_LINEAR_Z
+_FINE, _FINE_X, _FINE_Z = 2 ** 30, 2 ** 21, 2 ** 21                      # GDN2_LINEAR_FINE, _X, _Z
 
 
 def _addr(t):
@@ -55,8 +55,9 @@ def _product(form, a, b, M, K, N, out, bias=None, residual=None, act=0, z=None):
 def _fine(M, K, N, dtype):
     """Whether the gradients of a product of 16 bits are formed from dz and what its rounding leaves out.  Rounded alone, dz makes
     their error 1.42 times that of rounding them, in products of 32 to 100 rows or columns up to twice.  (With silu, us on the GPU,
-    rounded and both: 1 x 5412 x 127 27, 32; 2 x 1793 x 4407 66, 82; 300 x 677 x 811 51, 63; 2048 x 768 x 512 39, 57.)"""
-    return dtype != torch.float32 and 2 * M * K * N <= _FINE
+    rounded and both: 1 x 5412 x 127 27, 32; 2 x 1793 x 4407 66, 82; 300 x 677 x 811 51, 63; 2048 x 768 x 512 39, 57.
+    x is copied for it, so that a long one is left out: 16384 x 4096 x 1 118, 547.)"""
+    return dtype != torch.float32 and 2 * M * K * N <= _FINE and M * K <= _FINE_X
 
 
 def _z_dtype(M, K, N, dtype):
@@ -146,7 +147,8 @@ def linear(x, weight, bias=None, residual=None, activation=None, out_dtype=None)
     to out_dtype.  activation: None, "silu", "gelu" (z Phi(z)) or "gelu_tanh".  x and residual may be rows of wider
     matrices.  Gradients of all four, each summed in float32 and in its tensor's dtype; with an activation
     z = x W + bias is kept for them in x's dtype, and the gradient of z has x's dtype; a product of up to 2^30
-    operations keeps z in float32 and rounds no gradient on its way, results of up to 2^21 elements keep z in float32.  Once differentiable.  A row
+    operations over an x of up to 2^21 elements keeps z in float32 and rounds no gradient on its way, and results of up to
+    2^21 elements keep z in float32.  Once differentiable.  A row
     of x with an infinity or NaN gives nothing finite in float32 (an infinity may come out as NaN: larger float32 products
     take it in pieces), and touches no other row."""
     if activation in _ACTS and isinstance(x, torch.Tensor) and x.is_cuda and out_dtype in (None, x.dtype, torch.float32):

@@ -48,7 +48,7 @@ bool product(int form, int64_t M, int64_t K, int64_t N, const Tensor& a, int64_t
 // Whether the gradients of a product of 16 bits are formed from dz and what its rounding leaves out, and what z is kept in
 // (linear.py, _fine and _z_dtype)
 bool fine_gradients(int64_t M, int64_t K, int64_t N, at::ScalarType dt) {
-  return dt != at::kFloat && 2.0 * (double)M * (double)K * (double)N <= GDN2_LINEAR_FINE;
+  return dt != at::kFloat && 2.0 * (double)M * (double)K * (double)N <= GDN2_LINEAR_FINE && M * K <= GDN2_LINEAR_X;
 }
 at::ScalarType z_type(int64_t M, int64_t K, int64_t N, at::ScalarType dt) {
   return fine_gradients(M, K, N, dt) || M * N <= GDN2_LINEAR_Z ? at::kFloat : dt;

@@ -382,10 +382,11 @@ enum { GDN2_ACT_NONE = 0, GDN2_ACT_SILU = 1, GDN2_ACT_GELU = 2, GDN2_ACT_GELU_TA
 /* Added to an activation.  GDN2_Z_F32: z is float32.  GDN2_DZ_LOW (gdn2_linear_slope, 16 bits): dz holds 2 M rows, and row M + m
  * what the rounding of row m left out, rounded. */
 enum { GDN2_Z_F32 = 16, GDN2_DZ_LOW = 32 };
-/* The gradients of a product of 16 bits with 2 M K N up to GDN2_LINEAR_FINE operations are formed from both of dz's numbers, and
- * z is kept in float32 for them, and for other results of up to GDN2_LINEAR_Z elements: there it costs little, and few numbers
- * average a rounding out. */
+/* The gradients of a product of 16 bits with 2 M K N up to GDN2_LINEAR_FINE operations, and x of up to GDN2_LINEAR_X elements,
+ * are formed from both of dz's numbers, and z is kept in float32 for them, and for other results of up to GDN2_LINEAR_Z
+ * elements: there it costs little, and few numbers average a rounding out. */
 #define GDN2_LINEAR_FINE 1073741824
+#define GDN2_LINEAR_X 2097152
 #define GDN2_LINEAR_Z 2097152
 typedef struct gdn2_product {
   int32_t M, K, N, form, dtype, out_dtype, bias_dtype, activation;

@@ -95,7 +95,7 @@ def test_no_worse_than_one_rounding(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("M,K,N", [(1000, 1000, 1000), (1400, 700, 1498), (1400, 700, 1500), (5000, 2000, 60)])
+@pytest.mark.parametrize("M,K,N", [(1000, 1000, 1000), (1400, 700, 1498), (1400, 700, 1500), (5000, 2000, 60), (2100, 2000, 50), (5000, 4096, 1)])
 def test_larger_ones_round_dz_once(dtype, M, K, N):
     """Beyond: dz is rounded (u of it), z as well from 2^21 results on (u |z| of the slope, whose derivative is below 1)."""
     from atomic_gdn2.linear import linear
