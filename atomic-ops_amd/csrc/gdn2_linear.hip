@@ -98,19 +98,21 @@ __device__ __forceinline__ float lin_left(int dt, float v) {
   const float r = dt == LIN_BF16 ? bf16_val((uint16_t)bf16_bits(v)) : (float)(_Float16)v;
   return fabsf(r) < INFINITY ? v - r : 0.f;
 }
+template <bool LOW>
 __device__ __forceinline__ void lin_dz4(const LinSlope& a, size_t at, const float4& v) {
   lin_put4(a.dtype, a.dz, at, v);
-  if (a.low)
+  if constexpr (LOW)
     lin_put4(a.dtype, a.dz, (size_t)a.M * a.N + at, make_float4(lin_left(a.dtype, v.x), lin_left(a.dtype, v.y), lin_left(a.dtype, v.z), lin_left(a.dtype, v.w)));
 }
+template <bool LOW>
 __device__ __forceinline__ void lin_dz(const LinSlope& a, size_t at, float v) {
   lin_put(a.dtype, a.dz, at, v);
-  if (a.low) lin_put(a.dtype, a.dz, (size_t)a.M * a.N + at, lin_left(a.dtype, v));
+  if constexpr (LOW) lin_put(a.dtype, a.dz, (size_t)a.M * a.N + at, lin_left(a.dtype, v));
 }
 
 // A workgroup takes 256 columns, a wave every fourth of `rows` rows, a lane four columns; part: sums of its rows, [row
 // block][N].  vec: whole groups of four columns, and every pointer takes 16 bytes.
-template <int ACT>
+template <int ACT, bool LOW>
 __global__ __launch_bounds__(256) void lin_slope_kernel(LinSlope a, float* part, int rows, int vec) {
   __shared__ float4 sums[4][64];
   const int l = lane_id(), w = wave_id(), n = blockIdx.x * 256 + 4 * l;
@@ -126,7 +128,7 @@ __global__ __launch_bounds__(256) void lin_slope_kernel(LinSlope a, float* part,
         const float4 z = lin_get4(a.z_dtype, a.z, at);
         f[0] *= lin_slope<ACT>(z.x); f[1] *= lin_slope<ACT>(z.y); f[2] *= lin_slope<ACT>(z.z); f[3] *= lin_slope<ACT>(z.w);
       }
-      if (a.dz) lin_dz4(a, at, make_float4(f[0], f[1], f[2], f[3]));
+      if (a.dz) lin_dz4<LOW>(a, at, make_float4(f[0], f[1], f[2], f[3]));
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[e] += f[e];
     }
@@ -138,7 +140,7 @@ __global__ __launch_bounds__(256) void lin_slope_kernel(LinSlope a, float* part,
         const size_t at = (size_t)m * a.N + n + e;
         float d = lin_get(a.dy_dtype, a.dy, at);
         if constexpr (ACT != LIN_NONE) d *= lin_slope<ACT>(lin_get(a.z_dtype, a.z, at));
-        if (a.dz) lin_dz(a, at, d);
+        if (a.dz) lin_dz<LOW>(a, at, d);
         s[e] += d;
       }
   }
@@ -153,7 +155,7 @@ __global__ __launch_bounds__(256) void lin_slope_kernel(LinSlope a, float* part,
 }
 // Without a bias the rows do not matter: dy, z and dz are arrays of `total` values, whatever a row's width.  vec: every
 // pointer takes 16 bytes.
-template <int ACT>
+template <int ACT, bool LOW>
 __global__ __launch_bounds__(256) void lin_slope_flat_kernel(LinSlope a, size_t total, int vec) {
   const size_t x = (size_t)blockIdx.x * 256 + threadIdx.x, step = (size_t)gridDim.x * 256, whole = vec ? total / 4 : 0;
 #pragma unroll 4
@@ -163,12 +165,12 @@ __global__ __launch_bounds__(256) void lin_slope_flat_kernel(LinSlope a, size_t 
       const float4 z = lin_get4(a.z_dtype, a.z, 4 * i);
       d.x *= lin_slope<ACT>(z.x); d.y *= lin_slope<ACT>(z.y); d.z *= lin_slope<ACT>(z.z); d.w *= lin_slope<ACT>(z.w);
     }
-    lin_dz4(a, 4 * i, d);
+    lin_dz4<LOW>(a, 4 * i, d);
   }
   for (size_t i = 4 * whole + x; i < total; i += step) {
     float d = lin_get(a.dy_dtype, a.dy, i);
     if constexpr (ACT != LIN_NONE) d *= lin_slope<ACT>(lin_get(a.z_dtype, a.z, i));
-    lin_dz(a, i, d);
+    lin_dz<LOW>(a, i, d);
   }
 }
 // Sixteen groups of sixteen threads: a group's columns, every sixteenth block each
@@ -373,25 +375,29 @@ static int slope_blocks(const LinSlope& a) {
   return (a.M + rows - 1) / rows;
 }
 size_t linear_slope_workspace_bytes(const LinSlope& a) { return a.dbias ? (size_t)slope_blocks(a) * a.N * 4 : 0; }
-template <int ACT>
+template <int ACT, bool LOW>
 static void slope_go(const LinSlope& a, float* part, hipStream_t s) {
   auto low = [](const void* q) { return reinterpret_cast<uintptr_t>(q); };
   const bool wide = (low(a.dy) | low(a.z) | low(a.dz)) % 16 == 0;
   if (!part) {
     const size_t total = (size_t)a.M * a.N, wgs = (total + 4095) / 4096;
-    hipLaunchKernelGGL(lin_slope_flat_kernel<ACT>, dim3(wgs < 16384 ? wgs : 16384), dim3(256), 0, s, a, total, wide && (!a.low || total % 4 == 0));
+    hipLaunchKernelGGL((lin_slope_flat_kernel<ACT, LOW>), dim3(wgs < 16384 ? wgs : 16384), dim3(256), 0, s, a, total, wide && (!LOW || total % 4 == 0));
     return;
   }
   const int rows = slope_rows(a), blocks = slope_blocks(a);
-  hipLaunchKernelGGL(lin_slope_kernel<ACT>, dim3((a.N + 255) / 256, blocks), dim3(256), 0, s, a, part, rows, a.N % 4 == 0 && wide);
+  hipLaunchKernelGGL((lin_slope_kernel<ACT, LOW>), dim3((a.N + 255) / 256, blocks), dim3(256), 0, s, a, part, rows, a.N % 4 == 0 && wide);
   hipLaunchKernelGGL(lin_bias_kernel, dim3((a.N + 15) / 16), dim3(256), 0, s, a, part, blocks);
+}
+template <bool LOW>
+static void slope_act(const LinSlope& a, float* part, hipStream_t s) {
+  if (a.act == LIN_SILU) slope_go<LIN_SILU, LOW>(a, part, s);
+  else if (a.act == LIN_GELU) slope_go<LIN_GELU, LOW>(a, part, s);
+  else if (a.act == LIN_TANH) slope_go<LIN_TANH, LOW>(a, part, s);
+  else slope_go<LIN_NONE, LOW>(a, part, s);
 }
 hipError_t launch_linear_slope(const LinSlope& a, void* workspace, hipStream_t s) {
   float* part = a.dbias ? static_cast<float*>(workspace) : nullptr;
-  if (a.act == LIN_SILU) slope_go<LIN_SILU>(a, part, s);
-  else if (a.act == LIN_GELU) slope_go<LIN_GELU>(a, part, s);
-  else if (a.act == LIN_TANH) slope_go<LIN_TANH>(a, part, s);
-  else slope_go<LIN_NONE>(a, part, s);
+  a.low ? slope_act<true>(a, part, s) : slope_act<false>(a, part, s);
   return hipGetLastError();
 }
 

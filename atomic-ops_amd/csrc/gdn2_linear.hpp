@@ -154,20 +154,19 @@ __device__ __forceinline__ float lin_act(float z) {
   else if constexpr (ACT == LIN_TANH) return z * lin_logistic(LIN_TANH_C * (z + 0.044715f * z * z * z));
   else return z;
 }
-// (far out a slope is 0 or 1 and its terms are 0 times an infinity: z goes no further than where that is so.  float16 keeps a
-// z beyond 65504 as an infinity.  NaN stays NaN.)
+// (far out a slope is 0 or 1, and its terms 0 times an infinity: as a factor z goes no further than where that is so.  float16
+// keeps a z beyond 65504 as an infinity.  NaN stays NaN by the other factors.)
 template <int ACT>
 __device__ __forceinline__ float lin_slope(float z) {
-  constexpr float FAR = 1e18f;
-  z = z > FAR ? FAR : z < -FAR ? -FAR : z;
+  const float near = __builtin_amdgcn_fmed3f(z, -1e18f, 1e18f);
   if constexpr (ACT == LIN_SILU) {
     const float s = lin_logistic(z);
-    return s * (1.f + z * (1.f - s));
+    return s * (1.f + near * (1.f - s));
   } else if constexpr (ACT == LIN_GELU) {
-    return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);
+    return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + near * 0.39894228040143268f * __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);
   } else if constexpr (ACT == LIN_TANH) {
     const float s = lin_logistic(LIN_TANH_C * (z + 0.044715f * z * z * z));
-    return s + z * s * (1.f - s) * (LIN_TANH_C * (1.f + 0.134145f * z * z));
+    return s + near * s * (1.f - s) * (LIN_TANH_C * (1.f + 0.134145f * near * near));
   } else {
     return 1.f;
   }
