@@ -219,7 +219,7 @@ static LinSide lin_side(const LinProduct& p, bool b) {
 // 512^3 10.6, 16.3; 2048 x 768 x 512 21.2, 29.0; 1024^3 28, 33; 2048 x 1024 x 768 46.5, 37.4; 4096 x 2048 x 1024 160, 103); in rows
 // that 16-byte accesses do not take 300 x 677 x 811 17.9, 22.0; 500 x 999 x 1001 24.9, 27.0; 2047 x 767 x 513 43.8, 33.3
 constexpr double LIN_DIRECT_MOST = 2.5e9, LIN_DIRECT_ODD = 1.2e9;
-// float32 as pieces that a pass over memory has cut before (cut by each wave, by the pass): large tiles over a long sum, 4096^3
+// float32 as pieces that a pass over memory has cut before (cut by each wave, by the pass, on one card): large tiles over a long sum, 4096^3
 // 698, 667, but 4096 x 2048 x 1024 103, 128; odd rows, where an operand is used often enough, which M N / (M + N) says: 2048 x
 // 4095 x 4097 754, 535 (1365); 16383 x 255 x 513 75, 69 (497); 2047 x 767 x 513 33.3, 34.9 (410); 218 x 8190 x 7626 265, 358 (212)
 constexpr int64_t LIN_PACK_K = 4096, LIN_PACK_USE = 450;

@@ -10,11 +10,13 @@
 // What takes a product (the rules, with both sides measured, are in gdn2_linear.hip):
 //   lin_tile_kernel     tiles of 256 x 256 (float32 256 x 128), 128 x 128 or 64 x 64, operands into LDS by DMA a block ahead of
 //                       their use, sums in parts where there are few tiles; float32 as three bfloat16 pieces, six
-//                       products.  Bound by the matrix cores: 8192 x 4096 x 4096 bfloat16 225 us, 1.22 PFLOP/s;
-//                       4096^3 float32 660 us, 208 TFLOP/s (a library product on the float32 matrix cores 911).  Each
-//                       tile's epilogue waits for its products: with bias, activation, z and residual 296.  CUT:
+//                       products.  Bound by the matrix cores: 8192 x 4096 x 4096 bfloat16 215 to 232
+//                       us by card, 1.18 to 1.28 PFLOP/s; 4096^3 float32 647 to 671, 205 to 212 TFLOP/s (a library product on
+//                       the float32 matrix cores 917).  Each tile's epilogue waits for its products: with bias,
+//                       activation, z and residual 260.  CUT:
 //                       float32 stays as it is up to LDS and each wave cuts what it reads, no pass over memory before it:
-//                       218 x 8192 x 7680 197 us (by a pass 357, the library 237), 4096 x 2048 x 1024 103 (128, 119);
+//                       218 x 8192 x 7680 181 to 188 us (the library 208 to 216), 4096 x 2048 x 1024 103 (by a pass 128, the
+//                       library 119);
 //   lin_direct_kernel   small float32 products: 2048 x 768 x 512 21 us (the library's 18), 512^3 10.6 (17), bound by what
 //                       its small tiles draw from the caches;
 //   lin_rows_kernel, lin_columns_kernel, lin_dots_kernel   up to 8 rows, bound by W's bytes: one row of 4096 x 14336 bfloat16
@@ -605,7 +607,7 @@ __global__ __launch_bounds__(C::W * WAVE) void lin_tile_kernel(LinArgs a) {
 #pragma unroll
       for (int t = 0; t < MT; ++t) acc[q][i][t] = f4{0.f, 0.f, 0.f, 0.f};
   // Operands are read ahead of their use, those of A by AHEAD tiles, those of B by one step of the sum, a few beside each
-  // group of products (8192 x 4096 x 4096 bfloat16: 225 us, 1224 TFLOP/s; read where they are used 248)
+  // group of products (8192 x 4096 x 4096 bfloat16, on one card: 225 us; read where they are used 248)
   auto products = [&](int t, const s8 (&n)[NP][NT], const s8 (&m)[NP]) __attribute__((always_inline)) {
     // (float32: the smallest pieces' products first)
 #pragma unroll
